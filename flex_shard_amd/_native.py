@@ -120,6 +120,33 @@ class MuonGroup(Structure):
     ]
 
 
+class MxFp4Product(Structure):
+    """``fsh_mxfp4_product``."""
+
+    _fields_ = [
+        ("a_dev", c_void_p),
+        ("a_scales_dev", c_void_p),
+        ("b_dev", c_void_p),
+        ("b_scales_dev", c_void_p),
+        ("out_dev", c_void_p),
+        ("bias_dev", c_void_p),
+        ("offsets_dev", c_void_p),
+        ("source_dev", c_void_p),
+        ("m", c_int64),
+        ("n", c_int64),
+        ("k", c_int64),
+        ("a_rows", c_int64),
+        ("b_rows", c_int64),
+        ("ldo", c_int64),
+        ("out_dtype", c_int32),
+        ("mode", c_int32),
+        ("experts", c_int32),
+        ("top_k", c_int32),
+    ]
+
+
+MXFP4_DENSE, MXFP4_ROWS, MXFP4_OVER_ROWS = 0, 1, 2
+MAX_EXPERTS = 1024
 MAX_NS_PROBLEMS = 16
 MUON_PADDED = 1
 MAX_COPY_ROWS = 32
@@ -217,6 +244,33 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [POINTER(MuonGroup), c_int32, c_float, c_float, c_int32, c_float, c_float, c_float, c_float, c_int32, c_float,
          c_void_p],
+    ),
+    "fsh_mxfp4_quantize": (
+        c_int,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "fsh_mxfp4_quantize_segments": (
+        c_int,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "fsh_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_void_p]),
+    "fsh_sum_runs": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
+    "fsh_mxfp4_gemm": (c_int, [POINTER(MxFp4Product), c_void_p]),
+    "fsh_expert_route_workspace_bytes": (c_int64, [c_int64, c_int32]),
+    "fsh_expert_route": (
+        c_int, [c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    ),
+    "fsh_expert_dispatch": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p],
+    ),
+    "fsh_expert_combine": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p],
+    ),
+    "fsh_expert_combine_backward": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p,
+         c_void_p, c_void_p],
     ),
 }
 

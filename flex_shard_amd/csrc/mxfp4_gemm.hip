@@ -1,0 +1,100 @@
+// Products of microscaled 4-bit matrices: a linear layer's forward, its input
+// gradient and its weight gradient are all a b^T of operands quantized along the
+// contraction; the experts' layers are the same with rows (or the contraction)
+// in segments.
+#include "mxfp4_tiles.hpp"
+
+namespace fsh {
+namespace {
+
+template <typename Cfg, int kProblem>
+int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t stream) {
+  GemmParams& s = p.schedule;
+  const int64_t tiles_n = ceil_div(p.n, static_cast<int64_t>(Cfg::BN)), tiles = tiles_m * tiles_n;
+  if (tiles * batch > 0x3FFFFFLL) return fail(FSH_ENOTSUP, "fsh_mxfp4_gemm: too many tiles");
+  s.tiles_m = static_cast<int32_t>(tiles_m);
+  s.tiles_n = static_cast<int32_t>(tiles_n);
+  s.tiles_per_matrix = static_cast<int32_t>(tiles);
+  s.work_items = tiles * batch;
+  s.items_per_xcd = ceil_div(s.work_items, static_cast<int64_t>(kXcds));
+  const dim3 grid(static_cast<uint32_t>(s.items_per_xcd * kXcds)), block(Cfg::kThreads);
+  int rc = FSH_OK;
+  by_dtype(p.out_dtype, [&](auto dt) {
+    static LdsReservation reserved;
+    const auto kernel = &mxfp4_gemm_kernel<Cfg, kProblem, dt.value>;
+    rc = reserve_lds_once(reserved, kernel, Cfg::kLdsBytes);
+    if (rc == FSH_OK) hipLaunchKernelGGL(kernel, grid, block, Cfg::kLdsBytes, stream, p);
+  });
+  return rc != FSH_OK ? rc : check_launch("mxfp4_gemm_kernel");
+}
+
+// Tiles of BM rows that the segments of p.m rows take at most: each of the
+// experts and the rows behind the last can end inside a tile.
+template <typename Cfg>
+int64_t segment_tiles(const MxGemmParams& p) { return p.m / Cfg::BM + p.experts + 1; }
+
+using MxLarge = MxTile<4, 2, 4, 8, 2>;
+using MxSmall = MxTile<2, 2, 2, 2, 3>;
+
+template <typename Cfg>
+int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
+  const int64_t tiles_m = ceil_div(p.m, static_cast<int64_t>(Cfg::BM));
+  if (problem == kMxRows) return launch_mx_tiles<Cfg, kMxRows>(p, segment_tiles<Cfg>(p), 1, stream);
+  if (problem == kMxOverRows) return launch_mx_tiles<Cfg, kMxOverRows>(p, tiles_m, p.experts, stream);
+  return launch_mx_tiles<Cfg, kMxDense>(p, tiles_m, 1, stream);
+}
+
+}  // namespace
+}  // namespace fsh
+
+FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_mxfp4_gemm";
+  if (!product) return fail(FSH_EINVAL, "%s: null product", who);
+  const fsh_mxfp4_product& q = *product;
+  if (q.m < 0 || q.n < 0 || q.k < 0) return fail(FSH_EINVAL, "%s: negative size", who);
+  if (q.mode != FSH_MXFP4_DENSE && q.mode != FSH_MXFP4_ROWS && q.mode != FSH_MXFP4_OVER_ROWS)
+    return fail(FSH_EINVAL, "%s: unknown mode %d", who, q.mode);
+  if (q.mode != FSH_MXFP4_DENSE && q.experts <= 0) return fail(FSH_EINVAL, "%s: no expert", who);
+  if (q.m == 0 || q.n == 0) return FSH_OK;
+  if (!known_dtype(q.out_dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, q.out_dtype);
+  if (!q.a_dev || !q.a_scales_dev || !q.b_dev || !q.b_scales_dev || !q.out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (q.k == 0 || q.k % kMxColumns)
+    return fail(FSH_ENOTSUP, "%s: k must be a positive multiple of %d (operands are padded), got %lld", who, kMxColumns, (long long)q.k);
+  if (q.k >= (1LL << 31) || q.m >= (1LL << 28) || q.n >= (1LL << 28) || q.a_rows >= (1LL << 28) || q.b_rows >= (1LL << 28))
+    return fail(FSH_ENOTSUP, "%s: sizes beyond 2^28 rows or 2^31 columns", who);
+  if (q.ldo < q.n) return fail(FSH_EINVAL, "%s: ldo %lld < n %lld", who, (long long)q.ldo, (long long)q.n);
+  const bool segments = q.mode == FSH_MXFP4_ROWS;
+  if (q.mode != FSH_MXFP4_DENSE && !q.offsets_dev) return fail(FSH_EINVAL, "%s: segments without offsets", who);
+  if (segments && q.top_k <= 0) return fail(FSH_EINVAL, "%s: top_k must be positive", who);
+  if (q.a_rows < (q.source_dev ? 1 : q.m) || q.b_rows < q.n * (segments ? q.experts : 1))
+    return fail(FSH_EINVAL, "%s: operands of %lld and %lld rows are too few", who, (long long)q.a_rows, (long long)q.b_rows);
+  if (q.source_dev && !segments) return fail(FSH_EINVAL, "%s: gathered rows belong to segments of rows", who);
+  if (q.mode == FSH_MXFP4_OVER_ROWS && (q.bias_dev || q.ldo != q.n))
+    return fail(FSH_EINVAL, "%s: products over rows are contiguous and have no bias", who);
+  if (segments && q.bias_dev) return fail(FSH_ENOTSUP, "%s: segments have no bias", who);
+  if (!aligned(q.a_dev, 16) || !aligned(q.b_dev, 16) || !aligned(q.a_scales_dev, 8) || !aligned(q.b_scales_dev, 8) ||
+      !aligned(q.out_dev, dtype_bytes(q.out_dtype)) || !aligned(q.bias_dev, dtype_bytes(q.out_dtype)))
+    return fail(FSH_ENOTSUP, "%s: data must be 16-byte and scales 8-byte aligned, out and bias to their elements", who);
+  // The lanes' offsets are 32 bits from a tile's first row, or from the matrix for gathered rows.
+  if (256 * (q.k / 2) >= (1LL << 32) || (q.source_dev && q.a_rows * (q.k / 2) >= (1LL << 32)))
+    return fail(FSH_ENOTSUP, "%s: rows that are gathered, or a tile of them, span 4 GiB or more", who);
+  MxGemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
+  p.b = static_cast<const uint8_t*>(q.b_dev); p.bs = static_cast<const uint8_t*>(q.b_scales_dev);
+  p.out = q.out_dev; p.bias = q.bias_dev;
+  p.m = q.m; p.n = q.n; p.k = q.k;
+  p.a_rows = q.a_rows; p.b_rows = q.b_rows;
+  p.lda = p.ldb = q.k / 2;
+  p.ldo = q.ldo;
+  p.out_dtype = q.out_dtype;
+  p.experts = q.experts; p.top_k = q.top_k;
+  p.offsets = p.padded_offsets = q.offsets_dev;
+  p.source = q.source_dev;
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  const MxProblem problem = segments ? kMxRows : q.mode == FSH_MXFP4_OVER_ROWS ? kMxOverRows : kMxDense;
+  const int64_t rows = segments ? q.m / q.experts : q.m;
+  if (rows * q.n >= 128 * 128 * 64) return launch_mx<MxLarge>(p, problem, on);
+  return launch_mx<MxSmall>(p, problem, on);
+}

@@ -36,10 +36,11 @@ __all__ = [
     "REDUCE_PREMUL", "REDUCE_SUM", "SRC_BF16", "SRC_F16", "SRC_F32", "SRC_F32_AS_BF16", "SRC_F32_AS_F16",
     "MuonStepPlan", "QuantChunkSpec", "QuantPackPlan", "accumulate_grad", "act_quant_128x1_transposed", "act_quant_1x128", "act_quant_both",
     "copy_row_segments", "copy_segments", "fp8_gemm_1x128_128x1", "fp8_gemm_1x128_128x128", "fp8_gemm_1x128_128x128_dgrad",
+    "expert_combine", "expert_combine_backward", "expert_dispatch", "expert_route",
     "fp8_gemm_tiles", "fp8_linear_backward", "fp8_transpose", "gemm_nt", "gemm_nt_group", "gemm_tiles", "muon_apply",
-    "muon_prepare", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
+    "muon_prepare", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
     "newton_schulz_product_tiles",
-    "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "stream_ptr", "unpack_dequant", "zero_segments",
+    "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
 ]
 
 
@@ -1012,3 +1013,271 @@ class MuonStepPlan:
             steps, eps, stream_ptr(self._device),
         )
         _native.check(status, "fsh_muon_step")
+
+
+def _float_dt(dtype: torch.dtype) -> int:
+    return DT_F16 if dtype == torch.float16 else _dt(dtype)
+
+
+def _mxfp4_empty(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Data and scales of a quantized matrix [rows, cols]."""
+    steps = -(-cols // 256)
+    return (
+        torch.empty((rows, steps * 128), dtype=torch.uint8, device=device),
+        torch.empty((steps, rows, 8), dtype=torch.uint8, device=device),
+    )
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    """The row stride of a matrix whose rows are contiguous and apart."""
+    if x.ndim != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"expected a matrix with contiguous, separate rows, got {tuple(x.shape)} / {x.stride()}")
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def mxfp4_quantize(
+    x: torch.Tensor, *, rows: bool = True, columns: bool = False, column_sums: bool = False
+) -> tuple[tuple[torch.Tensor, torch.Tensor] | None, tuple[torch.Tensor, torch.Tensor] | None, torch.Tensor | None]:
+    """Quantize a bf16, fp16 or fp32 matrix (or contiguous stack [b, r, c]) to
+    microscaled 4-bit floats in one pass.  Returns ``(row form, column form,
+    sums)``: the row form is data and scales of [b * r, c], the column form those
+    of the transposes [b * c, r], None where not asked for; ``sums`` the fp32
+    column sums over 128 rows each, [ceil(r / 128), c] (a matrix with its column
+    form), which :func:`sum_runs` adds up."""
+    _require_gpu(x)
+    if x.ndim == 3:
+        if not x.is_contiguous():
+            raise ValueError("a stack of matrices must be contiguous")
+        batch, r, c = x.shape
+        ldx = c
+    else:
+        ldx = _row_stride(x)
+        batch, (r, c) = 1, x.shape
+    if not (rows or columns) or (column_sums and (not columns or x.ndim != 2)):
+        raise ValueError("ask for rows or columns; column sums come with the column form of a matrix")
+    row_form = _mxfp4_empty(batch * r, c, x.device) if rows else None
+    column_form = _mxfp4_empty(batch * c, r, x.device) if columns else None
+    sums = torch.empty((-(-r // 128), c), dtype=torch.float32, device=x.device) if column_sums else None
+    status = _native.lib().fsh_mxfp4_quantize(
+        x.data_ptr(), _float_dt(x.dtype), batch, r, c, ldx, *(map(_ptr, row_form) if rows else (None, None)),
+        *(map(_ptr, column_form) if columns else (None, None)), _ptr(sums), stream_ptr(x.device),
+    )
+    _native.check(status, "fsh_mxfp4_quantize")
+    return row_form, column_form, sums
+
+
+def mxfp4_quantize_segments(
+    x: torch.Tensor, offsets: torch.Tensor, padded_offsets: torch.Tensor, padded_rows: int, *, choices: int,
+    source: torch.Tensor | None = None, top_k: int = 1, rows: bool = False,
+) -> tuple[tuple[torch.Tensor, torch.Tensor] | None, tuple[torch.Tensor, torch.Tensor]]:
+    """The column form of rows sorted by expert, [cols, padded_rows]: segment
+    ``e`` from column ``padded_offsets[e]`` on, padded with zeros.  ``x`` holds the
+    ``choices`` sorted rows, or with ``source`` the rows ``source[i] // top_k`` of
+    them.  ``rows`` (without ``source``): the row form of [choices, cols] too."""
+    _require_gpu(x, offsets, padded_offsets, *([] if source is None else [source]))
+    ldx = _row_stride(x)
+    if source is None and x.shape[0] != choices:
+        raise ValueError(f"{choices} sorted rows expected, got {x.shape[0]}")
+    if rows and source is not None:
+        raise ValueError("the row form of gathered rows is that of x itself")
+    experts = _check_routing(offsets, padded_offsets)
+    cols = x.shape[1]
+    row_form = _mxfp4_empty(choices, cols, x.device) if rows else None
+    column_form = _mxfp4_empty(cols, padded_rows, x.device)
+    status = _native.lib().fsh_mxfp4_quantize_segments(
+        x.data_ptr(), _float_dt(x.dtype), choices, cols, ldx, offsets.data_ptr(), padded_offsets.data_ptr(), experts,
+        _ptr(source), top_k, *(map(_ptr, row_form) if rows else (None, None)), *map(_ptr, column_form), padded_rows,
+        stream_ptr(x.device),
+    )
+    _native.check(status, "fsh_mxfp4_quantize_segments")
+    return row_form, column_form
+
+
+def _check_routing(*offsets: torch.Tensor) -> int:
+    """The number of experts of int32 offset tables."""
+    for t in offsets:
+        if t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or t.numel() != offsets[0].numel() or t.numel() < 2:
+            raise ValueError("offsets must be contiguous int32 [experts + 1]")
+    return offsets[0].numel() - 1
+
+
+def _mxfp4_operand(name: str, pair: tuple[torch.Tensor, torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    data, scales = pair
+    if data.dtype != torch.uint8 or data.ndim != 2 or not data.is_contiguous() or data.shape[1] % 128:
+        raise ValueError(f"{name}'s data must be contiguous uint8 [rows, a multiple of 128]")
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (data.shape[1] // 128, data.shape[0], 8):
+        raise ValueError(f"{name}'s scales must be contiguous uint8 {(data.shape[1] // 128, data.shape[0], 8)}, got {tuple(scales.shape)}")
+    return data, scales
+
+
+def mxfp4_dequantize(
+    data: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype, out: torch.Tensor | None = None
+) -> torch.Tensor:
+    """The values [rows, cols] that a quantized matrix stands for."""
+    _require_gpu(data, scales)
+    _mxfp4_operand("the matrix", (data, scales))
+    rows = data.shape[0]
+    if -(-cols // 256) * 128 != data.shape[1]:
+        raise ValueError(f"{cols} columns take {-(-cols // 256) * 128} bytes a row, got {data.shape[1]}")
+    if out is None:
+        out = torch.empty((rows, cols), dtype=dtype, device=data.device)
+    _require_gpu(data, out)
+    if out.dtype != dtype or tuple(out.shape) != (rows, cols):
+        raise ValueError(f"out must be {dtype} [{rows}, {cols}]")
+    status = _native.lib().fsh_mxfp4_dequantize(
+        data.data_ptr(), scales.data_ptr(), rows, cols, out.data_ptr(), _float_dt(dtype), _row_stride(out), stream_ptr(data.device)
+    )
+    _native.check(status, "fsh_mxfp4_dequantize")
+    return out
+
+
+def sum_runs(sums: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The column sums of an fp32 [runs, cols] table in ``dtype``."""
+    _require_gpu(sums)
+    if sums.dtype != torch.float32 or sums.ndim != 2 or not sums.is_contiguous():
+        raise ValueError("sums must be contiguous fp32 [runs, cols]")
+    out = torch.empty((sums.shape[1],), dtype=dtype, device=sums.device)
+    status = _native.lib().fsh_sum_runs(
+        sums.data_ptr(), sums.shape[0], sums.shape[1], out.data_ptr(), _float_dt(dtype), stream_ptr(sums.device)
+    )
+    _native.check(status, "fsh_sum_runs")
+    return out
+
+
+def mxfp4_gemm(
+    a: tuple[torch.Tensor, torch.Tensor], b: tuple[torch.Tensor, torch.Tensor], dtype: torch.dtype, *,
+    bias: torch.Tensor | None = None, mode: int = _native.MXFP4_DENSE, offsets: torch.Tensor | None = None,
+    source: torch.Tensor | None = None, top_k: int = 1, choices: int | None = None, out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``a @ b.T (+ bias)`` of quantized matrices (data, scales) over the same
+    padded columns, fp32 sums rounded once to ``dtype``.  ``mode``: the whole
+    product; ``MXFP4_ROWS``: the ``choices`` rows in segments of ``offsets``, expert
+    ``e``'s times b's rows [e n, (e + 1) n), row i of a or, with ``source``, row
+    ``source[i] // top_k``; ``MXFP4_OVER_ROWS``: [experts, m, n], per expert the
+    product over the columns between two offsets."""
+    present = [t for t in (bias, offsets, source, out) if t is not None]
+    (a_data, a_scales), (b_data, b_scales) = _mxfp4_operand("a", a), _mxfp4_operand("b", b)
+    _require_gpu(a_data, a_scales, b_data, b_scales, *present)
+    if a_data.shape[1] != b_data.shape[1]:
+        raise ValueError(f"inner dimensions differ: {a_data.shape[1] * 2} and {b_data.shape[1] * 2} padded columns")
+    m, n, experts = a_data.shape[0], b_data.shape[0], 0
+    if mode != _native.MXFP4_DENSE:
+        if offsets is None:
+            raise ValueError("segments need their offsets")
+        experts = _check_routing(offsets)
+    if mode == _native.MXFP4_ROWS:
+        if n % experts:
+            raise ValueError(f"{n} rows of b do not belong to {experts} experts")
+        n //= experts
+        m = m if choices is None else choices
+        if source is not None and (source.dtype != torch.int32 or source.numel() != m or not source.is_contiguous()):
+            raise ValueError(f"source must be contiguous int32 [{m}]")
+    shape = (experts, m, n) if mode == _native.MXFP4_OVER_ROWS else (m, n)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=a_data.device)
+    if out.dtype != dtype or tuple(out.shape) != shape or (mode == _native.MXFP4_OVER_ROWS and not out.is_contiguous()):
+        raise ValueError(f"out must be {dtype} {shape}")
+    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be {dtype} of {n} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
+    q = _native.MxFp4Product()
+    q.a_dev, q.a_scales_dev, q.b_dev, q.b_scales_dev = a_data.data_ptr(), a_scales.data_ptr(), b_data.data_ptr(), b_scales.data_ptr()
+    q.out_dev, q.bias_dev, q.offsets_dev, q.source_dev = out.data_ptr(), _ptr(bias), _ptr(offsets), _ptr(source)
+    q.m, q.n, q.k = m, n, a_data.shape[1] * 2
+    q.a_rows, q.b_rows = a_data.shape[0], b_data.shape[0]
+    q.ldo = n if mode == _native.MXFP4_OVER_ROWS else _row_stride(out)
+    q.out_dtype, q.mode, q.experts, q.top_k = _float_dt(dtype), mode, experts, top_k
+    status = _native.lib().fsh_mxfp4_gemm(ctypes.byref(q), stream_ptr(a_data.device))
+    _native.check(status, "fsh_mxfp4_gemm")
+    return out
+
+
+def expert_route(expert_ids: torch.Tensor, experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The stable order of a router's choices ``expert_ids`` (int64 or int32,
+    contiguous) by expert: ``(position, offsets, source, padded_offsets)``, int32.
+    An id outside [0, experts) is a choice of no expert here."""
+    _require_gpu(expert_ids)
+    if expert_ids.dtype not in (torch.int64, torch.int32) or not expert_ids.is_contiguous():
+        raise ValueError(f"expert_ids must be contiguous int64 or int32, got {expert_ids.dtype}")
+    choices, device = expert_ids.numel(), expert_ids.device
+    lib = _native.lib()
+    position = torch.empty(expert_ids.shape, dtype=torch.int32, device=device)
+    source = torch.empty((choices,), dtype=torch.int32, device=device)
+    offsets, padded_offsets = torch.empty((2, max(experts, 0) + 1), dtype=torch.int32, device=device).unbind()
+    nbytes = lib.fsh_expert_route_workspace_bytes(choices, experts)
+    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+    status = lib.fsh_expert_route(
+        expert_ids.data_ptr(), expert_ids.element_size(), choices, experts, position.data_ptr(), offsets.data_ptr(),
+        source.data_ptr(), padded_offsets.data_ptr(), _ptr(workspace), nbytes, stream_ptr(device),
+    )
+    _native.check(status, "fsh_expert_route")
+    return position, offsets, source, padded_offsets
+
+
+def _check_positions(position: torch.Tensor, tokens: int) -> int:
+    if position.dtype != torch.int32 or position.ndim != 2 or position.shape[0] != tokens or not position.is_contiguous():
+        raise ValueError(f"position must be contiguous int32 [{tokens}, top_k], got {position.dtype} {tuple(position.shape)}")
+    return position.shape[1]
+
+
+def _check_rows(name: str, rows: torch.Tensor, count: int, width: int, dtype: torch.dtype) -> None:
+    if rows.dtype != dtype or tuple(rows.shape) != (count, width) or not rows.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} [{count}, {width}], got {rows.dtype} {tuple(rows.shape)}")
+
+
+def expert_dispatch(x: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """``out[position[t, j]] = x[t]`` for contiguous rows; rows of no expert are zero."""
+    _require_gpu(x, position, offsets)
+    tokens, width = x.shape
+    top_k = _check_positions(position, tokens)
+    _check_rows("x", x, tokens, width, x.dtype)
+    out = torch.empty((tokens * top_k, width), dtype=x.dtype, device=x.device)
+    status = _native.lib().fsh_expert_dispatch(
+        x.data_ptr(), position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), tokens, top_k, width,
+        _float_dt(x.dtype), out.data_ptr(), stream_ptr(x.device),
+    )
+    _native.check(status, "fsh_expert_dispatch")
+    return out
+
+
+def expert_combine(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * rows[position[t, j]]`` (weights None: 1),
+    fp32 sums in the order of j, rounded once."""
+    _require_gpu(rows, position, *([] if weights is None else [weights]))
+    tokens, width = position.shape[0], rows.shape[1]
+    top_k = _check_positions(position, tokens)
+    _check_rows("rows", rows, tokens * top_k, width, rows.dtype)
+    if weights is not None:
+        _check_rows("weights", weights, tokens, top_k, weights.dtype)
+    out = torch.empty((tokens, width), dtype=rows.dtype, device=rows.device)
+    status = _native.lib().fsh_expert_combine(
+        rows.data_ptr(), position.data_ptr(), _ptr(weights), DT_F32 if weights is None else _float_dt(weights.dtype), tokens, top_k,
+        width, _float_dt(rows.dtype), out.data_ptr(), stream_ptr(rows.device),
+    )
+    _native.check(status, "fsh_expert_combine")
+    return out
+
+
+def expert_combine_backward(
+    grad: torch.Tensor, rows: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor, weights: torch.Tensor
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of :func:`expert_combine` for ``rows`` and ``weights``."""
+    _require_gpu(grad, rows, position, offsets, weights)
+    tokens, width = position.shape[0], rows.shape[1]
+    top_k = _check_positions(position, tokens)
+    _check_rows("grad", grad, tokens, width, rows.dtype)
+    _check_rows("rows", rows, tokens * top_k, width, rows.dtype)
+    _check_rows("weights", weights, tokens, top_k, weights.dtype)
+    grad_rows, grad_weights = torch.empty_like(rows), torch.empty_like(weights)
+    if width == 0:
+        return grad_rows, grad_weights.zero_()
+    status = _native.lib().fsh_expert_combine_backward(
+        grad.data_ptr(), rows.data_ptr(), position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), weights.data_ptr(),
+        _float_dt(weights.dtype), tokens, top_k, width, _float_dt(rows.dtype), grad_rows.data_ptr(), grad_weights.data_ptr(),
+        stream_ptr(rows.device),
+    )
+    _native.check(status, "fsh_expert_combine_backward")
+    return grad_rows, grad_weights

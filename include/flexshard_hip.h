@@ -517,6 +517,115 @@ int fsh_muon_step(const fsh_muon_group* groups, int32_t count, float lerp_weight
                   float nesterov_weight /* mu */, int32_t nesterov, float decay_factor /* 1 - lr*wd */, float a,
                   float b, float c, int32_t steps, float eps, void* stream);
 
+/* ------------------------------------------------------------------------
+ * 11. Microscaled 4-bit floats.  An E2M1 element has the magnitudes 0, 0.5, 1,
+ * 1.5, 2, 3, 4 and 6; 32 consecutive ones share an E8M0 byte, the power of two
+ * 2^(byte - 127).  A run's byte is the exponent of its largest magnitude less 2
+ * (not below 0; 255, not a number, for a run with an infinity or a NaN); an
+ * element is its value over the scale, to nearest, ties to the even code, at
+ * most 6.  The reference has no 4-bit format; the layer is its blockwise FP8
+ * linear (blockwise_fp8/fp8_blockwise_linear.py) in that format.
+ *
+ * A quantized matrix [rows, cols]: data [rows][P / 2] bytes, P = cols rounded
+ * up to 256, the lower column in the low half, the pad zero; scales
+ * [P / 256][rows][8] bytes.  dtype: FSH_DT_* of x, of an output or of a bias.
+ *
+ * fsh_mxfp4_quantize: `batch` matrices [rows, cols] of row stride ldx behind
+ * one another (contiguous if batch > 1 and columns are asked for).  q_rows /
+ * s_rows: the matrix [batch * rows, cols], runs along the rows.  q_cols /
+ * s_cols: the transposes, a matrix [batch * cols, rows] with runs along the
+ * columns of x.  Either pair may be null; both come from one read of x.
+ * column_sums: [ceil(rows / 128)][cols] sums over 128 rows each, or null (with
+ * q_cols, batch 1); fsh_sum_runs adds them up.
+ *
+ * fsh_mxfp4_quantize_segments: rows sorted by expert (section 13).  The column
+ * form is [cols, padded_rows], segment e from column padded_offsets[e] on and
+ * padded with zeros to padded_offsets[e + 1]; columns behind the last segment
+ * are not written.  With source, sorted row r is row source[r] / top_k of x
+ * (then without the row form); the row form is [rows, cols] as above, for rows
+ * that belong to a segment.
+ *
+ * fsh_mxfp4_dequantize: the values, in dtype, at out [rows, cols] of stride ldo.
+ * ---------------------------------------------------------------------- */
+int fsh_mxfp4_quantize(const void* x_dev, int32_t dtype, int64_t batch, int64_t rows, int64_t cols, int64_t ldx,
+                       void* q_rows_dev, void* s_rows_dev, void* q_cols_dev, void* s_cols_dev,
+                       float* column_sums_dev, void* stream);
+int fsh_mxfp4_quantize_segments(const void* x_dev, int32_t dtype, int64_t rows, int64_t cols, int64_t ldx,
+                                const int32_t* offsets_dev, const int32_t* padded_offsets_dev, int32_t experts,
+                                const int32_t* source_dev, int32_t top_k, void* q_rows_dev, void* s_rows_dev,
+                                void* q_cols_dev, void* s_cols_dev, int64_t padded_rows, void* stream);
+int fsh_mxfp4_dequantize(const void* q_dev, const void* s_dev, int64_t rows, int64_t cols, void* out_dev, int32_t dtype,
+                         int64_t ldo, void* stream);
+int fsh_sum_runs(const float* sums_dev, int64_t runs, int64_t cols, void* out_dev, int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 12. Products of quantized matrices: out = a . b^T (+ bias), fp32 sums, one
+ * rounding to out_dtype.  Both operands are quantized along the contraction, of
+ * k columns (padded: a multiple of 256).
+ *   FSH_MXFP4_DENSE      a [a_rows >= m, k], b [b_rows >= n, k], out [m, n] of
+ *                        stride ldo; bias [n] of out_dtype or null, added before
+ *                        the rounding
+ *   FSH_MXFP4_ROWS       rows [offsets[e], offsets[e + 1]) of a's m rows times
+ *                        b's rows [e n, (e + 1) n); out rows behind the last
+ *                        segment are zero.  With source, row r is row
+ *                        source[r] / top_k of a
+ *   FSH_MXFP4_OVER_ROWS  out [experts, m, n]: per expert the product over the
+ *                        columns [offsets[e], offsets[e + 1]) alone (multiples
+ *                        of 256: section 13's padded offsets); zero where empty
+ * ---------------------------------------------------------------------- */
+#define FSH_MXFP4_DENSE 0
+#define FSH_MXFP4_ROWS 1
+#define FSH_MXFP4_OVER_ROWS 2
+typedef struct fsh_mxfp4_product {
+  const void* a_dev;
+  const void* a_scales_dev;
+  const void* b_dev;
+  const void* b_scales_dev;
+  void* out_dev;
+  const void* bias_dev;
+  const int32_t* offsets_dev; /* [experts + 1] */
+  const int32_t* source_dev;
+  int64_t m, n, k;
+  int64_t a_rows, b_rows, ldo;
+  int32_t out_dtype, mode, experts, top_k;
+} fsh_mxfp4_product;
+int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 13. Tokens sorted by expert and back.  expert_ids [tokens, top_k] (int64 or
+ * int32): the experts that a router chose for each token; an id outside
+ * [0, experts) is a choice of no expert here (of another rank, or none).
+ *
+ * fsh_expert_route: the choices in stable order by expert.  position [tokens *
+ * top_k]: the sorted row of each choice, -1 for none.  offsets [experts + 1]:
+ * expert e has rows [offsets[e], offsets[e + 1]).  source [tokens * top_k]: the
+ * choice t * top_k + j of each sorted row, -1 behind offsets[experts].
+ * padded_offsets [experts + 1]: the same segments, each rounded up to 256 rows.
+ * workspace: at least fsh_expert_route_workspace_bytes(...) bytes.
+ *
+ * fsh_expert_dispatch: out[position[t, j]] = x[t]; rows behind offsets[experts]
+ * are zero.  fsh_expert_combine: out[t] = sum over j, in that order, of
+ * weights[t, j] * rows[position[t, j]] in fp32, rounded once (weights null: 1),
+ * choices of no expert left out; it is also the gradient of the dispatch.
+ * fsh_expert_combine_backward: grad_rows[position[t, j]] = weights[t, j] *
+ * grad[t], zero behind offsets[experts]; grad_weights[t, j] = <grad[t],
+ * rows[position[t, j]]>, zero for no expert.  Rows of `width` elements,
+ * contiguous; x, rows and their gradients of one dtype, weights of its own.
+ * ---------------------------------------------------------------------- */
+#define FSH_MAX_EXPERTS 1024
+int64_t fsh_expert_route_workspace_bytes(int64_t choices, int32_t experts);
+int fsh_expert_route(const void* expert_ids_dev, int32_t id_bytes, int64_t choices, int32_t experts, int32_t* position_dev,
+                     int32_t* offsets_dev, int32_t* source_dev, int32_t* padded_offsets_dev, void* workspace_dev,
+                     int64_t workspace_nbytes, void* stream);
+int fsh_expert_dispatch(const void* x_dev, const int32_t* position_dev, const int32_t* offsets_dev, int32_t experts,
+                        int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream);
+int fsh_expert_combine(const void* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
+                       int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream);
+int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, const int32_t* position_dev,
+                                const int32_t* offsets_dev, int32_t experts, const void* weights_dev, int32_t weights_dtype,
+                                int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* grad_rows_dev,
+                                void* grad_weights_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
