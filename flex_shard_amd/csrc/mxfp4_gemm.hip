@@ -17,7 +17,12 @@ int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t
   s.tiles_per_matrix = static_cast<int32_t>(tiles);
   s.work_items = tiles * batch;
   s.items_per_xcd = ceil_div(s.work_items, static_cast<int64_t>(kXcds));
-  const dim3 grid(static_cast<uint32_t>(s.items_per_xcd * kXcds)), block(Cfg::kThreads);
+  int64_t blocks = s.items_per_xcd * kXcds;
+  if (Cfg::kResident) {
+    const int64_t units = compute_units(), resident = units >= kXcds ? units / kXcds * kXcds : kXcds;
+    blocks = blocks < resident ? blocks : resident;
+  }
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(Cfg::kThreads);
   int rc = FSH_OK;
   by_dtype(p.out_dtype, [&](auto dt) {
     static LdsReservation reserved;
@@ -33,8 +38,8 @@ int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t
 template <typename Cfg>
 int64_t segment_tiles(const MxGemmParams& p) { return p.m / Cfg::BM + p.experts + 1; }
 
-using MxLarge = MxTile<4, 2, 4, 8, 2>;
-using MxSmall = MxTile<2, 2, 2, 2, 3>;
+using MxLarge = MxTile<2, 2, 4, 4, 2, 5, true>;
+using MxSmall = MxTile<2, 2, 1, 1, 4, 0, false>;
 
 template <typename Cfg>
 int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
