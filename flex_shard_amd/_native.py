@@ -146,6 +146,7 @@ class MxFp4Product(Structure):
 
 
 MXFP4_DENSE, MXFP4_ROWS, MXFP4_OVER_ROWS = 0, 1, 2
+MXFP4_FEW_ROWS = 4
 MAX_EXPERTS = 1024
 MAX_NS_PROBLEMS = 16
 MUON_PADDED = 1
@@ -257,6 +258,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "fsh_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_void_p]),
     "fsh_sum_runs": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
     "fsh_mxfp4_gemm": (c_int, [POINTER(MxFp4Product), c_void_p]),
+    "fsh_mxfp4_matrix_bytes": (c_int64, [c_int64, c_int64]),
+    "fsh_mxfp4_linear": (
+        c_int, [c_void_p, c_int32, c_int64, c_int64, POINTER(MxFp4Product), c_int64, c_void_p, c_int64, c_void_p],
+    ),
     "fsh_expert_route_workspace_bytes": (c_int64, [c_int64, c_int32]),
     "fsh_expert_route": (
         c_int, [c_void_p, c_int32, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],

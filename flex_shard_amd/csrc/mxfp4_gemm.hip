@@ -2,7 +2,7 @@
 // gradient and its weight gradient are all a b^T of operands quantized along the
 // contraction; the experts' layers are the same with rows (or the contraction)
 // in segments.
-#include "mxfp4_tiles.hpp"
+#include "mxfp4_few.hpp"
 
 namespace fsh {
 namespace {
@@ -49,6 +49,51 @@ int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
   return launch_mx_tiles<Cfg, kMxDense>(p, tiles_m, 1, stream);
 }
 
+// Few rows: which kernel, and how many waves share a workgroup's contraction.
+constexpr int64_t kFewMaxRows = 64;
+int few_waves(int64_t workgroups, int64_t steps) {
+  int waves = 4;
+  while (waves < 16 && workgroups * waves < 2048 && 2 * waves <= steps) waves *= 2;
+  return static_cast<int>(waves < steps ? waves : steps);
+}
+int few_lds_bytes(const MxFewParams& p, int token_blocks, bool quantize) {
+  return p.waves * token_blocks * 16 * 17 * 4 + (quantize ? kFewQuantize * (static_cast<int>(p.ld) + 16 + 8 * p.steps) : 0);
+}
+
+// kDense: p.m rows at most kFewMaxRows; kExperts: any rows, 16 of an expert at a time.
+template <bool kExperts, bool kQuantize>
+int launch_few(MxFewParams& p, int32_t dtype, hipStream_t stream) {
+  const int64_t tiles_n = ceil_div(p.n, static_cast<int64_t>(kFewRows)), blocks = tiles_n * (kExperts ? p.experts + 1 : 1);
+  if (blocks > 0x3FFFFFLL) return fail(FSH_ENOTSUP, "fsh_mxfp4_gemm: too many tiles");
+  p.tiles_n = static_cast<int32_t>(tiles_n);
+  p.waves = few_waves(blocks, p.steps);
+  const dim3 grid(static_cast<uint32_t>(blocks)), block(64 * p.waves);
+  const int token_blocks = kExperts || p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+  const int lds = few_lds_bytes(p, token_blocks, kQuantize);
+  by_dtype(dtype, [&](auto dt) {
+    if (token_blocks == 1) hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 1, kExperts, kQuantize>), grid, block, lds, stream, p);
+    else if constexpr (!kExperts && !kQuantize) {
+      if (token_blocks == 2) hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 2, false, false>), grid, block, lds, stream, p);
+      else hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 4, false, false>), grid, block, lds, stream, p);
+    }
+  });
+  return check_launch("mxfp4_few_rows_kernel");
+}
+
+MxFewParams few_params(const fsh_mxfp4_product& q) {
+  MxFewParams p;
+  memset(&p, 0, sizeof(p));
+  p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
+  p.b = static_cast<const uint8_t*>(q.b_dev); p.bs = static_cast<const uint8_t*>(q.b_scales_dev);
+  p.out = q.out_dev; p.bias = q.bias_dev;
+  p.m = q.m; p.n = q.n; p.a_rows = q.a_rows; p.b_rows = q.b_rows;
+  p.ld = q.k / 2; p.ldo = q.ldo;
+  p.steps = static_cast<int32_t>(q.k / kMxColumns);
+  p.experts = q.experts; p.top_k = q.top_k;
+  p.offsets = q.offsets_dev; p.source = q.source_dev;
+  return p;
+}
+
 }  // namespace
 }  // namespace fsh
 
@@ -84,6 +129,15 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   // The lanes' offsets are 32 bits from a tile's first row, or from the matrix for gathered rows.
   if (256 * (q.k / 2) >= (1LL << 32) || (q.source_dev && q.a_rows * (q.k / 2) >= (1LL << 32)))
     return fail(FSH_ENOTSUP, "%s: rows that are gathered, or a tile of them, span 4 GiB or more", who);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (q.mode == FSH_MXFP4_DENSE && q.m <= kFewMaxRows) {
+    MxFewParams few = few_params(q);
+    return launch_few<false, false>(few, q.out_dtype, on);
+  }
+  if (segments && q.m <= 16 * static_cast<int64_t>(q.experts)) {
+    MxFewParams few = few_params(q);
+    return launch_few<true, false>(few, q.out_dtype, on);
+  }
   MxGemmParams p;
   memset(&p, 0, sizeof(p));
   p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
@@ -97,9 +151,54 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   p.experts = q.experts; p.top_k = q.top_k;
   p.offsets = p.padded_offsets = q.offsets_dev;
   p.source = q.source_dev;
-  const hipStream_t on = static_cast<hipStream_t>(stream);
   const MxProblem problem = segments ? kMxRows : q.mode == FSH_MXFP4_OVER_ROWS ? kMxOverRows : kMxDense;
   const int64_t rows = segments ? q.m / q.experts : q.m;
   if (rows * q.n >= 128 * 128 * 64) return launch_mx<MxLarge>(p, problem, on);
   return launch_mx<MxSmall>(p, problem, on);
+}
+
+FSH_API int64_t fsh_mxfp4_matrix_bytes(int64_t rows, int64_t cols) {
+  using namespace fsh;
+  if (rows <= 0 || cols <= 0) return 0;
+  return rows * ceil_div(cols, (int64_t)kMxColumns) * (kMxColumns / 2 + 8);
+}
+
+FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int64_t ldx, const fsh_mxfp4_product* product,
+                             int64_t in_dim, void* scratch_dev, int64_t scratch_nbytes, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_mxfp4_linear";
+  if (!product) return fail(FSH_EINVAL, "%s: null product", who);
+  if (rows < 0 || in_dim < 0) return fail(FSH_EINVAL, "%s: negative shape", who);
+  fsh_mxfp4_product q = *product;
+  if (q.k != ceil_div(in_dim, (int64_t)kMxColumns) * kMxColumns)
+    return fail(FSH_EINVAL, "%s: k %lld is not in_dim %lld rounded up to %d", who, (long long)q.k, (long long)in_dim, kMxColumns);
+  if (q.out_dtype != dtype) return fail(FSH_EINVAL, "%s: the output has the activation's dtype", who);
+  if (q.m == 0 || q.n == 0 || rows == 0) return FSH_OK;
+  q.a_rows = rows;
+  if (q.mode == FSH_MXFP4_DENSE && q.m <= kFewQuantize) {
+    MxFewParams p = few_params(q);
+    p.waves = 16;
+    if (few_lds_bytes(p, 1, true) <= 64 * 1024) {
+      if (!known_dtype(dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, dtype);
+      if (rows < q.m || ldx < in_dim || q.ldo < q.n || q.b_rows < q.n)
+        return fail(FSH_EINVAL, "%s: rows or leading dimensions too small", who);
+      if (!x_dev || !q.b_dev || !q.b_scales_dev || !q.out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+      const int bytes = dtype_bytes(dtype);
+      if (!aligned(x_dev, bytes) || !aligned(q.b_dev, 16) || !aligned(q.b_scales_dev, 8) || !aligned(q.out_dev, bytes) || !aligned(q.bias_dev, bytes))
+        return fail(FSH_ENOTSUP, "%s: weights must be 16-byte and scales 8-byte aligned, x, out and bias to their elements", who);
+      p.a = static_cast<const uint8_t*>(x_dev);
+      p.cols = in_dim; p.ldx = ldx;
+      p.vec = aligned(x_dev, 16) && ldx * bytes % 16 == 0;
+      return launch_few<false, true>(p, dtype, static_cast<hipStream_t>(stream));
+    }
+  }
+  const int64_t need = fsh_mxfp4_matrix_bytes(rows, in_dim);
+  if (!scratch_dev || scratch_nbytes < need)
+    return fail(FSH_EINVAL, "%s: scratch of %lld bytes, needs %lld", who, (long long)scratch_nbytes, (long long)need);
+  uint8_t* data = static_cast<uint8_t*>(scratch_dev);
+  uint8_t* scales = data + rows * (q.k / 2);
+  if (int rc = fsh_mxfp4_quantize(x_dev, dtype, 1, rows, in_dim, ldx, data, scales, nullptr, nullptr, nullptr, stream)) return rc;
+  q.a_dev = data;
+  q.a_scales_dev = scales;
+  return fsh_mxfp4_gemm(&q, stream);
 }

@@ -34,11 +34,12 @@ from ._native import (
 __all__ = [
     "DT_BF16", "DT_F16", "DT_F32", "EPS_FP32", "EPS_INPUT_DTYPE", "REDUCE_POSTDIV", "REDUCE_POSTMUL",
     "REDUCE_PREMUL", "REDUCE_SUM", "SRC_BF16", "SRC_F16", "SRC_F32", "SRC_F32_AS_BF16", "SRC_F32_AS_F16",
-    "MuonStepPlan", "QuantChunkSpec", "QuantPackPlan", "accumulate_grad", "act_quant_128x1_transposed", "act_quant_1x128", "act_quant_both",
+    "MuonStepPlan", "MxFp4Matrix", "QuantChunkSpec", "QuantPackPlan", "accumulate_grad", "act_quant_128x1_transposed", "act_quant_1x128", "act_quant_both",
     "copy_row_segments", "copy_segments", "fp8_gemm_1x128_128x1", "fp8_gemm_1x128_128x128", "fp8_gemm_1x128_128x128_dgrad",
-    "expert_combine", "expert_combine_backward", "expert_dispatch", "expert_route",
+    "expert_combine", "expert_combine_at", "expert_combine_backward", "expert_combine_backward_at", "expert_dispatch",
+    "expert_dispatch_at", "expert_route", "expert_route_buffer", "expert_route_into",
     "fp8_gemm_tiles", "fp8_linear_backward", "fp8_transpose", "gemm_nt", "gemm_nt_group", "gemm_tiles", "muon_apply",
-    "muon_prepare", "mxfp4_dequantize", "mxfp4_gemm", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
+    "muon_prepare", "mxfp4_dequantize", "mxfp4_expert_linear", "mxfp4_gemm", "mxfp4_linear", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
     "newton_schulz_product_tiles",
     "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
 ]
@@ -1015,39 +1016,98 @@ class MuonStepPlan:
         _native.check(status, "fsh_muon_step")
 
 
+_FLOAT_DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
+
+
 def _float_dt(dtype: torch.dtype) -> int:
-    return DT_F16 if dtype == torch.float16 else _dt(dtype)
+    code = _FLOAT_DT.get(dtype)
+    if code is None:
+        raise NotImplementedError(f"dtype {dtype} is not supported by the HIP kernels (bf16, fp16 and fp32 are)")
+    return code
 
 
-def _mxfp4_empty(rows: int, cols: int, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-    """Data and scales of a quantized matrix [rows, cols]."""
-    steps = -(-cols // 256)
-    return (
-        torch.empty((rows, steps * 128), dtype=torch.uint8, device=device),
-        torch.empty((steps, rows, 8), dtype=torch.uint8, device=device),
-    )
+class MxFp4Matrix:
+    """A matrix of microscaled 4-bit floats, in one buffer.  ``data`` is uint8
+    [rows, P / 2], P = ``cols`` rounded up to 256 (the lower column in a byte's low
+    half, the pad zero); ``scales`` uint8 [P / 256, rows, 8], the bytes of a row's
+    256 columns next to one another.  Unpacks into the two."""
+
+    __slots__ = ("buffer", "rows", "cols")
+
+    def __init__(self, buffer: torch.Tensor, rows: int, cols: int) -> None:
+        self.buffer = buffer
+        self.rows = rows
+        self.cols = cols
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, device: torch.device) -> "MxFp4Matrix":
+        return cls(torch.empty(rows * -(-cols // 256) * 136, dtype=torch.uint8, device=device), rows, cols)
+
+    @property
+    def steps(self) -> int:
+        return -(-self.cols // 256)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self.buffer[: self.rows * self.steps * 128].view(self.rows, self.steps * 128)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self.buffer[self.rows * self.steps * 128 :].view(self.steps, self.rows, 8)
+
+    @property
+    def pair(self) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.data, self.scales
+
+    def __iter__(self):
+        return iter(self.pair)
+
+    def __getitem__(self, index: int) -> torch.Tensor:
+        return self.pair[index]
+
+    def pointers(self) -> tuple[int, int]:
+        data = self.buffer.data_ptr()
+        return data, data + self.rows * -(-self.cols // 256) * 128
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values [rows, cols] in bf16, fp16 or fp32."""
+        buffer, rows, cols = self.buffer, self.rows, self.cols
+        out = torch.empty((rows, cols), dtype=dtype, device=buffer.device)
+        data, scales = self.pointers()
+        status = _native.lib().fsh_mxfp4_dequantize(
+            data, scales, rows, cols, out.data_ptr(), _float_dt(dtype), cols, stream_ptr(buffer.device)
+        )
+        if status:
+            _native.check(status, "fsh_mxfp4_dequantize")
+        return out
 
 
 def _row_stride(x: torch.Tensor) -> int:
     """The row stride of a matrix whose rows are contiguous and apart."""
-    if x.ndim != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        raise ValueError(f"expected a matrix with contiguous, separate rows, got {tuple(x.shape)} / {x.stride()}")
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if x.ndim == 2:
+        rows, cols = x.shape
+        along, across = x.stride()
+        if (cols <= 1 or across == 1) and (rows <= 1 or along >= cols):
+            return along if rows > 1 else cols
+    raise ValueError(f"expected a matrix with contiguous, separate rows, got {tuple(x.shape)} / {x.stride()}")
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_NO_FORM = (None, None)
+
+
 def mxfp4_quantize(
     x: torch.Tensor, *, rows: bool = True, columns: bool = False, column_sums: bool = False
-) -> tuple[tuple[torch.Tensor, torch.Tensor] | None, tuple[torch.Tensor, torch.Tensor] | None, torch.Tensor | None]:
+) -> tuple[MxFp4Matrix | None, MxFp4Matrix | None, torch.Tensor | None]:
     """Quantize a bf16, fp16 or fp32 matrix (or contiguous stack [b, r, c]) to
     microscaled 4-bit floats in one pass.  Returns ``(row form, column form,
-    sums)``: the row form is data and scales of [b * r, c], the column form those
-    of the transposes [b * c, r], None where not asked for; ``sums`` the fp32
-    column sums over 128 rows each, [ceil(r / 128), c] (a matrix with its column
-    form), which :func:`sum_runs` adds up."""
+    sums)``: the row form is the matrix [b * r, c], the column form that of the
+    transposes [b * c, r], None where not asked for; ``sums`` the fp32 column sums
+    over 128 rows each, [ceil(r / 128), c] (a matrix with its column form), which
+    :func:`sum_runs` adds up."""
     _require_gpu(x)
     if x.ndim == 3:
         if not x.is_contiguous():
@@ -1059,21 +1119,23 @@ def mxfp4_quantize(
         batch, (r, c) = 1, x.shape
     if not (rows or columns) or (column_sums and (not columns or x.ndim != 2)):
         raise ValueError("ask for rows or columns; column sums come with the column form of a matrix")
-    row_form = _mxfp4_empty(batch * r, c, x.device) if rows else None
-    column_form = _mxfp4_empty(batch * c, r, x.device) if columns else None
-    sums = torch.empty((-(-r // 128), c), dtype=torch.float32, device=x.device) if column_sums else None
+    device = x.device
+    row_form = MxFp4Matrix.empty(batch * r, c, device) if rows else None
+    column_form = MxFp4Matrix.empty(batch * c, r, device) if columns else None
+    sums = torch.empty((-(-r // 128), c), dtype=torch.float32, device=device) if column_sums else None
     status = _native.lib().fsh_mxfp4_quantize(
-        x.data_ptr(), _float_dt(x.dtype), batch, r, c, ldx, *(map(_ptr, row_form) if rows else (None, None)),
-        *(map(_ptr, column_form) if columns else (None, None)), _ptr(sums), stream_ptr(x.device),
+        x.data_ptr(), _float_dt(x.dtype), batch, r, c, ldx, *(row_form.pointers() if rows else _NO_FORM),
+        *(column_form.pointers() if columns else _NO_FORM), None if sums is None else sums.data_ptr(), stream_ptr(device),
     )
-    _native.check(status, "fsh_mxfp4_quantize")
+    if status:
+        _native.check(status, "fsh_mxfp4_quantize")
     return row_form, column_form, sums
 
 
 def mxfp4_quantize_segments(
     x: torch.Tensor, offsets: torch.Tensor, padded_offsets: torch.Tensor, padded_rows: int, *, choices: int,
     source: torch.Tensor | None = None, top_k: int = 1, rows: bool = False,
-) -> tuple[tuple[torch.Tensor, torch.Tensor] | None, tuple[torch.Tensor, torch.Tensor]]:
+) -> tuple[MxFp4Matrix | None, MxFp4Matrix]:
     """The column form of rows sorted by expert, [cols, padded_rows]: segment
     ``e`` from column ``padded_offsets[e]`` on, padded with zeros.  ``x`` holds the
     ``choices`` sorted rows, or with ``source`` the rows ``source[i] // top_k`` of
@@ -1084,13 +1146,15 @@ def mxfp4_quantize_segments(
         raise ValueError(f"{choices} sorted rows expected, got {x.shape[0]}")
     if rows and source is not None:
         raise ValueError("the row form of gathered rows is that of x itself")
+    if source is not None and (source.dtype != torch.int32 or source.numel() != choices or not source.is_contiguous()):
+        raise ValueError(f"source must be contiguous int32 [{choices}]")
     experts = _check_routing(offsets, padded_offsets)
     cols = x.shape[1]
-    row_form = _mxfp4_empty(choices, cols, x.device) if rows else None
-    column_form = _mxfp4_empty(cols, padded_rows, x.device)
+    row_form = MxFp4Matrix.empty(choices, cols, x.device) if rows else None
+    column_form = MxFp4Matrix.empty(cols, padded_rows, x.device)
     status = _native.lib().fsh_mxfp4_quantize_segments(
         x.data_ptr(), _float_dt(x.dtype), choices, cols, ldx, offsets.data_ptr(), padded_offsets.data_ptr(), experts,
-        _ptr(source), top_k, *(map(_ptr, row_form) if rows else (None, None)), *map(_ptr, column_form), padded_rows,
+        _ptr(source), top_k, *(row_form.pointers() if rows else _NO_FORM), *column_form.pointers(), padded_rows,
         stream_ptr(x.device),
     )
     _native.check(status, "fsh_mxfp4_quantize_segments")
@@ -1105,24 +1169,19 @@ def _check_routing(*offsets: torch.Tensor) -> int:
     return offsets[0].numel() - 1
 
 
-def _mxfp4_operand(name: str, pair: tuple[torch.Tensor, torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
-    data, scales = pair
-    if data.dtype != torch.uint8 or data.ndim != 2 or not data.is_contiguous() or data.shape[1] % 128:
-        raise ValueError(f"{name}'s data must be contiguous uint8 [rows, a multiple of 128]")
-    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (data.shape[1] // 128, data.shape[0], 8):
-        raise ValueError(f"{name}'s scales must be contiguous uint8 {(data.shape[1] // 128, data.shape[0], 8)}, got {tuple(scales.shape)}")
-    return data, scales
-
-
 def mxfp4_dequantize(
     data: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype, out: torch.Tensor | None = None
 ) -> torch.Tensor:
-    """The values [rows, cols] that a quantized matrix stands for."""
+    """The values [rows, cols] that a quantized matrix stands for, from its data
+    and scales (see :class:`MxFp4Matrix`)."""
     _require_gpu(data, scales)
-    _mxfp4_operand("the matrix", (data, scales))
+    if data.dtype != torch.uint8 or data.ndim != 2 or not data.is_contiguous():
+        raise ValueError("data must be contiguous uint8 [rows, bytes]")
     rows = data.shape[0]
     if -(-cols // 256) * 128 != data.shape[1]:
         raise ValueError(f"{cols} columns take {-(-cols // 256) * 128} bytes a row, got {data.shape[1]}")
+    if scales.dtype != torch.uint8 or not scales.is_contiguous() or tuple(scales.shape) != (-(-cols // 256), rows, 8):
+        raise ValueError(f"scales must be contiguous uint8 {(-(-cols // 256), rows, 8)}, got {tuple(scales.shape)}")
     if out is None:
         out = torch.empty((rows, cols), dtype=dtype, device=data.device)
     _require_gpu(data, out)
@@ -1148,23 +1207,39 @@ def sum_runs(sums: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
+def _mxfp4_product(
+    b: MxFp4Matrix, out: torch.Tensor, dtype: int, mode: int, m: int, n: int, bias: torch.Tensor | None, experts: int, top_k: int,
+    offsets_ptr: int | None, source_ptr: int | None,
+) -> "_native.MxFp4Product":
+    q = _native.MxFp4Product()
+    q.b_dev, q.b_scales_dev = b.pointers()
+    q.out_dev = out.data_ptr()
+    if bias is not None:
+        q.bias_dev = bias.data_ptr()
+    q.m, q.n, q.k = m, n, -(-b.cols // 256) * 256
+    q.b_rows = b.rows
+    q.ldo = out.stride(-2) if m > 1 else n
+    q.out_dtype = dtype
+    if mode != _native.MXFP4_DENSE:
+        q.mode, q.experts, q.top_k, q.offsets_dev, q.source_dev = mode, experts, top_k, offsets_ptr, source_ptr
+    return q
+
+
 def mxfp4_gemm(
-    a: tuple[torch.Tensor, torch.Tensor], b: tuple[torch.Tensor, torch.Tensor], dtype: torch.dtype, *,
-    bias: torch.Tensor | None = None, mode: int = _native.MXFP4_DENSE, offsets: torch.Tensor | None = None,
-    source: torch.Tensor | None = None, top_k: int = 1, choices: int | None = None, out: torch.Tensor | None = None,
+    a: MxFp4Matrix, b: MxFp4Matrix, dtype: torch.dtype, *, bias: torch.Tensor | None = None, mode: int = _native.MXFP4_DENSE,
+    offsets: torch.Tensor | None = None, source: torch.Tensor | None = None, top_k: int = 1, choices: int | None = None,
+    out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """``a @ b.T (+ bias)`` of quantized matrices (data, scales) over the same
-    padded columns, fp32 sums rounded once to ``dtype``.  ``mode``: the whole
-    product; ``MXFP4_ROWS``: the ``choices`` rows in segments of ``offsets``, expert
-    ``e``'s times b's rows [e n, (e + 1) n), row i of a or, with ``source``, row
-    ``source[i] // top_k``; ``MXFP4_OVER_ROWS``: [experts, m, n], per expert the
-    product over the columns between two offsets."""
-    present = [t for t in (bias, offsets, source, out) if t is not None]
-    (a_data, a_scales), (b_data, b_scales) = _mxfp4_operand("a", a), _mxfp4_operand("b", b)
-    _require_gpu(a_data, a_scales, b_data, b_scales, *present)
-    if a_data.shape[1] != b_data.shape[1]:
-        raise ValueError(f"inner dimensions differ: {a_data.shape[1] * 2} and {b_data.shape[1] * 2} padded columns")
-    m, n, experts = a_data.shape[0], b_data.shape[0], 0
+    """``a @ b.T (+ bias)`` of quantized matrices over the same padded columns, fp32
+    sums rounded once to ``dtype``.  ``mode``: the whole product; ``MXFP4_ROWS``: the
+    ``choices`` rows in segments of ``offsets``, expert ``e``'s times b's rows
+    [e n, (e + 1) n), row i of a or, with ``source``, row ``source[i] // top_k``;
+    ``MXFP4_OVER_ROWS``: [experts, m, n], per expert the product over the columns
+    between two offsets."""
+    _require_gpu(a.buffer, b.buffer, *[t for t in (bias, offsets, source, out) if t is not None])
+    if a.steps != b.steps:
+        raise ValueError(f"inner dimensions differ: {a.steps * 256} and {b.steps * 256} padded columns")
+    m, n, experts = a.rows, b.rows, 0
     if mode != _native.MXFP4_DENSE:
         if offsets is None:
             raise ValueError("segments need their offsets")
@@ -1178,43 +1253,110 @@ def mxfp4_gemm(
             raise ValueError(f"source must be contiguous int32 [{m}]")
     shape = (experts, m, n) if mode == _native.MXFP4_OVER_ROWS else (m, n)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=a_data.device)
-    if out.dtype != dtype or tuple(out.shape) != shape or (mode == _native.MXFP4_OVER_ROWS and not out.is_contiguous()):
+        out = torch.empty(shape, dtype=dtype, device=a.buffer.device)
+    elif out.dtype != dtype or tuple(out.shape) != shape or (mode == _native.MXFP4_OVER_ROWS and not out.is_contiguous()):
         raise ValueError(f"out must be {dtype} {shape}")
+    elif mode != _native.MXFP4_OVER_ROWS:
+        _row_stride(out)
     if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be {dtype} of {n} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
-    q = _native.MxFp4Product()
-    q.a_dev, q.a_scales_dev, q.b_dev, q.b_scales_dev = a_data.data_ptr(), a_scales.data_ptr(), b_data.data_ptr(), b_scales.data_ptr()
-    q.out_dev, q.bias_dev, q.offsets_dev, q.source_dev = out.data_ptr(), _ptr(bias), _ptr(offsets), _ptr(source)
-    q.m, q.n, q.k = m, n, a_data.shape[1] * 2
-    q.a_rows, q.b_rows = a_data.shape[0], b_data.shape[0]
-    q.ldo = n if mode == _native.MXFP4_OVER_ROWS else _row_stride(out)
-    q.out_dtype, q.mode, q.experts, q.top_k = _float_dt(dtype), mode, experts, top_k
-    status = _native.lib().fsh_mxfp4_gemm(ctypes.byref(q), stream_ptr(a_data.device))
-    _native.check(status, "fsh_mxfp4_gemm")
+    q = _mxfp4_product(b, out, _float_dt(dtype), mode, m, n, bias, experts, top_k, _ptr(offsets), _ptr(source))
+    q.a_dev, q.a_scales_dev = a.pointers()
+    q.a_rows = a.rows
+    status = _native.lib().fsh_mxfp4_gemm(ctypes.byref(q), stream_ptr(out.device))
+    if status:
+        _native.check(status, "fsh_mxfp4_gemm")
     return out
+
+
+def mxfp4_linear(x: torch.Tensor, weight: MxFp4Matrix, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`mxfp4_quantize` of ``x`` [rows, in] and :func:`mxfp4_gemm` in one
+    call; of a few rows in one launch."""
+    ldx = _row_stride(x)
+    rows, cols = x.shape
+    device = x.device
+    if cols != weight.cols:
+        raise ValueError(f"x {tuple(x.shape)} does not match a weight of {weight.cols} columns")
+    if bias is None:
+        _require_gpu(x, weight.buffer)
+    else:
+        _require_gpu(x, weight.buffer, bias)
+        if bias.dtype != x.dtype or bias.numel() != weight.rows or not bias.is_contiguous():
+            raise ValueError(f"bias must be {x.dtype} of {weight.rows} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
+    out = torch.empty((rows, weight.rows), dtype=x.dtype, device=device)
+    return _mxfp4_linear(x, ldx, weight, out, bias, _native.MXFP4_DENSE, rows, weight.rows, 0, 1, None, None)
+
+
+def mxfp4_expert_linear(
+    x: torch.Tensor, weight: MxFp4Matrix, experts: int, choices: int, top_k: int, offsets_ptr: int, source_ptr: int | None
+) -> torch.Tensor:
+    """The same for the experts' rows (``MXFP4_ROWS``); the routing's tables by address."""
+    _require_gpu(x, weight.buffer)
+    n = weight.rows // experts
+    out = torch.empty((choices, n), dtype=x.dtype, device=x.device)
+    return _mxfp4_linear(x, _row_stride(x), weight, out, None, _native.MXFP4_ROWS, choices, n, experts, top_k, offsets_ptr, source_ptr)
+
+
+def _mxfp4_linear(
+    x: torch.Tensor, ldx: int, weight: MxFp4Matrix, out: torch.Tensor, bias: torch.Tensor | None, mode: int, m: int, n: int,
+    experts: int, top_k: int, offsets_ptr: int | None, source_ptr: int | None,
+) -> torch.Tensor:
+    rows, cols = x.shape
+    dtype = _float_dt(x.dtype)
+    device = out.device
+    q = _mxfp4_product(weight, out, dtype, mode, m, n, bias, experts, top_k, offsets_ptr, source_ptr)
+    scratch, nbytes = None, 0
+    if mode != _native.MXFP4_DENSE or rows > _native.MXFP4_FEW_ROWS or cols > 16384:
+        nbytes = rows * -(-cols // 256) * 136
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    status = _native.lib().fsh_mxfp4_linear(
+        x.data_ptr(), dtype, rows, ldx, ctypes.byref(q), cols, None if scratch is None else scratch.data_ptr(), nbytes,
+        stream_ptr(device),
+    )
+    if status:
+        _native.check(status, "fsh_mxfp4_linear")
+    return out
+
+
+def expert_route_into(buffer: torch.Tensor, expert_ids: torch.Tensor, experts: int) -> None:
+    """Sort the choices ``expert_ids`` (contiguous int64 or int32) by expert into an
+    int32 ``buffer``: position, source [choices] each, offsets, padded offsets
+    [experts + 1] each, behind one another."""
+    choices = expert_ids.numel()
+    device = buffer.device
+    lib = _native.lib()
+    workspace, nbytes = None, lib.fsh_expert_route_workspace_bytes(choices, experts)
+    if nbytes:
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    position = buffer.data_ptr()
+    source = position + 4 * choices
+    offsets = source + 4 * choices
+    status = lib.fsh_expert_route(
+        expert_ids.data_ptr(), expert_ids.element_size(), choices, experts, position, offsets, source,
+        offsets + 4 * (experts + 1), None if workspace is None else workspace.data_ptr(), nbytes, stream_ptr(device),
+    )
+    if status:
+        _native.check(status, "fsh_expert_route")
 
 
 def expert_route(expert_ids: torch.Tensor, experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The stable order of a router's choices ``expert_ids`` (int64 or int32,
     contiguous) by expert: ``(position, offsets, source, padded_offsets)``, int32.
     An id outside [0, experts) is a choice of no expert here."""
+    buffer = expert_route_buffer(expert_ids, experts)
+    choices = expert_ids.numel()
+    offsets, padded_offsets = buffer[2 * choices :].view(2, experts + 1).unbind()
+    return buffer[:choices].view(expert_ids.shape), offsets, buffer[choices : 2 * choices], padded_offsets
+
+
+def expert_route_buffer(expert_ids: torch.Tensor, experts: int) -> torch.Tensor:
+    """:func:`expert_route`'s tables behind one another (see :func:`expert_route_into`)."""
     _require_gpu(expert_ids)
     if expert_ids.dtype not in (torch.int64, torch.int32) or not expert_ids.is_contiguous():
         raise ValueError(f"expert_ids must be contiguous int64 or int32, got {expert_ids.dtype}")
-    choices, device = expert_ids.numel(), expert_ids.device
-    lib = _native.lib()
-    position = torch.empty(expert_ids.shape, dtype=torch.int32, device=device)
-    source = torch.empty((choices,), dtype=torch.int32, device=device)
-    offsets, padded_offsets = torch.empty((2, max(experts, 0) + 1), dtype=torch.int32, device=device).unbind()
-    nbytes = lib.fsh_expert_route_workspace_bytes(choices, experts)
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
-    status = lib.fsh_expert_route(
-        expert_ids.data_ptr(), expert_ids.element_size(), choices, experts, position.data_ptr(), offsets.data_ptr(),
-        source.data_ptr(), padded_offsets.data_ptr(), _ptr(workspace), nbytes, stream_ptr(device),
-    )
-    _native.check(status, "fsh_expert_route")
-    return position, offsets, source, padded_offsets
+    buffer = torch.empty(2 * (expert_ids.numel() + max(experts, 0) + 1), dtype=torch.int32, device=expert_ids.device)
+    expert_route_into(buffer, expert_ids, experts)
+    return buffer
 
 
 def _check_positions(position: torch.Tensor, tokens: int) -> int:
@@ -1234,12 +1376,19 @@ def expert_dispatch(x: torch.Tensor, position: torch.Tensor, offsets: torch.Tens
     tokens, width = x.shape
     top_k = _check_positions(position, tokens)
     _check_rows("x", x, tokens, width, x.dtype)
-    out = torch.empty((tokens * top_k, width), dtype=x.dtype, device=x.device)
+    return expert_dispatch_at(x, position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), top_k)
+
+
+def expert_dispatch_at(x: torch.Tensor, position_ptr: int, offsets_ptr: int, experts: int, top_k: int) -> torch.Tensor:
+    """:func:`expert_dispatch` of contiguous ``x``; the routing's tables by address."""
+    tokens, width = x.shape
+    device = x.device
+    out = torch.empty((tokens * top_k, width), dtype=x.dtype, device=device)
     status = _native.lib().fsh_expert_dispatch(
-        x.data_ptr(), position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), tokens, top_k, width,
-        _float_dt(x.dtype), out.data_ptr(), stream_ptr(x.device),
+        x.data_ptr(), position_ptr, offsets_ptr, experts, tokens, top_k, width, _float_dt(x.dtype), out.data_ptr(), stream_ptr(device)
     )
-    _native.check(status, "fsh_expert_dispatch")
+    if status:
+        _native.check(status, "fsh_expert_dispatch")
     return out
 
 
@@ -1252,12 +1401,22 @@ def expert_combine(rows: torch.Tensor, position: torch.Tensor, weights: torch.Te
     _check_rows("rows", rows, tokens * top_k, width, rows.dtype)
     if weights is not None:
         _check_rows("weights", weights, tokens, top_k, weights.dtype)
-    out = torch.empty((tokens, width), dtype=rows.dtype, device=rows.device)
+    return expert_combine_at(rows, position.data_ptr(), tokens, top_k, weights)
+
+
+def expert_combine_at(
+    rows: torch.Tensor, position_ptr: int, tokens: int, top_k: int, weights: torch.Tensor | None = None
+) -> torch.Tensor:
+    """:func:`expert_combine` of contiguous ``rows`` and weights; the routing's table by address."""
+    width, device = rows.shape[1], rows.device
+    out = torch.empty((tokens, width), dtype=rows.dtype, device=device)
     status = _native.lib().fsh_expert_combine(
-        rows.data_ptr(), position.data_ptr(), _ptr(weights), DT_F32 if weights is None else _float_dt(weights.dtype), tokens, top_k,
-        width, _float_dt(rows.dtype), out.data_ptr(), stream_ptr(rows.device),
+        rows.data_ptr(), position_ptr, None if weights is None else weights.data_ptr(),
+        DT_F32 if weights is None else _float_dt(weights.dtype), tokens, top_k, width, _float_dt(rows.dtype), out.data_ptr(),
+        stream_ptr(device),
     )
-    _native.check(status, "fsh_expert_combine")
+    if status:
+        _native.check(status, "fsh_expert_combine")
     return out
 
 
@@ -1271,13 +1430,21 @@ def expert_combine_backward(
     _check_rows("grad", grad, tokens, width, rows.dtype)
     _check_rows("rows", rows, tokens * top_k, width, rows.dtype)
     _check_rows("weights", weights, tokens, top_k, weights.dtype)
+    return expert_combine_backward_at(grad, rows, position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), weights)
+
+
+def expert_combine_backward_at(
+    grad: torch.Tensor, rows: torch.Tensor, position_ptr: int, offsets_ptr: int, experts: int, weights: torch.Tensor
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`expert_combine_backward` of contiguous tensors; the routing's tables by address."""
+    (tokens, top_k), width, device = weights.shape, rows.shape[1], rows.device
     grad_rows, grad_weights = torch.empty_like(rows), torch.empty_like(weights)
     if width == 0:
         return grad_rows, grad_weights.zero_()
     status = _native.lib().fsh_expert_combine_backward(
-        grad.data_ptr(), rows.data_ptr(), position.data_ptr(), offsets.data_ptr(), _check_routing(offsets), weights.data_ptr(),
-        _float_dt(weights.dtype), tokens, top_k, width, _float_dt(rows.dtype), grad_rows.data_ptr(), grad_weights.data_ptr(),
-        stream_ptr(rows.device),
+        grad.data_ptr(), rows.data_ptr(), position_ptr, offsets_ptr, experts, weights.data_ptr(), _float_dt(weights.dtype), tokens,
+        top_k, width, _float_dt(rows.dtype), grad_rows.data_ptr(), grad_weights.data_ptr(), stream_ptr(device),
     )
-    _native.check(status, "fsh_expert_combine_backward")
+    if status:
+        _native.check(status, "fsh_expert_combine_backward")
     return grad_rows, grad_weights

@@ -17,11 +17,11 @@ from typing import Any
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native, hip_ops
-from ..experts import ExpertRouting
+from ..experts import ExpertRouting, differentiates
+from ..hip_ops import MxFp4Matrix
 from .mxfp4_matrix import MxFp4Weight, as_rows
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -36,11 +36,6 @@ def _check_input(x: torch.Tensor, in_dim: int) -> None:
         raise ValueError("the weight's input dim is zero")
 
 
-def _differentiates() -> bool:
-    """Whether a call may be recorded (or has to refuse a transform)."""
-    return torch.is_grad_enabled() or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
-
-
 def _weight_forms(weight: torch.Tensor | MxFp4Weight, needs_x: bool):
     """Row and column form of a weight, the latter where the input's gradient needs it."""
     if not isinstance(weight, MxFp4Weight):
@@ -50,42 +45,57 @@ def _weight_forms(weight: torch.Tensor | MxFp4Weight, needs_x: bool):
             "a gradient for the input of a quantized weight needs its transposed form: "
             "quantize_mxfp4_weight(weight, transposed=True)"
         )
-    return weight.matrix.pair, weight.transposed.pair if needs_x else None
+    return weight.matrix, weight.transposed if needs_x else None
 
 
-def _linear_forward(x: torch.Tensor, weight: torch.Tensor | MxFp4Weight, bias: torch.Tensor | None, needs_x: bool, needs_w: bool):
-    """The product, and the column forms of x and W that a backward needs."""
-    x_rows, x_columns, _ = hip_ops.mxfp4_quantize(x, columns=needs_w)
-    w_rows, w_columns = _weight_forms(weight, needs_x)
-    out = hip_ops.mxfp4_gemm(x_rows, w_rows, x.dtype, bias=None if bias is None else bias.to(x.dtype).contiguous())
-    return out, x_columns, w_columns
+def _bias_for(x: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor | None:
+    """The bias in the product's type (its epilogue adds it before the one rounding)."""
+    if bias is None or (bias.dtype == x.dtype and bias.is_contiguous()):
+        return bias
+    return bias.to(x.dtype).contiguous()
+
+
+def _keep(ctx: Any, x_columns: MxFp4Matrix | None, w_columns: MxFp4Matrix | None) -> None:
+    """Save the column forms that the backward reads."""
+    ctx.forms = [None if form is None else (form.rows, form.cols) for form in (x_columns, w_columns)]
+    ctx.save_for_backward(*[None if form is None else form.buffer for form in (x_columns, w_columns)])
+
+
+def _kept(ctx: Any) -> list[MxFp4Matrix | None]:
+    return [None if size is None else MxFp4Matrix(buffer, *size) for buffer, size in zip(ctx.saved_tensors, ctx.forms)]
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, frozen: MxFp4Weight | None):
         needs_x, needs_w = ctx.needs_input_grad[0], frozen is None and ctx.needs_input_grad[1]
-        out, x_columns, w_columns = _linear_forward(x, frozen or weight, bias, needs_x, needs_w)
+        w_rows, w_columns = _weight_forms(frozen or weight, needs_x)
+        x_columns = None
+        if needs_w:
+            x_rows, x_columns, _ = hip_ops.mxfp4_quantize(x, columns=True)
+            out = hip_ops.mxfp4_gemm(x_rows, w_rows, x.dtype, bias=_bias_for(x, bias))
+        else:
+            out = hip_ops.mxfp4_linear(x, w_rows, _bias_for(x, bias))
         ctx.dtype, ctx.weight_dtype = x.dtype, None if frozen else weight.dtype
         ctx.bias_dtype = None if bias is None else bias.dtype
-        ctx.save_for_backward(*(x_columns or (None, None)), *(w_columns or (None, None)))
+        _keep(ctx, x_columns, w_columns)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        x_data, x_scales, w_data, w_scales = ctx.saved_tensors
+        x_columns, w_columns = _kept(ctx)
         needs_bias = ctx.bias_dtype is not None and ctx.needs_input_grad[2]
-        grad = as_rows(grad)
-        columns = x_data is not None or needs_bias
-        g_rows, g_columns, sums = (None, None, None)
-        if w_data is not None or columns:
-            g_rows, g_columns, sums = hip_ops.mxfp4_quantize(grad, rows=w_data is not None, columns=columns, column_sums=needs_bias)
+        columns = x_columns is not None or needs_bias
         grad_x = grad_w = grad_b = None
-        if w_data is not None:
-            grad_x = hip_ops.mxfp4_gemm(g_rows, (w_data, w_scales), ctx.dtype)
-        if x_data is not None:
-            grad_w = hip_ops.mxfp4_gemm(g_columns, (x_data, x_scales), ctx.weight_dtype)
+        if w_columns is not None or columns:
+            g_rows, g_columns, sums = hip_ops.mxfp4_quantize(
+                as_rows(grad), rows=w_columns is not None, columns=columns, column_sums=needs_bias
+            )
+        if w_columns is not None:
+            grad_x = hip_ops.mxfp4_gemm(g_rows, w_columns, ctx.dtype)
+        if x_columns is not None:
+            grad_w = hip_ops.mxfp4_gemm(g_columns, x_columns, ctx.weight_dtype)
         if needs_bias:
             grad_b = hip_ops.sum_runs(sums, ctx.bias_dtype)
         return grad_x, grad_w, grad_b, None
@@ -111,31 +121,18 @@ def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor | MxFp4Weight, bias: torc
         dense = x.new_empty((out_dim, in_dim)) if frozen is not None else weight.to(x.dtype)
         return nn.functional.linear(x, dense, None if bias is None else bias.to(x.dtype))
     x_2d = as_rows(x if x.ndim == 2 else x.reshape(-1, in_dim))
-    if _differentiates():
+    if differentiates(x_2d, None if frozen else weight, bias):
         out = _Linear.apply(x_2d, None if frozen else weight, bias, frozen)
     else:
-        out = _linear_forward(x_2d, weight, bias, False, False)[0]
+        out = hip_ops.mxfp4_linear(x_2d, _weight_forms(weight, False)[0], _bias_for(x, bias))
     return out if x.ndim == 2 else out.reshape(*x.shape[:-1], out_dim)
 
 
-def _expert_forward(
-    x: torch.Tensor, weight: torch.Tensor | MxFp4Weight, routing: ExpertRouting, sorted_rows: bool, needs_x: bool, needs_w: bool
-):
-    source = None if sorted_rows else routing.source
-    x_rows = x_columns = None
-    if needs_w:
-        x_rows, x_columns = hip_ops.mxfp4_quantize_segments(
-            x, routing.offsets, routing.padded_offsets, routing.padded_rows, choices=routing.rows, source=source,
-            top_k=routing.top_k, rows=sorted_rows,
-        )
-    if x_rows is None:
-        x_rows, _, _ = hip_ops.mxfp4_quantize(x)
-    w_rows, w_columns = _weight_forms(weight, needs_x)
-    out = hip_ops.mxfp4_gemm(
-        x_rows, w_rows, x.dtype, mode=_native.MXFP4_ROWS, offsets=routing.offsets, source=source, top_k=routing.top_k,
-        choices=routing.rows,
+def _expert_forward(x: torch.Tensor, w_rows: MxFp4Matrix, routing: ExpertRouting, sorted_rows: bool) -> torch.Tensor:
+    _, source, offsets, _ = routing.pointers()
+    return hip_ops.mxfp4_expert_linear(
+        x, w_rows, routing.experts, routing.rows, routing.top_k, offsets, None if sorted_rows else source
     )
-    return out, x_columns, w_columns
 
 
 class _ExpertLinear(torch.autograd.Function):
@@ -144,36 +141,44 @@ class _ExpertLinear(torch.autograd.Function):
         ctx: Any, x: torch.Tensor, weight: torch.Tensor | None, routing: ExpertRouting, sorted_rows: bool, frozen: MxFp4Weight | None
     ):
         needs_x, needs_w = ctx.needs_input_grad[0], frozen is None and ctx.needs_input_grad[1]
-        out, x_columns, w_columns = _expert_forward(x, frozen or weight, routing, sorted_rows, needs_x, needs_w)
+        w_rows, w_columns = _weight_forms(frozen or weight, needs_x)
+        x_rows = x_columns = None
+        if needs_w:
+            x_rows, x_columns = hip_ops.mxfp4_quantize_segments(
+                x, routing.offsets, routing.padded_offsets, routing.padded_rows, choices=routing.rows,
+                source=None if sorted_rows else routing.source, top_k=routing.top_k, rows=sorted_rows,
+            )
+        if x_rows is not None:
+            out = hip_ops.mxfp4_gemm(x_rows, w_rows, x.dtype, mode=_native.MXFP4_ROWS, offsets=routing.offsets)
+        else:
+            out = _expert_forward(x, w_rows, routing, sorted_rows)
         ctx.routing, ctx.sorted_rows = routing, sorted_rows
         ctx.dtype, ctx.weight_dtype = x.dtype, None if frozen else weight.dtype
-        ctx.save_for_backward(*(x_columns or (None, None)), *(w_columns or (None, None)))
+        _keep(ctx, x_columns, w_columns)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor):
-        x_data, x_scales, w_data, w_scales = ctx.saved_tensors
+        x_columns, w_columns = _kept(ctx)
         routing = ctx.routing
         grad = as_rows(grad)
         grad_x = grad_w = g_rows = None
-        if x_data is not None:
+        if x_columns is not None:
             g_rows, g_columns = hip_ops.mxfp4_quantize_segments(
-                grad, routing.offsets, routing.padded_offsets, routing.padded_rows, choices=routing.rows, rows=w_data is not None,
+                grad, routing.offsets, routing.padded_offsets, routing.padded_rows, choices=routing.rows, rows=w_columns is not None,
             )
             grad_w = hip_ops.mxfp4_gemm(
-                g_columns, (x_data, x_scales), ctx.weight_dtype, mode=_native.MXFP4_OVER_ROWS, offsets=routing.padded_offsets
+                g_columns, x_columns, ctx.weight_dtype, mode=_native.MXFP4_OVER_ROWS, offsets=routing.padded_offsets
             )
-        elif w_data is not None:
+        elif w_columns is not None:
             g_rows, _, _ = hip_ops.mxfp4_quantize(grad)
-        if w_data is not None:
-            grad_x = hip_ops.mxfp4_gemm(
-                g_rows, (w_data, w_scales), ctx.dtype, mode=_native.MXFP4_ROWS, offsets=routing.offsets
-            )
+        if w_columns is not None:
+            grad_x = hip_ops.mxfp4_gemm(g_rows, w_columns, ctx.dtype, mode=_native.MXFP4_ROWS, offsets=routing.offsets)
             if not ctx.sorted_rows:
                 # The choices' gradients are rounded to the activation's type before they are added up in
                 # fp32: half the bytes of fp32 rows, for an error of the size of the result's own rounding.
-                grad_x = hip_ops.expert_combine(grad_x, routing.position)
+                grad_x = hip_ops.expert_combine_at(grad_x, routing.pointers()[0], routing.tokens, routing.top_k)
         return grad_x, grad_w, None, None, None
 
 
@@ -198,9 +203,11 @@ def mxfp4_expert_linear(
     if routing.rows == 0 or out_dim == 0:
         dense = x.new_empty((out_dim, in_dim)) if frozen is not None else weight[0].to(x.dtype)
         return nn.functional.linear(x.new_zeros((routing.rows, in_dim)) + 0 * x.sum(), dense)
-    if _differentiates():
-        return _ExpertLinear.apply(as_rows(x), None if frozen else weight, routing, sorted_rows, frozen)
-    return _expert_forward(as_rows(x), weight, routing, sorted_rows, False, False)[0]
+    hip_ops._require_gpu(routing.buffer, x)
+    x = as_rows(x)
+    if differentiates(x, None if frozen else weight):
+        return _ExpertLinear.apply(x, None if frozen else weight, routing, sorted_rows, frozen)
+    return _expert_forward(x, _weight_forms(weight, False)[0], routing, sorted_rows)
 
 
 class FlexShardMxFp4Linear(nn.Linear):

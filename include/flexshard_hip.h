@@ -591,6 +591,19 @@ typedef struct fsh_mxfp4_product {
 } fsh_mxfp4_product;
 int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream);
 
+/* The forward of a linear layer, or of the experts', on an activation x [rows,
+ * in_dim] of row stride ldx that is quantized on the way: product as above with k =
+ * in_dim rounded up to 256, out_dtype = dtype, mode DENSE or ROWS; its a_dev,
+ * a_scales_dev and a_rows are not read.  scratch: 16-byte aligned, at least
+ * fsh_mxfp4_matrix_bytes(rows, in_dim) bytes (the size of a quantized matrix, data
+ * and scales behind one another); null will do for a dense product of at most
+ * FSH_MXFP4_FEW_ROWS rows and 16384 columns, whose workgroups quantize x for
+ * themselves. */
+#define FSH_MXFP4_FEW_ROWS 4
+int64_t fsh_mxfp4_matrix_bytes(int64_t rows, int64_t cols);
+int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int64_t ldx, const fsh_mxfp4_product* product,
+                     int64_t in_dim, void* scratch_dev, int64_t scratch_nbytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * 13. Tokens sorted by expert and back.  expert_ids [tokens, top_k] (int64 or
  * int32): the experts that a router chose for each token; an id outside
