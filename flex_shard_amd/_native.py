@@ -258,6 +258,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "fsh_mxfp4_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_int64, c_void_p]),
     "fsh_sum_runs": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
     "fsh_mxfp4_gemm": (c_int, [POINTER(MxFp4Product), c_void_p]),
+    "fsh_mxfp4_gemm_tiles": (c_int, [c_int64, c_int64, c_int64, c_int32, c_int32]),
     "fsh_mxfp4_matrix_bytes": (c_int64, [c_int64, c_int64]),
     "fsh_mxfp4_linear": (
         c_int, [c_void_p, c_int32, c_int64, c_int64, POINTER(MxFp4Product), c_int64, c_void_p, c_int64, c_void_p],

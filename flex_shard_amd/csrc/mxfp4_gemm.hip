@@ -7,17 +7,18 @@
 namespace fsh {
 namespace {
 
+constexpr int64_t kFewMaxRows = 16;
+
 template <typename Cfg, int kProblem>
 int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t stream) {
-  GemmParams& s = p.schedule;
+  MxSchedule& s = p.schedule;
   const int64_t tiles_n = ceil_div(p.n, static_cast<int64_t>(Cfg::BN)), tiles = tiles_m * tiles_n;
   if (tiles * batch > 0x3FFFFFLL) return fail(FSH_ENOTSUP, "fsh_mxfp4_gemm: too many tiles");
   s.tiles_m = static_cast<int32_t>(tiles_m);
   s.tiles_n = static_cast<int32_t>(tiles_n);
-  s.tiles_per_matrix = static_cast<int32_t>(tiles);
-  s.work_items = tiles * batch;
-  s.items_per_xcd = ceil_div(s.work_items, static_cast<int64_t>(kXcds));
-  int64_t blocks = s.items_per_xcd * kXcds;
+  s.items = static_cast<int32_t>(tiles * batch);
+  s.items_per_xcd = (s.items + kXcds - 1) / kXcds;
+  int64_t blocks = static_cast<int64_t>(s.items_per_xcd) * kXcds;
   if (Cfg::kResident) {
     const int64_t units = compute_units(), resident = units >= kXcds ? units / kXcds * kXcds : kXcds;
     blocks = blocks < resident ? blocks : resident;
@@ -38,8 +39,10 @@ int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t
 template <typename Cfg>
 int64_t segment_tiles(const MxGemmParams& p) { return p.m / Cfg::BM + p.experts + 1; }
 
-using MxLarge = MxTile<2, 2, 4, 4, 2, 5, true>;
-using MxSmall = MxTile<2, 2, 1, 1, 4, 0, false>;
+using MxLarge = MxTile<2, 2, 4, 4, 2, 5, true>;     // 256 x 256, one workgroup per compute unit
+using MxMid = MxTile<2, 2, 2, 2, 2, 0, false>;      // 128 x 128, two
+using MxMidDeep = MxTile<2, 2, 2, 2, 4, 0, false>;  // 128 x 128, one, four steps in flight
+using MxSmall = MxTile<2, 2, 1, 1, 4, 0, false>;    // 64 x 64, two
 
 template <typename Cfg>
 int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
@@ -49,33 +52,85 @@ int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
   return launch_mx_tiles<Cfg, kMxDense>(p, tiles_m, 1, stream);
 }
 
-// Few rows: which kernel, and how many waves share a workgroup's contraction.
-constexpr int64_t kFewMaxRows = 64;
-int few_waves(int64_t workgroups, int64_t steps) {
-  int waves = 4;
-  while (waves < 16 && workgroups * waves < 2048 && 2 * waves <= steps) waves *= 2;
-  return static_cast<int>(waves < steps ? waves : steps);
-}
-int few_lds_bytes(const MxFewParams& p, int token_blocks, bool quantize) {
-  return p.waves * token_blocks * 16 * 17 * 4 + (quantize ? kFewQuantize * (static_cast<int>(p.ld) + 16 + 8 * p.steps) : 0);
+// Which tiles a product takes: those with the lowest estimated time, from what
+// the four measured (us, 64 x 64 / 128 x 128 / 128 x 128 deep / 256 x 256):
+//   48 x 14336, k 4096      8.2  14.8  11.1  24.2    128 x 14336, k 4096    11.0  15.2  11.6  23.8
+//   256 x 1024, k 4096      6.5  10.0   9.7  23.4    512 x 4096, k 4096     10.9  14.9  11.7  24.4
+//   64 x 4096, k 14336     16.0  39.3  24.2  63.5    445 x 3932, k 11071    24.3  35.8  25.3  60.4
+//   1000 x 5120, k 2048    15.7  12.4  15.4  18.0    1000 x 2048, k 5120    13.0  18.0  13.2  29.1
+//   3000 x 1024, k 1500     9.5   8.2   7.8  14.5    2048 x 2048, k 2048    12.7  10.2   9.1  16.8
+//   1024 x 4096, k 8192    35.0  28.8  22.6  42.2    512 x 14336, k 4096    33.7  22.0  24.0  26.9
+//   2048 x 4096, k 4096    36.9  22.6  24.3  27.2    4096 x 4096, k 4096    67.8  41.4  46.4  35.3
+//   4096 x 14336, k 4096    221   154   173   126    14336 x 4096, k 1000   92.5  51.8  66.5  46.7
+// Rows of 32 experts, 7168 to 2048 columns, by rows per expert:
+//   4   51.2  49.4  55.2  73.5    64  74.2  52.3  57.0  66.6    128  107  93.9  84.1  70.9    512  292  217  244  176
+// Over rows of 32 experts, [2048, 7168] each, by rows per expert:
+//   64  480  257  368  254    256  547  295  443  338    1024  829  506  642  477
+// Few rows have a kernel of their own (mxfp4_few.hpp); us, it / 64 x 64 tiles, by rows (1, 4, 16):
+//   14336, k 4096  8.5 / 9.0  9.0 / 9.1  10.9 / 9.4    4096, k 4096  4.2 / 7.5  4.4 / 7.6  4.9 / 7.6
+//   4096, k 14336  9.6 / 17   9.9 / 17   11.5 / 18     1024, k 4096  3.5 / 7.1  3.7 / 7.1  4.3 / 7.2
+bool takes_few_rows(int64_t m, int64_t n) { return m <= kFewMaxRows && (m <= kFewQuantize || n <= 8192); }
+
+enum MxTileKind { kMxTiles64, kMxTiles128, kMxTiles128Deep, kMxTiles256, kMxFewRows };
+MxTileKind mx_tile_kind(const MxGemmParams& p, MxProblem problem, int64_t units) {
+  static constexpr TileShape kShapes[] = {
+      {64, 64, 512.0, 0.18, 0.34, 0.49, 1.2},
+      {128, 128, 512.0, 0.75, 0.80, 1.20, 2.8},
+      {128, 128, 256.0, 0.42, 0.54, 0.60, 2.2},
+      {256, 256, 256.0, 1.34, 1.50, 2.05, 5.0},
+  };
+  const bool segments = problem == kMxRows;
+  if (problem == kMxDense && takes_few_rows(p.m, p.n)) return kMxFewRows;
+  // Experts that have rows, and their rows: evenly spread for all that is known here.
+  const double experts = segments ? static_cast<double>(p.m < p.experts ? p.m : p.experts) : 1.0;
+  const double rows = static_cast<double>(p.m) / experts;
+  double steps = static_cast<double>(p.k / kMxColumns);
+  if (problem == kMxOverRows) steps = steps / p.experts < 1.0 ? 1.0 : steps / p.experts;
+  // Every expert's weight comes from memory.
+  const double memory_us = segments ? experts * static_cast<double>(p.n) * static_cast<double>(p.k) * (17.0 / 32.0) / 5.2e6 : 0.0;
+  MxTileKind best = kMxTiles64;
+  double best_us = 0.0;
+  for (int i = 0; i < 4; ++i) {
+    TileShape shape = kShapes[i];
+    shape.round *= static_cast<double>(units) / 256.0;
+    double tiles_m = ceil(rows / static_cast<double>(shape.m));
+    if (segments && 2.0 * rows > static_cast<double>(shape.m)) tiles_m = rows / static_cast<double>(shape.m) + 0.5;  // (some have more rows)
+    double tiles = experts * tiles_m * static_cast<double>(ceil_div(p.n, shape.m));
+    if (problem == kMxOverRows) tiles *= p.experts;
+    if (segments && i < 3) {  // (two tile rows of an expert do not meet in the L2 as those of one matrix do)
+      shape.empty *= 1.4;
+      shape.half *= 1.4;
+      shape.full *= 1.4;
+    }
+    double us = rounds_us(shape, tiles, tiles * steps, steps);
+    if (us < memory_us) us = memory_us;
+    if (i == 0 || us < best_us) {
+      best = static_cast<MxTileKind>(i);
+      best_us = us;
+    }
+  }
+  return best;
 }
 
-// kDense: p.m rows at most kFewMaxRows; kExperts: any rows, 16 of an expert at a time.
-template <bool kExperts, bool kQuantize>
+// How many waves share a workgroup's contraction: enough to fill the chip.
+int few_waves(int64_t workgroups, int64_t steps) {
+  int waves = 4;
+  while (waves < kFewMaxWaves && workgroups * waves < 2048 && 2 * waves <= steps) waves *= 2;
+  return static_cast<int>(waves < steps ? waves : steps);
+}
+int few_lds_bytes(const MxFewParams& p, int waves, bool quantize) {
+  return waves * 16 * 17 * 4 + (quantize ? kFewQuantize * (static_cast<int>(p.ld) + 16 + 8 * p.steps) : 0);
+}
+
+template <bool kQuantize>
 int launch_few(MxFewParams& p, int32_t dtype, hipStream_t stream) {
-  const int64_t tiles_n = ceil_div(p.n, static_cast<int64_t>(kFewRows)), blocks = tiles_n * (kExperts ? p.experts + 1 : 1);
+  const int64_t blocks = ceil_div(p.n, static_cast<int64_t>(kFewRows));
   if (blocks > 0x3FFFFFLL) return fail(FSH_ENOTSUP, "fsh_mxfp4_gemm: too many tiles");
-  p.tiles_n = static_cast<int32_t>(tiles_n);
   p.waves = few_waves(blocks, p.steps);
   const dim3 grid(static_cast<uint32_t>(blocks)), block(64 * p.waves);
-  const int token_blocks = kExperts || p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-  const int lds = few_lds_bytes(p, token_blocks, kQuantize);
+  const int lds = few_lds_bytes(p, p.waves, kQuantize);
   by_dtype(dtype, [&](auto dt) {
-    if (token_blocks == 1) hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 1, kExperts, kQuantize>), grid, block, lds, stream, p);
-    else if constexpr (!kExperts && !kQuantize) {
-      if (token_blocks == 2) hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 2, false, false>), grid, block, lds, stream, p);
-      else hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, 4, false, false>), grid, block, lds, stream, p);
-    }
+    hipLaunchKernelGGL((mxfp4_few_rows_kernel<dt.value, kQuantize>), grid, block, lds, stream, p);
   });
   return check_launch("mxfp4_few_rows_kernel");
 }
@@ -89,8 +144,6 @@ MxFewParams few_params(const fsh_mxfp4_product& q) {
   p.m = q.m; p.n = q.n; p.a_rows = q.a_rows; p.b_rows = q.b_rows;
   p.ld = q.k / 2; p.ldo = q.ldo;
   p.steps = static_cast<int32_t>(q.k / kMxColumns);
-  p.experts = q.experts; p.top_k = q.top_k;
-  p.offsets = q.offsets_dev; p.source = q.source_dev;
   return p;
 }
 
@@ -130,14 +183,6 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   if (256 * (q.k / 2) >= (1LL << 32) || (q.source_dev && q.a_rows * (q.k / 2) >= (1LL << 32)))
     return fail(FSH_ENOTSUP, "%s: rows that are gathered, or a tile of them, span 4 GiB or more", who);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (q.mode == FSH_MXFP4_DENSE && q.m <= kFewMaxRows) {
-    MxFewParams few = few_params(q);
-    return launch_few<false, false>(few, q.out_dtype, on);
-  }
-  if (segments && q.m <= 16 * static_cast<int64_t>(q.experts)) {
-    MxFewParams few = few_params(q);
-    return launch_few<true, false>(few, q.out_dtype, on);
-  }
   MxGemmParams p;
   memset(&p, 0, sizeof(p));
   p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
@@ -151,10 +196,38 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   p.experts = q.experts; p.top_k = q.top_k;
   p.offsets = p.padded_offsets = q.offsets_dev;
   p.source = q.source_dev;
+  if (p.top_k > 0) {
+    // ceil(2^(31 + b) / top_k), 2^b >= top_k: exact for choices below 2^31
+    int bits = 0;
+    while ((1LL << bits) < p.top_k) ++bits;
+    p.top_k_shift = 31 + bits;
+    p.top_k_factor = static_cast<uint32_t>(((1ULL << p.top_k_shift) + p.top_k - 1) / p.top_k);
+  }
   const MxProblem problem = segments ? kMxRows : q.mode == FSH_MXFP4_OVER_ROWS ? kMxOverRows : kMxDense;
-  const int64_t rows = segments ? q.m / q.experts : q.m;
-  if (rows * q.n >= 128 * 128 * 64) return launch_mx<MxLarge>(p, problem, on);
-  return launch_mx<MxSmall>(p, problem, on);
+  const int64_t units = compute_units();
+  switch (mx_tile_kind(p, problem, units > 0 ? units : 256)) {
+    case kMxTiles64: return launch_mx<MxSmall>(p, problem, on);
+    case kMxTiles128: return launch_mx<MxMid>(p, problem, on);
+    case kMxTiles128Deep: return launch_mx<MxMidDeep>(p, problem, on);
+    case kMxFewRows: {
+      MxFewParams few = few_params(q);
+      return launch_few<false>(few, q.out_dtype, on);
+    }
+    default: return launch_mx<MxLarge>(p, problem, on);
+  }
+}
+
+FSH_API int fsh_mxfp4_gemm_tiles(int64_t m, int64_t n, int64_t k, int32_t mode, int32_t experts) {
+  using namespace fsh;
+  if (m <= 0 || n <= 0 || k <= 0 || mode < FSH_MXFP4_DENSE || mode > FSH_MXFP4_OVER_ROWS || (mode != FSH_MXFP4_DENSE && experts <= 0))
+    return fail(FSH_EINVAL, "fsh_mxfp4_gemm_tiles: bad sizes");
+  MxGemmParams p;
+  memset(&p, 0, sizeof(p));
+  p.m = m; p.n = n; p.k = ceil_div(k, (int64_t)kMxColumns) * kMxColumns;
+  p.experts = experts;
+  const int64_t units = compute_units();
+  static constexpr int kNames[] = {FSH_TILES_64, FSH_TILES_128, FSH_TILES_128_DEEP, FSH_TILES_256, FSH_TILES_FEW_ROWS};
+  return kNames[mx_tile_kind(p, mode == FSH_MXFP4_ROWS ? kMxRows : mode == FSH_MXFP4_OVER_ROWS ? kMxOverRows : kMxDense, units > 0 ? units : 256)];
 }
 
 FSH_API int64_t fsh_mxfp4_matrix_bytes(int64_t rows, int64_t cols) {
@@ -177,8 +250,7 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
   q.a_rows = rows;
   if (q.mode == FSH_MXFP4_DENSE && q.m <= kFewQuantize) {
     MxFewParams p = few_params(q);
-    p.waves = 16;
-    if (few_lds_bytes(p, 1, true) <= 64 * 1024) {
+    if (few_lds_bytes(p, kFewMaxWaves, true) <= 64 * 1024) {
       if (!known_dtype(dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, dtype);
       if (rows < q.m || ldx < in_dim || q.ldo < q.n || q.b_rows < q.n)
         return fail(FSH_EINVAL, "%s: rows or leading dimensions too small", who);
@@ -189,7 +261,7 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
       p.a = static_cast<const uint8_t*>(x_dev);
       p.cols = in_dim; p.ldx = ldx;
       p.vec = aligned(x_dev, 16) && ldx * bytes % 16 == 0;
-      return launch_few<false, true>(p, dtype, static_cast<hipStream_t>(stream));
+      return launch_few<true>(p, dtype, static_cast<hipStream_t>(stream));
     }
   }
   const int64_t need = fsh_mxfp4_matrix_bytes(rows, in_dim);

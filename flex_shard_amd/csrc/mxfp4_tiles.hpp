@@ -49,6 +49,12 @@ enum MxProblem {
   kMxOverRows,   // per expert the product over its own (padded) columns of a and b: [experts][m][n]
 };
 
+// The order of the tiles: XCD x takes the run [x, x + 1) * items_per_xcd of an order in which kGroupTilesM tile rows are
+// walked together, so that the tiles that its compute units hold at a time share operands in its L2.
+struct MxSchedule {
+  int32_t tiles_m, tiles_n, items, items_per_xcd;  // items: tiles of all matrices
+};
+
 struct MxGemmParams {
   const uint8_t* a;   // [a_rows][lda]
   const uint8_t* as;  // [k / 256][a_rows][8]
@@ -63,7 +69,9 @@ struct MxGemmParams {
   const int32_t* offsets;         // [experts + 1]
   const int32_t* padded_offsets;  // [experts + 1] (kMxOverRows)
   const int32_t* source;          // kMxRows: row r of the segments is row source[r] / top_k of a, or null
-  GemmParams schedule;            // tile order
+  uint32_t top_k_factor;          // choice / top_k is choice * top_k_factor >> top_k_shift
+  int32_t top_k_shift;
+  MxSchedule schedule;
 };
 
 // A tile of WM x WN waves, each TM x TN blocks of 32 x 32.  A k-step is 256
@@ -157,14 +165,16 @@ struct MxStores {
 
 // The tile of a workgroup's turn (0 for the first) in the order of `schedule`.
 template <typename Cfg, int kProblem>
-__device__ __forceinline__ bool place_of_turn(const MxGemmParams& p, const GemmParams& schedule, const int32_t* table, int64_t turn,
+__device__ __forceinline__ bool place_of_turn(const MxGemmParams& p, const MxSchedule& schedule, const int32_t* table, int turn,
                                               MxTilePlace* place) {
-  int64_t batch;
-  int tm, tn;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) + turn * gridDim.x;
-  if (id / kXcds >= schedule.items_per_xcd || !tile_of_workgroup(schedule, id, &batch, &tm, &tn)) return false;
-  tm = uniform_i32(tm);
-  tn = uniform_i32(tn);
+  const int id = static_cast<int>(blockIdx.x) + turn * static_cast<int>(gridDim.x);
+  const int item = id % kXcds * schedule.items_per_xcd + id / kXcds;
+  if (id / kXcds >= schedule.items_per_xcd || item >= schedule.items) return false;
+  const int tiles = schedule.tiles_m * schedule.tiles_n;
+  const int batch = kProblem == kMxOverRows ? item / tiles : 0;
+  const int t = item - batch * tiles, span = kGroupTilesM * schedule.tiles_n, first_m = t / span * kGroupTilesM;
+  const int within = t - first_m * schedule.tiles_n, rows = min(schedule.tiles_m - first_m, kGroupTilesM);
+  const int tn = rows == kGroupTilesM ? within / kGroupTilesM : within / rows, tm = first_m + within - tn * rows;
   place->zero = false;
   place->out_offset = 0;
   place->first_step = 0;
@@ -183,7 +193,7 @@ __device__ __forceinline__ bool place_of_turn(const MxGemmParams& p, const GemmP
     place->row0 = static_cast<int64_t>(tm) * Cfg::BM;
     place->rows = p.m - place->row0 < Cfg::BM ? p.m - place->row0 : Cfg::BM;
     if (kProblem == kMxOverRows) {
-      const int expert = uniform_i32(static_cast<int>(batch));
+      const int expert = batch;
       const int32_t begin = load_uniform(p.padded_offsets + expert), end = load_uniform(p.padded_offsets + expert + 1);
       place->first_step = begin / kMxColumns;
       place->steps = (end - begin) / kMxColumns;
@@ -225,13 +235,12 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
   int32_t* const table = reinterpret_cast<int32_t*>(lds_bytes + Cfg::kTableOffset);
   float* const bias_of_tile = reinterpret_cast<float*>(lds_bytes + Cfg::kTableOffset);
 
-  GemmParams schedule = p.schedule;
+  MxSchedule schedule = p.schedule;
   if (kProblem == kMxRows) {
     // How many tiles the segments have is known here only.
     schedule.tiles_m = fill_segment_table<Cfg::BM>(p, table);
-    schedule.tiles_per_matrix = schedule.tiles_m * schedule.tiles_n;
-    schedule.work_items = schedule.tiles_per_matrix;
-    schedule.items_per_xcd = ceil_div(schedule.work_items, static_cast<int64_t>(kXcds));
+    schedule.items = schedule.tiles_m * schedule.tiles_n;
+    schedule.items_per_xcd = (schedule.items + kXcds - 1) / kXcds;
   }
   MxTilePlace place;
   if (!place_of_turn<Cfg, kProblem>(p, schedule, table, 0, &place)) return;  // whole workgroup
@@ -272,13 +281,16 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
   const uint8_t* scale_src[kScaleRequests];
   int64_t scale_step[kScaleRequests];
   uint32_t scale_lds[kScaleRequests];
+  const auto token_of = [&](int choice) FSH_INLINE {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(choice)) * p.top_k_factor >> p.top_k_shift);
+  };
   const auto aim = [&](const MxTilePlace& at, const Rows& rows) FSH_INLINE {
     const int64_t a_first = gathered ? 0 : at.row0, b_first = at.b_row0 + at.col0;
     const int b_last = static_cast<int>(p.n - at.col0 < Cfg::BN ? p.n - at.col0 : Cfg::BN) - 1;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (c < kChunksA) {
-        voff[c] = static_cast<uint32_t>(gathered ? rows.data[c] / p.top_k : rows.data[c]) * static_cast<uint32_t>(p.lda);
+        voff[c] = static_cast<uint32_t>(gathered ? token_of(rows.data[c]) : rows.data[c]) * static_cast<uint32_t>(p.lda);
       } else {
         const int r = Cfg::kChunkRows * (c - kChunksA) + 8 * wave + fill_row;
         voff[c] = static_cast<uint32_t>(r < b_last ? r : b_last) * static_cast<uint32_t>(p.ldb);
@@ -292,7 +304,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
       const int q = kScaleRequests * wave + i, first = 64 * (q >> 1);
       const bool of_a = first < Cfg::BM;
       const int r = first - Cfg::BM + lane;
-      const int row = of_a ? (gathered ? rows.scales[i] / p.top_k : rows.scales[i]) : (r < b_last ? r : b_last);
+      const int row = of_a ? (gathered ? token_of(rows.scales[i]) : rows.scales[i]) : (r < b_last ? r : b_last);
       scale_voff[i] = static_cast<uint32_t>(row) * 8;
       scale_step[i] = (of_a ? p.a_rows : p.b_rows) * 8;
       scale_src[i] = uniform_ptr((of_a ? p.as + a_first * 8 : p.bs + b_first * 8) + at.first_step * scale_step[i] + 4 * (q & 1));
@@ -377,7 +389,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
   if (!place.zero) request_all_first(place.steps);
   using Stores = MxStores<Cfg, DT>;
   bool counted_stores = false;  // the last tile left between this one's first requests, in whole parts
-  for (int64_t turn = 1;; ++turn) {
+  for (int turn = 1;; ++turn) {
     MxTilePlace next_place;
     bool more_tiles = false;
     Rows next_rows;
@@ -519,28 +531,30 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     const bool vec = p.ldo * kElement % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     const bool whole = vec && wave_row + Cfg::kWaveM <= row_end && wave_col + Cfg::kWaveN <= p.n;
     const int store_row = lane / kLanesPerRow, store_col = lane % kLanesPerRow * kPerLane;
+    const int rows_left = static_cast<int>(row_end - wave_row), cols_left = static_cast<int>(p.n - wave_col < Cfg::kWaveN ? p.n - wave_col : Cfg::kWaveN);
+    const int vec_cols = vec ? (cols_left > 0 ? cols_left : 0) / kPerLane * kPerLane : 0;  // those that leave 16 bytes at a time
+    uint8_t* const wave_out = out + (wave_row * p.ldo + wave_col) * kElement;
+    uint8_t* const lane_out = wave_out + (store_row * p.ldo + store_col) * kElement;
+    const int64_t row_bytes = p.ldo * kElement;
     u32x4 leaving[Stores::kStores];
-    const auto store_part = [&](int part) FSH_INLINE {
-      const int64_t row = wave_row + part / (Cfg::kWaveN / kCols) * 32 + store_row, col = wave_col + part % (Cfg::kWaveN / kCols) * kCols + store_col;
-      uint8_t* to = out + (row * p.ldo + col) * kElement;
-      if (whole) {
-#pragma unroll
-        for (int s = 0; s < Stores::kStores; ++s) *reinterpret_cast<u32x4*>(to + s * kRowsPerStore * p.ldo * kElement) = leaving[s];
-      } else {
-#pragma unroll
-        for (int s = 0; s < Stores::kStores; ++s) {
-          if (row + s * kRowsPerStore >= row_end) break;
-          uint8_t* there = to + s * kRowsPerStore * p.ldo * kElement;
-          if (vec && col + kPerLane <= p.n) {
-            *reinterpret_cast<u32x4*>(there) = leaving[s];
-          } else {
-#pragma unroll
-            for (int t = 0; t < kPerLane; ++t)
-              if (col + t < p.n) {
-                if (kElement == 4) reinterpret_cast<uint32_t*>(there)[t] = leaving[s][t % 4];
-                else reinterpret_cast<uint16_t*>(there)[t] = static_cast<uint16_t>(leaving[s][t / 2 % 4] >> (16 * (t % 2)));
-              }
-          }
+    const auto store_one = [&](int part, int s) FSH_INLINE {
+      const int row = part / (Cfg::kWaveN / kCols) * 32 + s * kRowsPerStore, col = part % (Cfg::kWaveN / kCols) * kCols;
+      if (row + store_row < rows_left && col + store_col < vec_cols)
+        *reinterpret_cast<u32x4*>(lane_out + row * row_bytes + col * kElement) = leaving[s];
+    };
+    const auto store_rest = [&](int part) FSH_INLINE {
+      const int row = part / (Cfg::kWaveN / kCols) * 32, col = part % (Cfg::kWaveN / kCols) * kCols;
+      // What is left of rows that are not whole 16-byte pieces, out of the staging.  Not unrolled: the code of whole
+      // tiles has to stay in the instruction cache.
+      if (vec_cols < cols_left) {
+#pragma unroll 1
+        for (int e = lane; e < 32 * kCols; e += 64) {
+          const int r = e / kCols, c = e % kCols;
+          if (row + r >= rows_left || col + c < vec_cols || col + c >= cols_left) continue;
+          const uint8_t* from = region + r * Cfg::kPitch + c * kElement;
+          uint8_t* there = wave_out + (row + r) * row_bytes + (col + c) * kElement;
+          if (kElement == 4) *reinterpret_cast<uint32_t*>(there) = *reinterpret_cast<const uint32_t*>(from);
+          else *reinterpret_cast<uint16_t*>(there) = *reinterpret_cast<const uint16_t*>(from);
         }
       }
     };
@@ -565,15 +579,22 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
             for (int t = 0; t < 4; ++t) v[j][4 * q + t] += add[t];
           }
       }
+      // (the part before leaves between the conversions)
       uint32_t words[Stores::kWords];
+      constexpr int kPerStore = Stores::kWords / Stores::kStores;
+      static_for<Stores::kStores>([&](auto s_tag) FSH_INLINE {
+        constexpr int s = decltype(s_tag)::value;
 #pragma unroll
-      for (int w = 0; w < Stores::kWords; ++w) {
-        if (DT == FSH_DT_F32) words[w] = f32_as_u32(v[0][w]);
-        else if (DT == FSH_DT_BF16) words[w] = pack_bf16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
-        else words[w] = f32_to_f16_bits(v[w / 8][2 * w % 16]) | (f32_to_f16_bits(v[w / 8][2 * w % 16 + 1]) << 16);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (part > 0) store_part(part - 1);
+        for (int w = s * kPerStore; w < (s + 1) * kPerStore; ++w) {
+          if (DT == FSH_DT_F32) words[w] = f32_as_u32(v[0][w]);
+          else if (DT == FSH_DT_BF16) words[w] = pack_bf16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
+          else words[w] = f32_to_f16_bits(v[w / 8][2 * w % 16]) | (f32_to_f16_bits(v[w / 8][2 * w % 16 + 1]) << 16);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (part > 0) store_one(part - 1, s);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if (part > 0) store_rest(part - 1);
       wave_lds_sync();
       constexpr int kPerPiece = kElement;  // dwords of four columns, less what 16 bits save: 2 or 4
 #pragma unroll
@@ -594,7 +615,8 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
         });
       __builtin_amdgcn_sched_barrier(0);
     });
-    store_part(kParts - 1);
+    static_for<Stores::kStores>([&](auto s) FSH_INLINE { store_one(kParts - 1, decltype(s)::value); });
+    store_rest(kParts - 1);
     counted_stores = whole;
     if (!more_tiles) return;
     // The staging's slot is the third step's: every wave has to be done with it.

@@ -39,7 +39,8 @@ __all__ = [
     "expert_combine", "expert_combine_at", "expert_combine_backward", "expert_combine_backward_at", "expert_dispatch",
     "expert_dispatch_at", "expert_route", "expert_route_buffer", "expert_route_into",
     "fp8_gemm_tiles", "fp8_linear_backward", "fp8_transpose", "gemm_nt", "gemm_nt_group", "gemm_tiles", "muon_apply",
-    "muon_prepare", "mxfp4_dequantize", "mxfp4_expert_linear", "mxfp4_gemm", "mxfp4_linear", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
+    "muon_prepare", "mxfp4_dequantize", "mxfp4_expert_linear", "mxfp4_gemm", "mxfp4_gemm_tiles",
+    "mxfp4_linear", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
     "newton_schulz_product_tiles",
     "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
 ]
@@ -530,7 +531,7 @@ def gemm_nt(
 
 
 #: the tiles a product can take, as ``gemm_tiles`` and ``fp8_gemm_tiles`` name them
-GEMM_TILES = ("64", "64 deep", "128", "128 deep", "256x128", "256", "256 long k")
+GEMM_TILES = ("64", "64 deep", "128", "128 deep", "256x128", "256", "256 long k", "few rows")
 
 
 def gemm_tiles(*problems: tuple) -> tuple[str, ...]:
@@ -1267,6 +1268,14 @@ def mxfp4_gemm(
     if status:
         _native.check(status, "fsh_mxfp4_gemm")
     return out
+
+
+def mxfp4_gemm_tiles(m: int, n: int, k: int, *, mode: int = _native.MXFP4_DENSE, experts: int = 0) -> str:
+    """The kernel of an [m, n] product over ``k`` (as :func:`mxfp4_gemm` counts them;
+    no GPU needed)."""
+    kind = _native.lib().fsh_mxfp4_gemm_tiles(m, n, k, mode, experts)
+    _native.check(min(kind, 0), "fsh_mxfp4_gemm_tiles")
+    return GEMM_TILES[kind]
 
 
 def mxfp4_linear(x: torch.Tensor, weight: MxFp4Matrix, bias: torch.Tensor | None = None) -> torch.Tensor:

@@ -591,6 +591,11 @@ typedef struct fsh_mxfp4_product {
 } fsh_mxfp4_product;
 int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream);
 
+/* Which kernel such a product takes (FSH_TILES_*, or a negative status), without
+ * a GPU; k: columns before padding (OVER_ROWS: of all experts, padded). */
+#define FSH_TILES_FEW_ROWS 7
+int fsh_mxfp4_gemm_tiles(int64_t m, int64_t n, int64_t k, int32_t mode, int32_t experts);
+
 /* The forward of a linear layer, or of the experts', on an activation x [rows,
  * in_dim] of row stride ldx that is quantized on the way: product as above with k =
  * in_dim rounded up to 256, out_dtype = dtype, mode DENSE or ROWS; its a_dev,

@@ -6,12 +6,14 @@ import torch
 import torch.nn as nn
 from mxfp4_definition import ROUNDING, assert_product, through
 
+from flex_shard_amd import _native, hip_ops
 from flex_shard_amd.experts import combine_tokens, dispatch_tokens, route_tokens
 from flex_shard_amd.mxfp4 import (
     FlexShardMxFp4Linear,
     convert_to_flex_shard_mxfp4_linear,
     mxfp4_expert_linear,
     mxfp4_linear,
+    mxfp4_quantize,
     quantize_mxfp4_weight,
 )
 
@@ -61,6 +63,32 @@ def test_gradients(device, tokens, out_dim, in_dim, dtype):
         others[i] = leaf
         (alone,) = torch.autograd.grad(mxfp4_linear(*others), leaf, g.to(device))
         assert torch.equal(alone, (gx, gw, gb)[i])
+
+
+# every kernel of the dense product: sizes that end inside its tiles, contractions of few and of many steps,
+# more tiles than the chip holds at a time (256 x 256: a workgroup takes several)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(
+    "tiles,m,n,k",
+    [("few rows", 4, 14340, 700), ("few rows", 16, 1001, 5000), ("64", 50, 3001, 1100), ("64", 300, 2048, 2048), ("128", 1000, 5123, 600),
+     ("128", 8192, 1024, 1024), ("128 deep", 2040, 2040, 2300), ("128 deep", 2035, 2041, 700), ("256", 7950, 4096, 200),
+     ("256", 8190, 4088, 520), ("256", 8001, 4091, 1030), ("256", 4090, 8192, 1792)],
+)
+def test_every_kernel(device, tiles, m, n, k, dtype):
+    assert hip_ops.mxfp4_gemm_tiles(m, n, k) == tiles
+    gen = torch.Generator(device=device).manual_seed(m + n)
+    x, w = (torch.randn(rows, k, generator=gen, device=device).to(dtype) for rows in (m, n))
+    a, b = mxfp4_quantize(x), mxfp4_quantize(w)
+    bias = torch.randn(n, generator=gen, device=device).to(dtype)
+    got = hip_ops.mxfp4_gemm(a, b, dtype, bias=bias)
+    assert torch.equal(got, hip_ops.mxfp4_gemm(a, b, dtype, bias=bias))
+    a64, b64 = a.dequantize(torch.float32).double(), b.dequantize(torch.float32).double()
+    want, size = torch.mm(a64, b64.t()) + bias.double(), torch.mm(a64.abs(), b64.abs().t()) + bias.double().abs()
+    assert ((got.double() - want).abs() <= (k + 1) * 2.0**-23 * size + ROUNDING[dtype] * want.abs()).all()
+    # rows of a wider output, and nothing beside them
+    wide = torch.full((m, n + 24), 7.0, dtype=dtype, device=device)
+    assert torch.equal(hip_ops.mxfp4_gemm(a, b, dtype, bias=bias, out=wide[:, 5 : n + 5]), got)
+    assert (wide[:, :5] == 7.0).all() and (wide[:, n + 5 :] == 7.0).all()
 
 
 def test_fp32_master_weight_and_bias_with_bf16_activations(device):
@@ -225,6 +253,47 @@ def test_experts(device, tokens, top_k, experts, out_dim, in_dim, kind, sorted_r
     if dtype == torch.float16:
         bound += (top_k + 1) * 2.0**-25
     assert ((gx.double().cpu() - want_gx).abs() <= bound + 2.0**-133).all()
+
+
+@pytest.mark.parametrize(
+    "tiles,tokens,top_k,experts,n,k,absent",
+    [("64", 30, 2, 9, 300, 700, 0.1), ("128", 900, 4, 30, 2100, 500, 0.0), ("256", 2100, 4, 17, 1290, 600, 0.3)],
+)
+def test_every_kernel_of_the_experts(device, tiles, tokens, top_k, experts, n, k, absent):
+    assert hip_ops.mxfp4_gemm_tiles(tokens * top_k, n, k, mode=_native.MXFP4_ROWS, experts=experts) == tiles
+    gen = torch.Generator(device=device).manual_seed(tokens)
+    ids = torch.randint(0, experts, (tokens, top_k), generator=gen, device=device)
+    ids[: tokens // 3] = experts - 2  # one of them much liked
+    ids = torch.where(torch.rand(tokens, top_k, generator=gen, device=device) < absent, -1, ids)
+    routing = route_tokens(ids, experts)
+    x, w = (torch.randn(*s, generator=gen, device=device) for s in ((tokens, k), (experts, n, k)))
+    x.requires_grad_()
+    w.requires_grad_()
+    g = torch.randn(tokens * top_k, n, generator=gen, device=device)
+    y = mxfp4_expert_linear(x, w, routing)
+    gx, gw = torch.autograd.grad(y, (x, w), g)
+
+    def on(t):  # the values, in 64 bits
+        return mxfp4_quantize(t.detach()).dequantize(torch.float32).double()
+
+    offsets, source = routing.offsets.tolist(), routing.source.long()
+    want_gx = torch.zeros(tokens, k, dtype=torch.float64, device=device)
+    size_gx = torch.zeros_like(want_gx)
+    for e in range(experts):
+        part = slice(offsets[e], offsets[e + 1])
+        if part.start == part.stop:
+            assert not gw[e].any()
+            continue
+        of = source[part] // top_k
+        x_e, w_e, g_e = x[of], w[e], g[part]
+        for got, a, b in ((y[part], on(x_e), on(w_e)), (gw[e], on(g_e.t()), on(x_e.t()))):
+            want, size = torch.mm(a, b.t()), torch.mm(a.abs(), b.abs().t())
+            assert ((got.double() - want).abs() <= a.shape[1] * 2.0**-23 * size + 2.0**-24 * want.abs()).all()
+        a, b = on(g_e), on(w_e.t())
+        want_gx.index_add_(0, of, torch.mm(a, b.t()))
+        size_gx.index_add_(0, of, torch.mm(a.abs(), b.abs().t()))
+    assert not y[offsets[-1] :].any()
+    assert ((gx.double() - want_gx).abs() <= (n + 2 * top_k) * 2.0**-23 * size_gx).all()
 
 
 def test_expert_layer_through_the_whole_path(device):
