@@ -540,7 +540,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     const auto store_one = [&](int part, int s) FSH_INLINE {
       const int row = part / (Cfg::kWaveN / kCols) * 32 + s * kRowsPerStore, col = part % (Cfg::kWaveN / kCols) * kCols;
       if (row + store_row < rows_left && col + store_col < vec_cols)
-        *reinterpret_cast<u32x4*>(lane_out + row * row_bytes + col * kElement) = leaving[s];
+        __builtin_nontemporal_store(leaving[s], reinterpret_cast<u32x4*>(lane_out + row * row_bytes + col * kElement));
     };
     const auto store_rest = [&](int part) FSH_INLINE {
       const int row = part / (Cfg::kWaveN / kCols) * 32, col = part % (Cfg::kWaveN / kCols) * kCols;
