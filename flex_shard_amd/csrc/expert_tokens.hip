@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kThreads) void expert_count_kernel(const RouteParam
 // rank among the 64 is the number of earlier lanes with its expert.
 __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParams p) {
   __shared__ int32_t next[kWaves][kMaxExperts];  // first the waves' counts, then the next row of each expert
-  __shared__ int32_t total[kMaxExperts + 1];
+  __shared__ int32_t total[kMaxExperts + 1], before[kMaxExperts];  // of all blocks, of those before this one
   __shared__ int32_t wave_sum[2][kWaves];
   constexpr int kPerWave = kChoicesPerBlock / kWaves, kRounds = kPerWave / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -79,37 +79,45 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
     const int64_t at = first + 64 * i + lane;
     mine[i] = at < p.choices ? expert_of(p, at) : p.experts;
   }
-  for (int e = tid; e < p.experts; e += kThreads)
+  for (int e = tid; e < p.experts; e += kThreads) {
+    total[e] = before[e] = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) next[w][e] = 0;
+  }
   __syncthreads();
+  // (whole numbers: the order of the additions does not matter)
 #pragma unroll
   for (int i = 0; i < kRounds; ++i)
     if (mine[i] < p.experts) atomicAdd(&next[wave][mine[i]], 1);
+  if (p.blocks > 1) {
+    const int own = static_cast<int>(blockIdx.x) * p.experts, counts = p.blocks * p.experts;
+#pragma unroll 4
+    for (int i = tid; i < counts; i += kThreads) {
+      const int32_t c = p.counts[i];
+      const int e = i % p.experts;
+      if (c) atomicAdd(&total[e], c);
+      if (c && i < own) atomicAdd(&before[e], c);
+    }
+  }
   __syncthreads();
-  // Per expert: the choices of earlier blocks, and of all.  A thread has
-  // neighbouring experts, for the scan over them.
+  // A thread has neighbouring experts, for the scan over them.
   constexpr int kPerThread = kMaxExperts / kThreads;
-  const int used = static_cast<int>(ceil_div(p.experts, static_cast<int64_t>(kThreads)));  // experts per thread
-  int32_t before[kPerThread], all[kPerThread];
+  const int used = (p.experts + kThreads - 1) / kThreads;  // experts per thread
+  int32_t all[kPerThread];
   int32_t sum = 0, padded_sum = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     const int e = tid * used + i;
-    before[i] = all[i] = 0;
+    all[i] = 0;
     if (i >= used || e >= p.experts) continue;
-    if (p.blocks == 1) {
+    if (p.blocks > 1) {
+      all[i] = total[e];
+    } else {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) all[i] += next[w][e];
-    } else {
-      for (int b = 0; b < p.blocks; ++b) {
-        const int32_t c = p.counts[static_cast<int64_t>(b) * p.experts + e];
-        all[i] += c;
-        if (b < static_cast<int>(blockIdx.x)) before[i] += c;
-      }
     }
     sum += all[i];
-    padded_sum += static_cast<int32_t>(ceil_div(all[i], static_cast<int64_t>(kSegmentPad))) * kSegmentPad;
+    padded_sum += (all[i] + kSegmentPad - 1) / kSegmentPad * kSegmentPad;
   }
   int32_t scan = sum, padded_scan = padded_sum;
 #pragma unroll
@@ -134,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
   for (int i = 0; i < kPerThread; ++i) {
     const int e = tid * used + i;
     if (i >= used || e >= p.experts) continue;
-    int32_t at = row + before[i];
+    int32_t at = row + before[e];
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       const int32_t c = next[w][e];
@@ -142,8 +150,8 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
       at += c;
     }
     row += all[i];
-    padded += static_cast<int32_t>(ceil_div(all[i], static_cast<int64_t>(kSegmentPad))) * kSegmentPad;
-    total[e + 1] = row;
+    padded += (all[i] + kSegmentPad - 1) / kSegmentPad * kSegmentPad;
+    if (e + 1 == p.experts) total[p.experts] = row;
     if (blockIdx.x == 0) {
       p.offsets[e + 1] = row;
       p.padded_offsets[e + 1] = padded;
@@ -155,6 +163,7 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
   while ((1 << bits) <= p.experts) ++bits;
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
+    if (first + 64 * i >= p.choices) break;  // (the whole wave)
     const int e = mine[i];
     uint64_t same = ~0ull;
     for (int b = 0; b < bits; ++b) {
@@ -184,9 +193,12 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
 template <int DT, bool kVec>
 struct Piece {
   static constexpr int kElements = kVec ? 16 / element_bytes<DT>() : 1;
+  // kStream: a row that is read once
+  template <bool kStream>
   static __device__ __forceinline__ void load(const uint8_t* row, int64_t piece, float (&f)[kElements]) {
     if (kVec) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(row + piece * 16);
+      const u32x4* at = reinterpret_cast<const u32x4*>(row + piece * 16);
+      const u32x4 v = kStream ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
       for (int i = 0; i < kElements; ++i) f[i] = DT == FSH_DT_F32 ? u32_as_f32(v[i % 4]) : half_of_pair<DT>(v[i / 2 % 4], i % 2);
     } else {
@@ -197,9 +209,9 @@ struct Piece {
     if constexpr (!kVec) {
       store_element<DT>(row, piece, f[0]);
     } else if constexpr (DT == FSH_DT_F32) {
-      *reinterpret_cast<f32x4*>(row + piece * 16) = f32x4{f[0], f[1], f[2], f[3]};
+      __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4*>(row + piece * 16));
     } else {
-      store_raw8<DT>(row + piece * 16, f, 8, true);
+      __builtin_nontemporal_store(pack8<DT>(f), reinterpret_cast<u32x4*>(row + piece * 16));
     }
   }
 };
@@ -244,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void expert_dispatch_kernel(const RowsPar
   }
   if (piece >= p.pieces) return;
   float f[P::kElements];
-  P::load(p.x + token * p.row_bytes, piece, f);
+  P::template load<false>(p.x + token * p.row_bytes, piece, f);
   for (int j = 0; j < p.top_k; ++j) {
     const int64_t row = p.position[token * p.top_k + j];
     if (row >= 0) P::store(p.out + row * p.row_bytes, piece, f);
@@ -268,7 +280,7 @@ __global__ __launch_bounds__(kThreads) void expert_combine_kernel(const RowsPara
       for (int i = 0; i < P::kElements; ++i) f[j][i] = 0.0f;
       if (row >= 0) {
         w[j] = weight_of(p, choice);
-        P::load(p.rows + row * p.row_bytes, piece, f[j]);
+        P::template load<true>(p.rows + row * p.row_bytes, piece, f[j]);
       }
     }
 #pragma unroll
@@ -280,8 +292,8 @@ __global__ __launch_bounds__(kThreads) void expert_combine_kernel(const RowsPara
   P::store(p.out + token * p.row_bytes, piece, sum);
 }
 
-// One token: its gradient's pieces stay in registers a slab at a time while the
-// choices' rows pass; the dot products are joined over the workgroup in a fixed order.
+// One token: a piece of its gradient is read once for eight choices, whose rows are
+// in flight together; the dot products are joined over the workgroup in a fixed order.
 constexpr int kMaxTopK = 64;
 template <int DT, bool kVec>
 __global__ __launch_bounds__(kThreads) void expert_combine_backward_kernel(const RowsParams p) {
@@ -293,25 +305,39 @@ __global__ __launch_bounds__(kThreads) void expert_combine_backward_kernel(const
     return;
   }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int j = 0; j < p.top_k; ++j) {
-    const int64_t choice = token * p.top_k + j, row = p.position[choice];
-    float dot = 0.0f;
-    if (row >= 0) {
-      const float w = weight_of(p, choice);
-      for (int64_t piece = threadIdx.x; piece < p.pieces; piece += kThreads) {
-        float g[P::kElements], f[P::kElements];
-        P::load(p.x + token * p.row_bytes, piece, g);
-        P::load(p.rows + row * p.row_bytes, piece, f);
+  for (int j0 = 0; j0 < p.top_k; j0 += 8) {
+    int64_t row[8];
+    float w[8], dot[8];
 #pragma unroll
-        for (int i = 0; i < P::kElements; ++i) {
-          dot = __builtin_fmaf(g[i], f[i], dot);
-          g[i] *= w;
-        }
-        P::store(p.out + row * p.row_bytes, piece, g);
-      }
+    for (int j = 0; j < 8; ++j) {
+      const int64_t choice = token * p.top_k + j0 + j;
+      row[j] = j0 + j < p.top_k ? p.position[choice] : -1;
+      w[j] = row[j] >= 0 ? weight_of(p, choice) : 0.0f;
+      dot[j] = 0.0f;
     }
-    dot = wave_sum_f32(dot);
-    if (lane == 0) dots[wave][j] = dot;
+    for (int64_t piece = threadIdx.x; piece < p.pieces; piece += kThreads) {
+      float g[P::kElements], f[8][P::kElements];
+      P::template load<false>(p.x + token * p.row_bytes, piece, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (row[j] >= 0) P::template load<true>(p.rows + row[j] * p.row_bytes, piece, f[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (row[j] >= 0) {
+          float out[P::kElements];
+#pragma unroll
+          for (int i = 0; i < P::kElements; ++i) {
+            dot[j] = __builtin_fmaf(g[i], f[j][i], dot[j]);
+            out[i] = g[i] * w[j];
+          }
+          P::store(p.out + row[j] * p.row_bytes, piece, out);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float sum = wave_sum_f32(dot[j]);
+      if (lane == 0 && j0 + j < p.top_k) dots[wave][j0 + j] = sum;
+    }
   }
   __syncthreads();
   const int j = threadIdx.x;

@@ -84,25 +84,16 @@ __device__ __forceinline__ void store_element(void* base, int64_t i, float f) {
   if (DT == FSH_DT_F32) static_cast<float*>(base)[i] = f;
   else static_cast<uint16_t*>(base)[i] = static_cast<uint16_t>(round_to_16_bits(f, DT));
 }
-// Elements [0, count) of eight to `at`; `vec` as above.
+// Eight floats to 16-bit elements.
 template <int DT>
-__device__ __forceinline__ void store_raw8(uint8_t* at, const float (&f)[8], int64_t count, bool vec) {
-  if (vec && count >= 8) {
-    if (DT == FSH_DT_F32) {
-      reinterpret_cast<f32x4*>(at)[0] = f32x4{f[0], f[1], f[2], f[3]};
-      reinterpret_cast<f32x4*>(at)[1] = f32x4{f[4], f[5], f[6], f[7]};
-    } else if (DT == FSH_DT_BF16) {
-      *reinterpret_cast<u32x4*>(at) = pack8_bf16(f);
-    } else {
-      u32x4 w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = f32_to_f16_bits(f[2 * j]) | (f32_to_f16_bits(f[2 * j + 1]) << 16);
-      *reinterpret_cast<u32x4*>(at) = w;
-    }
+__device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
+  if constexpr (DT == FSH_DT_BF16) {
+    return pack8_bf16(f);
   } else {
+    u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < count) store_element<DT>(at, i, f[i]);
+    for (int j = 0; j < 4; ++j) w[j] = f32_to_f16_bits(f[2 * j]) | (f32_to_f16_bits(f[2 * j + 1]) << 16);
+    return w;
   }
 }
 
@@ -127,14 +118,52 @@ __device__ __forceinline__ uint32_t mx_quantize8(const float (&f)[8], float scal
   w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
   return w;
 }
-__device__ __forceinline__ uint32_t max_magnitude8(const float (&f)[8]) {
-  uint32_t m = 0;
+// Eight elements as they lie in memory: 16-bit magnitudes compare as whole
+// numbers, and pairs of bf16 or fp16 convert without being taken apart.
+template <int DT>
+__device__ __forceinline__ uint32_t magnitude_bits_to_f32(uint32_t m) {  // of a 16-bit magnitude, or fp32 bits
+  if (DT == FSH_DT_F32) return m;
+  return DT == FSH_DT_F16 ? f32_as_u32(f16_bits_to_f32(m)) : m << 16;
+}
+__device__ __forceinline__ uint32_t larger_half(uint32_t pair) { return (pair & 0xFFFFu) > (pair >> 16) ? pair & 0xFFFFu : pair >> 16; }
+template <int DT>
+__device__ __forceinline__ uint32_t max_magnitude8(const Raw8<DT>& r) {  // in the element's own bits
+  if constexpr (DT == FSH_DT_F32) {
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t b = f32_as_u32(f[i]) & 0x7FFFFFFFu;
-    m = b > m ? b : m;
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t b = r.v[i / 4][i % 4] & 0x7FFFFFFFu;
+      m = b > m ? b : m;
+    }
+    return m;
+  } else {
+    const u32x4 a = r.v[0] & 0x7FFF7FFFu;
+    return larger_half(pk_max_u16(pk_max_u16(a.x, a.y), pk_max_u16(a.z, a.w)));
   }
-  return m;
+}
+// Two neighbouring elements (16-bit: a dword that holds both) to byte kByte of `old`.
+template <int DT, int kByte>
+__device__ __forceinline__ uint32_t mx_quantize_pair(uint32_t old, uint32_t pair, float scale) {
+  if constexpr (DT == FSH_DT_F16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, pair), scale, kByte);
+  } else {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, pair), scale, kByte);
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint32_t mx_quantize8(const Raw8<DT>& r, float scale) {
+  if constexpr (DT == FSH_DT_F32) {
+    float f[8];
+    unpack_raw8<DT>(r, f);
+    return mx_quantize8(f, scale);
+  } else {
+    uint32_t w = 0;
+    w = mx_quantize_pair<DT, 0>(w, r.v[0].x, scale);
+    w = mx_quantize_pair<DT, 1>(w, r.v[0].y, scale);
+    w = mx_quantize_pair<DT, 2>(w, r.v[0].z, scale);
+    return mx_quantize_pair<DT, 3>(w, r.v[0].w, scale);
+  }
 }
 
 // Experts: the rows of expert e are [offsets[e], offsets[e + 1]) of the sorted

@@ -117,14 +117,12 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void mxfp4_few_rows_kernel(const
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int i = i0 + u * static_cast<int>(blockDim.x), x_row = i / pieces, col = (i - x_row * pieces) * 8;
-        float f[8];
-        unpack_raw8<DT>(raw[u], f);
-        uint32_t m = max_magnitude8(f);
+        uint32_t m = max_magnitude8(raw[u]);
         m = dpp_max_u32<0xB1, 0xF>(m);
         m = dpp_max_u32<0x4E, 0xF>(m);
-        const uint32_t byte = mx_scale_byte(m);
+        const uint32_t byte = mx_scale_byte(magnitude_bits_to_f32<DT>(m));
         if (i >= total) break;
-        *reinterpret_cast<uint32_t*>(x_data + x_row * x_pitch + col / 2) = mx_quantize8(f, mx_scale(byte));
+        *reinterpret_cast<uint32_t*>(x_data + x_row * x_pitch + col / 2) = mx_quantize8(raw[u], mx_scale(byte));
         if ((i & 3) == 0) x_scales[x_row * s_pitch + col / kMxBlock] = static_cast<uint8_t>(byte);
       }
     }

@@ -42,18 +42,19 @@ struct MxQuantParams {
 
 // A lane's eight columns of a row, 16 lanes 128 columns, quantized: the data of
 // the lane and, in lane 0 of the 16, the four scale bytes.
-__device__ __forceinline__ uint32_t quantize_row_piece(const float (&f)[8], uint32_t* scales) {
-  uint32_t m = max_magnitude8(f);
+template <int DT>
+__device__ __forceinline__ uint32_t quantize_row_piece(const Raw8<DT>& raw, uint32_t* scales) {
+  uint32_t m = max_magnitude8(raw);
   m = dpp_max_u32<0xB1, 0xF>(m);  // quad_perm [1,0,3,2]
   m = dpp_max_u32<0x4E, 0xF>(m);  // quad_perm [2,3,0,1]: the four lanes of a run
-  const uint32_t byte = mx_scale_byte(m);
+  const uint32_t byte = mx_scale_byte(magnitude_bits_to_f32<DT>(m));
   // lanes 4, 8 and 12 of the 16 to lane 0 (row_shl)
   uint32_t all = byte;
   all |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(byte), 0x104, 0xF, 0xF, true)) << 8;
   all |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(byte), 0x108, 0xF, 0xF, true)) << 16;
   all |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(byte), 0x10C, 0xF, 0xF, true)) << 24;
   *scales = all;
-  return mx_quantize8(f, mx_scale(byte));
+  return mx_quantize8(raw, mx_scale(byte));
 }
 
 // Stores what quantize_row_piece gave for columns [col, col + 8) of table row `row`.
@@ -80,10 +81,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows_kernel(const MxQ
 #pragma unroll
   for (int i = 0; i < kRowTileRows / 4; ++i) {
     const int64_t row = tile_r * kRowTileRows + 4 * i + wave;
-    float f[8];
-    unpack_raw8<DT>(raw[i], f);
     uint32_t scales;
-    const uint32_t data = quantize_row_piece(f, &scales);
+    const uint32_t data = quantize_row_piece(raw[i], &scales);
     if (row < p.rows) store_row_piece4(p, row, col, data, scales);
   }
 }
@@ -129,10 +128,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_columns_kernel(const 
 #pragma unroll
     for (int i = 0; i < kTile / 16; ++i) {
       const int r = 16 * i + (tid >> 4);
-      float f[8];
-      unpack_raw8<DT>(raw[i], f);
       uint32_t scales;
-      const uint32_t data = quantize_row_piece(f, &scales);
+      const uint32_t data = quantize_row_piece(raw[i], &scales);
       if (r < rows_left) store_row_piece4(p, batch * p.rows + r0 + r, col, data, scales);
     }
   }
@@ -140,40 +137,61 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_columns_kernel(const 
   __syncthreads();
 
   const int pair = tid & 63, block = tid >> 6;
-  float f[2][32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const uint8_t* at = tile + (block * 32 + i) * kPitch + pair * 2 * kElement;
-    if (DT == FSH_DT_F32) {
-      const f32x2 v = *reinterpret_cast<const f32x2*>(at);
-      f[0][i] = v.x;
-      f[1][i] = v.y;
-    } else {
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(at);
-      f[0][i] = half_of_pair<DT>(v, 0);
-      f[1][i] = half_of_pair<DT>(v, 1);
-    }
-  }
   u32x4 data[2];
   uint32_t bytes[2];
   float sums[2] = {0.0f, 0.0f};
+  const uint8_t* const columns = tile + block * 32 * kPitch + pair * 2 * kElement;
+  if constexpr (DT == FSH_DT_F32) {
+    f32x2 f[32];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t m = 0;
+    for (int i = 0; i < 32; ++i) f[i] = *reinterpret_cast<const f32x2*>(columns + i * kPitch);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const uint32_t b = f32_as_u32(f[c][i]) & 0x7FFFFFFFu;
-      m = b > m ? b : m;
-      sums[c] += f[c][i];
+    for (int c = 0; c < 2; ++c) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t b = f32_as_u32(f[i][c]) & 0x7FFFFFFFu;
+        m = b > m ? b : m;
+      }
+      bytes[c] = mx_scale_byte(m);
+      const float scale = mx_scale(bytes[c]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = f[8 * w + i][c];
+        data[c][w] = mx_quantize8(g, scale);
+      }
+      if (p.column_sums) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sums[c] += f[i][c];
+      }
     }
-    bytes[c] = mx_scale_byte(m);
-    const float scale = mx_scale(bytes[c]);
+  } else {
+    uint32_t f[32], m = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float g[8];
+    for (int i = 0; i < 32; ++i) f[i] = *reinterpret_cast<const uint32_t*>(columns + i * kPitch);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) g[i] = f[c][8 * w + i];
-      data[c][w] = mx_quantize8(g, scale);
+    for (int i = 0; i < 32; ++i) m = pk_max_u16(m, f[i] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bytes[c] = mx_scale_byte(magnitude_bits_to_f32<DT>(c ? m >> 16 : m & 0xFFFFu));
+      const float scale = mx_scale(bytes[c]);
+      constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;  // the halves of two rows that are a column's
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t pick = c ? kHigh : kLow;
+        uint32_t d = 0;
+        d = mx_quantize_pair<DT, 0>(d, __builtin_amdgcn_perm(f[8 * w + 1], f[8 * w], pick), scale);
+        d = mx_quantize_pair<DT, 1>(d, __builtin_amdgcn_perm(f[8 * w + 3], f[8 * w + 2], pick), scale);
+        d = mx_quantize_pair<DT, 2>(d, __builtin_amdgcn_perm(f[8 * w + 5], f[8 * w + 4], pick), scale);
+        d = mx_quantize_pair<DT, 3>(d, __builtin_amdgcn_perm(f[8 * w + 7], f[8 * w + 6], pick), scale);
+        data[c][w] = d;
+      }
+      if (p.column_sums) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sums[c] += half_of_pair<DT>(f[i], c);
+      }
     }
   }
   __syncthreads();
@@ -208,20 +226,32 @@ struct MxDequantParams {
   const uint8_t* q;
   const uint8_t* s;
   uint8_t* out;
-  int64_t rows, cols, ldq, ldo, groups;  // groups of eight columns per row
+  int64_t rows, cols, ldq, ldo, groups;  // groups of 16 bytes' columns per row
   int32_t vec;
 };
+// A thread writes 16 bytes, past the caches: 8192 x 14336 to bf16 69 us with plain
+// stores, 46 so; with 32 bytes of fp32 in two stores they do harm (14336 x 4096 55 / 91).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const MxDequantParams p) {
+  constexpr int kColumns = 16 / element_bytes<DT>();
   const int64_t total = p.rows * p.groups;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t row = i / p.groups, col = (i - row * p.groups) * 8;
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p.q + row * p.ldq + col / 2);
+    const int64_t row = i / p.groups, col = (i - row * p.groups) * kColumns;
+    const uint8_t* at = p.q + row * p.ldq + col / 2;
+    const uint32_t w = kColumns == 8 ? *reinterpret_cast<const uint32_t*>(at) : *reinterpret_cast<const uint16_t*>(at);
     const float scale = mx_scale(p.s[((col / kMxColumns) * p.rows + row) * 8 + (col % kMxColumns) / kMxBlock]);
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
     const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
     const float f[8] = {a.x * scale, a.y * scale, b.x * scale, b.y * scale, c.x * scale, c.y * scale, d.x * scale, d.y * scale};
-    store_raw8<DT>(p.out + (row * p.ldo + col) * element_bytes<DT>(), f, p.cols - col, p.vec);
+    uint8_t* out = p.out + (row * p.ldo + col) * element_bytes<DT>();
+    if (p.vec && col + kColumns <= p.cols) {
+      if constexpr (DT == FSH_DT_F32) __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4*>(out));
+      else __builtin_nontemporal_store(pack8<DT>(f), reinterpret_cast<u32x4*>(out));
+    } else {
+#pragma unroll
+      for (int c2 = 0; c2 < kColumns; ++c2)
+        if (col + c2 < p.cols) store_element<DT>(out, c2, f[c2]);
+    }
   }
 }
 
@@ -343,14 +373,14 @@ FSH_API int fsh_mxfp4_dequantize(const void* q_dev, const void* s_dev, int64_t r
   if (!known_dtype(dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, dtype);
   if (!q_dev || !s_dev || !out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
   if (ldo < cols) return fail(FSH_EINVAL, "%s: ldo %lld < cols %lld", who, (long long)ldo, (long long)cols);
-  if (!aligned(q_dev, 4) || !aligned(out_dev, dtype_bytes(dtype))) return fail(FSH_ENOTSUP, "%s: misaligned pointer", who);
+  if (!aligned(q_dev, 16) || !aligned(out_dev, dtype_bytes(dtype))) return fail(FSH_ENOTSUP, "%s: misaligned pointer", who);
   MxDequantParams p;
   p.q = static_cast<const uint8_t*>(q_dev);
   p.s = static_cast<const uint8_t*>(s_dev);
   p.out = static_cast<uint8_t*>(out_dev);
   p.rows = rows; p.cols = cols; p.ldo = ldo;
   p.ldq = ceil_div(cols, (int64_t)kMxColumns) * (kMxColumns / 2);
-  p.groups = ceil_div(cols, (int64_t)8);
+  p.groups = ceil_div(cols, (int64_t)(16 / dtype_bytes(dtype)));
   p.vec = aligned(out_dev, 16) && ldo * dtype_bytes(dtype) % 16 == 0;
   const int64_t blocks = ceil_div(rows * p.groups, (int64_t)kThreads);
   const dim3 grid(static_cast<uint32_t>(blocks < kMaxGrid ? blocks : kMaxGrid)), block(kThreads);
