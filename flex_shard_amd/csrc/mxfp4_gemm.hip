@@ -18,6 +18,11 @@ int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t
   s.tiles_n = static_cast<int32_t>(tiles_n);
   s.items = static_cast<int32_t>(tiles * batch);
   s.items_per_xcd = (s.items + kXcds - 1) / kXcds;
+  const int32_t eighth = static_cast<int32_t>(ceil_div(tiles, static_cast<int64_t>(kXcds)));
+  s.run = eighth < kGroupTilesM ? kGroupTilesM : eighth;
+  s.by_span = Divisor::of(static_cast<uint32_t>(kGroupTilesM * tiles_n));
+  s.by_run = Divisor::of(static_cast<uint32_t>(s.run));
+  s.by_round = Divisor::of(static_cast<uint32_t>(s.run * batch));
   int64_t blocks = static_cast<int64_t>(s.items_per_xcd) * kXcds;
   if (Cfg::kResident) {
     const int64_t units = compute_units(), resident = units >= kXcds ? units / kXcds * kXcds : kXcds;
@@ -196,13 +201,7 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   p.experts = q.experts; p.top_k = q.top_k;
   p.offsets = p.padded_offsets = q.offsets_dev;
   p.source = q.source_dev;
-  if (p.top_k > 0) {
-    // ceil(2^(31 + b) / top_k), 2^b >= top_k: exact for choices below 2^31
-    int bits = 0;
-    while ((1LL << bits) < p.top_k) ++bits;
-    p.top_k_shift = 31 + bits;
-    p.top_k_factor = static_cast<uint32_t>(((1ULL << p.top_k_shift) + p.top_k - 1) / p.top_k);
-  }
+  if (p.top_k > 0) p.by_top_k = Divisor::of(static_cast<uint32_t>(p.top_k));
   const MxProblem problem = segments ? kMxRows : q.mode == FSH_MXFP4_OVER_ROWS ? kMxOverRows : kMxDense;
   const int64_t units = compute_units();
   switch (mx_tile_kind(p, problem, units > 0 ? units : 256)) {

@@ -49,10 +49,29 @@ enum MxProblem {
   kMxOverRows,   // per expert the product over its own (padded) columns of a and b: [experts][m][n]
 };
 
+// Division by a number that the host knows: x / d is x * factor >> shift for x
+// below 2^31, with factor = ceil(2^shift / d) and shift = 31 + ceil(log2 d).
+struct Divisor {
+  uint32_t factor;
+  int32_t shift;
+  __host__ static Divisor of(uint32_t d) {
+    int32_t b = 0;
+    while ((1ULL << b) < d) ++b;
+    return Divisor{static_cast<uint32_t>(((1ULL << (31 + b)) + d - 1) / d), 31 + b};
+  }
+  __device__ __forceinline__ int quotient(int x) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(x)) * factor >> shift);
+  }
+};
+
 // The order of the tiles: XCD x takes the run [x, x + 1) * items_per_xcd of an order in which kGroupTilesM tile rows are
-// walked together, so that the tiles that its compute units hold at a time share operands in its L2.
+// walked together, so that the tiles that its compute units hold at a time share operands in its L2.  Products of
+// different lengths (kMxOverRows) are cut into runs of `run` tiles, and the first runs of all experts come before the
+// second ones: every XCD then has an eighth of every expert, whatever their rows.
 struct MxSchedule {
   int32_t tiles_m, tiles_n, items, items_per_xcd;  // items: tiles of all matrices
+  int32_t run;
+  Divisor by_span, by_run, by_round;  // kGroupTilesM tile rows, a run, the runs of all experts
 };
 
 struct MxGemmParams {
@@ -69,8 +88,7 @@ struct MxGemmParams {
   const int32_t* offsets;         // [experts + 1]
   const int32_t* padded_offsets;  // [experts + 1] (kMxOverRows)
   const int32_t* source;          // kMxRows: row r of the segments is row source[r] / top_k of a, or null
-  uint32_t top_k_factor;          // choice / top_k is choice * top_k_factor >> top_k_shift
-  int32_t top_k_shift;
+  Divisor by_top_k;
   MxSchedule schedule;
 };
 
@@ -171,10 +189,17 @@ __device__ __forceinline__ bool place_of_turn(const MxGemmParams& p, const MxSch
   const int item = id % kXcds * schedule.items_per_xcd + id / kXcds;
   if (id / kXcds >= schedule.items_per_xcd || item >= schedule.items) return false;
   const int tiles = schedule.tiles_m * schedule.tiles_n;
-  const int batch = kProblem == kMxOverRows ? item / tiles : 0;
-  const int t = item - batch * tiles, span = kGroupTilesM * schedule.tiles_n, first_m = t / span * kGroupTilesM;
+  int batch = 0, t = item;
+  if (kProblem == kMxOverRows) {
+    const int round = schedule.by_round.quotient(item), first = round * schedule.run, left = tiles - first;
+    const int run = left < schedule.run ? left : schedule.run, of_round = item - first * p.experts;
+    batch = run == schedule.run ? schedule.by_run.quotient(of_round) : of_round / run;
+    t = first + of_round - batch * run;
+  }
+  const int first_m = schedule.by_span.quotient(t) * kGroupTilesM;
   const int within = t - first_m * schedule.tiles_n, rows = min(schedule.tiles_m - first_m, kGroupTilesM);
-  const int tn = rows == kGroupTilesM ? within / kGroupTilesM : within / rows, tm = first_m + within - tn * rows;
+  static_assert(kGroupTilesM == 4, "the divisions");
+  const int tn = rows == 4 ? within / 4 : rows == 3 ? within / 3 : rows == 2 ? within / 2 : within, tm = first_m + within - tn * rows;
   place->zero = false;
   place->out_offset = 0;
   place->first_step = 0;
@@ -281,16 +306,13 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
   const uint8_t* scale_src[kScaleRequests];
   int64_t scale_step[kScaleRequests];
   uint32_t scale_lds[kScaleRequests];
-  const auto token_of = [&](int choice) FSH_INLINE {
-    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(choice)) * p.top_k_factor >> p.top_k_shift);
-  };
   const auto aim = [&](const MxTilePlace& at, const Rows& rows) FSH_INLINE {
     const int64_t a_first = gathered ? 0 : at.row0, b_first = at.b_row0 + at.col0;
     const int b_last = static_cast<int>(p.n - at.col0 < Cfg::BN ? p.n - at.col0 : Cfg::BN) - 1;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (c < kChunksA) {
-        voff[c] = static_cast<uint32_t>(gathered ? token_of(rows.data[c]) : rows.data[c]) * static_cast<uint32_t>(p.lda);
+        voff[c] = static_cast<uint32_t>(gathered ? p.by_top_k.quotient(rows.data[c]) : rows.data[c]) * static_cast<uint32_t>(p.lda);
       } else {
         const int r = Cfg::kChunkRows * (c - kChunksA) + 8 * wave + fill_row;
         voff[c] = static_cast<uint32_t>(r < b_last ? r : b_last) * static_cast<uint32_t>(p.ldb);
@@ -304,7 +326,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
       const int q = kScaleRequests * wave + i, first = 64 * (q >> 1);
       const bool of_a = first < Cfg::BM;
       const int r = first - Cfg::BM + lane;
-      const int row = of_a ? (gathered ? token_of(rows.scales[i]) : rows.scales[i]) : (r < b_last ? r : b_last);
+      const int row = of_a ? (gathered ? p.by_top_k.quotient(rows.scales[i]) : rows.scales[i]) : (r < b_last ? r : b_last);
       scale_voff[i] = static_cast<uint32_t>(row) * 8;
       scale_step[i] = (of_a ? p.a_rows : p.b_rows) * 8;
       scale_src[i] = uniform_ptr((of_a ? p.as + a_first * 8 : p.bs + b_first * 8) + at.first_step * scale_step[i] + 4 * (q & 1));
@@ -333,10 +355,10 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     dma_touch_4(scale_voff[i], scale_src[i] + step * scale_step[i], lds_base + at.scales + scale_lds[i]);
   };
   // Request r of the first kDepth steps of a tile, of kRequests each; then the early chunks of one more.
-  const auto request_first = [&](int steps, auto r_tag) FSH_INLINE {
+  const auto request_first = [&](auto long_enough, int steps, auto r_tag) FSH_INLINE {
     constexpr int d = decltype(r_tag)::value / kRequests, q = decltype(r_tag)::value % kRequests;
     constexpr Place at{d * Cfg::kEarlyBytes, kFirst.late + d * Cfg::kLateBytes, kFirst.scales + d * Cfg::kScaleBytes};
-    if (d < steps) {
+    if (long_enough.value || d == 0 || d < steps) {
       if constexpr (q < kScaleRequests) request_scales(d, at, q);
       else request(d, at, q - kScaleRequests);
     }
@@ -347,7 +369,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
       if (kDepth < steps) request(kDepth, Place{kDepth * Cfg::kEarlyBytes, 0, 0}, c);
   };
   const auto request_all_first = [&](int steps) FSH_INLINE {
-    static_for<kDepth * kRequests>([&](auto r) FSH_INLINE { request_first(steps, r); });
+    static_for<kDepth * kRequests>([&](auto r) FSH_INLINE { request_first(std::false_type{}, steps, r); });
     request_first_early(steps);
   };
 
@@ -411,12 +433,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     const int steps = place.steps;
     // Lane (r = l & 31, g) accumulates, of row r of a block, columns 8 q + 4 g + 0 .. 3, q = 0 .. 3.
     f32x16 acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int t = 0; t < 16; ++t) acc[i][j][t] = 0.0f;
+    constexpr f32x16 kZeros = {};
     // Step 0 has landed; what was queued behind it stays in flight.
     if (kDepth < steps) {
       if (Cfg::kResident && counted_stores) wait_for_dma_loads_but<at_most_63((kDepth - 1) * kRequests + kEarly + Stores::behind_step(0))>();
@@ -444,7 +461,9 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     // and scales of the step at `at`, the next one (quarter 3), or the fragments of
     // this one's next quarter; requests of the iteration that began with step
     // `left`, into that step's slots.
-    const auto quarter = [&](auto s_tag, auto more_tag, auto late_tag, auto early_tag, const Place& at, int left, const Place& freed) FSH_INLINE {
+    const auto quarter = [&](auto s_tag, auto first_tag, auto more_tag, auto late_tag, auto early_tag, const Place& at, int left,
+                             const Place& freed) FSH_INLINE {
+      constexpr bool of_first = decltype(first_tag)::value;
       constexpr int s = decltype(s_tag)::value;
       constexpr bool more = decltype(more_tag)::value, late = decltype(late_tag)::value, early = decltype(early_tag)::value;
 #pragma unroll
@@ -453,7 +472,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
         const u32x4 a = af[s & 1][i], b = bf[s & 1][j];
         const v8i32 av = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
         const v8i32 bv = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv, av, acc[i][j], 4, 4, s, sb[j], s, sa[i]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv, av, s == 0 && of_first ? kZeros : acc[i][j], 4, 4, s, sb[j], s, sa[i]);
         __builtin_amdgcn_sched_barrier(0);
         if (s == 3 && more && m == 0) {
           if (late) {
@@ -495,24 +514,24 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     };
     const auto iteration = [&](int step, auto late, auto early) FSH_INLINE {
       const Place freed = now, next = place_after(now);
-      quarter(q3, yes, late, early, next, step, freed);
+      quarter(q3, no, yes, late, early, next, step, freed);
 #pragma unroll
       for (int i = 0; i < TM; ++i) sa[i] = next_sa[i];
 #pragma unroll
       for (int j = 0; j < TN; ++j) sb[j] = next_sb[j];
-      quarter(q0, yes, late, early, next, step, freed);
-      quarter(q1, yes, late, early, next, step, freed);
-      quarter(q2, yes, late, early, next, step, freed);
+      quarter(q0, no, yes, late, early, next, step, freed);
+      quarter(q1, no, yes, late, early, next, step, freed);
+      quarter(q2, no, yes, late, early, next, step, freed);
       now = next;
     };
-    quarter(q0, yes, no, no, now, 0, now);
-    quarter(q1, yes, no, no, now, 0, now);
-    quarter(q2, yes, no, no, now, 0, now);
+    quarter(q0, yes, yes, no, no, now, 0, now);
+    quarter(q1, yes, yes, no, no, now, 0, now);
+    quarter(q2, yes, yes, no, no, now, 0, now);
     int step = 0;
     for (; step + kDepth + 1 < steps; ++step) iteration(step, yes, yes);
     if (step + kDepth < steps) iteration(step++, yes, no);
     for (; step + 1 < steps; ++step) iteration(step, no, no);
-    quarter(q3, no, no, no, now, 0, now);
+    quarter(q3, no, no, no, no, now, 0, now);
     if (kProblem == kMxDense && tid < Cfg::BN) bias_of_tile[tid] = bias;
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the slots are free
 
@@ -537,10 +556,13 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
     uint8_t* const lane_out = wave_out + (store_row * p.ldo + store_col) * kElement;
     const int64_t row_bytes = p.ldo * kElement;
     u32x4 leaving[Stores::kStores];
-    const auto store_one = [&](int part, int s) FSH_INLINE {
+    // (opaque: the compiler multiplies it out ahead of all tiles otherwise, and spills)
+    int64_t store_bytes = kRowsPerStore * row_bytes;
+    asm volatile("" : "+s"(store_bytes));
+    const auto store_one = [&](auto plain, int part, int s) FSH_INLINE {
       const int row = part / (Cfg::kWaveN / kCols) * 32 + s * kRowsPerStore, col = part % (Cfg::kWaveN / kCols) * kCols;
-      if (row + store_row < rows_left && col + store_col < vec_cols)
-        __builtin_nontemporal_store(leaving[s], reinterpret_cast<u32x4*>(lane_out + row * row_bytes + col * kElement));
+      if (plain.value || (row + store_row < rows_left && col + store_col < vec_cols))
+        __builtin_nontemporal_store(leaving[s], reinterpret_cast<u32x4*>(lane_out + row / kRowsPerStore * store_bytes + col * kElement));
     };
     const auto store_rest = [&](int part) FSH_INLINE {
       const int row = part / (Cfg::kWaveN / kCols) * 32, col = part % (Cfg::kWaveN / kCols) * kCols;
@@ -558,65 +580,70 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
         }
       }
     };
-    static_for<kParts>([&](auto part_tag) FSH_INLINE {
-      constexpr int part = decltype(part_tag)::value;
-      constexpr int i = part / (Cfg::kWaveN / kCols), j0 = part % (Cfg::kWaveN / kCols) * (kCols / 32);
-      // (said to be in accumulation registers up to here: the compiler copies them all out ahead otherwise, and spills)
-      float v[kCols / 32][16];
+    const auto leave = [&](auto plain) FSH_INLINE {
+      static_for<kParts>([&](auto part_tag) FSH_INLINE {
+        constexpr int part = decltype(part_tag)::value;
+        constexpr int i = part / (Cfg::kWaveN / kCols), j0 = part % (Cfg::kWaveN / kCols) * (kCols / 32);
+        // (said to be in accumulation registers up to here: the compiler copies them all out ahead otherwise, and spills)
+        float v[kCols / 32][16];
 #pragma unroll
-      for (int j = 0; j < kCols / 32; ++j) {
-        asm volatile("" : "+a"(acc[i][j0 + j]));
+        for (int j = 0; j < kCols / 32; ++j) {
+          asm volatile("" : "+a"(acc[i][j0 + j]));
 #pragma unroll
-        for (int t = 0; t < 16; ++t) v[j][t] = acc[i][j0 + j][t];
-      }
-      if (kProblem == kMxDense && p.bias) {
-#pragma unroll
-        for (int j = 0; j < kCols / 32; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 add = *reinterpret_cast<const f32x4*>(bias_of_tile + wn * Cfg::kWaveN + 32 * (j0 + j) + 8 * q + 4 * group);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) v[j][4 * q + t] += add[t];
-          }
-      }
-      // (the part before leaves between the conversions)
-      uint32_t words[Stores::kWords];
-      constexpr int kPerStore = Stores::kWords / Stores::kStores;
-      static_for<Stores::kStores>([&](auto s_tag) FSH_INLINE {
-        constexpr int s = decltype(s_tag)::value;
-#pragma unroll
-        for (int w = s * kPerStore; w < (s + 1) * kPerStore; ++w) {
-          if (DT == FSH_DT_F32) words[w] = f32_as_u32(v[0][w]);
-          else if (DT == FSH_DT_BF16) words[w] = pack_bf16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
-          else words[w] = f32_to_f16_bits(v[w / 8][2 * w % 16]) | (f32_to_f16_bits(v[w / 8][2 * w % 16 + 1]) << 16);
+          for (int t = 0; t < 16; ++t) v[j][t] = acc[i][j0 + j][t];
         }
+        if (kProblem == kMxDense && p.bias) {
+#pragma unroll
+          for (int j = 0; j < kCols / 32; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 add = *reinterpret_cast<const f32x4*>(bias_of_tile + wn * Cfg::kWaveN + 32 * (j0 + j) + 8 * q + 4 * group);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) v[j][4 * q + t] += add[t];
+            }
+        }
+        // (the part before leaves between the conversions)
+        uint32_t words[Stores::kWords];
+        constexpr int kPerStore = Stores::kWords / Stores::kStores;
+        static_for<Stores::kStores>([&](auto s_tag) FSH_INLINE {
+          constexpr int s = decltype(s_tag)::value;
+#pragma unroll
+          for (int w = s * kPerStore; w < (s + 1) * kPerStore; ++w) {
+            if (DT == FSH_DT_F32) words[w] = f32_as_u32(v[0][w]);
+            else if (DT == FSH_DT_BF16) words[w] = pack_bf16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
+            else words[w] = f32_to_f16_bits(v[w / 8][2 * w % 16]) | (f32_to_f16_bits(v[w / 8][2 * w % 16 + 1]) << 16);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          if (part > 0) store_one(plain, part - 1, s);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        if (part > 0 && !plain.value) store_rest(part - 1);
+        wave_lds_sync();
+        constexpr int kPerPiece = kElement;  // dwords of four columns, less what 16 bits save: 2 or 4
+#pragma unroll
+        for (int piece = 0; piece < Stores::kWords / kPerPiece; ++piece) {
+          uint8_t* at = region + frag_row * Cfg::kPitch + (32 * (piece / 4) + 8 * (piece % 4) + 4 * group) * kElement;
+          const uint32_t* w = words + piece * kPerPiece;
+          if constexpr (kElement == 4) *reinterpret_cast<u32x4*>(at) = u32x4{w[0], w[1], w[2], w[3]};
+          else *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
+        }
+        wave_lds_sync();
+#pragma unroll
+        for (int s = 0; s < Stores::kStores; ++s)
+          leaving[s] = *reinterpret_cast<const u32x4*>(region + (s * kRowsPerStore + store_row) * Cfg::kPitch + store_col * kElement);
         __builtin_amdgcn_sched_barrier(0);
-        if (part > 0) store_one(part - 1, s);
+        if (plain.value || request_next)
+          static_for<2 * kRequests>([&](auto r) FSH_INLINE {
+            if constexpr (Cfg::kResident && Stores::part_of_request(decltype(r)::value) == part) request_first(plain, place.steps, r);
+          });
         __builtin_amdgcn_sched_barrier(0);
       });
-      if (part > 0) store_rest(part - 1);
-      wave_lds_sync();
-      constexpr int kPerPiece = kElement;  // dwords of four columns, less what 16 bits save: 2 or 4
-#pragma unroll
-      for (int piece = 0; piece < Stores::kWords / kPerPiece; ++piece) {
-        uint8_t* at = region + frag_row * Cfg::kPitch + (32 * (piece / 4) + 8 * (piece % 4) + 4 * group) * kElement;
-        const uint32_t* w = words + piece * kPerPiece;
-        if constexpr (kElement == 4) *reinterpret_cast<u32x4*>(at) = u32x4{w[0], w[1], w[2], w[3]};
-        else *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
-      }
-      wave_lds_sync();
-#pragma unroll
-      for (int s = 0; s < Stores::kStores; ++s)
-        leaving[s] = *reinterpret_cast<const u32x4*>(region + (s * kRowsPerStore + store_row) * Cfg::kPitch + store_col * kElement);
-      __builtin_amdgcn_sched_barrier(0);
-      if (request_next)
-        static_for<2 * kRequests>([&](auto r) FSH_INLINE {
-          if constexpr (Cfg::kResident && Stores::part_of_request(decltype(r)::value) == part) request_first(place.steps, r);
-        });
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    static_for<Stores::kStores>([&](auto s) FSH_INLINE { store_one(kParts - 1, decltype(s)::value); });
-    store_rest(kParts - 1);
+      static_for<Stores::kStores>([&](auto s) FSH_INLINE { store_one(plain, kParts - 1, decltype(s)::value); });
+      if (!plain.value) store_rest(kParts - 1);
+    };
+    // A whole tile before a tile of some length, as most are, leaves without a branch.
+    if (Cfg::kResident && whole && request_next && kDepth < place.steps) leave(yes);
+    else leave(no);
     counted_stores = whole;
     if (!more_tiles) return;
     // The staging's slot is the third step's: every wave has to be done with it.
