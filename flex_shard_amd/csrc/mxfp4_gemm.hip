@@ -44,6 +44,7 @@ int launch_mx_tiles(MxGemmParams& p, int64_t tiles_m, int64_t batch, hipStream_t
 template <typename Cfg>
 int64_t segment_tiles(const MxGemmParams& p) { return p.m / Cfg::BM + p.experts + 1; }
 
+// (see mx_tile_kind for what each is good at)
 using MxLarge = MxTile<2, 2, 4, 4, 2, 5, true>;     // 256 x 256, one workgroup per compute unit
 using MxMid = MxTile<2, 2, 2, 2, 2, 0, false>;      // 128 x 128, two
 using MxMidDeep = MxTile<2, 2, 2, 2, 4, 0, false>;  // 128 x 128, one, four steps in flight
@@ -59,18 +60,18 @@ int launch_mx(MxGemmParams& p, MxProblem problem, hipStream_t stream) {
 
 // Which tiles a product takes: those with the lowest estimated time, from what
 // the four measured (us, 64 x 64 / 128 x 128 / 128 x 128 deep / 256 x 256):
-//   48 x 14336, k 4096      8.2  14.8  11.1  24.2    128 x 14336, k 4096    11.0  15.2  11.6  23.8
-//   256 x 1024, k 4096      6.5  10.0   9.7  23.4    512 x 4096, k 4096     10.9  14.9  11.7  24.4
-//   64 x 4096, k 14336     16.0  39.3  24.2  63.5    445 x 3932, k 11071    24.3  35.8  25.3  60.4
-//   1000 x 5120, k 2048    15.7  12.4  15.4  18.0    1000 x 2048, k 5120    13.0  18.0  13.2  29.1
-//   3000 x 1024, k 1500     9.5   8.2   7.8  14.5    2048 x 2048, k 2048    12.7  10.2   9.1  16.8
-//   1024 x 4096, k 8192    35.0  28.8  22.6  42.2    512 x 14336, k 4096    33.7  22.0  24.0  26.9
-//   2048 x 4096, k 4096    36.9  22.6  24.3  27.2    4096 x 4096, k 4096    67.8  41.4  46.4  35.3
-//   4096 x 14336, k 4096    221   154   173   126    14336 x 4096, k 1000   92.5  51.8  66.5  46.7
+//   48 x 14336, k 4096      7.8  14.4  10.6  24.8    128 x 14336, k 4096    10.3  15.0  11.1  24.7
+//   256 x 1024, k 4096      6.3  10.0   9.6  24.6    512 x 4096, k 4096     10.7  14.6  11.2  25.3
+//   64 x 4096, k 14336     15.3  39.4  24.2  64.1    445 x 3932, k 11071    23.4  36.6  26.4  71.0
+//   1000 x 5120, k 2048    14.9  11.5  14.3  17.1    1000 x 2048, k 5120    12.8  18.0  13.1  29.8
+//   3000 x 1024, k 1500     8.6   7.9   7.4  15.3    2048 x 2048, k 2048    11.8   9.5   8.9  17.3
+//   1024 x 4096, k 8192    36.6  29.6  25.2  41.8    512 x 14336, k 4096    34.1  21.0  26.2  25.9
+//   2048 x 4096, k 4096    35.4  22.2  24.9  27.3    4096 x 4096, k 4096    69.2  42.9  47.6  35.7
+//   4096 x 14336, k 4096    221   136   155   120    14336 x 4096, k 1000   83.0  50.0  66.1  50.8
 // Rows of 32 experts, 7168 to 2048 columns, by rows per expert:
-//   4   51.2  49.4  55.2  73.5    64  74.2  52.3  57.0  66.6    128  107  93.9  84.1  70.9    512  292  217  244  176
+//   4   50.5  50.3  56.8  77.1    64  79.4  53.9  58.6  66.9    128  111  93.8  85.4  72.2    512  288  209  221  174
 // Over rows of 32 experts, [2048, 7168] each, by rows per expert:
-//   64  480  257  368  254    256  547  295  443  338    1024  829  506  642  477
+//   64  421  207  324  207    256  462  243  342  238    1024  731  411  551  364
 // Few rows have a kernel of their own (mxfp4_few.hpp); us, it / 64 x 64 tiles, by rows (1, 4, 16):
 //   14336, k 4096  8.5 / 9.0  9.0 / 9.1  10.9 / 9.4    4096, k 4096  4.2 / 7.5  4.4 / 7.6  4.9 / 7.6
 //   4096, k 14336  9.6 / 17   9.9 / 17   11.5 / 18     1024, k 4096  3.5 / 7.1  3.7 / 7.1  4.3 / 7.2

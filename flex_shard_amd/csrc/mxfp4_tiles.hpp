@@ -248,6 +248,14 @@ __device__ __forceinline__ void zero_tile(const MxGemmParams& p, const MxTilePla
 // A resident workgroup requests the first two steps of its next tile before it
 // stores the one it has finished: the start of a tile (a chain of loads) and the
 // end of one (128 KB of stores) then pass behind one another and behind products.
+//
+// Measured, 256 x 256 tiles: 2340 cycles a step (2048 of MFMA), 8000 to 9000 between
+// two tiles' steps, at the 1.7 GHz that the power allows.  8192 x 4096, k 14336 206
+// us, 4.7 PFLOP/s; 8192 x 14336, k 4096 250 us, 3.9; 4096 x 4096, k 4096 36 us, 3.9.
+// Outputs go past the caches, which hold the operands: rows of 32 experts' weight
+// gradients, [2048, 7168] each of 1024 rows, 484 us through them, 364 so.
+// The staging pays for whole 128-byte stores: swapping halves and quarters of a
+// wave instead (64-byte pieces, no LDS) took 63 us for 47, 14336 x 4096, k 1024.
 template <typename Cfg, int kProblem, int DT>
 __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_kernel(const MxGemmParams p) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds_bytes[];
