@@ -619,7 +619,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
           for (int w = s * kPerStore; w < (s + 1) * kPerStore; ++w) {
             if (DT == FSH_DT_F32) words[w] = f32_as_u32(v[0][w]);
             else if (DT == FSH_DT_BF16) words[w] = pack_bf16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
-            else words[w] = f32_to_f16_bits(v[w / 8][2 * w % 16]) | (f32_to_f16_bits(v[w / 8][2 * w % 16 + 1]) << 16);
+            else words[w] = pack_f16x2(v[w / 8][2 * w % 16], v[w / 8][2 * w % 16 + 1]);
           }
           __builtin_amdgcn_sched_barrier(0);
           if (part > 0) store_one(plain, part - 1, s);
