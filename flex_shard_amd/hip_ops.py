@@ -531,7 +531,9 @@ def gemm_nt(
 
 
 #: the tiles a product can take, as ``gemm_tiles`` and ``fp8_gemm_tiles`` name them
-GEMM_TILES = ("64", "64 deep", "128", "128 deep", "256x128", "256", "256 long k", "few rows")
+GEMM_TILES = ("64", "64 deep", "128", "128 deep", "256x128", "256", "256 long k")
+#: and as ``mxfp4_gemm_tiles`` does
+MXFP4_TILES = (*GEMM_TILES, "few rows")
 
 
 def gemm_tiles(*problems: tuple) -> tuple[str, ...]:
@@ -1275,7 +1277,7 @@ def mxfp4_gemm_tiles(m: int, n: int, k: int, *, mode: int = _native.MXFP4_DENSE,
     no GPU needed)."""
     kind = _native.lib().fsh_mxfp4_gemm_tiles(m, n, k, mode, experts)
     _native.check(min(kind, 0), "fsh_mxfp4_gemm_tiles")
-    return GEMM_TILES[kind]
+    return MXFP4_TILES[kind]
 
 
 def mxfp4_linear(x: torch.Tensor, weight: MxFp4Matrix, bias: torch.Tensor | None = None) -> torch.Tensor:
