@@ -249,7 +249,7 @@ __device__ __forceinline__ void zero_tile(const MxGemmParams& p, const MxTilePla
 // stores the one it has finished: the start of a tile (a chain of loads) and the
 // end of one (128 KB of stores) then pass behind one another and behind products.
 //
-// Measured, 256 x 256 tiles: 2340 cycles a step (2048 of MFMA), 8000 to 9000 between
+// Measured, 256 x 256 tiles: 2340 cycles a step (2048 of MFMA), 10 000 to 12 000 between
 // two tiles' steps, at the 1.7 GHz that the power allows.  8192 x 4096, k 14336 206
 // us, 4.7 PFLOP/s; 8192 x 14336, k 4096 250 us, 3.9; 4096 x 4096, k 4096 36 us, 3.9.
 // Outputs go past the caches, which hold the operands: rows of 32 experts' weight
