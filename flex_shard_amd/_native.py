@@ -273,6 +273,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "fsh_expert_combine": (
         c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p],
     ),
+    "fsh_expert_combine_f32": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p],
+    ),
     "fsh_expert_combine_backward": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p,

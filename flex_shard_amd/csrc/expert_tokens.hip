@@ -11,7 +11,7 @@
 // The sort is bound by latency; the others by memory: every row of the experts
 // is read or written once, the tokens' rows once.  Measured, 8192 tokens of 7168
 // bf16, 8 of 32 experts each: sort 13 us; dispatch 187 us, 5.7 TB/s; combine 212 us,
-// 5.0; its gradient 393 us, 5.1.  16 tokens: 3.6, 4.2 and 4.8 us, a launch's chain
+// 5.0; its gradient 393 us, 5.1; 4096 tokens' fp32 rows to bf16 194 us, 5.1.  16 tokens: 3.6, 4.2 and 4.8 us, a launch's chain
 // of loads each.
 #include "mxfp4.hpp"
 
@@ -191,24 +191,30 @@ __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParam
 }
 
 // ------------------------------------------------------------------ the rows
-// A thread has kUnit bytes' worth of neighbouring elements: 16 bytes where all
-// rows are 16-byte aligned, one element otherwise.
-template <int DT, bool kVec>
+// A thread has neighbouring elements: where all rows are 16-byte aligned 16 bytes'
+// worth (kCount: as many as 16 bytes of another type hold), one otherwise.
+template <int DT, bool kVec, int kCount = 16 / element_bytes<DT>()>
 struct Piece {
-  static constexpr int kElements = kVec ? 16 / element_bytes<DT>() : 1;
+  static constexpr int kElements = kVec ? kCount : 1;
   // kStream: a row that is read once
   template <bool kStream>
   static __device__ __forceinline__ void load(const uint8_t* row, int64_t piece, float (&f)[kElements]) {
-    if (kVec) {
-      const u32x4* at = reinterpret_cast<const u32x4*>(row + piece * 16);
-      const u32x4 v = kStream ? __builtin_nontemporal_load(at) : *at;
+    if constexpr (kVec) {
+      constexpr int kLoads = kElements * element_bytes<DT>() / 16, kPerLoad = kElements / kLoads;
+      const u32x4* at = reinterpret_cast<const u32x4*>(row) + piece * kLoads;
 #pragma unroll
-      for (int i = 0; i < kElements; ++i) f[i] = DT == FSH_DT_F32 ? u32_as_f32(v[i % 4]) : half_of_pair<DT>(v[i / 2 % 4], i % 2);
+      for (int l = 0; l < kLoads; ++l) {
+        const u32x4 v = kStream ? __builtin_nontemporal_load(at + l) : at[l];
+#pragma unroll
+        for (int i = 0; i < kPerLoad; ++i)
+          f[l * kPerLoad + i] = DT == FSH_DT_F32 ? u32_as_f32(v[i % 4]) : half_of_pair<DT>(v[i / 2 % 4], i % 2);
+      }
     } else {
       f[0] = load_element<DT>(row, piece);
     }
   }
   static __device__ __forceinline__ void store(uint8_t* row, int64_t piece, const float (&f)[kElements]) {
+    static_assert(!kVec || kCount * element_bytes<DT>() == 16, "one store");
     if constexpr (!kVec) {
       store_element<DT>(row, piece, f[0]);
     } else if constexpr (DT == FSH_DT_F32) {
@@ -229,6 +235,7 @@ struct RowsParams {
   void* grad_weights;
   int32_t weights_dtype, experts, top_k;
   int64_t tokens, pieces, row_bytes, slabs;
+  int64_t out_row_bytes;  // combine: of its output's rows, whose type may differ
 };
 
 __device__ __forceinline__ float weight_of(const RowsParams& p, int64_t choice) {
@@ -266,10 +273,11 @@ __global__ __launch_bounds__(kThreads) void expert_dispatch_kernel(const RowsPar
   }
 }
 
-// One token, kThreads pieces of its row.  Eight rows are in flight at a time.
-template <int DT, bool kVec>
+// One token, kThreads pieces of its row.  Eight rows are in flight at a time.  OUT:
+// the output's type; fp32 rows can leave as 16 bits, rounded after their sum.
+template <int DT, int OUT, bool kVec>
 __global__ __launch_bounds__(kThreads) void expert_combine_kernel(const RowsParams p) {
-  using P = Piece<DT, kVec>;
+  using P = Piece<DT, kVec, 16 / element_bytes<OUT>()>;
   const int64_t token = blockIdx.x / p.slabs, piece = blockIdx.x % p.slabs * kThreads + threadIdx.x;
   if (piece >= p.pieces) return;
   float sum[P::kElements] = {};
@@ -292,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void expert_combine_kernel(const RowsPara
 #pragma unroll
         for (int i = 0; i < P::kElements; ++i) sum[i] = __builtin_fmaf(w[j], f[j][i], sum[i]);
   }
-  P::store(p.out + token * p.row_bytes, piece, sum);
+  Piece<OUT, kVec>::store(p.out + token * p.out_row_bytes, piece, sum);
 }
 
 // One token: a piece of its gradient is read once for eight choices, whose rows are
@@ -354,19 +362,20 @@ __global__ __launch_bounds__(kThreads) void expert_combine_backward_kernel(const
 }
 
 // Checks that the row kernels share, and the sizes that follow from the dtype and the pointers.
-int rows_checks(RowsParams& p, int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, bool* vec, const char* who) {
+int rows_checks(RowsParams& p, int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, int32_t out_dtype, bool* vec, const char* who) {
   if (tokens < 0 || width < 0 || top_k <= 0) return fail(FSH_EINVAL, "%s: negative shape, or top_k not positive", who);
-  if (!known_dtype(dtype) || (p.weights && !known_dtype(p.weights_dtype))) return fail(FSH_EINVAL, "%s: unknown dtype", who);
+  if (!known_dtype(dtype) || !known_dtype(out_dtype) || (p.weights && !known_dtype(p.weights_dtype))) return fail(FSH_EINVAL, "%s: unknown dtype", who);
   if (top_k > kMaxTopK) return fail(FSH_ENOTSUP, "%s: at most %d choices per token, got %d", who, kMaxTopK, top_k);
   if (tokens * top_k >= (1LL << 31)) return fail(FSH_ENOTSUP, "%s: 2^31 choices or more", who);
   if (tokens == 0 || width == 0) return FSH_OK;
   if (!p.position || !p.out) return fail(FSH_EINVAL, "%s: null pointer", who);
-  const int bytes = dtype_bytes(dtype);
-  if (!aligned(p.x, bytes) || !aligned(p.rows, bytes) || !aligned(p.out, bytes)) return fail(FSH_ENOTSUP, "%s: misaligned pointer", who);
+  const int bytes = dtype_bytes(dtype), out_bytes = dtype_bytes(out_dtype);
+  if (!aligned(p.x, bytes) || !aligned(p.rows, bytes) || !aligned(p.out, out_bytes)) return fail(FSH_ENOTSUP, "%s: misaligned pointer", who);
   p.tokens = tokens; p.top_k = top_k;
   p.row_bytes = width * bytes;
-  *vec = p.row_bytes % 16 == 0 && aligned(p.x, 16) && aligned(p.rows, 16) && aligned(p.out, 16);
-  p.pieces = *vec ? p.row_bytes / 16 : width;
+  p.out_row_bytes = width * out_bytes;
+  *vec = p.row_bytes % 16 == 0 && p.out_row_bytes % 16 == 0 && aligned(p.x, 16) && aligned(p.rows, 16) && aligned(p.out, 16);
+  p.pieces = *vec ? p.out_row_bytes / 16 : width;
   p.slabs = ceil_div(p.pieces, static_cast<int64_t>(kThreads));
   if (tokens * p.slabs + kZeroBlocks > kMaxGrid) return fail(FSH_ENOTSUP, "%s: too many rows", who);
   return FSH_OK;
@@ -425,7 +434,7 @@ FSH_API int fsh_expert_dispatch(const void* x_dev, const int32_t* position_dev, 
   p.out = static_cast<uint8_t*>(out_dev);
   p.position = position_dev; p.offsets = offsets_dev; p.experts = experts;
   bool vec = false;
-  if (int rc = rows_checks(p, tokens, top_k, width, dtype, &vec, who)) return rc;
+  if (int rc = rows_checks(p, tokens, top_k, width, dtype, dtype, &vec, who)) return rc;
   if (tokens == 0 || width == 0) return FSH_OK;
   if (!x_dev || !offsets_dev || experts <= 0) return fail(FSH_EINVAL, "%s: null pointer, or no expert", who);
   const dim3 grid(static_cast<uint32_t>(tokens * p.slabs + kZeroBlocks)), block(kThreads);
@@ -437,10 +446,11 @@ FSH_API int fsh_expert_dispatch(const void* x_dev, const int32_t* position_dev, 
   return check_launch("expert_dispatch_kernel");
 }
 
-FSH_API int fsh_expert_combine(const void* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
-                               int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream) {
-  using namespace fsh;
-  const char* who = "fsh_expert_combine";
+namespace fsh {
+namespace {
+
+int combine(const void* rows_dev, int32_t dtype, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype, int64_t tokens,
+            int32_t top_k, int64_t width, int32_t out_dtype, void* out_dev, void* stream, const char* who) {
   RowsParams p;
   memset(&p, 0, sizeof(p));
   p.rows = static_cast<const uint8_t*>(rows_dev);
@@ -448,16 +458,35 @@ FSH_API int fsh_expert_combine(const void* rows_dev, const int32_t* position_dev
   p.position = position_dev;
   p.weights = weights_dev; p.weights_dtype = weights_dtype;
   bool vec = false;
-  if (int rc = rows_checks(p, tokens, top_k, width, dtype, &vec, who)) return rc;
+  if (int rc = rows_checks(p, tokens, top_k, width, dtype, out_dtype, &vec, who)) return rc;
   if (tokens == 0 || width == 0) return FSH_OK;
   if (!rows_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
   const dim3 grid(static_cast<uint32_t>(tokens * p.slabs)), block(kThreads);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  by_dtype(dtype, [&](auto dt) {
-    if (vec) hipLaunchKernelGGL((expert_combine_kernel<dt.value, true>), grid, block, 0, on, p);
-    else hipLaunchKernelGGL((expert_combine_kernel<dt.value, false>), grid, block, 0, on, p);
+  by_dtype(out_dtype, [&](auto out) {
+    const auto launch = [&](auto rows) {
+      if (vec) hipLaunchKernelGGL((expert_combine_kernel<rows.value, out.value, true>), grid, block, 0, on, p);
+      else hipLaunchKernelGGL((expert_combine_kernel<rows.value, out.value, false>), grid, block, 0, on, p);
+    };
+    if (dtype == FSH_DT_F32) launch(std::integral_constant<int, FSH_DT_F32>{});
+    else launch(out);
   });
   return check_launch("expert_combine_kernel");
+}
+
+}  // namespace
+}  // namespace fsh
+
+FSH_API int fsh_expert_combine(const void* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
+                               int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream) {
+  return fsh::combine(rows_dev, dtype, position_dev, weights_dev, weights_dtype, tokens, top_k, width, dtype, out_dev, stream,
+                      "fsh_expert_combine");
+}
+
+FSH_API int fsh_expert_combine_f32(const float* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
+                                   int64_t tokens, int32_t top_k, int64_t width, int32_t out_dtype, void* out_dev, void* stream) {
+  return fsh::combine(rows_dev, FSH_DT_F32, position_dev, weights_dev, weights_dtype, tokens, top_k, width, out_dtype, out_dev, stream,
+                      "fsh_expert_combine_f32");
 }
 
 FSH_API int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, const int32_t* position_dev,
@@ -475,7 +504,7 @@ FSH_API int fsh_expert_combine_backward(const void* grad_dev, const void* rows_d
   p.weights = weights_dev; p.weights_dtype = weights_dtype;
   p.grad_weights = grad_weights_dev;
   bool vec = false;
-  if (int rc = rows_checks(p, tokens, top_k, width, dtype, &vec, who)) return rc;
+  if (int rc = rows_checks(p, tokens, top_k, width, dtype, dtype, &vec, who)) return rc;
   if (tokens == 0 || width == 0) return FSH_OK;
   if (!grad_dev || !rows_dev || !offsets_dev || experts <= 0 || !weights_dev || !grad_weights_dev)
     return fail(FSH_EINVAL, "%s: null pointer, or no expert", who);

@@ -1416,18 +1416,24 @@ def expert_combine(rows: torch.Tensor, position: torch.Tensor, weights: torch.Te
 
 
 def expert_combine_at(
-    rows: torch.Tensor, position_ptr: int, tokens: int, top_k: int, weights: torch.Tensor | None = None
+    rows: torch.Tensor, position_ptr: int, tokens: int, top_k: int, weights: torch.Tensor | None = None, dtype: torch.dtype | None = None
 ) -> torch.Tensor:
-    """:func:`expert_combine` of contiguous ``rows`` and weights; the routing's table by address."""
+    """:func:`expert_combine` of contiguous ``rows`` and weights; the routing's table by address.  ``dtype``: that of
+    the sums, which fp32 rows are rounded to (None: as the rows)."""
     width, device = rows.shape[1], rows.device
-    out = torch.empty((tokens, width), dtype=rows.dtype, device=device)
-    status = _native.lib().fsh_expert_combine(
+    out = torch.empty((tokens, width), dtype=dtype or rows.dtype, device=device)
+    name = "fsh_expert_combine"
+    if out.dtype != rows.dtype:
+        if rows.dtype != torch.float32:
+            raise NotImplementedError(f"rows of {rows.dtype} are combined to their own type, not to {dtype}")
+        name = "fsh_expert_combine_f32"
+    status = getattr(_native.lib(), name)(
         rows.data_ptr(), position_ptr, None if weights is None else weights.data_ptr(),
-        DT_F32 if weights is None else _float_dt(weights.dtype), tokens, top_k, width, _float_dt(rows.dtype), out.data_ptr(),
+        DT_F32 if weights is None else _float_dt(weights.dtype), tokens, top_k, width, _float_dt(out.dtype), out.data_ptr(),
         stream_ptr(device),
     )
     if status:
-        _native.check(status, "fsh_expert_combine")
+        _native.check(status, name)
     return out
 
 

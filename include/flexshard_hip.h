@@ -625,6 +625,7 @@ int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int64_t ldx
  * are zero.  fsh_expert_combine: out[t] = sum over j, in that order, of
  * weights[t, j] * rows[position[t, j]] in fp32, rounded once (weights null: 1),
  * choices of no expert left out; it is also the gradient of the dispatch.
+ * fsh_expert_combine_f32: the same of fp32 rows, rounded once to out_dtype.
  * fsh_expert_combine_backward: grad_rows[position[t, j]] = weights[t, j] *
  * grad[t], zero behind offsets[experts]; grad_weights[t, j] = <grad[t],
  * rows[position[t, j]]>, zero for no expert.  Rows of `width` elements,
@@ -639,6 +640,8 @@ int fsh_expert_dispatch(const void* x_dev, const int32_t* position_dev, const in
                         int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream);
 int fsh_expert_combine(const void* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
                        int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* out_dev, void* stream);
+int fsh_expert_combine_f32(const float* rows_dev, const int32_t* position_dev, const void* weights_dev, int32_t weights_dtype,
+                           int64_t tokens, int32_t top_k, int64_t width, int32_t out_dtype, void* out_dev, void* stream);
 int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, const int32_t* position_dev,
                                 const int32_t* offsets_dev, int32_t experts, const void* weights_dev, int32_t weights_dtype,
                                 int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* grad_rows_dev,

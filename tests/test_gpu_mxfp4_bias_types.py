@@ -1,0 +1,57 @@
+"""A bias of another type than the activation is added to the fp32 sums as it is: one rounding, that of the result."""
+
+import pytest
+import torch
+from mxfp4_definition import assert_product, through
+
+from flex_shard_amd import hip_ops
+from flex_shard_amd.mxfp4 import mxfp4_linear, quantize_mxfp4_weight
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.bfloat16, torch.float16]
+
+
+# a size for every kernel of the dense product
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize(
+    "tiles,m,n,k",
+    [("few rows", 1, 130, 96), ("few rows", 4, 1001, 300), ("few rows", 16, 1001, 5000), ("64", 50, 3001, 1100), ("128", 1000, 5123, 600),
+     ("128 deep", 2035, 2041, 700), ("256", 8001, 4091, 1030)],
+)
+def test_low_bits_of_an_fp32_bias_survive(device, tiles, m, n, k, dtype):
+    assert hip_ops.mxfp4_gemm_tiles(m, n, k) == tiles
+    x, w = torch.zeros(m, k, dtype=dtype, device=device), torch.zeros(n, k, dtype=dtype, device=device)
+    x[:, 7], w[:, 7] = 1.0, -1.0
+    small = (torch.arange(n, device=device) % 200) * 2.0**-14
+    want = small.to(dtype).expand(m, n)  # -1 + (1 + small), eight bits of it
+    frozen = quantize_mxfp4_weight(w)
+    bias = 1.0 + small
+    assert torch.equal(mxfp4_linear(x, frozen, bias), want)
+    leaves = [w.requires_grad_(), bias.requires_grad_()]  # the training call quantizes ahead of the product
+    y = mxfp4_linear(x, *leaves)
+    assert y.dtype == dtype and torch.equal(y, want)
+    gw, gb = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    assert gw.dtype == dtype and gb.dtype == torch.float32 and torch.equal(gb, torch.full_like(gb, m))
+
+
+def test_bf16_bias_beyond_fp16(device):
+    x, w = torch.zeros(3, 64, dtype=torch.float16, device=device), torch.zeros(40, 64, dtype=torch.float16, device=device)
+    x[:, 1], w[:, 1] = 256.0, -512.0
+    bias = torch.full((40,), 131072.0 + 1024.0, dtype=torch.bfloat16, device=device)  # an infinity in fp16
+    assert torch.equal(mxfp4_linear(x, w, bias), torch.full((3, 40), 1024.0, dtype=torch.float16, device=device))
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 4, 9, 200])
+def test_against_the_unrounded_sum(device, tokens, bias_dtype, dtype):
+    gen = torch.Generator().manual_seed(tokens)
+    x, w = torch.randn(tokens, 96, generator=gen).to(dtype), (torch.randn(70, 96, generator=gen) * 0.05).to(dtype)
+    bias = torch.randn(70, generator=gen).to(bias_dtype)
+    got = mxfp4_linear(x.to(device), w.to(device), bias.to(device))
+    assert got.dtype == dtype
+    assert_product(got, through(x), through(w), bias.double())
+    strided = torch.randn(70, 2, generator=gen).to(bias_dtype)
+    got = mxfp4_linear(x.to(device), w.to(device), strided.to(device)[:, 1])
+    assert_product(got, through(x), through(w), strided[:, 1].double())
