@@ -79,6 +79,11 @@ __device__ __forceinline__ float load_element(const void* base, int64_t i) {
 __device__ __forceinline__ uint32_t round_to_16_bits(float f, int dtype) {
   return dtype == FSH_DT_F16 ? f32_to_f16_bits(f) : f32_to_bf16_bits(f);
 }
+// Element i of a bias: of the output's type DT, or fp32.
+template <int DT>
+__device__ __forceinline__ float load_bias(const void* bias, int64_t i, int32_t is_f32) {
+  return is_f32 ? load_element<FSH_DT_F32>(bias, i) : load_element<DT>(bias, i);
+}
 template <int DT>
 __device__ __forceinline__ void store_element(void* base, int64_t i, float f) {
   if (DT == FSH_DT_F32) static_cast<float*>(base)[i] = f;

@@ -24,6 +24,7 @@ struct MxFewParams {
   int64_t m, n, a_rows, b_rows, ld, ldo;  // ld: bytes of a quantized row
   int64_t cols, ldx;                      // kQuantize: columns and row stride of the activation, elements
   int32_t steps, waves, vec;
+  int32_t bias_f32;  // the bias is fp32, whatever the output
 };
 
 constexpr int kFewRows = 16;  // of the weight, per workgroup
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * kFewMaxWaves) void mxfp4_few_rows_kernel(const
     float sum = 0.0f;
     for (int w = 0; w < p.waves; ++w) sum += sums[w * kWaveSums + (i / 16) * kPitch + i % 16];
     if (out_row < p.m && col < p.n) {
-      if (p.bias) sum += load_element<DT>(p.bias, col);
+      if (p.bias) sum += load_bias<DT>(p.bias, col, p.bias_f32);
       store_element<DT>(p.out, out_row * p.ldo + col, sum);
     }
   }

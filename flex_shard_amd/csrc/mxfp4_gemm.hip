@@ -141,12 +141,23 @@ int launch_few(MxFewParams& p, int32_t dtype, hipStream_t stream) {
   return check_launch("mxfp4_few_rows_kernel");
 }
 
+// A product's mode and whether its bias is fp32 (FSH_MXFP4_BIAS_F32 is added to the mode of a dense one).
+struct MxMode {
+  int32_t mode;
+  bool bias_f32;
+  explicit MxMode(int32_t m) : mode(m & ~FSH_MXFP4_BIAS_F32), bias_f32((m & FSH_MXFP4_BIAS_F32) != 0) {}
+  bool known() const { return mode == FSH_MXFP4_DENSE || (!bias_f32 && (mode == FSH_MXFP4_ROWS || mode == FSH_MXFP4_OVER_ROWS)); }
+  bool dense() const { return mode == FSH_MXFP4_DENSE; }
+  int bias_bytes(int32_t out_dtype) const { return bias_f32 ? 4 : dtype_bytes(out_dtype); }
+};
+
 MxFewParams few_params(const fsh_mxfp4_product& q) {
   MxFewParams p;
   memset(&p, 0, sizeof(p));
   p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
   p.b = static_cast<const uint8_t*>(q.b_dev); p.bs = static_cast<const uint8_t*>(q.b_scales_dev);
   p.out = q.out_dev; p.bias = q.bias_dev;
+  p.bias_f32 = MxMode(q.mode).bias_f32;
   p.m = q.m; p.n = q.n; p.a_rows = q.a_rows; p.b_rows = q.b_rows;
   p.ld = q.k / 2; p.ldo = q.ldo;
   p.steps = static_cast<int32_t>(q.k / kMxColumns);
@@ -162,9 +173,9 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   if (!product) return fail(FSH_EINVAL, "%s: null product", who);
   const fsh_mxfp4_product& q = *product;
   if (q.m < 0 || q.n < 0 || q.k < 0) return fail(FSH_EINVAL, "%s: negative size", who);
-  if (q.mode != FSH_MXFP4_DENSE && q.mode != FSH_MXFP4_ROWS && q.mode != FSH_MXFP4_OVER_ROWS)
-    return fail(FSH_EINVAL, "%s: unknown mode %d", who, q.mode);
-  if (q.mode != FSH_MXFP4_DENSE && q.experts <= 0) return fail(FSH_EINVAL, "%s: no expert", who);
+  const MxMode mode(q.mode);
+  if (!mode.known()) return fail(FSH_EINVAL, "%s: unknown mode %d", who, q.mode);
+  if (!mode.dense() && q.experts <= 0) return fail(FSH_EINVAL, "%s: no expert", who);
   if (q.m == 0 || q.n == 0) return FSH_OK;
   if (!known_dtype(q.out_dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, q.out_dtype);
   if (!q.a_dev || !q.a_scales_dev || !q.b_dev || !q.b_scales_dev || !q.out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
@@ -174,7 +185,7 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
     return fail(FSH_ENOTSUP, "%s: sizes beyond 2^28 rows or 2^31 columns", who);
   if (q.ldo < q.n) return fail(FSH_EINVAL, "%s: ldo %lld < n %lld", who, (long long)q.ldo, (long long)q.n);
   const bool segments = q.mode == FSH_MXFP4_ROWS;
-  if (q.mode != FSH_MXFP4_DENSE && !q.offsets_dev) return fail(FSH_EINVAL, "%s: segments without offsets", who);
+  if (!mode.dense() && !q.offsets_dev) return fail(FSH_EINVAL, "%s: segments without offsets", who);
   if (segments && q.top_k <= 0) return fail(FSH_EINVAL, "%s: top_k must be positive", who);
   if (q.a_rows < (q.source_dev ? 1 : q.m) || q.b_rows < q.n * (segments ? q.experts : 1))
     return fail(FSH_EINVAL, "%s: operands of %lld and %lld rows are too few", who, (long long)q.a_rows, (long long)q.b_rows);
@@ -183,7 +194,7 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
     return fail(FSH_EINVAL, "%s: products over rows are contiguous and have no bias", who);
   if (segments && q.bias_dev) return fail(FSH_ENOTSUP, "%s: segments have no bias", who);
   if (!aligned(q.a_dev, 16) || !aligned(q.b_dev, 16) || !aligned(q.a_scales_dev, 8) || !aligned(q.b_scales_dev, 8) ||
-      !aligned(q.out_dev, dtype_bytes(q.out_dtype)) || !aligned(q.bias_dev, dtype_bytes(q.out_dtype)))
+      !aligned(q.out_dev, dtype_bytes(q.out_dtype)) || !aligned(q.bias_dev, mode.bias_bytes(q.out_dtype)))
     return fail(FSH_ENOTSUP, "%s: data must be 16-byte and scales 8-byte aligned, out and bias to their elements", who);
   // The lanes' offsets are 32 bits from a tile's first row, or from the matrix for gathered rows.
   if (256 * (q.k / 2) >= (1LL << 32) || (q.source_dev && q.a_rows * (q.k / 2) >= (1LL << 32)))
@@ -194,6 +205,7 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   p.a = static_cast<const uint8_t*>(q.a_dev); p.as = static_cast<const uint8_t*>(q.a_scales_dev);
   p.b = static_cast<const uint8_t*>(q.b_dev); p.bs = static_cast<const uint8_t*>(q.b_scales_dev);
   p.out = q.out_dev; p.bias = q.bias_dev;
+  p.bias_f32 = mode.bias_f32;
   p.m = q.m; p.n = q.n; p.k = q.k;
   p.a_rows = q.a_rows; p.b_rows = q.b_rows;
   p.lda = p.ldb = q.k / 2;
@@ -248,7 +260,8 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
   if (q.out_dtype != dtype) return fail(FSH_EINVAL, "%s: the output has the activation's dtype", who);
   if (q.m == 0 || q.n == 0 || rows == 0) return FSH_OK;
   q.a_rows = rows;
-  if (q.mode == FSH_MXFP4_DENSE && q.m <= kFewQuantize) {
+  const MxMode mode(q.mode);
+  if (mode.dense() && q.m <= kFewQuantize) {
     MxFewParams p = few_params(q);
     if (few_lds_bytes(p, kFewMaxWaves, true) <= 64 * 1024) {
       if (!known_dtype(dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, dtype);
@@ -256,7 +269,8 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
         return fail(FSH_EINVAL, "%s: rows or leading dimensions too small", who);
       if (!x_dev || !q.b_dev || !q.b_scales_dev || !q.out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
       const int bytes = dtype_bytes(dtype);
-      if (!aligned(x_dev, bytes) || !aligned(q.b_dev, 16) || !aligned(q.b_scales_dev, 8) || !aligned(q.out_dev, bytes) || !aligned(q.bias_dev, bytes))
+      if (!aligned(x_dev, bytes) || !aligned(q.b_dev, 16) || !aligned(q.b_scales_dev, 8) || !aligned(q.out_dev, bytes) ||
+          !aligned(q.bias_dev, mode.bias_bytes(dtype)))
         return fail(FSH_ENOTSUP, "%s: weights must be 16-byte and scales 8-byte aligned, x, out and bias to their elements", who);
       p.a = static_cast<const uint8_t*>(x_dev);
       p.cols = in_dim; p.ldx = ldx;

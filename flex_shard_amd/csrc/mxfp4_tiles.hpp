@@ -80,10 +80,10 @@ struct MxGemmParams {
   const uint8_t* b;
   const uint8_t* bs;
   void* out;
-  const void* bias;  // [n] of the output's type, or null
+  const void* bias;  // [n] of the output's type, or fp32 (bias_f32), or null
   int64_t m, n, k;   // k a multiple of 256; kMxOverRows: of all segments
   int64_t a_rows, b_rows, lda, ldb, ldo;
-  int32_t out_dtype;
+  int32_t out_dtype, bias_f32;
   int32_t experts, top_k;
   const int32_t* offsets;         // [experts + 1]
   const int32_t* padded_offsets;  // [experts + 1] (kMxOverRows)
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(Cfg::kThreads, Cfg::kWaves / 4) void mxfp4_gemm_ker
       more_tiles = place_of_turn<Cfg, kProblem>(p, schedule, table, turn, &next_place);
       if (more_tiles) next_rows = rows_of(next_place);
     }
-    if (kProblem == kMxDense && p.bias && tid < Cfg::BN && place.col0 + tid < p.n) bias = load_element<DT>(p.bias, place.col0 + tid);
+    if (kProblem == kMxDense && p.bias && tid < Cfg::BN && place.col0 + tid < p.n) bias = load_bias<DT>(p.bias, place.col0 + tid, p.bias_f32);
     if (place.zero) {
       zero_tile<DT, Cfg>(p, place);
       if (!more_tiles) return;

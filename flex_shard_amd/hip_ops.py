@@ -1219,6 +1219,8 @@ def _mxfp4_product(
     q.out_dev = out.data_ptr()
     if bias is not None:
         q.bias_dev = bias.data_ptr()
+        if dtype != DT_F32 and bias.dtype == torch.float32:
+            q.mode = _native.MXFP4_BIAS_F32
     q.m, q.n, q.k = m, n, -(-b.cols // 256) * 256
     q.b_rows = b.rows
     q.ldo = out.stride(-2) if m > 1 else n
@@ -1228,13 +1230,18 @@ def _mxfp4_product(
     return q
 
 
+def _check_bias(bias: torch.Tensor, dtype: torch.dtype, n: int) -> None:
+    if (bias.dtype is not dtype and bias.dtype is not torch.float32) or tuple(bias.shape) != (n,) or not bias.is_contiguous():
+        raise ValueError(f"bias must be {dtype} or fp32 of {n} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
+
+
 def mxfp4_gemm(
     a: MxFp4Matrix, b: MxFp4Matrix, dtype: torch.dtype, *, bias: torch.Tensor | None = None, mode: int = _native.MXFP4_DENSE,
     offsets: torch.Tensor | None = None, source: torch.Tensor | None = None, top_k: int = 1, choices: int | None = None,
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """``a @ b.T (+ bias)`` of quantized matrices over the same padded columns, fp32
-    sums rounded once to ``dtype``.  ``mode``: the whole product; ``MXFP4_ROWS``: the
+    sums rounded once to ``dtype``, of which the bias is, or fp32.  ``mode``: the whole product; ``MXFP4_ROWS``: the
     ``choices`` rows in segments of ``offsets``, expert ``e``'s times b's rows
     [e n, (e + 1) n), row i of a or, with ``source``, row ``source[i] // top_k``;
     ``MXFP4_OVER_ROWS``: [experts, m, n], per expert the product over the columns
@@ -1261,8 +1268,8 @@ def mxfp4_gemm(
         raise ValueError(f"out must be {dtype} {shape}")
     elif mode != _native.MXFP4_OVER_ROWS:
         _row_stride(out)
-    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
-        raise ValueError(f"bias must be {dtype} of {n} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
+    if bias is not None:
+        _check_bias(bias, dtype, n)
     q = _mxfp4_product(b, out, _float_dt(dtype), mode, m, n, bias, experts, top_k, _ptr(offsets), _ptr(source))
     q.a_dev, q.a_scales_dev = a.pointers()
     q.a_rows = a.rows
@@ -1292,8 +1299,7 @@ def mxfp4_linear(x: torch.Tensor, weight: MxFp4Matrix, bias: torch.Tensor | None
         _require_gpu(x, weight.buffer)
     else:
         _require_gpu(x, weight.buffer, bias)
-        if bias.dtype != x.dtype or bias.numel() != weight.rows or not bias.is_contiguous():
-            raise ValueError(f"bias must be {x.dtype} of {weight.rows} contiguous elements, got {bias.dtype} {tuple(bias.shape)}")
+        _check_bias(bias, x.dtype, weight.rows)
     out = torch.empty((rows, weight.rows), dtype=x.dtype, device=device)
     return _mxfp4_linear(x, ldx, weight, out, bias, _native.MXFP4_DENSE, rows, weight.rows, 0, 1, None, None)
 

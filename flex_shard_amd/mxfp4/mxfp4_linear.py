@@ -49,10 +49,11 @@ def _weight_forms(weight: torch.Tensor | MxFp4Weight, needs_x: bool):
 
 
 def _bias_for(x: torch.Tensor, bias: torch.Tensor | None) -> torch.Tensor | None:
-    """The bias in the product's type (its epilogue adds it before the one rounding)."""
-    if bias is None or (bias.dtype == x.dtype and bias.is_contiguous()):
+    """The bias as the product's epilogue adds it, before the one rounding: of the
+    activation's type or fp32, which any other becomes without a rounding."""
+    if bias is None:
         return bias
-    return bias.to(x.dtype).contiguous()
+    return (bias if bias.dtype == x.dtype else bias.float()).contiguous()
 
 
 def _keep(ctx: Any, x_columns: MxFp4Matrix | None, w_columns: MxFp4Matrix | None) -> None:
@@ -103,7 +104,8 @@ class _Linear(torch.autograd.Function):
 
 def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor | MxFp4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ W.T + bias`` with both operands in microscaled 4-bit floats and fp32
-    sums, rounded once to the type of ``x`` (bf16, fp16 or fp32).  ``weight``
+    sums, rounded once to the type of ``x`` (bf16, fp16 or fp32); a bias of another
+    of these types is added unrounded.  ``weight``
     [out, in]: quantized within the call, with gradients for all three; an
     :class:`MxFp4Weight`: as it is, with gradients for ``x`` (if it has its
     transposed form) and ``bias``."""

@@ -564,7 +564,8 @@ int fsh_sum_runs(const float* sums_dev, int64_t runs, int64_t cols, void* out_de
  * k columns (padded: a multiple of 256).
  *   FSH_MXFP4_DENSE      a [a_rows >= m, k], b [b_rows >= n, k], out [m, n] of
  *                        stride ldo; bias [n] of out_dtype or null, added before
- *                        the rounding
+ *                        the rounding; with FSH_MXFP4_BIAS_F32 added to the mode
+ *                        the bias is fp32
  *   FSH_MXFP4_ROWS       rows [offsets[e], offsets[e + 1]) of a's m rows times
  *                        b's rows [e n, (e + 1) n); out rows behind the last
  *                        segment are zero.  With source, row r is row
@@ -576,6 +577,7 @@ int fsh_sum_runs(const float* sums_dev, int64_t runs, int64_t cols, void* out_de
 #define FSH_MXFP4_DENSE 0
 #define FSH_MXFP4_ROWS 1
 #define FSH_MXFP4_OVER_ROWS 2
+#define FSH_MXFP4_BIAS_F32 256
 typedef struct fsh_mxfp4_product {
   const void* a_dev;
   const void* a_scales_dev;

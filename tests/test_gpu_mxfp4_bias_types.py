@@ -55,3 +55,18 @@ def test_against_the_unrounded_sum(device, tokens, bias_dtype, dtype):
     strided = torch.randn(70, 2, generator=gen).to(bias_dtype)
     got = mxfp4_linear(x.to(device), w.to(device), strided.to(device)[:, 1])
     assert_product(got, through(x), through(w), strided[:, 1].double())
+
+
+def test_fp32_master_weight_and_bias(device):
+    gen = torch.Generator().manual_seed(3)
+    x, w, b = torch.randn(40, 96, generator=gen).bfloat16(), torch.randn(70, 96, generator=gen) * 0.05, torch.randn(70, generator=gen)
+    g = (torch.randn(40, 70, generator=gen) * 0.01).bfloat16()
+    leaves = [t.to(device).requires_grad_() for t in (x, w, b)]
+    y = mxfp4_linear(*leaves)
+    assert y.dtype == torch.bfloat16
+    assert_product(y, through(x), through(w), b.double())
+    gx, gw, gb = torch.autograd.grad(y, leaves, g.to(device))
+    assert gx.dtype == torch.bfloat16 and gw.dtype == gb.dtype == torch.float32
+    assert_product(gx, through(g), through(w.t()))
+    assert_product(gw, through(g.t()), through(x.t()))
+    assert ((gb.double().cpu() - g.double().sum(0)).abs() <= 41 * 2.0**-24 * g.double().abs().sum(0)).all()

@@ -1,5 +1,9 @@
 """Calls of the 4-bit and expert entry points that have to be refused on the host, before a kernel sees their operands."""
 
+import ctypes
+
+import pytest
+
 from flex_shard_amd import _native
 
 OK, EINVAL, ENOTSUP = 0, -22, -95
@@ -18,3 +22,36 @@ def test_combine_of_fp32_rows():
         assert call(*args[:at], value, *args[at + 1 :]) == status, (at, value)
         assert _message().startswith("fsh_expert_combine_f32")
     assert call(SOMEWHERE, SOMEWHERE, None, 1, 0, 2, 8, 0, SOMEWHERE, None) == OK
+
+
+def _product(**fields):
+    q = _native.MxFp4Product()
+    for name in ("a_dev", "a_scales_dev", "b_dev", "b_scales_dev", "out_dev"):
+        setattr(q, name, SOMEWHERE)
+    q.m, q.n, q.k, q.a_rows, q.b_rows, q.ldo, q.top_k = 8, 16, 256, 8, 16, 16, 1
+    for name, value in fields.items():
+        setattr(q, name, value)
+    return ctypes.byref(q)
+
+
+BIAS_F32 = _native.MXFP4_BIAS_F32
+
+
+@pytest.mark.parametrize(
+    "fields,status,word",
+    [
+        (dict(mode=BIAS_F32 + 1, experts=1, offsets_dev=SOMEWHERE), EINVAL, "mode"),
+        (dict(mode=BIAS_F32 + 2, experts=1, offsets_dev=SOMEWHERE), EINVAL, "mode"),
+        (dict(mode=2 * BIAS_F32), EINVAL, "mode"),
+        (dict(mode=BIAS_F32, bias_dev=SOMEWHERE + 2), ENOTSUP, "aligned"),
+    ],
+)
+def test_fp32_bias(fields, status, word):
+    assert _native.lib().fsh_mxfp4_gemm(_product(**fields), None) == status
+    assert word in _message()
+
+
+def test_fp32_bias_of_a_few_rows():
+    call = _native.lib().fsh_mxfp4_linear
+    product = _product(m=2, a_rows=2, mode=BIAS_F32, bias_dev=SOMEWHERE + 2)
+    assert call(SOMEWHERE, 0, 2, 256, product, 256, None, 0, None) == ENOTSUP and "aligned" in _message()
