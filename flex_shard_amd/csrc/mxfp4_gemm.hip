@@ -151,6 +151,13 @@ struct MxMode {
   int bias_bytes(int32_t out_dtype) const { return bias_f32 ? 4 : dtype_bytes(out_dtype); }
 };
 
+// A tile of rows in segments holds the first tile of every segment in LDS (kTableBytes).
+int check_experts(MxMode mode, int32_t experts, const char* who) {
+  if (mode.mode == FSH_MXFP4_ROWS && experts > FSH_MAX_EXPERTS)
+    return fail(FSH_ENOTSUP, "%s: rows in segments of at most %d experts, got %d", who, FSH_MAX_EXPERTS, experts);
+  return FSH_OK;
+}
+
 MxFewParams few_params(const fsh_mxfp4_product& q) {
   MxFewParams p;
   memset(&p, 0, sizeof(p));
@@ -176,6 +183,7 @@ FSH_API int fsh_mxfp4_gemm(const fsh_mxfp4_product* product, void* stream) {
   const MxMode mode(q.mode);
   if (!mode.known()) return fail(FSH_EINVAL, "%s: unknown mode %d", who, q.mode);
   if (!mode.dense() && q.experts <= 0) return fail(FSH_EINVAL, "%s: no expert", who);
+  if (int rc = check_experts(mode, q.experts, who)) return rc;
   if (q.m == 0 || q.n == 0) return FSH_OK;
   if (!known_dtype(q.out_dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, q.out_dtype);
   if (!q.a_dev || !q.a_scales_dev || !q.b_dev || !q.b_scales_dev || !q.out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
@@ -233,6 +241,7 @@ FSH_API int fsh_mxfp4_gemm_tiles(int64_t m, int64_t n, int64_t k, int32_t mode, 
   using namespace fsh;
   if (m <= 0 || n <= 0 || k <= 0 || mode < FSH_MXFP4_DENSE || mode > FSH_MXFP4_OVER_ROWS || (mode != FSH_MXFP4_DENSE && experts <= 0))
     return fail(FSH_EINVAL, "fsh_mxfp4_gemm_tiles: bad sizes");
+  if (int rc = check_experts(MxMode(mode), experts, "fsh_mxfp4_gemm_tiles")) return rc;
   MxGemmParams p;
   memset(&p, 0, sizeof(p));
   p.m = m; p.n = n; p.k = ceil_div(k, (int64_t)kMxColumns) * kMxColumns;
@@ -261,6 +270,7 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
   if (q.m == 0 || q.n == 0 || rows == 0) return FSH_OK;
   q.a_rows = rows;
   const MxMode mode(q.mode);
+  if (int rc = check_experts(mode, q.experts, who)) return rc;
   if (mode.dense() && q.m <= kFewQuantize) {
     MxFewParams p = few_params(q);
     if (few_lds_bytes(p, kFewMaxWaves, true) <= 64 * 1024) {

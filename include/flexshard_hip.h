@@ -569,7 +569,8 @@ int fsh_sum_runs(const float* sums_dev, int64_t runs, int64_t cols, void* out_de
  *   FSH_MXFP4_ROWS       rows [offsets[e], offsets[e + 1]) of a's m rows times
  *                        b's rows [e n, (e + 1) n); out rows behind the last
  *                        segment are zero.  With source, row r is row
- *                        source[r] / top_k of a
+ *                        source[r] / top_k of a.  At most FSH_MAX_EXPERTS
+ *                        experts
  *   FSH_MXFP4_OVER_ROWS  out [experts, m, n]: per expert the product over the
  *                        columns [offsets[e], offsets[e + 1]) alone (multiples
  *                        of 256: section 13's padded offsets); zero where empty

@@ -55,3 +55,14 @@ def test_fp32_bias_of_a_few_rows():
     call = _native.lib().fsh_mxfp4_linear
     product = _product(m=2, a_rows=2, mode=BIAS_F32, bias_dev=SOMEWHERE + 2)
     assert call(SOMEWHERE, 0, 2, 256, product, 256, None, 0, None) == ENOTSUP and "aligned" in _message()
+
+
+@pytest.mark.parametrize("experts", [1025, 1 << 20])
+def test_more_experts_than_a_tile_has_a_table_for(experts):
+    fields = dict(mode=_native.MXFP4_ROWS, experts=experts, offsets_dev=SOMEWHERE, b_rows=16 * experts)
+    assert _native.lib().fsh_mxfp4_gemm(_product(**fields), None) == ENOTSUP and "1024 experts" in _message()
+    # (ahead of the quantizer's launch)
+    status = _native.lib().fsh_mxfp4_linear(SOMEWHERE, 0, 8, 256, _product(**fields), 256, SOMEWHERE, 1 << 20, None)
+    assert status == ENOTSUP and "1024 experts" in _message()
+    assert _native.lib().fsh_mxfp4_gemm_tiles(8, 16, 256, _native.MXFP4_ROWS, experts) == ENOTSUP
+    assert _native.lib().fsh_mxfp4_gemm_tiles(8, 16, 256, _native.MXFP4_ROWS, _native.MAX_EXPERTS) >= 0
