@@ -14,7 +14,7 @@ import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
-from .. import hip_ops
+from .. import _native, hip_ops
 
 
 class ExpertRouting:
@@ -27,26 +27,67 @@ class ExpertRouting:
     ``offsets[e + 1]``.  ``source`` [tokens * top_k]: the choice ``t * top_k + j`` of
     each sorted row, -1 behind the last.  ``padded_offsets`` [experts + 1]: the
     segments, each rounded up to 256 rows (a product over an expert's rows).  All
-    int32, behind one another in one buffer."""
+    int32, behind one another in one buffer.
 
-    __slots__ = ("experts", "tokens", "top_k", "rows", "buffer")
+    :func:`route_tokens` makes them.  Kernels index by what the tables hold, so
+    tables of another origin are checked before the first use of a routing
+    (:meth:`check`), which waits for the GPU once."""
+
+    __slots__ = ("experts", "tokens", "top_k", "rows", "buffer", "_sizes", "_checked")
 
     def __init__(
         self, experts: int, position: torch.Tensor, offsets: torch.Tensor, source: torch.Tensor, padded_offsets: torch.Tensor
     ) -> None:
-        self._set(experts, position.shape, torch.cat([position.flatten(), source, offsets, padded_offsets]))
+        tables = (position.flatten(), source.flatten(), offsets.flatten(), padded_offsets.flatten())
+        self._set(experts, position.shape, torch.cat(tables), tuple(t.numel() for t in tables))
 
     @classmethod
     def of_buffer(cls, experts: int, shape: torch.Size, buffer: torch.Tensor) -> "ExpertRouting":
         routing = cls.__new__(cls)
-        routing._set(experts, shape, buffer)
+        routing._set(experts, shape, buffer, None)
         return routing
 
-    def _set(self, experts: int, shape: torch.Size, buffer: torch.Tensor) -> None:
+    def _set(self, experts: int, shape: torch.Size, buffer: torch.Tensor, sizes: tuple[int, ...] | None) -> None:
         self.experts = experts
         self.tokens, self.top_k = shape
         self.rows = self.tokens * self.top_k
         self.buffer = buffer
+        self._sizes = sizes
+        self._checked = False
+
+    def check(self) -> None:
+        """Raise ``ValueError`` unless the tables are an order of the choices by
+        expert as described above.  Nothing to do for those of :func:`route_tokens`."""
+        if not self._checked:
+            self._check_tables()
+            self._checked = True
+
+    def _check_tables(self) -> None:
+        experts, rows, buffer = self.experts, self.rows, self.buffer
+        if not 1 <= experts <= _native.MAX_EXPERTS or self.top_k < 1:
+            raise ValueError(f"a routing has 1 to {_native.MAX_EXPERTS} experts and at least one choice per token, got {experts}, {self.top_k}")
+        sizes = (rows, rows, experts + 1, experts + 1)
+        if buffer.dtype != torch.int32:
+            raise ValueError(f"a routing's tables are int32, got {buffer.dtype}")
+        if buffer.ndim != 1 or not buffer.is_contiguous() or buffer.numel() != sum(sizes) or self._sizes not in (None, sizes):
+            raise ValueError(
+                f"position, source, offsets and padded_offsets must have {sizes} elements, got {self._sizes or tuple(buffer.shape)}"
+            )
+        position, source, offsets, padded = (t.long() for t in buffer.split(sizes))
+        row = torch.arange(rows, device=buffer.device)
+        used = offsets[-1]
+        here = row < used
+        lengths = offsets.diff()
+        right = (
+            (offsets[0] == 0) & (lengths >= 0).all() & (used <= rows)
+            # as many choices with a row as there are rows, and each row that of its choice: one to one
+            & ((position >= -1) & (position < rows)).all() & ((position >= 0).sum() == used)
+            & torch.where(here, (source >= 0) & (source < rows), source == -1).all()
+            & ((position[source.clamp(0, max(rows - 1, 0))] == row) | ~here).all()
+            & (padded[0] == 0) & (padded.diff() == (lengths + 255) // 256 * 256).all()
+        )
+        if not bool(right):
+            raise ValueError("position, offsets, source and padded_offsets are not one order of the choices by expert")
 
     @property
     def position(self) -> torch.Tensor:
@@ -66,6 +107,7 @@ class ExpertRouting:
 
     def pointers(self) -> tuple[int, int, int, int]:
         """Device addresses of position, source, offsets and padded_offsets."""
+        self.check()
         position = self.buffer.data_ptr()
         offsets = position + 8 * self.rows
         return position, position + 4 * self.rows, offsets, offsets + 4 * (self.experts + 1)
@@ -86,7 +128,9 @@ def route_tokens(expert_ids: torch.Tensor, experts: int) -> ExpertRouting:
         raise ValueError(f"at least one expert, got {experts}")
     if not expert_ids.is_contiguous():
         expert_ids = expert_ids.contiguous()
-    return ExpertRouting.of_buffer(experts, expert_ids.shape, hip_ops.expert_route_buffer(expert_ids, experts))
+    routing = ExpertRouting.of_buffer(experts, expert_ids.shape, hip_ops.expert_route_buffer(expert_ids, experts))
+    routing._checked = True
+    return routing
 
 
 def differentiates(*tensors: torch.Tensor | None) -> bool:
@@ -98,8 +142,10 @@ def differentiates(*tensors: torch.Tensor | None) -> bool:
     return torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
 
 
-def _check_device(routing: ExpertRouting, *tensors: torch.Tensor) -> None:
+def check_routing(routing: ExpertRouting, *tensors: torch.Tensor) -> None:
+    """The routing's tables and the tensors of a call are on one GPU, and the tables in order."""
     hip_ops._require_gpu(routing.buffer, *tensors)
+    routing.check()
 
 
 class _Dispatch(torch.autograd.Function):
@@ -145,7 +191,7 @@ def dispatch_tokens(x: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
     its rows' gradients, in fp32 in the order of its choices."""
     if x.ndim != 2 or x.shape[0] != routing.tokens:
         raise ValueError(f"x must be [{routing.tokens}, width], got {tuple(x.shape)}")
-    _check_device(routing, x)
+    check_routing(routing, x)
     x = x.contiguous()
     return _Dispatch.apply(x, routing) if differentiates(x) else _dispatch(x, routing)
 
@@ -158,7 +204,7 @@ def combine_tokens(rows: torch.Tensor, routing: ExpertRouting, weights: torch.Te
         raise ValueError(f"rows must be [{routing.rows}, width], got {tuple(rows.shape)}")
     if tuple(weights.shape) != (routing.tokens, routing.top_k):
         raise ValueError(f"weights must be {(routing.tokens, routing.top_k)}, got {tuple(weights.shape)}")
-    _check_device(routing, rows, weights)
+    check_routing(routing, rows, weights)
     rows, weights = rows.contiguous(), weights.contiguous()
     return _Combine.apply(rows, weights, routing) if differentiates(rows, weights) else _combine(rows, weights, routing)
 

@@ -20,7 +20,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .. import _native, hip_ops
-from ..experts import ExpertRouting, differentiates
+from ..experts import ExpertRouting, check_routing, differentiates
 from ..hip_ops import MxFp4Matrix
 from .mxfp4_matrix import MxFp4Weight, as_rows
 
@@ -207,7 +207,7 @@ def mxfp4_expert_linear(
     if routing.rows == 0 or out_dim == 0:
         dense = x.new_empty((out_dim, in_dim)) if frozen is not None else weight[0].to(x.dtype)
         return nn.functional.linear(x.new_zeros((routing.rows, in_dim)) + 0 * x.sum(), dense)
-    hip_ops._require_gpu(routing.buffer, x)
+    check_routing(routing, x)
     x = as_rows(x)
     if differentiates(x, None if frozen else weight):
         return _ExpertLinear.apply(x, None if frozen else weight, routing, sorted_rows, frozen)
