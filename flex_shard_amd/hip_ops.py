@@ -1038,13 +1038,26 @@ class MxFp4Matrix:
     __slots__ = ("buffer", "rows", "cols")
 
     def __init__(self, buffer: torch.Tensor, rows: int, cols: int) -> None:
+        # kernels read as many bytes as the sizes say
+        nbytes = rows * -(-cols // 256) * 136
+        if (
+            rows < 0 or cols < 0 or buffer.dtype is not torch.uint8 or buffer.ndim != 1 or buffer.numel() != nbytes
+            or not buffer.is_contiguous()
+        ):
+            raise ValueError(
+                f"a 4-bit matrix [{rows}, {cols}] is {nbytes} contiguous uint8, got {buffer.dtype} {tuple(buffer.shape)} / {buffer.stride()}"
+            )
         self.buffer = buffer
         self.rows = rows
         self.cols = cols
 
     @classmethod
     def empty(cls, rows: int, cols: int, device: torch.device) -> "MxFp4Matrix":
-        return cls(torch.empty(rows * -(-cols // 256) * 136, dtype=torch.uint8, device=device), rows, cols)
+        matrix = cls.__new__(cls)
+        matrix.buffer = torch.empty(rows * -(-cols // 256) * 136, dtype=torch.uint8, device=device)
+        matrix.rows = rows
+        matrix.cols = cols
+        return matrix
 
     @property
     def steps(self) -> int:
@@ -1075,6 +1088,7 @@ class MxFp4Matrix:
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values [rows, cols] in bf16, fp16 or fp32."""
         buffer, rows, cols = self.buffer, self.rows, self.cols
+        _require_gpu(buffer)
         out = torch.empty((rows, cols), dtype=dtype, device=buffer.device)
         data, scales = self.pointers()
         status = _native.lib().fsh_mxfp4_dequantize(

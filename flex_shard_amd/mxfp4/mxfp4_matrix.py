@@ -52,6 +52,15 @@ class MxFp4Weight:
     matrix: MxFp4Matrix
     transposed: MxFp4Matrix | None = None
 
+    def __post_init__(self) -> None:
+        if len(self.shape) not in (2, 3):
+            raise ValueError(f"a weight is [out, in] or [experts, out, in], got {tuple(self.shape)}")
+        *experts, rows, cols = self.shape
+        count = experts[0] if experts else 1
+        for form, want in ((self.matrix, (count * rows, cols)), (self.transposed, (count * cols, rows))):
+            if form is not None and (form.rows, form.cols) != want:
+                raise ValueError(f"a weight {tuple(self.shape)} has a form {want}, got {(form.rows, form.cols)}")
+
 
 def quantize_mxfp4_weight(weight: torch.Tensor, *, transposed: bool = False) -> MxFp4Weight:
     """Quantize a weight that stays as it is: serving, or a frozen layer
