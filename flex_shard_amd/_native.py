@@ -149,6 +149,7 @@ MXFP4_DENSE, MXFP4_ROWS, MXFP4_OVER_ROWS = 0, 1, 2
 MXFP4_BIAS_F32 = 256
 MXFP4_FEW_ROWS = 4
 MAX_EXPERTS = 1024
+MAX_CHOICES = 64
 MAX_NS_PROBLEMS = 16
 MUON_PADDED = 1
 MAX_COPY_ROWS = 32

@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void expert_combine_kernel(const RowsPara
 
 // One token: a piece of its gradient is read once for eight choices, whose rows are
 // in flight together; the dot products are joined over the workgroup in a fixed order.
-constexpr int kMaxTopK = 64;
+constexpr int kMaxTopK = FSH_MAX_CHOICES;
 template <int DT, bool kVec>
 __global__ __launch_bounds__(kThreads) void expert_combine_backward_kernel(const RowsParams p) {
   using P = Piece<DT, kVec>;

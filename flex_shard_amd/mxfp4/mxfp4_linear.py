@@ -210,6 +210,11 @@ def mxfp4_expert_linear(
     check_routing(routing, x)
     x = as_rows(x)
     if differentiates(x, None if frozen else weight):
+        if x.requires_grad and not sorted_rows and routing.top_k > _native.MAX_CHOICES:
+            raise NotImplementedError(
+                f"a gradient for the tokens adds up at most {_native.MAX_CHOICES} choices each, got {routing.top_k} (rows in sorted order, "
+                "sorted_rows=True, have no such limit)"
+            )
         return _ExpertLinear.apply(x, None if frozen else weight, routing, sorted_rows, frozen)
     return _expert_forward(x, _weight_forms(weight, False)[0], routing, sorted_rows)
 

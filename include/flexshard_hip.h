@@ -632,9 +632,11 @@ int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int64_t ldx
  * fsh_expert_combine_backward: grad_rows[position[t, j]] = weights[t, j] *
  * grad[t], zero behind offsets[experts]; grad_weights[t, j] = <grad[t],
  * rows[position[t, j]]>, zero for no expert.  Rows of `width` elements,
- * contiguous; x, rows and their gradients of one dtype, weights of its own.
+ * contiguous; x, rows and their gradients of one dtype, weights of its own.  At
+ * most FSH_MAX_CHOICES choices per token in these.
  * ---------------------------------------------------------------------- */
 #define FSH_MAX_EXPERTS 1024
+#define FSH_MAX_CHOICES 64
 int64_t fsh_expert_route_workspace_bytes(int64_t choices, int32_t experts);
 int fsh_expert_route(const void* expert_ids_dev, int32_t id_bytes, int64_t choices, int32_t experts, int32_t* position_dev,
                      int32_t* offsets_dev, int32_t* source_dev, int32_t* padded_offsets_dev, void* workspace_dev,
