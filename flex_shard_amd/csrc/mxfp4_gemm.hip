@@ -262,12 +262,13 @@ FSH_API int fsh_mxfp4_linear(const void* x_dev, int32_t dtype, int64_t rows, int
   using namespace fsh;
   const char* who = "fsh_mxfp4_linear";
   if (!product) return fail(FSH_EINVAL, "%s: null product", who);
-  if (rows < 0 || in_dim < 0) return fail(FSH_EINVAL, "%s: negative shape", who);
   fsh_mxfp4_product q = *product;
+  if (rows < 0 || in_dim < 0 || q.m < 0 || q.n < 0) return fail(FSH_EINVAL, "%s: negative shape", who);
   if (q.k != ceil_div(in_dim, (int64_t)kMxColumns) * kMxColumns)
     return fail(FSH_EINVAL, "%s: k %lld is not in_dim %lld rounded up to %d", who, (long long)q.k, (long long)in_dim, kMxColumns);
   if (q.out_dtype != dtype) return fail(FSH_EINVAL, "%s: the output has the activation's dtype", who);
-  if (q.m == 0 || q.n == 0 || rows == 0) return FSH_OK;
+  if (q.m == 0 || q.n == 0) return FSH_OK;
+  if (q.k == 0) return fail(FSH_ENOTSUP, "%s: in_dim must be positive", who);
   q.a_rows = rows;
   const MxMode mode(q.mode);
   if (int rc = check_experts(mode, q.experts, who)) return rc;

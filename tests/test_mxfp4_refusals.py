@@ -66,3 +66,21 @@ def test_more_experts_than_a_tile_has_a_table_for(experts):
     assert status == ENOTSUP and "1024 experts" in _message()
     assert _native.lib().fsh_mxfp4_gemm_tiles(8, 16, 256, _native.MXFP4_ROWS, experts) == ENOTSUP
     assert _native.lib().fsh_mxfp4_gemm_tiles(8, 16, 256, _native.MXFP4_ROWS, _native.MAX_EXPERTS) >= 0
+
+
+@pytest.mark.parametrize(
+    "fields,in_dim,status,word",
+    [(dict(m=-1), 256, EINVAL, "negative"), (dict(m=2, n=-100, ldo=16), 256, EINVAL, "negative"), (dict(m=2, k=0), 0, ENOTSUP, "positive"),
+     (dict(m=8, k=0), 0, ENOTSUP, "positive"), (dict(m=2, k=-256), 256, EINVAL, "in_dim")],
+)
+def test_linear_sizes(fields, in_dim, status, word):
+    call = _native.lib().fsh_mxfp4_linear
+    assert call(SOMEWHERE, 0, 8, 256, _product(**fields), in_dim, SOMEWHERE, 1 << 20, None) == status
+    assert word in _message()
+
+
+@pytest.mark.parametrize("m", [2, 8])
+def test_linear_of_no_rows_has_no_outputs(m):
+    call = _native.lib().fsh_mxfp4_linear
+    assert call(SOMEWHERE, 0, 0, 256, _product(m=m), 256, SOMEWHERE, 1 << 20, None) == EINVAL  # outputs that nothing would write
+    assert call(SOMEWHERE, 0, 0, 256, _product(m=0), 256, None, 0, None) == OK
