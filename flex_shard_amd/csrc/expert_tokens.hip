@@ -11,8 +11,8 @@
 // The sort is bound by latency; the others by memory: every row of the experts
 // is read or written once, the tokens' rows once.  Measured, 8192 tokens of 7168
 // bf16, 8 of 32 experts each: sort 13 us; dispatch 187 us, 5.7 TB/s; combine 212 us,
-// 5.0; its gradient 393 us, 5.1; 4096 tokens' fp32 rows to bf16 194 us, 5.1.  16 tokens: 3.6, 4.2 and 4.8 us, a launch's chain
-// of loads each.
+// 5.0; its gradient 393 us, 5.1.  4096 tokens' fp32 rows combined to bf16: 205 us,
+// 4.9.  16 tokens: 3.6, 4.2 and 4.8 us, a launch's chain of loads each.
 #include "mxfp4.hpp"
 
 namespace fsh {
@@ -68,7 +68,9 @@ __global__ __launch_bounds__(kThreads) void expert_count_kernel(const RouteParam
 }
 
 // Each wave places a quarter of the block's choices, 64 at a time: a choice's
-// rank among the 64 is the number of earlier lanes with its expert.
+// rank among the 64 is the number of earlier lanes with its expert.  Every block
+// reads all blocks' counts, which in all is quadratic in the choices: 32 blocks of
+// 32 counts for 8192 tokens of 8 choices, 4 KB a block.
 __global__ __launch_bounds__(kThreads) void expert_place_kernel(const RouteParams p) {
   __shared__ int32_t next[kWaves][kMaxExperts];  // first the waves' counts, then the next row of each expert
   __shared__ int32_t total[kMaxExperts + 1], before[kMaxExperts];  // of all blocks, of those before this one

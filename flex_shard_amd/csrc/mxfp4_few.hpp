@@ -1,7 +1,7 @@
 // The product of few rows with a microscaled 4-bit weight: a token, or a few.
 // Bound by the weight's bytes, and where those are few by the chain of one launch:
-// loads, products, sums.  One row: 14336, k 4096 (31 MB) 8.8 us, 3.6 TB/s; 4096, k
-// 4096 4.1; 4096, k 14336 9.6; 1024, k 4096 3.2.
+// loads, products, sums.  One row: 14336, k 4096 (31 MB) 8.5 to 8.8 us, 3.6 TB/s;
+// 4096, k 4096 4.1 to 4.3; 4096, k 14336 9.6; 1024, k 4096 3.2 to 3.5.
 //
 // A workgroup owns 16 rows of the weight and all (at most 16) rows of the
 // activation; its waves take the contraction's steps of 256 columns in turn,

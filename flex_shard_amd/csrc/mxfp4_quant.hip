@@ -95,9 +95,12 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_rows_kernel(const MxQ
 // so a column's run lies in one thread.  Its 16 bytes go through LDS once more to
 // leave as 64 bytes per column.  With kRows the row runs leave from the registers
 // that the tile was loaded into.  Gathered rows (65536 x 7168 of 8192 tokens' rows,
-// 234 us) cost what as many rows of a matrix do, though each comes from memory
-// once: per element the conversions bound it then.  Neighbouring tiles on one XCD
-// were slower (8192 x 14336 both 77 to 84 us).
+// 234 us) cost what as many rows of a matrix do: a token's choices are in the tiles
+// of different experts, so its row crosses into an L2 once for each, out of the
+// memory-side cache if not from memory.  By the counters the L2s miss 1.14 GB (1.19
+// of a matrix), 4.9 TB/s, the rate of a copy; the 9 vector instructions an element
+// (5) would take about half of the time.  Neighbouring tiles on one XCD were slower
+// (8192 x 14336 both 77 to 84 us).
 constexpr int kTile = 128;
 template <int DT, bool kRows>
 __global__ __launch_bounds__(kThreads) void mxfp4_quantize_columns_kernel(const MxQuantParams p) {
