@@ -70,3 +70,20 @@ def test_fp32_master_weight_and_bias(device):
     assert_product(gx, through(g), through(w.t()))
     assert_product(gw, through(g.t()), through(x.t()))
     assert ((gb.double().cpu() - g.double().sum(0)).abs() <= 41 * 2.0**-24 * g.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("needs_x", [False, True])
+def test_bias_gradient_beside_a_frozen_weight(device, needs_x, bias_dtype):
+    gen = torch.Generator().manual_seed(6)
+    x, w = torch.randn(300, 96, generator=gen).bfloat16(), torch.randn(70, 96, generator=gen) * 0.05
+    g, bias = torch.randn(300, 70, generator=gen).bfloat16(), torch.randn(70, generator=gen).to(bias_dtype)
+    leaves = [bias.to(device).requires_grad_()] + ([x.to(device).requires_grad_()] if needs_x else [])
+    y = mxfp4_linear(leaves[1] if needs_x else x.to(device), quantize_mxfp4_weight(w.to(device), transposed=needs_x), leaves[0])
+    assert_product(y, through(x), through(w), bias.double())
+    gb, *gx = torch.autograd.grad(y, leaves, g.to(device))
+    size, want = g.double().abs().sum(0), g.double().sum(0)
+    assert gb.dtype == bias_dtype
+    assert ((gb.double().cpu() - want).abs() <= 300 * 2.0**-24 * size + (2.0**-8 if bias_dtype == torch.bfloat16 else 2.0**-24) * want.abs()).all()
+    if needs_x:
+        assert_product(gx[0], through(g), through(w.t()))
