@@ -336,10 +336,12 @@ def _through_8_bits(y: torch.Tensor) -> torch.Tensor:
 # 2**-100).  A code stands for the fp32 number whose upper bits, 3 of the mantissa
 # and those of the exponent, it counts down from 1.0 = 1016 * 2**20: the first
 # moment has a sign and the codes 1 to 127 (to 1.0), the second the codes 1 to 255; 0
-# is zero.  Rounding up or down goes by a dither that runs evenly through [0, 1) over
-# the elements and over the steps.
-def _dither(index: torch.Tensor, t: int, over_elements: int, over_steps: int) -> torch.Tensor:
-    return (index.long() * over_elements + t * over_steps) & 0xFFFFFFFF
+# is zero.  Rounding up or down goes by a dither in [0, 1) that every element has anew
+# in every step: half of a word that is mixed from the element's index and the step's.
+def _dither(index: torch.Tensor, t: int) -> torch.Tensor:
+    z = (index.long() * 0x9E3779B9 + t * 0x6A09E667) & 0xFFFFFFFF
+    z = ((z ^ (z >> 16)) * 0xBB67AE85) & 0xFFFFFFFF
+    return z ^ (z >> 15)
 
 
 def _scaled(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -350,7 +352,7 @@ def _scaled(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _first_moment_codes(m: torch.Tensor, index: torch.Tensor, t: int) -> tuple[torch.Tensor, torch.Tensor]:
     size, scale = _scaled(m)
-    u = _dither(index, t, 0xC13FA9A9, 0x91E10DA5)
+    u = (_dither(index, t) & 0xFFFF) << 16
     code = ((size.view(torch.int32) + (u >> 12)) >> 20) - 889
     smallest = 1.25 * 2.0**-16
     few = (size * (1.0 / smallest) > (u >> 8).float() * 2.0**-24).long()
@@ -360,7 +362,7 @@ def _first_moment_codes(m: torch.Tensor, index: torch.Tensor, t: int) -> tuple[t
 
 def _second_moment_codes(v: torch.Tensor, index: torch.Tensor, t: int) -> tuple[torch.Tensor, torch.Tensor]:
     size, scale = _scaled(v)
-    u = _dither(index, t, 0x9E3779B9, 0x6A09E667)
+    u = _dither(index, t) >> 16 << 16
     code = ((size.view(torch.int32) + (u >> 12)) >> 20) - 761
     # (what is not zero stays so: a first moment is never divided by nothing)
     return torch.where(size > 0, code.clamp(min=1), 0).to(torch.uint8), scale
@@ -450,8 +452,7 @@ def _exact_adamw(state: dict):
         v = b2 * v + (1 - b2) * g**2
         p = p - lr * DECAY * p - lr * (m / (1 - b1**t)) / (torch.sqrt(v / (1 - b2**t)) + ADAM_EPS)
         if eight:
-            m = _exact_state(m, t, (0xC13FA9A9, 0x91E10DA5), 127)
-            v = _exact_state(v, t, (0x9E3779B9, 0x6A09E667), 255)
+            m, v = _exact_state(m, t, 127), _exact_state(v, t, 255)
         for kept, value in zip((params, firsts, seconds), (p, m, v)):
             kept.append(value.view(shape))
     return params, firsts, seconds
@@ -463,7 +464,7 @@ def _at(place: torch.Tensor) -> torch.Tensor:
     return (1.0 + (place - 8 * octave) / 8.0) * torch.exp2(octave.double())
 
 
-def _exact_state(x: torch.Tensor, t: int, steps: tuple[int, int], codes: int) -> torch.Tensor:
+def _exact_state(x: torch.Tensor, t: int, codes: int) -> torch.Tensor:
     """Up to the next of the numbers of a code where the dither is less than what
     is missing of the step above it, down otherwise."""
     count = x.numel()
@@ -473,7 +474,10 @@ def _exact_state(x: torch.Tensor, t: int, steps: tuple[int, int], codes: int) ->
     scale = blocks.abs().max(dim=1, keepdim=True).values.clamp(min=2.0**-100)
     size = blocks.abs() / scale
     index = torch.arange(blocks.numel(), device=x.device).view_as(blocks)
-    u = ((index * steps[0] + t * steps[1]) % 2**32).double() / 2**32
+    word = (index * 0x9E3779B9 + t * 0x6A09E667) % 2**32
+    word = (word ^ word // 2**16) * 0xBB67AE85 % 2**32
+    word = word ^ word // 2**15
+    u = (word % 2**16 if codes == 127 else word // 2**16).double() / 2**16
     _, exponent = torch.frexp(size)
     step = torch.exp2((exponent - 4).double())
     below = torch.floor(size / step)
