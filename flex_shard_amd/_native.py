@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libflexshard_hip.so")
@@ -142,6 +142,44 @@ class MxFp4Product(Structure):
         ("mode", c_int32),
         ("experts", c_int32),
         ("top_k", c_int32),
+    ]
+
+
+NORM_VALUES, NORM_FP8 = 0, 1
+
+
+class Norm(Structure):  # fsh_norm
+    _fields_ = [
+        *((name, c_void_p) for name in ("x_dev", "residual_dev", "weight_dev", "total_dev", "out_dev", "scales_dev", "rstd_dev")),
+        *((name, c_int64) for name in ("rows", "cols", "ldx", "ldr")),
+        *((name, c_int32) for name in ("x_dtype", "residual_dtype", "weight_dtype", "form")),
+        ("eps", c_float),
+        ("reserved", c_int32),
+    ]
+
+
+class NormGradient(Structure):  # fsh_norm_gradient
+    _fields_ = [
+        *(
+            (name, c_void_p)
+            for name in (
+                "grad_dev", "total_dev", "weight_dev", "rstd_dev", "grad_total_dev", "grad_x_dev", "grad_residual_dev",
+                "grad_weight_dev", "workspace_dev",
+            )
+        ),
+        *((name, c_int64) for name in ("workspace_nbytes", "rows", "cols", "ldg", "ldh", "ldt")),
+        *((name, c_int32) for name in ("grad_dtype", "total_dtype", "x_dtype", "weight_dtype")),
+    ]
+
+
+ADAMW_BLOCK, ADAMW_GROUPS = 128, 16
+ADAMW_TENSOR_INT64S = 12  # fsh_adamw_tensor
+
+
+class AdamWGroup(Structure):  # fsh_adamw_group
+    _fields_ = [
+        ("lr", c_double), ("lr_dev", c_void_p), ("beta1", c_double), ("beta2", c_double), ("eps", c_double),
+        ("weight_decay", c_double),
     ]
 
 
@@ -282,6 +320,23 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p,
          c_void_p, c_void_p],
+    ),
+    "fsh_rms_norm": (c_int, [POINTER(Norm), c_void_p]),
+    "fsh_rms_norm_backward_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "fsh_rms_norm_backward": (c_int, [POINTER(NormGradient), c_void_p]),
+    "fsh_rms_norm_token_runs": (
+        c_int,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p],
+    ),
+    "fsh_act_dequant_1x128": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
+    "fsh_grad_square_sum_workspace_bytes": (c_int64, [POINTER(c_int64), c_int32]),
+    "fsh_grad_square_sum": (c_int, [POINTER(c_int64), c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fsh_adamw_step_workspace_bytes": (c_int64, [c_int32]),
+    "fsh_adamw_step": (
+        c_int, [POINTER(c_int64), c_int32, POINTER(AdamWGroup), c_int32, c_void_p, c_double, c_void_p, c_int64, c_void_p],
+    ),
+    "fsh_adamw_state_values": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p],
     ),
 }
 

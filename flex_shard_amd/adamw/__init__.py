@@ -1,0 +1,210 @@
+"""AdamW for what Muon does not update (or for everything), many tensors at a time.
+
+:class:`FlexShardAdamW` is a ``torch.optim.Optimizer`` whose step is one table of
+tensors on the HIP kernels, with fp32 states or with 8-bit ones.  Clipping by the
+gradients' norm is part of the step's one pass over them:
+
+    square_sum = grad_square_sum([p.grad for p in params])   # all_reduce it over the ranks' shards
+    optimizer.step(square_sum=square_sum, max_norm=1.0)
+"""
+
+from __future__ import annotations
+
+from typing import Any, Iterable, Sequence
+
+import torch
+
+from .. import _native, hip_ops
+from .._native import ADAMW_BLOCK, ADAMW_GROUPS, DT_BF16, DT_F32
+
+_DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
+
+
+def grad_square_sum(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
+    """The sum of the squares of the gradients' elements (bf16, fp16 or fp32, all on
+    one GPU; None is left out), a float64 scalar there: the square of their
+    common norm.  Products and sums in 64 bits, in an order that the sizes alone decide.  Of
+    sharded gradients it is this rank's part: add the ranks' up before it is used."""
+    present = [g.detach() if g.is_contiguous() else g.detach().contiguous() for g in grads if g is not None]
+    if not present:
+        raise ValueError("at least one gradient")
+    return hip_ops.grad_square_sum(present)
+
+
+class FlexShardAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) on contiguous bf16 or fp32 parameters, each
+    with a gradient of either type, all on one GPU.
+
+    ``state_bits`` 32: ``exp_avg`` and ``exp_avg_sq`` are fp32 whatever the parameter's type.
+    8: they are uint8 codes with fp32 scales for every 128 elements (``exp_avg_scale``,
+    ``exp_avg_sq_scale``; :meth:`state_values` gives what they stand for): 2 1/16
+    bytes an element for 8.  Arithmetic is in fp32, the parameter rounded once.  ``step`` is
+    an int32 on the GPU, so that a captured step counts on; ``lr`` may be an fp32 scalar
+    there, which a captured step reads anew.  Parameters without a gradient are left alone."""
+
+    def __init__(
+        self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+        weight_decay: float = 1e-2, *, state_bits: int = 32,
+    ) -> None:
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group: dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            beta1, beta2 = group["betas"]
+            if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
+                raise ValueError(f"betas must be in [0, 1), got {group['betas']}")
+            for name in ("eps", "weight_decay"):
+                if not group[name] >= 0:
+                    raise ValueError(f"{name} must not be negative, got {group[name]}")
+            if not isinstance(group["lr"], torch.Tensor) and not group["lr"] >= 0:
+                raise ValueError(f"lr must not be negative, got {group['lr']}")
+            if group["state_bits"] not in (8, 32):
+                raise NotImplementedError(f"states have 8 or 32 bits, got {group['state_bits']}")
+            for p in group["params"]:
+                if p.dtype not in _DT:
+                    raise NotImplementedError(f"the AdamW kernels update bf16 or fp32 parameters, got {p.dtype}")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    # ------------------------------------------------------------------- states
+    def _new_state(self, p: torch.Tensor, bits: int) -> dict[str, torch.Tensor]:
+        if torch.cuda.is_current_stream_capturing():
+            # the zeros would be part of the graph, and every replay would begin with them
+            raise RuntimeError("the states of an AdamW step must exist before it is captured: run one step, or load them")
+        blocks = -(-p.numel() // ADAMW_BLOCK)
+        kind, device = torch.float32 if bits == 32 else torch.uint8, p.device
+        state = {"step": torch.zeros((), dtype=torch.int32, device=device)}
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros(p.shape, dtype=kind, device=device)
+            if bits == 8:
+                state[f"{name}_scale"] = torch.zeros((blocks,), dtype=torch.float32, device=device)
+        return state
+
+    def state_values(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+        """``exp_avg`` and ``exp_avg_sq`` of a parameter as numbers."""
+        state = self.state.get(param)
+        if not state:
+            raise KeyError("this parameter has no state yet")
+        if state["exp_avg"].dtype != torch.uint8:
+            return state["exp_avg"].to(dtype), state["exp_avg_sq"].to(dtype)
+        return hip_ops.adamw_state_values(
+            state["exp_avg"], state["exp_avg_scale"], state["exp_avg_sq"], state["exp_avg_sq_scale"], dtype
+        )
+
+    def load_state_dict(self, state_dict: dict[str, Any]) -> None:
+        """Copies of the saved states, of the types that they have here (``torch``'s
+        own loading would cast them to the parameters')."""
+        saved_groups = state_dict["param_groups"]
+        loaded = {}
+        if [len(g["params"]) for g in saved_groups] == [len(g["params"]) for g in self.param_groups]:
+            for group, saved in zip(self.param_groups, saved_groups):
+                for p, index in zip(group["params"], saved["params"]):
+                    if index in state_dict["state"]:
+                        loaded[p] = self._copy_of(p, saved.get("state_bits", 32), state_dict["state"][index])
+        super().load_state_dict({**state_dict, "state": {}})
+        self.state.update(loaded)
+
+    def _copy_of(self, p: torch.Tensor, bits: int, saved: dict[str, Any]) -> dict[str, torch.Tensor]:
+        state = self._new_state(p, bits)
+        state["step"].fill_(int(saved["step"]))
+        for name, mine in state.items():
+            if name == "step":
+                continue
+            value = saved.get(name)
+            if value is None or value.shape != mine.shape or (value.dtype == torch.uint8) != (mine.dtype == torch.uint8):
+                got = None if value is None else f"{value.dtype} {tuple(value.shape)}"
+                raise ValueError(f"{bits}-bit states need {name} as {mine.dtype} {tuple(mine.shape)}, got {got}")
+            mine.copy_(value)
+        return state
+
+    # --------------------------------------------------------------------- step
+    @torch.no_grad()
+    def step(self, closure=None, *, square_sum: torch.Tensor | None = None, max_norm: float | None = None):
+        """One step on the parameters' ``.grad``.  With ``square_sum`` (of
+        :func:`grad_square_sum`) and ``max_norm`` the gradients are scaled by min(1, max_norm /
+        (sqrt(square_sum) + 1e-6)) as they are read.  A ``square_sum`` that is an infinity
+        or not a number leaves parameters, states and step counts as they are."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if max_norm is not None and (square_sum is None or not max_norm > 0):
+            raise ValueError(f"clipping needs the gradients' square_sum and a positive max_norm, got {max_norm}")
+        device = None
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is not None:
+                    device = p.device if device is None else device
+                    _check_pair(p, p.grad, device)
+        if device is None:
+            return loss
+        if square_sum is not None and (square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device):
+            raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
+        groups: list[tuple] = []
+        table: list[int] = []
+        calls = [(table, groups)]
+        stepped, copies = [], []  # (the queued kernels read the copies)
+        for group in self.param_groups:
+            lr, address = group["lr"], None
+            if isinstance(lr, torch.Tensor):
+                lr, address = _learning_rate(lr, device)
+            if len(groups) == ADAMW_GROUPS:
+                table, groups = [], []
+                calls.append((table, groups))
+            bits, index = group["state_bits"], len(groups)
+            for p in group["params"]:
+                if p.grad is not None:
+                    stepped.append(p)
+                    table += self._row(p, bits, index, copies)
+            groups.append((lr, address, *group["betas"], group["eps"], group["weight_decay"]))
+        for table, groups in calls:  # (nothing is queued before all of it has been checked)
+            hip_ops.adamw_step(table, groups, device, square_sum, max_norm or 0.0)
+        torch.autograd.graph.increment_version(stepped)
+        return loss
+
+    def _row(self, p: torch.Tensor, bits: int, group: int, copies: list) -> Sequence[int]:
+        """The twelve numbers of an ``fsh_adamw_tensor``."""
+        g = p.grad
+        if not g.is_contiguous():
+            g = g.contiguous()
+            copies.append(g)
+        state = self.state[p]
+        if not state:
+            state.update(self._new_state(p, bits))
+        m, v = state["exp_avg"], state["exp_avg_sq"]
+        if (m.dtype == torch.uint8) != (bits == 8):
+            raise ValueError(f"states of {m.dtype} do not go with state_bits={bits}")
+        scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if bits == 8 else (0, 0)
+        return (
+            p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), *scales, state["step"].data_ptr(), p.numel(),
+            _DT[p.dtype], _DT[g.dtype], bits, group,
+        )
+
+
+def _check_pair(p: torch.Tensor, g: torch.Tensor, device: torch.device) -> None:
+    """That the kernels can take a parameter and its gradient."""
+    if p.device.type != "cuda":
+        raise RuntimeError("flex_shard_amd kernels run on the GPU only; there is no CPU path.")
+    if p.dtype not in _DT or g.dtype not in _DT or g.layout != torch.strided:
+        raise NotImplementedError(f"the AdamW kernels take dense bf16 or fp32 parameters and gradients, got {p.dtype} and {g.dtype} ({g.layout})")
+    if p.device != device or g.device != device:
+        raise ValueError(f"all parameters and gradients of a step must live on {device}, got {p.device} and {g.device}")
+    if not p.is_contiguous() or g.shape != p.shape:
+        raise ValueError(f"contiguous parameters with gradients of their shape, got {tuple(p.shape)} / {p.stride()} and {tuple(g.shape)}")
+
+
+def _learning_rate(lr: torch.Tensor, device: torch.device) -> tuple[float, int | None]:
+    """A learning rate in a tensor: as a number, and its address on the GPU."""
+    if lr.numel() != 1:
+        raise ValueError(f"lr must be one number, got {tuple(lr.shape)}")
+    if lr.device.type == "cpu":
+        return float(lr), None
+    if lr.device != device or lr.dtype != torch.float32:
+        raise ValueError(f"lr on the GPU must be fp32 on {device}, got {lr.dtype} on {lr.device}")
+    return 0.0, lr.data_ptr()
+
+
+__all__ = ["FlexShardAdamW", "grad_square_sum"]

@@ -1,0 +1,77 @@
+"""An activation that is already quantized when a linear reads it."""
+
+from __future__ import annotations
+
+from typing import Any, Callable
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import hip_ops
+
+
+class Fp8Activation:
+    """Rows of E4M3 bytes with a scale for every run of 128 columns, as the FP8
+    linear's quantizer writes them: ``q`` float8_e4m3fn [rows, cols rounded up to
+    128], ``scales`` fp32 [that / 128, rows], for an activation of ``shape`` [..., cols].
+
+    ``FlexShardFloat8BlockwiseLinear`` and ``prequantized_linear`` take one in place of
+    an activation.  ``carrier`` stands for it in autograd: a bf16 tensor of that
+    shape without values of its own, through which the linears' gradients reach what
+    made the activation, unrounded by the quantizer (straight through)."""
+
+    __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_runs")
+
+    def __init__(
+        self, q: torch.Tensor, scales: torch.Tensor, carrier: torch.Tensor,
+        make_token_runs: Callable[[], tuple[torch.Tensor, torch.Tensor]],
+    ) -> None:
+        self.q = q
+        self.scales = scales
+        self.shape = carrier.shape
+        self.carrier = carrier
+        self._make_runs = make_token_runs
+        self._runs: tuple | None = None
+
+    @property
+    def ndim(self) -> int:
+        return len(self.shape)
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+    def token_runs(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The activation in runs of 128 tokens, transposed, with its scales: what a
+        weight gradient contracts over.  Made when the first linear asks for it, for
+        all that do so on the same stream."""
+        stream = hip_ops.stream_ptr(self.q.device)
+        if self._runs is None or self._runs[0] != stream:
+            self._runs = (stream, self._make_runs())
+        return self._runs[1]
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The values, differentiable straight through the quantizer."""
+        if torch.is_grad_enabled() and self.carrier.requires_grad:
+            return _Dequantize.apply(self.carrier, self, dtype)
+        return self._values(dtype)
+
+    def _values(self, dtype: torch.dtype) -> torch.Tensor:
+        return hip_ops.act_dequant_1x128(self.q, self.scales, self.shape[-1], dtype).view(self.shape)
+
+    def __repr__(self) -> str:
+        return f"Fp8Activation(shape={tuple(self.shape)})"
+
+
+class _Dequantize(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, carrier: torch.Tensor, activation: Fp8Activation, dtype: torch.dtype) -> torch.Tensor:
+        return activation._values(dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: torch.Tensor):
+        return grad.to(torch.bfloat16), None, None
+
+
+__all__ = ["Fp8Activation"]

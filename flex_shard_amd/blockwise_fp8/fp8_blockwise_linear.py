@@ -33,6 +33,7 @@ from torch.autograd import forward_ad
 
 from .. import hip_ops
 from .blockwise_fp8_weight import BlockwiseFp8Weight
+from .fp8_activation import Fp8Activation
 
 
 def _pad_last_dim_to(tensor: torch.Tensor, target_dim: int) -> torch.Tensor:
@@ -133,18 +134,26 @@ class Fp8BlockwiseGemms:
         if x_2d.shape[1] != in_dim:
             raise ValueError(f"input last dim {x_2d.shape[1]} does not match weight input dim {in_dim}")
         x_2d = _as_quantizer_input(x_2d)
-        # The quantizer pads the activation to whole 128-element runs itself;
-        # only a weight whose rows are not whole runs has to be copied.
-        token_runs = None
         if with_token_runs:
             x_fp8, x_scale, *token_runs = shared_activation_quantizer.quantize_both(x_2d)
-            token_runs = tuple(token_runs)
-        else:
-            x_fp8, x_scale = shared_activation_quantizer.quantize("rows", x_2d, hip_ops.act_quant_1x128)
+            return self._product(x_fp8, x_scale, weight, bias), tuple(token_runs)
+        x_fp8, x_scale = shared_activation_quantizer.quantize("rows", x_2d, hip_ops.act_quant_1x128)
+        return self._product(x_fp8, x_scale, weight, bias), None
+
+    def _forward_quantized(self, x: Fp8Activation, weight: BlockwiseFp8Weight, with_token_runs: bool, bias: torch.Tensor | None):
+        """:meth:`_forward` of an activation that is quantized already."""
+        self._check(weight)
+        out = self._product(x.q, x.scales, weight, bias)
+        return out, x.token_runs() if with_token_runs else None
+
+    def _product(self, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None) -> torch.Tensor:
+        # The quantizer pads the activation to whole 128-element runs itself;
+        # only a weight whose rows are not whole runs has to be copied.
+        weight_matrix = _weight_matrix(weight)
         padded_in_dim = x_fp8.shape[1]
         if weight_matrix.shape[1] != padded_in_dim or weight_matrix.stride(1) != 1 or weight_matrix.stride(0) % 16:
             weight_matrix = _pad_last_dim_to(weight_matrix.view(torch.uint8), padded_in_dim).view(torch.float8_e4m3fn)
-        return hip_ops.fp8_gemm_1x128_128x128(x_fp8, x_scale, weight_matrix, weight.recip_scale, bias=bias), token_runs
+        return hip_ops.fp8_gemm_1x128_128x128(x_fp8, x_scale, weight_matrix, weight.recip_scale, bias=bias)
 
     def _check(self, weight: BlockwiseFp8Weight) -> None:
         if self.block_size != weight.block_size:
@@ -251,14 +260,16 @@ class _PrequantizedLinearFunction(torch.autograd.Function):
     (reference: blockwise_quant/linear.py:74-123)."""
 
     @staticmethod
-    def forward(ctx: Any, x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms):
+    def forward(
+        ctx: Any, x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms, quantized: Fp8Activation | None
+    ):
         # With a weight gradient to come, the pass that quantizes x for the
         # product also writes the form the weight gradient contracts over, and
         # that (1 byte per element) is kept instead of x.
         keeps_token_runs = (
             ctx.needs_input_grad[1] and hasattr(gemms, "forward_with_token_runs") and not torch.compiler.is_compiling()
         )
-        out, token_runs = _linear_forward(x, weight, bias, gemms, keeps_token_runs)
+        out, token_runs = _linear_forward(x if quantized is None else quantized, weight, bias, gemms, keeps_token_runs)
         if keeps_token_runs:
             ctx.save_for_backward(weight, *token_runs)
         else:
@@ -300,12 +311,13 @@ class _PrequantizedLinearFunction(torch.autograd.Function):
             grad_x = grad_x.reshape(ctx.x_shape)
         if grad_bias is not None and weight.ndim != 2:
             grad_bias = grad_bias.view(weight.shape[:-1])
-        return grad_x, grad_weight, grad_bias, None
+        return grad_x, grad_weight, grad_bias, None, None
 
 
-def _linear_forward(x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms, with_token_runs: bool):
+def _linear_forward(x: torch.Tensor | Fp8Activation, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms, with_token_runs: bool):
     """``(x @ W.T + bias, the activation's token runs or None)``."""
-    x_2d = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    quantized = isinstance(x, Fp8Activation)
+    x_2d = x if x.ndim == 2 or quantized else x.reshape(-1, x.shape[-1])
     if x_2d.shape[-1] != weight.shape[-1]:
         raise ValueError(f"input last dim {x_2d.shape[-1]} does not match weight input dim {weight.shape[-1]}")
     token_runs = None
@@ -315,7 +327,9 @@ def _linear_forward(x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Ten
         fused = None
         if bias is not None and bias.dtype == torch.bfloat16 and bias.shape == weight.shape[:-1] and bias.is_contiguous():
             fused, bias = bias, None
-        out, token_runs = gemms._forward(x_2d, weight, with_token_runs, fused)
+        out, token_runs = (gemms._forward_quantized if quantized else gemms._forward)(x_2d, weight, with_token_runs, fused)
+    elif quantized:
+        raise TypeError(f"{type(gemms).__name__} takes no Fp8Activation: give it the values, dequantize()")
     elif with_token_runs:
         out, token_runs = gemms.forward_with_token_runs(x_2d, weight)
     else:
@@ -327,20 +341,23 @@ def _linear_forward(x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Ten
     return out, token_runs
 
 
-def _apply_linear(x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms) -> torch.Tensor:
+def _apply_linear(x: torch.Tensor | Fp8Activation, weight: BlockwiseFp8Weight, bias: torch.Tensor | None, gemms) -> torch.Tensor:
     # (inside a forward-mode level too: the function refuses a tangent, which the kernels would drop)
     if torch.is_grad_enabled() or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
-        return _PrequantizedLinearFunction.apply(x, weight, bias, gemms)
+        quantized = x if isinstance(x, Fp8Activation) else None
+        return _PrequantizedLinearFunction.apply(x if quantized is None else x.carrier, weight, bias, gemms, quantized)
     # Nothing to differentiate: no graph node, and the activation is quantized
     # in the one form that the product reads (host time of 48 tokens 34 -> 21 us).
     return _linear_forward(x, weight, bias, gemms, False)[0]
 
 
 def prequantized_linear(
-    x: torch.Tensor, weight: BlockwiseFp8Weight, bias: torch.Tensor | None = None, gemms: Fp8BlockwiseGemms | None = None
+    x: torch.Tensor | Fp8Activation, weight: BlockwiseFp8Weight, bias: torch.Tensor | None = None,
+    gemms: Fp8BlockwiseGemms | None = None,
 ) -> torch.Tensor:
     """Differentiable ``x @ W.T + bias`` on a gathered blockwise FP8 weight; a
-    stacked ``[*stack, out, in]`` weight returns ``[..., *stack, out]``."""
+    stacked ``[*stack, out, in]`` weight returns ``[..., *stack, out]``.  An
+    :class:`Fp8Activation` is multiplied as it is."""
     if not isinstance(weight, BlockwiseFp8Weight):
         raise TypeError(
             f"prequantized_linear requires a BlockwiseFp8Weight produced by an FP8 unshard, got {type(weight).__name__}."
@@ -365,7 +382,7 @@ class FlexShardFloat8BlockwiseLinear(nn.Linear):
         new_mod.train(mod.training)
         return new_mod
 
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: torch.Tensor | Fp8Activation) -> torch.Tensor:
         weight = self.weight
         if not isinstance(weight, self.weight_type):
             raise TypeError(

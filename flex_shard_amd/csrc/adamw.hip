@@ -1,0 +1,558 @@
+// One AdamW step of many tensors, with states in 32 or in 8 bits, and the sum of
+// the squares of many gradients, by which they are clipped.
+//
+//   c = min(1, max_norm / (sqrt(S) + 1e-6))            S: the sum of squares, or c = 1
+//   g = c g;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// in fp32, the parameter rounded to its type once.  S that is an infinity or not a
+// number leaves parameters, states and step counts as they are.
+//
+// Bound by memory: everything is read once and written once, 22 bytes an element
+// (bf16 parameters and gradients, 32-bit states), 10 1/8 with 8-bit states.  The
+// tensors of a launch come with its arguments, so that nothing is uploaded and a captured
+// launch keeps its own table.
+//
+// Eight-bit states.  128 consecutive elements share a scale, their largest
+// magnitude (at least 2^-100).  A value over its scale is at most 1; of its fp32 bits
+// the exponent and 3 bits of the mantissa are kept, counted from those of 1.0 (1016)
+// down: the first moment has a sign and codes 1 to 127, 16 octaves; the second, never
+// negative, codes 1 to 255, 32 octaves, which are 16 of the gradient's.  Code 0 is
+// zero.  Rounding is dithered: a number from [0, 1), which every element has anew in
+// every step, is added to the bits below, and the carry decides.  To nearest, a second
+// moment that changes by 1 - b2 of itself, less than half a step, would never leave its code; this
+// way it moves at the right rate on average, and the bits are the same every time.  (Multiples of an irrational
+// number modulo 1 do not do: the rounding's own past goes along with them, and a moment that is to fall to 0.049
+// in 300 steps falls to 0.038.)  A first moment below the smallest code becomes that or zero, evenly
+// too; a second one never becomes zero, for the first is divided by its root.
+// What is an infinity or not a number makes the whole block not a number.
+#include "rows.hpp"
+
+namespace fsh {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kStateBlock = FSH_ADAMW_BLOCK;
+constexpr int64_t kMaxGrid = (1LL << 32) / kThreads - 1;
+
+// -------------------------------------------------- per-tensor factors of a step
+struct alignas(16) StepFactors {
+  float b1, one_b1, b2, one_b2;
+  float eps, decay, step_size, root_factor;  // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  float clip;
+  uint32_t t;
+  int32_t skip, unused;
+};
+
+constexpr int kFactorTensors = 240;  // of one launch: 12 bytes each beside the groups
+struct FactorParams {
+  fsh_adamw_group groups[FSH_ADAMW_GROUPS];
+  int32_t* step[kFactorTensors];
+  uint8_t group[kFactorTensors];
+  StepFactors* factors;
+  const double* square_sum;
+  double max_norm;
+  int32_t count;
+};
+static_assert(sizeof(FactorParams) <= 4096, "kernel arguments");
+
+// b^t by squaring, in 64 bits: 1 - b^t loses ten bits at b = 0.999 and t = 1.
+__device__ double power(double b, uint32_t t) {
+  double r = 1.0;
+  for (; t; t >>= 1, b *= b)
+    if (t & 1) r *= b;
+  return r;
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_factors_kernel(const FactorParams p) {
+  const int i = threadIdx.x;
+  if (i >= p.count) return;
+  float clip = 1.0f;
+  bool skip = false;
+  if (p.square_sum) {
+    const double sum = *p.square_sum;
+    skip = !(fabs(sum) <= 1.7976931348623157e308);
+    if (p.max_norm > 0.0) {
+      const double factor = p.max_norm / (sqrt(sum) + 1e-6);
+      clip = static_cast<float>(factor < 1.0 ? factor : 1.0);
+    }
+  }
+  const fsh_adamw_group g = p.groups[p.group[i]];
+  const double lr = g.lr_dev ? static_cast<double>(*g.lr_dev) : g.lr;
+  const uint32_t t = static_cast<uint32_t>(*p.step[i]) + (skip ? 0u : 1u);
+  if (!skip) *p.step[i] = static_cast<int32_t>(t);
+  StepFactors f;
+  f.b1 = static_cast<float>(g.beta1);
+  f.one_b1 = static_cast<float>(1.0 - g.beta1);
+  f.b2 = static_cast<float>(g.beta2);
+  f.one_b2 = static_cast<float>(1.0 - g.beta2);
+  f.eps = static_cast<float>(g.eps);
+  f.decay = static_cast<float>(1.0 - lr * g.weight_decay);
+  f.step_size = static_cast<float>(lr / (1.0 - power(g.beta1, t)));
+  f.root_factor = static_cast<float>(1.0 / sqrt(1.0 - power(g.beta2, t)));
+  f.clip = clip;
+  f.t = t;
+  f.skip = skip;
+  f.unused = 0;
+  p.factors[i] = f;
+}
+
+// ------------------------------------------------------------- the tensors' table
+// Tensors of one launch, cut into chunks that are numbered through.
+constexpr int kTensors = 60;
+struct AdamTable {
+  void* param[kTensors];
+  const void* grad[kTensors];
+  void* m[kTensors];
+  void* v[kTensors];
+  float* m_scale[kTensors];
+  float* v_scale[kTensors];
+  int64_t numel[kTensors];
+  uint32_t factors[kTensors];
+  uint32_t first_chunk[kTensors];  // 0xFFFFFFFF behind the last
+  const StepFactors* all_factors;
+  int64_t chunks;
+};
+static_assert(sizeof(AdamTable) <= 4096, "kernel arguments");
+
+// The tensor that a chunk belongs to: the last that begins at or before it (a lane each).
+template <int N>
+__device__ __forceinline__ int tensor_of(const uint32_t (&first)[N], uint32_t chunk) {
+  const int lane = threadIdx.x & 63;
+  int at = -1;
+#pragma unroll
+  for (int base = 0; base < N; base += 64)
+    at += __popcll(__ballot(base + lane < N && first[base + lane < N ? base + lane : 0] <= chunk));
+  return __builtin_amdgcn_readfirstlane(at);
+}
+
+// ------------------------------------------------------------------ 8-bit codes
+constexpr int kOne = 1016;  // the upper 12 bits of 1.0f
+__device__ __forceinline__ float code_value(uint32_t code, int codes) {
+  return code ? u32_as_f32((code + kOne - codes) << 20) : 0.0f;
+}
+__device__ __forceinline__ float first_value(uint32_t code) {
+  return u32_as_f32(f32_as_u32(code_value(code & 127u, 127)) | ((code & 128u) << 24));
+}
+// size in [0, 1]; u: the dither.
+__device__ __forceinline__ uint32_t first_code(float size, uint32_t sign, uint32_t u) {
+  constexpr float kSmallest = 1.25f / 65536.0f;
+  const uint32_t up = ((f32_as_u32(size) + (u >> 12)) >> 20) - (kOne - 127);
+  const uint32_t few = size * (1.0f / kSmallest) > static_cast<float>(u >> 8) * (1.0f / 16777216.0f) ? 1u : 0u;
+  return (size < kSmallest ? few : up) | (sign ? 128u : 0u);
+}
+__device__ __forceinline__ uint32_t second_code(float size, uint32_t u) {
+  const int up = static_cast<int>((f32_as_u32(size) + (u >> 12)) >> 20) - (kOne - 255);
+  return size > 0.0f ? static_cast<uint32_t>(up > 1 ? up : 1) : 0u;
+}
+// The dither of an element in a step, 16 bits for each moment: multiples of the
+// golden ratio and of the square root of 2, modulo 2^32, mixed by one product with the
+// square root of 3 between two shifts, which leaves no correlation beyond chance between
+// neighbours, steps or the halves (2^20 elements).
+__device__ __forceinline__ uint32_t dither(uint32_t index, uint32_t t) {
+  uint32_t z = index * 0x9E3779B9u + t * 0x6A09E667u;
+  z = (z ^ (z >> 16)) * 0xBB67AE85u;
+  return z ^ (z >> 15);
+}
+
+// The scale of a block from its largest magnitude's bits, and 1 over it.
+__device__ __forceinline__ float block_scale(uint32_t largest, float& inverse) {
+  const float least = u32_as_f32(0x0D800000u);  // 2^-100
+  const float amax = u32_as_f32(largest >= 0x7F800000u ? 0x7FC00000u : largest);
+  const float scale = amax < least ? least : amax;  // (not a number stays)
+  inverse = 1.0f / scale;
+  return scale;
+}
+
+// --------------------------------------------------------------------- the step
+constexpr int kChunk = 4 * kThreads;  // elements: four neighbours a thread
+
+template <int PT, int GT, bool kEight>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamTable a) {
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
+    const StepFactors f = a.all_factors[a.factors[k]];
+    if (f.skip) continue;
+    const int64_t numel = a.numel[k];
+    const int64_t at = (chunk - a.first_chunk[k]) * kChunk + 4 * static_cast<int64_t>(threadIdx.x);
+    const int64_t count = numel - at;
+    const auto pr = load_vec<PT, 4>(a.param[k], at, count);
+    const auto gr = load_vec<GT, 4>(a.grad[k], at, count);
+    float m[4], v[4], p[4];
+    const int64_t block = at / kStateBlock;
+    if constexpr (kEight) {
+      // (codes lie in fours at 4-byte addresses; a tensor's last four may be fewer)
+      uint32_t mc = 0, vc = 0;
+      float ms = 0.0f, vs = 0.0f;
+      if (count > 0) {
+        ms = a.m_scale[k][block];
+        vs = a.v_scale[k][block];
+      }
+      if (count >= 4) {
+        __builtin_memcpy(&mc, static_cast<const uint8_t*>(a.m[k]) + at, 4);
+        __builtin_memcpy(&vc, static_cast<const uint8_t*>(a.v[k]) + at, 4);
+      } else {
+        for (int j = 0; j < count; ++j) {
+          mc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.m[k])[at + j]) << (8 * j);
+          vc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.v[k])[at + j]) << (8 * j);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = first_value((mc >> (8 * j)) & 255u) * ms;
+        v[j] = code_value((vc >> (8 * j)) & 255u, 255) * vs;
+      }
+    } else {
+      const auto mr = load_vec<FSH_DT_F32, 4>(a.m[k], at, count);
+      const auto vr = load_vec<FSH_DT_F32, 4>(a.v[k], at, count);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = element<FSH_DT_F32, 4>(mr, j);
+        v[j] = element<FSH_DT_F32, 4>(vr, j);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float g = element<GT, 4>(gr, j) * f.clip;
+      m[j] = m[j] * f.b1 + g * f.one_b1;
+      v[j] = v[j] * f.b2 + (g * g) * f.one_b2;
+      const float root = sqrtf(v[j]) * f.root_factor + f.eps;
+      p[j] = element<PT, 4>(pr, j) * f.decay - f.step_size * (m[j] / root);
+    }
+    if (count > 0) store_vec<PT, 4>(a.param[k], at, count, to_vec<PT, 4>(p));
+    if constexpr (kEight) {
+      // Half a wave has a block; elements behind the tensor's last are zero.
+      uint32_t m_max = 0, v_max = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= count) m[j] = v[j] = 0.0f;
+        m_max = max(m_max, f32_as_u32(m[j]) & 0x7FFFFFFFu);
+        v_max = max(v_max, f32_as_u32(v[j]) & 0x7FFFFFFFu);
+      }
+      float m_inverse, v_inverse;
+      const float ms = block_scale(max32_u32(m_max), m_inverse), vs = block_scale(max32_u32(v_max), v_inverse);
+      uint32_t mc = 0, vc = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = dither(static_cast<uint32_t>(at) + j, f.t);
+        const float m_size = fminf(u32_as_f32(f32_as_u32(m[j]) & 0x7FFFFFFFu) * m_inverse, 1.0f);
+        const float v_size = fminf(v[j] * v_inverse, 1.0f);
+        mc |= (first_code(m_size, m[j] < 0.0f, u << 16) & 255u) << (8 * j);
+        vc |= (second_code(v_size, u & 0xFFFF0000u) & 255u) << (8 * j);
+      }
+      if (count >= 4) {
+        __builtin_memcpy(static_cast<uint8_t*>(a.m[k]) + at, &mc, 4);
+        __builtin_memcpy(static_cast<uint8_t*>(a.v[k]) + at, &vc, 4);
+      } else {
+        for (int j = 0; j < count; ++j) {
+          static_cast<uint8_t*>(a.m[k])[at + j] = static_cast<uint8_t>(mc >> (8 * j));
+          static_cast<uint8_t*>(a.v[k])[at + j] = static_cast<uint8_t>(vc >> (8 * j));
+        }
+      }
+      if (count > 0 && at % kStateBlock == 0) {
+        a.m_scale[k][block] = ms;
+        a.v_scale[k][block] = vs;
+      }
+    } else if (count > 0) {
+      store_vec<FSH_DT_F32, 4>(a.m[k], at, count, to_vec<FSH_DT_F32, 4>(m));
+      store_vec<FSH_DT_F32, 4>(a.v[k], at, count, to_vec<FSH_DT_F32, 4>(v));
+    }
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void adamw_values_kernel(const uint8_t* m, const float* m_scale, const uint8_t* v, const float* v_scale,
+                                                                void* m_out, void* v_out, int64_t numel) {
+  for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 8; at < numel; at += static_cast<int64_t>(gridDim.x) * kThreads * 8) {
+    const int64_t count = numel - at;
+    uint8_t mc[8] = {}, vc[8] = {};
+    if (count >= 8) {
+      __builtin_memcpy(mc, m + at, 8);
+      __builtin_memcpy(vc, v + at, 8);
+    } else {
+      for (int j = 0; j < count; ++j) {
+        mc[j] = m[at + j];
+        vc[j] = v[at + j];
+      }
+    }
+    const float ms = m_scale[at / kStateBlock], vs = v_scale[at / kStateBlock];
+    float mf[8], vf[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      mf[j] = first_value(mc[j]) * ms;
+      vf[j] = code_value(vc[j], 255) * vs;
+    }
+    store_vec<DT, 8>(m_out, at, count, to_vec<DT, 8>(mf));
+    store_vec<DT, 8>(v_out, at, count, to_vec<DT, 8>(vf));
+  }
+}
+
+// --------------------------------------------------------------- sum of squares
+// In 64 bits, where the squares of bf16, fp16 and fp32 values are exact or nearly: a
+// workgroup adds up its chunks, its threads' sums are joined in a fixed order, and
+// one workgroup joins the workgroups'.
+constexpr int kSquareTensors = 160;
+constexpr int kSquareChunk = 8 * kThreads * 4;  // elements: four vectors of eight a thread
+constexpr int kSquareGroups = 2048;
+struct SquareTable {
+  const void* grad[kSquareTensors];
+  int64_t numel[kSquareTensors];
+  uint32_t first_chunk[kSquareTensors];
+  uint8_t dtype[kSquareTensors];
+  double* parts;
+  int64_t chunks;
+};
+static_assert(sizeof(SquareTable) <= 4096, "kernel arguments");
+
+template <int DT>
+__device__ __forceinline__ double squares_of(const void* g, int64_t at, int64_t numel) {
+  constexpr int VEC = DT == FSH_DT_F32 ? 4 : 8, kVectors = kSquareChunk / kThreads / VEC;
+  RawVec<DT, VEC> r[kVectors];
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const int64_t here = at + (static_cast<int64_t>(i) * kThreads + threadIdx.x) * VEC;
+    r[i] = load_vec<DT, VEC>(g, here, numel - here);
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const double x = static_cast<double>(element<DT, VEC>(r[i], j));
+      sum = __builtin_fma(x, x, sum);
+    }
+  return sum;
+}
+
+__device__ double workgroup_sum(double v, double* lds) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) sum += lds[w];
+  return sum;
+}
+
+__global__ __launch_bounds__(kThreads) void square_sum_kernel(const SquareTable a) {
+  __shared__ double lds[kThreads / 64];
+  double sum = 0.0;
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
+    const int64_t at = (chunk - a.first_chunk[k]) * kSquareChunk;
+    const int dtype = a.dtype[k];
+    if (dtype == FSH_DT_F32) sum += squares_of<FSH_DT_F32>(a.grad[k], at, a.numel[k]);
+    else if (dtype == FSH_DT_BF16) sum += squares_of<FSH_DT_BF16>(a.grad[k], at, a.numel[k]);
+    else sum += squares_of<FSH_DT_F16>(a.grad[k], at, a.numel[k]);
+  }
+  sum = workgroup_sum(sum, lds);
+  if (threadIdx.x == 0) a.parts[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kThreads) void square_join_kernel(const double* parts, int64_t count, double* out) {
+  __shared__ double lds[kThreads / 64];
+  double sum = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < count; i += kThreads) sum += parts[i];
+  sum = workgroup_sum(sum, lds);
+  if (threadIdx.x == 0) *out = sum;
+}
+
+// Chunks of one launch are numbered in 32 bits.
+constexpr int64_t kMaxChunks = 0xFFFFFFFELL;
+
+// Workgroups of each of the launches that the tensors take; their number.
+template <typename Each>
+int square_launches(const int64_t* tensors, int32_t count, Each each) {
+  int32_t begin = 0;
+  int launches = 0;
+  while (begin < count) {
+    int64_t chunks = 0;
+    int32_t end = begin;
+    while (end < count && end - begin < kSquareTensors) {
+      const int64_t more = ceil_div(tensors[3 * end + 1], (int64_t)kSquareChunk);
+      if (chunks + more > kMaxChunks) break;
+      chunks += more;
+      ++end;
+    }
+    if (end == begin) return -1;  // a tensor of more than 2^44 elements
+    if (chunks) each(begin, end, chunks, chunks < kSquareGroups ? chunks : static_cast<int64_t>(kSquareGroups));
+    ++launches;
+    begin = end;
+  }
+  return launches;
+}
+
+template <int PT, int GT>
+void launch_step(const AdamTable& a, bool eight, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(a.chunks < kMaxGrid ? a.chunks : kMaxGrid)), block(kThreads);
+  if (eight) hipLaunchKernelGGL((adamw_kernel<PT, GT, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((adamw_kernel<PT, GT, false>), grid, block, 0, stream, a);
+}
+
+}  // namespace
+}  // namespace fsh
+
+FSH_API int64_t fsh_grad_square_sum_workspace_bytes(const int64_t* tensors, int32_t count) {
+  using namespace fsh;
+  if (!tensors || count < 0) return 0;
+  int64_t groups = 0;
+  square_launches(tensors, count, [&](int32_t, int32_t, int64_t, int64_t mine) { groups += mine; });
+  return groups * static_cast<int64_t>(sizeof(double));
+}
+
+FSH_API int fsh_grad_square_sum(const int64_t* tensors, int32_t count, double* out_dev, void* workspace_dev, int64_t workspace_nbytes, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_grad_square_sum";
+  if (count < 0) return fail(FSH_EINVAL, "%s: negative count", who);
+  if (!out_dev || (count && !tensors)) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (!aligned(out_dev, 8) || !aligned(workspace_dev, 8)) return fail(FSH_ENOTSUP, "%s: the sum and the workspace must be 8-byte aligned", who);
+  for (int32_t i = 0; i < count; ++i) {
+    const int64_t address = tensors[3 * i], numel = tensors[3 * i + 1], dtype = tensors[3 * i + 2];
+    if (numel < 0) return fail(FSH_EINVAL, "%s: tensor %d has a negative size", who, i);
+    if (dtype < 0 || !is_dtype(static_cast<int32_t>(dtype < 99 ? dtype : 99))) return fail(FSH_EINVAL, "%s: tensor %d has an unknown dtype %lld", who, i, (long long)dtype);
+    if (numel && !address) return fail(FSH_EINVAL, "%s: null pointer", who);
+    if (address % bytes_of(static_cast<int>(dtype))) return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
+  }
+  const int64_t need = fsh_grad_square_sum_workspace_bytes(tensors, count);
+  if (need && (!workspace_dev || workspace_nbytes < need)) return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_nbytes, (long long)need);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  double* const parts = static_cast<double*>(workspace_dev);
+  int64_t used = 0;
+  int rc = FSH_OK;
+  const int launches = square_launches(tensors, count, [&](int32_t begin, int32_t end, int64_t chunks, int64_t groups) {
+    SquareTable a;
+    uint32_t first = 0;
+    for (int k = 0; k < kSquareTensors; ++k) {
+      const bool here = begin + k < end;
+      const int64_t* t = tensors + 3 * (here ? begin + k : begin);
+      a.grad[k] = reinterpret_cast<const void*>(t[0]);
+      a.numel[k] = t[1];
+      a.dtype[k] = static_cast<uint8_t>(t[2]);
+      a.first_chunk[k] = here ? first : 0xFFFFFFFFu;
+      if (here) first += static_cast<uint32_t>(ceil_div(t[1], (int64_t)kSquareChunk));
+    }
+    a.parts = parts + used;
+    a.chunks = chunks;
+    if (rc == FSH_OK) {
+      hipLaunchKernelGGL(square_sum_kernel, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, on, a);
+      rc = check_launch("square_sum_kernel");
+    }
+    used += groups;
+  });
+  if (launches < 0) return fail(FSH_ENOTSUP, "%s: a tensor is too long", who);
+  if (rc) return rc;
+  hipLaunchKernelGGL(square_join_kernel, dim3(1), dim3(kThreads), 0, on, parts, used, out_dev);
+  return check_launch("square_join_kernel");
+}
+
+FSH_API int64_t fsh_adamw_step_workspace_bytes(int32_t count) {
+  return count < 0 ? 0 : static_cast<int64_t>(count) * static_cast<int64_t>(sizeof(fsh::StepFactors));
+}
+
+FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const double* square_sum_dev,
+                           double max_norm, void* workspace_dev, int64_t workspace_nbytes, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_adamw_step";
+  if (count < 0) return fail(FSH_EINVAL, "%s: negative count", who);
+  if (count == 0) return FSH_OK;
+  if (!tensors || !groups || !workspace_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (group_count < 1 || group_count > FSH_ADAMW_GROUPS) return fail(FSH_ENOTSUP, "%s: 1 to %d groups, got %d", who, FSH_ADAMW_GROUPS, group_count);
+  if (workspace_nbytes < fsh_adamw_step_workspace_bytes(count) || !aligned(workspace_dev, 16))
+    return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", who, (long long)workspace_nbytes, (long long)fsh_adamw_step_workspace_bytes(count));
+  if (!aligned(square_sum_dev, 8)) return fail(FSH_ENOTSUP, "%s: the sum of squares must be 8-byte aligned", who);
+  if (max_norm != max_norm) return fail(FSH_EINVAL, "%s: max_norm is not a number", who);
+  for (int32_t i = 0; i < group_count; ++i) {
+    const fsh_adamw_group& g = groups[i];
+    if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return fail(FSH_EINVAL, "%s: group %d: betas in [0, 1), eps not negative", who, i);
+    if (!aligned(g.lr_dev, 4)) return fail(FSH_ENOTSUP, "%s: group %d: the learning rate must be 4-byte aligned", who, i);
+  }
+  for (int32_t i = 0; i < count; ++i) {
+    const fsh_adamw_tensor& t = tensors[i];
+    if (t.numel < 0 || t.group < 0 || t.group >= group_count) return fail(FSH_EINVAL, "%s: tensor %d: negative size, or group %lld of %d", who, i, (long long)t.group, group_count);
+    if ((t.param_dtype != FSH_DT_BF16 && t.param_dtype != FSH_DT_F32) || (t.grad_dtype != FSH_DT_BF16 && t.grad_dtype != FSH_DT_F32) || (t.state_bits != 8 && t.state_bits != 32))
+      return fail(FSH_EINVAL, "%s: tensor %d: bf16 or fp32 parameters and gradients, states of 8 or 32 bits", who, i);
+    if (!t.step_dev || (t.numel && (!t.param_dev || !t.grad_dev || !t.exp_avg_dev || !t.exp_avg_sq_dev || (t.state_bits == 8 && (!t.exp_avg_scale_dev || !t.exp_avg_sq_scale_dev)))))
+      return fail(FSH_EINVAL, "%s: tensor %d: null pointer", who, i);
+    if (!aligned(t.param_dev, bytes_of(t.param_dtype)) || !aligned(t.grad_dev, bytes_of(t.grad_dtype)) || !aligned(t.exp_avg_dev, t.state_bits == 8 ? 1 : 4) ||
+        !aligned(t.exp_avg_sq_dev, t.state_bits == 8 ? 1 : 4) || !aligned(t.exp_avg_scale_dev, 4) || !aligned(t.exp_avg_sq_scale_dev, 4) || !aligned(t.step_dev, 4))
+      return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
+    if (ceil_div(t.numel, (int64_t)kChunk) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
+  }
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  StepFactors* const factors = static_cast<StepFactors*>(workspace_dev);
+  for (int32_t begin = 0; begin < count; begin += kFactorTensors) {
+    FactorParams p = {};
+    for (int32_t i = 0; i < group_count; ++i) p.groups[i] = groups[i];
+    p.count = count - begin < kFactorTensors ? count - begin : kFactorTensors;
+    for (int32_t i = 0; i < p.count; ++i) {
+      p.step[i] = tensors[begin + i].step_dev;
+      p.group[i] = static_cast<uint8_t>(tensors[begin + i].group);
+    }
+    p.factors = factors + begin;
+    p.square_sum = square_sum_dev;
+    p.max_norm = max_norm;
+    hipLaunchKernelGGL(adamw_factors_kernel, dim3(1), dim3(kThreads), 0, on, p);
+    if (int rc = check_launch("adamw_factors_kernel")) return rc;
+  }
+  // Tensors of the same types share launches.
+  for (int kind = 0; kind < 8; ++kind) {
+    const int pt = kind & 1 ? FSH_DT_F32 : FSH_DT_BF16, gt = kind & 2 ? FSH_DT_F32 : FSH_DT_BF16;
+    const bool eight = (kind & 4) != 0;
+    for (int32_t next = 0; next < count;) {
+      AdamTable a;
+      int32_t n = 0;
+      a.chunks = 0;
+      for (; next < count && n < kTensors; ++next) {
+        const fsh_adamw_tensor& t = tensors[next];
+        if (t.param_dtype != pt || t.grad_dtype != gt || (t.state_bits == 8) != eight || t.numel == 0) continue;
+        const int64_t more = ceil_div(t.numel, (int64_t)kChunk);
+        if (a.chunks + more > kMaxChunks) break;
+        a.param[n] = t.param_dev;
+        a.grad[n] = t.grad_dev;
+        a.m[n] = t.exp_avg_dev;
+        a.v[n] = t.exp_avg_sq_dev;
+        a.m_scale[n] = t.exp_avg_scale_dev;
+        a.v_scale[n] = t.exp_avg_sq_scale_dev;
+        a.numel[n] = t.numel;
+        a.factors[n] = static_cast<uint32_t>(next);
+        a.first_chunk[n] = static_cast<uint32_t>(a.chunks);
+        a.chunks += more;
+        ++n;
+      }
+      if (n == 0) break;  // (no more of this kind)
+      for (int32_t i = n; i < kTensors; ++i) a.first_chunk[i] = 0xFFFFFFFFu;
+      a.all_factors = factors;
+      if (pt == FSH_DT_BF16 && gt == FSH_DT_BF16) launch_step<FSH_DT_BF16, FSH_DT_BF16>(a, eight, on);
+      else if (pt == FSH_DT_BF16) launch_step<FSH_DT_BF16, FSH_DT_F32>(a, eight, on);
+      else if (gt == FSH_DT_BF16) launch_step<FSH_DT_F32, FSH_DT_BF16>(a, eight, on);
+      else launch_step<FSH_DT_F32, FSH_DT_F32>(a, eight, on);
+      if (int rc = check_launch("adamw_kernel")) return rc;
+    }
+  }
+  return FSH_OK;
+}
+
+FSH_API int fsh_adamw_state_values(const void* exp_avg_dev, const float* exp_avg_scale_dev, const void* exp_avg_sq_dev, const float* exp_avg_sq_scale_dev,
+                                   int64_t numel, void* exp_avg_out_dev, void* exp_avg_sq_out_dev, int32_t dtype, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_adamw_state_values";
+  if (numel < 0) return fail(FSH_EINVAL, "%s: negative size", who);
+  if (!is_dtype(dtype)) return fail(FSH_EINVAL, "%s: unknown dtype %d", who, dtype);
+  if (numel == 0) return FSH_OK;
+  if (!exp_avg_dev || !exp_avg_scale_dev || !exp_avg_sq_dev || !exp_avg_sq_scale_dev || !exp_avg_out_dev || !exp_avg_sq_out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (!aligned(exp_avg_scale_dev, 4) || !aligned(exp_avg_sq_scale_dev, 4) || !aligned(exp_avg_out_dev, bytes_of(dtype)) || !aligned(exp_avg_sq_out_dev, bytes_of(dtype)))
+    return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements", who);
+  const int64_t blocks = ceil_div(numel, (int64_t)kThreads * 8);
+  const dim3 grid(static_cast<uint32_t>(blocks < kMaxGrid ? blocks : kMaxGrid)), block(kThreads);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, block, 0, on, static_cast<const uint8_t*>(exp_avg_dev), exp_avg_scale_dev, static_cast<const uint8_t*>(exp_avg_sq_dev),
+                       exp_avg_sq_scale_dev, exp_avg_out_dev, exp_avg_sq_out_dev, numel);
+  };
+  if (dtype == FSH_DT_BF16) go(adamw_values_kernel<FSH_DT_BF16>);
+  else if (dtype == FSH_DT_F16) go(adamw_values_kernel<FSH_DT_F16>);
+  else go(adamw_values_kernel<FSH_DT_F32>);
+  return check_launch("adamw_values_kernel");
+}

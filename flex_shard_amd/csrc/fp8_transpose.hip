@@ -17,7 +17,7 @@
 // The first three work on 128 x 128 tiles through LDS: rows go in as they are read
 // (16-byte global loads along the source rows), and come out along the
 // source columns as 16-byte runs of 16 source rows each.
-#include "common.hpp"
+#include "rows.hpp"
 
 namespace fsh {
 namespace {
@@ -120,8 +120,10 @@ static_assert(16 * kTileDim * 4 <= kTileDim * kTilePitch, "the column sums fit t
 // is the sum of the output gradient over the tokens) cost eight additions per
 // element row and 8 KB through LDS instead of a pass of its own over the
 // matrix (14.6 us at 1000 x 5120, and 4 us for a fill that the pass needed).
-template <bool kAlsoRowRuns>
-__device__ __forceinline__ void quantize_tile_transposed(const ActQuantTParams& p, ActQuantTShared<kAlsoRowRuns>& shared, uint32_t id) {
+//
+// load(v, row, col): the thread's columns of rows row + 16 k as bf16, zero outside the matrix.
+template <bool kAlsoRowRuns, typename Load>
+__device__ __forceinline__ void quantize_tile_transposed(const ActQuantTParams& p, ActQuantTShared<kAlsoRowRuns>& shared, uint32_t id, Load load) {
   uint8_t* const tile = shared.tile;
   uint16_t* const col_max = shared.col_max;
   float* const col_scale = shared.col_scale;
@@ -134,12 +136,7 @@ __device__ __forceinline__ void quantize_tile_transposed(const ActQuantTParams& 
   const int64_t col = c0 + cg * 8;
 
   u32x4 v[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int64_t row = r0 + rl + 16 * k;
-    v[k] = u32x4{0, 0, 0, 0};
-    if (row < p.rows && col < p.cols) v[k] = load_stream_u32x4(p.x + (row * p.ldx + col) * 2);  // cols % 8 == 0
-  }
+  load(v, r0 + rl, col);
   if (kAlsoRowRuns) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -230,10 +227,67 @@ __device__ __forceinline__ void quantize_tile_transposed(const ActQuantTParams& 
   store_tile_transposed(tile, p.q, c0, r0, p.cols, p.ldq, tid);
 }
 
+// The thread's part of a tile of the matrix itself.
+struct LoadMatrix {
+  const ActQuantTParams& p;
+  __device__ __forceinline__ void operator()(u32x4 (&v)[8], int64_t row0, int64_t col) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t row = row0 + 16 * k;
+      v[k] = u32x4{0, 0, 0, 0};
+      if (row < p.rows && col < p.cols) v[k] = load_stream_u32x4(p.x + (row * p.ldx + col) * 2);  // cols % 8 == 0
+    }
+  }
+};
+
+// The thread's part of a tile of a norm's output h s w (norm_forward.hip), made again
+// from its sum h [rows, cols], the rows' factors s and the weight, and rounded to bf16 as there.
+// (y itself is then never written, nor kept for the backward pass.)
+struct NormRunsParams {
+  const void* h;
+  const float* rstd;
+  const void* weight;
+  int64_t cols, ldh;  // (the quantizer's cols are these rounded up to 8)
+  int32_t weight_dtype;
+};
+template <int HT>
+struct LoadNorm {
+  const ActQuantTParams& p;
+  const NormRunsParams& norm;
+  __device__ __forceinline__ void operator()(u32x4 (&v)[8], int64_t row0, int64_t col) const {
+    const int64_t count = norm.cols - col;
+    RawVec<HT, 8> h[8];
+    float s[8], w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t row = row0 + 16 * k;
+      const bool here = row < p.rows && count > 0;
+      h[k] = load_vec<HT, 8>(norm.h, row * norm.ldh + col, here ? count : 0);
+      s[k] = here ? norm.rstd[row] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = 1.0f;
+    if (norm.weight && count > 0) load_floats<8>(norm.weight, norm.weight_dtype, col, count, w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = j < count && row0 + 16 * k < p.rows ? element<HT, 8>(h[k], j) * s[k] * w[j] : 0.0f;
+      v[k] = pack8_bf16(y);
+    }
+  }
+};
+
+template <int HT>
+__global__ __launch_bounds__(kTransposeThreads) void norm_token_runs_kernel(const ActQuantTParams p, const NormRunsParams norm) {
+  __shared__ ActQuantTShared<false> shared;
+  quantize_tile_transposed(p, shared, blockIdx.x, LoadNorm<HT>{p, norm});
+}
+
 template <bool kAlsoRowRuns>
 __global__ __launch_bounds__(kTransposeThreads) void act_quant_128x1_t_kernel(const ActQuantTParams p) {
   __shared__ ActQuantTShared<kAlsoRowRuns> shared;
-  quantize_tile_transposed(p, shared, blockIdx.x);
+  quantize_tile_transposed(p, shared, blockIdx.x, LoadMatrix{p});
 }
 
 // One launch for what the two backward products of a layer read: workgroups
@@ -244,7 +298,7 @@ __global__ __launch_bounds__(kTransposeThreads) void backward_operands_kernel(co
                                                                               uint32_t quant_tiles) {
   __shared__ ActQuantTShared<true> shared;
   if (blockIdx.x < quant_tiles)
-    quantize_tile_transposed(quant, shared, blockIdx.x);
+    quantize_tile_transposed(quant, shared, blockIdx.x, LoadMatrix{quant});
   else
     transpose_tile(transpose, shared.tile, blockIdx.x - quant_tiles);
 }
@@ -385,6 +439,33 @@ FSH_API int fsh_act_quant_128x1_transposed(const void* x_dev, int64_t rows, int6
   hipLaunchKernelGGL(act_quant_128x1_t_kernel<false>, dim3(static_cast<uint32_t>(tiles)), dim3(kTransposeThreads), 0,
                      static_cast<hipStream_t>(stream), p);
   return check_launch("act_quant_128x1_t_kernel");
+}
+
+FSH_API int fsh_rms_norm_token_runs(const void* total_dev, int32_t dtype, int64_t rows, int64_t cols, int64_t ldh, const float* rstd_dev,
+                                    const void* weight_dev, int32_t weight_dtype, void* q_dev, int64_t ldq, float* scales_dev, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_rms_norm_token_runs";
+  if (rows < 0 || cols < 0) return fail(FSH_EINVAL, "%s: negative shape", who);
+  if (!is_dtype(dtype) || (weight_dev && !is_dtype(weight_dtype))) return fail(FSH_EINVAL, "%s: unknown dtype %d or %d", who, dtype, weight_dtype);
+  if (rows == 0 || cols == 0) return FSH_OK;
+  if (!total_dev || !rstd_dev || !q_dev || !scales_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (ldh < cols) return fail(FSH_EINVAL, "%s: ldh %lld < cols %lld", who, (long long)ldh, (long long)cols);
+  if (!aligned(total_dev, bytes_of(dtype)) || !aligned(rstd_dev, 4) || (weight_dev && !aligned(weight_dev, bytes_of(weight_dtype))))
+    return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements", who);
+  ActQuantTParams p;
+  int64_t tiles = 0;
+  const int64_t padded = ceil_div(cols, (int64_t)8) * 8;
+  // (x is not read: the row stride and address stand for a matrix that the checks accept)
+  if (int rc = act_quant_params(p, tiles, nullptr, rows, padded, padded, nullptr, 0, nullptr, q_dev, ldq, scales_dev, nullptr, FSH_EPS_FP32, who))
+    return rc;
+  if (tiles > (1LL << 32) / kTransposeThreads - 1) return fail(FSH_ENOTSUP, "%s: too many tiles", who);  // a launch's threads are counted in 32 bits
+  const NormRunsParams norm = {total_dev, rstd_dev, weight_dev, cols, ldh, weight_dtype};
+  const dim3 grid(static_cast<uint32_t>(tiles)), block(kTransposeThreads);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (dtype == FSH_DT_BF16) hipLaunchKernelGGL(norm_token_runs_kernel<FSH_DT_BF16>, grid, block, 0, on, p, norm);
+  else if (dtype == FSH_DT_F16) hipLaunchKernelGGL(norm_token_runs_kernel<FSH_DT_F16>, grid, block, 0, on, p, norm);
+  else hipLaunchKernelGGL(norm_token_runs_kernel<FSH_DT_F32>, grid, block, 0, on, p, norm);
+  return check_launch("norm_token_runs_kernel");
 }
 
 FSH_API int fsh_act_quant_both(const void* x_dev, int64_t rows, int64_t cols, int64_t ldx, void* q_row_dev,

@@ -1,0 +1,278 @@
+// Gradients of the root-mean-square norm (norm_forward.hip):
+//
+//   n = h s,  a = dy w,  c = mean(a n) over the row
+//   dh = s (a - n c) + (the gradient of h from what reads it besides)
+//   dx = dr = dh, rounded to their types;  dw = sum over the rows of dy n
+//
+// Bound by memory: dy, h and the gradient of h are read once, dx is written once.
+// A workgroup takes rows in turn and keeps its part of dw in registers, in fp32;
+// the parts are added up in a fixed order by a second kernel.
+#include "norm_layout.hpp"
+
+namespace fsh {
+namespace {
+
+struct NormGradParams {
+  const void* grad;
+  const void* h;
+  const void* weight;
+  const float* rstd;
+  const void* grad_total;
+  void* grad_x;
+  void* grad_residual;
+  float* parts;  // [workgroups][cols], or null
+  int64_t rows, cols, ldg, ldh, ldt;
+  int64_t row_blocks;
+  int32_t weight_dtype;
+};
+
+constexpr int kGradGroups = 1024;      // workgroups of 256 threads: four a compute unit
+constexpr int kGradGroupsWide = 512;   // of 1024
+
+template <int GT, int HT, int XT, typename L>
+__global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGradParams p) {
+  constexpr int VEC = L::VEC, ITEMS = L::ITEMS;
+  __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : L::ROWS * L::LANES * L::PER];
+  const int lane = threadIdx.x % L::LANES, group = threadIdx.x / L::LANES;
+  float w[ITEMS][VEC], part[ITEMS][VEC];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      w[i][j] = 1.0f;
+      part[i][j] = 0.0f;
+    }
+    if (p.weight && col < p.cols) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w[i]);
+  }
+  int turn = 0;
+  for (int64_t block = blockIdx.x; block < p.row_blocks; block += gridDim.x, ++turn) {
+    const int64_t row = block * L::ROWS + group;
+    const bool live = row < p.rows;
+    RawVec<GT, VEC> g[ITEMS];
+    RawVec<HT, VEC> h[ITEMS], t[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+      const int64_t count = live ? p.cols - col : 0;
+      g[i] = load_vec<GT, VEC>(p.grad, row * p.ldg + col, count);
+      h[i] = load_vec<HT, VEC>(p.h, row * p.ldh + col, count);
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+      t[i] = load_vec<HT, VEC>(p.grad_total, row * p.ldt + col, live && p.grad_total ? p.cols - col : 0);
+    }
+    const float s = live ? p.rstd[row] : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
+        sum += dy * w[i][j] * n;
+        part[i][j] += dy * n;
+      }
+    const float c = sum_over_row<L::LANES>(sum, lds, turn) / static_cast<float>(p.cols);
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+      if (!live || col >= p.cols) continue;
+      float d[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
+        d[j] = s * (dy * w[i][j] - n * c) + element<HT, VEC>(t[i], j);
+      }
+      if (p.grad_x) store_vec<XT, VEC>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
+      if (HT != XT && p.grad_residual) store_vec<HT, VEC>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
+    }
+  }
+  if (!p.parts) return;
+  float* const mine = p.parts + blockIdx.x * p.cols;
+  if constexpr (L::ROWS == 1) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (col + j < p.cols) mine[col + j] = part[i][j];
+    }
+  } else {
+    // (LANES <= 64: no sum over a row goes through LDS)
+    constexpr int kWidth = L::LANES * L::PER;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) lds[group * kWidth + (i * L::LANES + lane) * VEC + j] = part[i][j];
+    __syncthreads();
+    for (int64_t col = threadIdx.x; col < p.cols; col += L::THREADS) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < L::ROWS; ++k) sum += lds[k * kWidth + col];
+      mine[col] = sum;
+    }
+  }
+}
+
+// Rows that do not fit the registers: the sum first, then the gradients, with dw's
+// part of a workgroup read and written for every row it takes.
+template <int GT, int HT, int XT, typename L>
+__global__ __launch_bounds__(L::THREADS) void rms_norm_grad_wide_kernel(const NormGradParams p) {
+  constexpr int VEC = L::VEC, STEP = L::THREADS * VEC;
+  __shared__ float lds[2 * L::THREADS / 64];
+  int turn = 0;
+  float* const mine = p.parts ? p.parts + blockIdx.x * p.cols : nullptr;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, ++turn) {
+    const float s = p.rstd[row];
+    float sum = 0.0f;
+    for (int64_t col = threadIdx.x * VEC; col < p.cols; col += STEP) {
+      const auto g = load_vec<GT, VEC>(p.grad, row * p.ldg + col, p.cols - col);
+      const auto h = load_vec<HT, VEC>(p.h, row * p.ldh + col, p.cols - col);
+      float w[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
+      if (p.weight) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dy = element<GT, VEC>(g, j), n = element<HT, VEC>(h, j) * s;
+        sum += dy * w[j] * n;
+        if (mine && col + j < p.cols) mine[col + j] = (turn ? mine[col + j] : 0.0f) + dy * n;
+      }
+    }
+    const float c = sum_over_row<L::THREADS>(sum, lds, turn) / static_cast<float>(p.cols);
+    for (int64_t col = threadIdx.x * VEC; col < p.cols; col += STEP) {
+      const auto g = load_vec<GT, VEC>(p.grad, row * p.ldg + col, p.cols - col);
+      const auto h = load_vec<HT, VEC>(p.h, row * p.ldh + col, p.cols - col);
+      const auto t = load_vec<HT, VEC>(p.grad_total, row * p.ldt + col, p.grad_total ? p.cols - col : 0);
+      float w[VEC], d[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
+      if (p.weight) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float dy = element<GT, VEC>(g, j), n = element<HT, VEC>(h, j) * s;
+        d[j] = s * (dy * w[j] - n * c) + element<HT, VEC>(t, j);
+      }
+      if (p.grad_x) store_vec<XT, VEC>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
+      if (HT != XT && p.grad_residual) store_vec<HT, VEC>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
+    }
+  }
+}
+
+// dw[c] = the sum of the workgroups' parts: 64 columns a workgroup, sixteen
+// threads a column, always in the same order.
+template <int DT>
+__global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* parts, void* out, int64_t groups, int64_t cols) {
+  __shared__ float lds[16][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float sum = 0.0f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = slice; r < groups; r += 16) sum += parts[r * cols + c];
+  }
+  lds[slice][lane] = sum;
+  __syncthreads();
+  if (slice == 0 && c < cols) {
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum += lds[k][lane];
+    if (DT == FSH_DT_F32) static_cast<float*>(out)[c] = sum;
+    else static_cast<uint16_t*>(out)[c] = static_cast<uint16_t>(bits_of<DT>(sum));
+  }
+}
+
+// Workgroups that a gradient's rows are dealt out to.
+template <typename L>
+int64_t grad_groups(int64_t rows) {
+  const int64_t blocks = ceil_div(rows, (int64_t)L::ROWS), most = L::THREADS == 256 ? kGradGroups : kGradGroupsWide;
+  return blocks < most ? blocks : most;
+}
+
+// Launches the gradients; returns how many parts of dw they leave.
+template <int GT, int HT, int XT>
+int64_t launch_grad(NormGradParams& p, hipStream_t stream) {
+  constexpr int VEC = GT == FSH_DT_F32 || HT == FSH_DT_F32 || XT == FSH_DT_F32 ? 4 : 8;
+  int64_t groups = 0;
+  by_columns<VEC>(p.cols, [&](auto layout) {
+    using L = decltype(layout);
+    p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS);
+    groups = grad_groups<L>(p.rows);
+    const dim3 grid(static_cast<uint32_t>(groups)), block(L::THREADS);
+    if constexpr (L::PER == 0)
+      hipLaunchKernelGGL((rms_norm_grad_wide_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
+    else
+      hipLaunchKernelGGL((rms_norm_grad_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
+  });
+  return groups;
+}
+
+}  // namespace
+}  // namespace fsh
+
+FSH_API int64_t fsh_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
+  using namespace fsh;
+  if (rows <= 0 || cols <= 0) return 0;
+  int64_t groups = 0;
+  by_columns<4>(cols, [&](auto layout) { groups = grad_groups<decltype(layout)>(rows); });  // (never fewer than with vectors of 8)
+  return groups * cols * static_cast<int64_t>(sizeof(float));
+}
+
+FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
+  using namespace fsh;
+  const char* who = "fsh_rms_norm_backward";
+  if (!q) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (q->rows < 0 || q->cols < 0) return fail(FSH_EINVAL, "%s: negative shape", who);
+  const int g = q->grad_dtype, h = q->total_dtype, x = q->x_dtype;
+  if (!is_dtype(g) || !is_dtype(h) || !is_dtype(x) || (q->weight_dev && !is_dtype(q->weight_dtype)))
+    return fail(FSH_EINVAL, "%s: unknown dtype (%d, %d, %d, %d)", who, g, h, x, q->weight_dtype);
+  if ((g != x && g != FSH_DT_BF16) || (h != x && h != FSH_DT_F32))
+    return fail(FSH_EINVAL, "%s: a gradient of dtype %d (that of x, %d, or bf16) of a sum of dtype %d (that of x, or fp32)", who, g, x, h);
+  if (q->grad_weight_dev && !q->weight_dev) return fail(FSH_EINVAL, "%s: a weight's gradient without a weight", who);
+  if (q->rows == 0 || q->cols == 0) {
+    if (q->grad_weight_dev && q->cols) return fail(FSH_ENOTSUP, "%s: a weight's gradient needs rows", who);
+    return FSH_OK;
+  }
+  if (!q->grad_dev || !q->total_dev || !q->rstd_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
+  if (q->ldg < q->cols || q->ldh < q->cols || (q->grad_total_dev && q->ldt < q->cols))
+    return fail(FSH_EINVAL, "%s: a row stride (%lld, %lld, %lld) is less than cols %lld", who, (long long)q->ldg, (long long)q->ldh, (long long)q->ldt,
+                (long long)q->cols);
+  if (!aligned(q->grad_dev, bytes_of(g)) || !aligned(q->total_dev, bytes_of(h)) || !aligned(q->rstd_dev, 4) || !aligned(q->grad_total_dev, bytes_of(h)) ||
+      !aligned(q->grad_x_dev, bytes_of(x)) || !aligned(q->grad_residual_dev, bytes_of(h)) || !aligned(q->workspace_dev, 4) ||
+      (q->weight_dev && (!aligned(q->weight_dev, bytes_of(q->weight_dtype)) || !aligned(q->grad_weight_dev, bytes_of(q->weight_dtype)))))
+    return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements", who);
+  if (q->grad_weight_dev && (!q->workspace_dev || q->workspace_nbytes < fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols)))
+    return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)q->workspace_nbytes,
+                (long long)fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols));
+  if (ceil_div(q->cols, (int64_t)64) > (1LL << 22) - 1) return fail(FSH_ENOTSUP, "%s: too many columns", who);
+  NormGradParams p = {};
+  p.grad = q->grad_dev;
+  p.h = q->total_dev;
+  p.weight = q->weight_dev;
+  p.rstd = q->rstd_dev;
+  p.grad_total = q->grad_total_dev;
+  p.grad_x = q->grad_x_dev;
+  p.grad_residual = q->grad_residual_dev;
+  p.parts = q->grad_weight_dev ? static_cast<float*>(q->workspace_dev) : nullptr;
+  p.rows = q->rows;
+  p.cols = q->cols;
+  p.ldg = q->ldg;
+  p.ldh = q->ldh;
+  p.ldt = q->ldt;
+  p.weight_dtype = q->weight_dtype;
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  int64_t groups;
+  if (x == FSH_DT_BF16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_BF16, FSH_DT_BF16>(p, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_BF16>(p, on);
+  else if (x == FSH_DT_F16 && g == x) groups = h == x ? launch_grad<FSH_DT_F16, FSH_DT_F16, FSH_DT_F16>(p, on) : launch_grad<FSH_DT_F16, FSH_DT_F32, FSH_DT_F16>(p, on);
+  else if (x == FSH_DT_F16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_F16, FSH_DT_F16>(p, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F16>(p, on);
+  else if (g == x) groups = launch_grad<FSH_DT_F32, FSH_DT_F32, FSH_DT_F32>(p, on);
+  else groups = launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F32>(p, on);
+  if (int rc = check_launch("rms_norm_grad_kernel")) return rc;
+  if (!q->grad_weight_dev) return FSH_OK;
+  const dim3 grid(static_cast<uint32_t>(ceil_div(q->cols, (int64_t)64))), block(1024);
+  if (q->weight_dtype == FSH_DT_BF16) hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_BF16>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);
+  else if (q->weight_dtype == FSH_DT_F16) hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_F16>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);
+  else hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_F32>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);
+  return check_launch("norm_weight_grad_kernel");
+}

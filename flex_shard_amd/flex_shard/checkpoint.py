@@ -18,10 +18,11 @@ from typing import Any, Iterable
 
 import torch
 
+from ..adamw import FlexShardAdamW
 from ..placement_contract import GlobalLayout, compose_global_layouts, set_global_layout
 
 # Their states other than ``step`` are elementwise, with the parameter's shape.
-_CHECKPOINTABLE_OPTIMIZERS = (torch.optim.Adam, torch.optim.AdamW)
+_CHECKPOINTABLE_OPTIMIZERS = (torch.optim.Adam, torch.optim.AdamW, FlexShardAdamW)
 _OPTIMIZER_CHECKPOINT_HOOK_ATTR = "_flex_shard_optimizer_checkpoint_hook"
 
 

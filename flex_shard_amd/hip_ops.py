@@ -34,15 +34,17 @@ from ._native import (
 __all__ = [
     "DT_BF16", "DT_F16", "DT_F32", "EPS_FP32", "EPS_INPUT_DTYPE", "REDUCE_POSTDIV", "REDUCE_POSTMUL",
     "REDUCE_PREMUL", "REDUCE_SUM", "SRC_BF16", "SRC_F16", "SRC_F32", "SRC_F32_AS_BF16", "SRC_F32_AS_F16",
-    "MuonStepPlan", "MxFp4Matrix", "QuantChunkSpec", "QuantPackPlan", "accumulate_grad", "act_quant_128x1_transposed", "act_quant_1x128", "act_quant_both",
+    "MuonStepPlan", "MxFp4Matrix", "QuantChunkSpec", "QuantPackPlan", "accumulate_grad", "act_dequant_1x128",
+    "act_quant_128x1_transposed", "act_quant_1x128", "act_quant_both", "adamw_state_values", "adamw_step",
     "copy_row_segments", "copy_segments", "fp8_gemm_1x128_128x1", "fp8_gemm_1x128_128x128", "fp8_gemm_1x128_128x128_dgrad",
     "expert_combine", "expert_combine_at", "expert_combine_backward", "expert_combine_backward_at", "expert_dispatch",
     "expert_dispatch_at", "expert_route", "expert_route_buffer", "expert_route_into",
-    "fp8_gemm_tiles", "fp8_linear_backward", "fp8_transpose", "gemm_nt", "gemm_nt_group", "gemm_tiles", "muon_apply",
+    "fp8_gemm_tiles", "fp8_linear_backward", "fp8_transpose", "gemm_nt", "gemm_nt_group", "gemm_tiles", "grad_square_sum", "muon_apply",
     "muon_prepare", "mxfp4_dequantize", "mxfp4_expert_linear", "mxfp4_gemm", "mxfp4_gemm_tiles",
     "mxfp4_linear", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
     "newton_schulz_product_tiles",
-    "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
+    "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "rms_norm", "rms_norm_backward",
+    "rms_norm_token_runs", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
 ]
 
 
@@ -1485,3 +1487,217 @@ def expert_combine_backward_at(
     if status:
         _native.check(status, "fsh_expert_combine_backward")
     return grad_rows, grad_weights
+
+
+def _queue(entry: str, device: torch.device, *args) -> None:
+    """Call a C entry with the current stream of ``device`` behind its arguments,
+    ``device`` being the current one meanwhile."""
+    fn = getattr(_native.lib(), entry)
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream_ptr(device))
+    if status:
+        _native.check(status, entry)
+
+
+def _norm_stride(name: str, t: torch.Tensor, shape: tuple[int, int]) -> int:
+    rows, cols = shape
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _check_norm_weight(weight: torch.Tensor | None, cols: int) -> int:
+    if weight is None:
+        return DT_F32
+    if tuple(weight.shape) != (cols,) or (cols > 1 and weight.stride(0) != 1):
+        raise ValueError(f"weight must be {[cols]}, contiguous, got {tuple(weight.shape)} / {weight.stride()}")
+    return _float_dt(weight.dtype)
+
+
+def rms_norm(
+    x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None, *, fp8: bool = False,
+    keep_rstd: bool = False,
+) -> tuple[torch.Tensor | tuple[torch.Tensor, torch.Tensor], torch.Tensor | None, torch.Tensor | None]:
+    """``(out, total, rstd)`` of the rows of ``x`` [rows, cols]: ``total`` = x +
+    residual (None without one), ``out`` its norm in the type of ``x``, or with ``fp8``
+    what :func:`act_quant_1x128` makes of it in bf16; ``rstd`` [rows] if kept."""
+    _require_gpu(x, *(t for t in (weight, residual) if t is not None))
+    if x.ndim != 2:
+        raise ValueError(f"expected rows [rows, cols], got {tuple(x.shape)}")
+    rows, cols = shape = tuple(x.shape)
+    q = _native.Norm()
+    q.x_dtype, q.weight_dtype = _float_dt(x.dtype), _check_norm_weight(weight, cols)
+    q.rows, q.cols, q.eps = rows, cols, eps
+    q.ldx = _norm_stride("x", x, shape)
+    q.x_dev = x.data_ptr()
+    total = rstd = scales = None
+    if weight is not None:
+        q.weight_dev = weight.data_ptr()
+    if residual is not None:
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise NotImplementedError(f"a residual is of the type of x ({x.dtype}) or fp32, got {residual.dtype}")
+        q.residual_dtype, q.ldr = _float_dt(residual.dtype), _norm_stride("residual", residual, shape)
+        total = torch.empty(shape, dtype=residual.dtype, device=x.device)
+        q.residual_dev, q.total_dev = residual.data_ptr(), total.data_ptr()
+    if fp8:
+        padded = -(-cols // 128) * 128
+        out = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=x.device)
+        scales = torch.empty((padded // 128, rows), dtype=torch.float32, device=x.device)
+        q.form, q.scales_dev = _native.NORM_FP8, scales.data_ptr()
+    else:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    q.out_dev = out.data_ptr()
+    if keep_rstd:
+        rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        q.rstd_dev = rstd.data_ptr()
+    if rows and cols:
+        _queue("fsh_rms_norm", x.device, ctypes.byref(q))
+    return (out, scales) if fp8 else out, total, rstd
+
+
+def rms_norm_backward(
+    grad: torch.Tensor, total: torch.Tensor, weight: torch.Tensor | None, rstd: torch.Tensor, x_dtype: torch.dtype,
+    grad_total: torch.Tensor | None = None, *, needs_x: bool = True, needs_residual: bool = False, needs_weight: bool = True,
+) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """``(grad_x, grad_residual, grad_weight)`` of :func:`rms_norm`; ``total`` is
+    what it normed (``x`` without a residual).  The first two are one tensor where
+    ``total`` is of ``x_dtype``."""
+    _require_gpu(grad, total, rstd, *(t for t in (weight, grad_total) if t is not None))
+    rows, cols = shape = tuple(total.shape)
+    same = total.dtype == x_dtype
+    q = _native.NormGradient()
+    q.grad_dtype, q.total_dtype, q.x_dtype = _float_dt(grad.dtype), _float_dt(total.dtype), _float_dt(x_dtype)
+    q.weight_dtype = _check_norm_weight(weight, cols)
+    q.rows, q.cols = shape
+    q.ldg, q.ldh = _norm_stride("grad", grad, shape), _norm_stride("total", total, shape)
+    if tuple(rstd.shape) != (rows,) or rstd.dtype != torch.float32 or not rstd.is_contiguous():
+        raise ValueError(f"rstd must be contiguous fp32 [{rows}], got {rstd.dtype} {tuple(rstd.shape)}")
+    q.grad_dev, q.total_dev, q.rstd_dev = grad.data_ptr(), total.data_ptr(), rstd.data_ptr()
+    if weight is not None:
+        q.weight_dev = weight.data_ptr()
+    if grad_total is not None:
+        if grad_total.dtype != total.dtype:
+            raise ValueError(f"the gradient of a sum of {total.dtype} is of that type, got {grad_total.dtype}")
+        q.ldt, q.grad_total_dev = _norm_stride("grad_total", grad_total, shape), grad_total.data_ptr()
+    grad_x = grad_residual = grad_weight = None
+    if needs_x or (same and needs_residual):
+        grad_x = torch.empty(shape, dtype=x_dtype, device=grad.device)
+        q.grad_x_dev = grad_x.data_ptr()
+    if needs_residual:
+        grad_residual = grad_x if same else torch.empty(shape, dtype=total.dtype, device=grad.device)
+        if not same:
+            q.grad_residual_dev = grad_residual.data_ptr()
+    if needs_weight and weight is not None:
+        grad_weight = torch.empty((cols,), dtype=weight.dtype, device=grad.device)
+        nbytes = _native.lib().fsh_rms_norm_backward_workspace_bytes(rows, cols)
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=grad.device)
+        q.grad_weight_dev, q.workspace_dev, q.workspace_nbytes = grad_weight.data_ptr(), workspace.data_ptr(), nbytes
+    _queue("fsh_rms_norm_backward", grad.device, ctypes.byref(q))
+    return grad_x if needs_x else None, grad_residual, grad_weight
+
+
+def rms_norm_token_runs(total: torch.Tensor, weight: torch.Tensor | None, rstd: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """What :func:`act_quant_128x1_transposed` makes of the norm in bf16 (its columns
+    padded with zeros to a multiple of 8), from what was normed and ``rstd``."""
+    _require_gpu(total, rstd, *(() if weight is None else (weight,)))
+    rows, cols = shape = tuple(total.shape)
+    if tuple(rstd.shape) != (rows,) or rstd.dtype != torch.float32 or not rstd.is_contiguous():
+        raise ValueError(f"rstd must be contiguous fp32 [{rows}], got {rstd.dtype} {tuple(rstd.shape)}")
+    width, padded = -(-cols // 8) * 8, -(-rows // 128) * 128
+    q = torch.empty((width, padded), dtype=torch.float8_e4m3fn, device=total.device)
+    scales = torch.empty((padded // 128, width), dtype=torch.float32, device=total.device)
+    if rows and cols:
+        _queue(
+            "fsh_rms_norm_token_runs", total.device, total.data_ptr(), _float_dt(total.dtype), rows, cols,
+            _norm_stride("total", total, shape), rstd.data_ptr(), None if weight is None else weight.data_ptr(),
+            _check_norm_weight(weight, cols), q.data_ptr(), padded, scales.data_ptr(),
+        )
+    return q, scales
+
+
+def act_dequant_1x128(q: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values [rows, cols] of what :func:`act_quant_1x128` returned."""
+    _require_gpu(q, scales)
+    _fp8_matrix("q", q)
+    rows, padded = q.shape
+    if padded != -(-cols // 128) * 128 or q.stride(0) % 8 or q.data_ptr() % 8:
+        raise ValueError(f"q must be [rows, {cols} rounded up to 128], rows 8-byte aligned, got {tuple(q.shape)} / {q.stride()}")
+    if scales.dtype != torch.float32 or not scales.is_contiguous() or tuple(scales.shape) != (padded // 128, rows):
+        raise ValueError(f"scales must be contiguous fp32 of shape {(padded // 128, rows)}, got {tuple(scales.shape)}")
+    out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    if rows and cols:
+        _queue(
+            "fsh_act_dequant_1x128", q.device, q.data_ptr(), scales.data_ptr(), rows, cols, q.stride(0) if rows > 1 else padded,
+            out.data_ptr(), _float_dt(dtype),
+        )
+    return out
+
+
+def grad_square_sum(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
+    """The sum of the squares of all elements of contiguous bf16, fp16 or fp32
+    tensors, a float64 scalar on their device."""
+    device = _require_gpu(*tensors)
+    table = []
+    for t in tensors:
+        if not t.is_contiguous():
+            raise ValueError(f"contiguous tensors, got strides {t.stride()} of {tuple(t.shape)}")
+        table += (t.data_ptr(), t.numel(), _float_dt(t.dtype))
+    table = (ctypes.c_int64 * len(table))(*table)
+    nbytes = _native.lib().fsh_grad_square_sum_workspace_bytes(table, len(tensors))
+    # the sum, and behind it the workgroups' parts
+    buffer = torch.empty((1 + nbytes // 8,), dtype=torch.float64, device=device)
+    out = buffer.data_ptr()
+    _queue("fsh_grad_square_sum", device, table, len(tensors), out, out + 8, nbytes)
+    return buffer[0]
+
+
+def adamw_step(
+    table: Sequence[int], groups: Sequence[tuple], device: torch.device, square_sum: torch.Tensor | None = None, max_norm: float = 0.0
+) -> None:
+    """``fsh_adamw_step``.  ``table``: the twelve numbers of an ``fsh_adamw_tensor``
+    for each tensor, one after the other; the caller answers for the memory that
+    they name.  ``groups``: ``(lr, address of a device lr or None, beta1, beta2, eps,
+    weight_decay)`` each, at most ``_native.ADAMW_GROUPS``."""
+    count, rest = divmod(len(table), _native.ADAMW_TENSOR_INT64S)
+    if rest:
+        raise ValueError(f"{_native.ADAMW_TENSOR_INT64S} numbers a tensor, got {len(table)}")
+    if square_sum is not None:
+        _require_gpu(square_sum)
+        if square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device:
+            raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
+    if not count:
+        return
+    of_groups = (_native.AdamWGroup * len(groups))(*groups)
+    nbytes = _native.lib().fsh_adamw_step_workspace_bytes(count)
+    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    _queue(
+        "fsh_adamw_step", device, (ctypes.c_int64 * len(table))(*table), count, of_groups, len(groups),
+        None if square_sum is None else square_sum.data_ptr(), max_norm, workspace.data_ptr(), nbytes,
+    )
+
+
+def adamw_state_values(
+    exp_avg: torch.Tensor, exp_avg_scale: torch.Tensor, exp_avg_sq: torch.Tensor, exp_avg_sq_scale: torch.Tensor, dtype: torch.dtype
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the 8-bit codes of both moments stand for."""
+    device = _require_gpu(exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale)
+    numel = exp_avg.numel()
+    blocks = -(-numel // _native.ADAMW_BLOCK)
+    for name, t, want, count in (
+        ("exp_avg", exp_avg, torch.uint8, numel), ("exp_avg_sq", exp_avg_sq, torch.uint8, numel),
+        ("exp_avg_scale", exp_avg_scale, torch.float32, blocks), ("exp_avg_sq_scale", exp_avg_sq_scale, torch.float32, blocks),
+    ):
+        if t.dtype != want or t.numel() != count or not t.is_contiguous():
+            raise ValueError(f"{name} must be {count} contiguous {want}, got {t.dtype} {tuple(t.shape)}")
+    out = [torch.empty(exp_avg.shape, dtype=dtype, device=device) for _ in range(2)]
+    if numel:
+        _queue(
+            "fsh_adamw_state_values", device, exp_avg.data_ptr(), exp_avg_scale.data_ptr(), exp_avg_sq.data_ptr(),
+            exp_avg_sq_scale.data_ptr(), numel, out[0].data_ptr(), out[1].data_ptr(), _float_dt(dtype),
+        )
+    return out[0], out[1]

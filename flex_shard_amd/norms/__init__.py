@@ -1,0 +1,187 @@
+"""Root-mean-square norms ahead of the linears, with the residual's addition:
+
+    h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
+
+:func:`rms_norm` gives y in the type of ``x``, :func:`rms_norm_fp8` in the 8 bits that
+the blockwise FP8 linears multiply (``flex_shard_amd.blockwise_fp8``), so that no linear
+quantizes it again.  Both also return h where there is a residual: the stream that the
+next layer adds to.  The norm is that of h as it is kept, rounded to the residual's type.
+"""
+
+from __future__ import annotations
+
+from functools import partial
+from typing import Any
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import hip_ops
+from ..blockwise_fp8.fp8_activation import Fp8Activation
+from ..experts import differentiates
+
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _as_rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] with contiguous rows that do not overlap; a copy if need be."""
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _check(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None) -> None:
+    if x.dtype not in _DTYPES:
+        raise NotImplementedError(f"the norm takes bf16, fp16 or fp32 rows, got {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError(f"expected rows [..., cols], got {tuple(x.shape)}")
+    if weight is not None and (tuple(weight.shape) != (x.shape[-1],) or weight.dtype not in _DTYPES):
+        raise ValueError(f"weight must be bf16, fp16 or fp32 [{x.shape[-1]}], got {weight.dtype} {tuple(weight.shape)}")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
+        if residual.dtype not in (x.dtype, torch.float32):
+            raise NotImplementedError(f"a residual is of the type of x ({x.dtype}) or fp32, got {residual.dtype}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
+def _carrier(shape, device: torch.device) -> torch.Tensor:
+    return torch.empty((), dtype=torch.bfloat16, device=device).expand(shape)
+
+
+class _Norm(torch.autograd.Function):
+    """``(y, total)``; in 8 bits y is the carrier, and ``kept`` gets the bytes, the
+    scales and what the token runs are made of."""
+
+    @staticmethod
+    def forward(ctx: Any, x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor | None, eps: float, kept: list | None):
+        out, total, rstd = hip_ops.rms_norm(x, weight, eps, residual, fp8=kept is not None, keep_rstd=True)
+        normed = x if total is None else total
+        if kept is not None:
+            kept += (*out, normed, rstd)
+            out = _carrier(x.shape, x.device)
+        ctx.save_for_backward(normed, weight, rstd)
+        ctx.x_dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        return out, total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
+        normed, weight, rstd = ctx.saved_tensors
+        needs_x, needs_residual, needs_weight = ctx.needs_input_grad[:3]
+        if grad is None:  # the stream alone was used
+            if grad_total is None:
+                return None, None, None, None, None
+            return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
+        grads = hip_ops.rms_norm_backward(
+            _as_rows(grad), normed, weight, rstd, ctx.x_dtype, None if grad_total is None else _as_rows(grad_total),
+            needs_x=needs_x, needs_residual=needs_residual, needs_weight=needs_weight,
+        )
+        return (*grads, None, None)
+
+
+def rms_norm(
+    x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *, residual: torch.Tensor | None = None
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """The norm of the rows of ``x`` [..., cols] (bf16, fp16 or fp32), in its type,
+    times ``weight`` [cols] (any of these types, or None).  With ``residual``, of the
+    shape of ``x`` and its type or fp32, ``(norm of x + residual, x + residual)``, the sum in
+    the residual's type.  Statistics in fp32, every output rounded once; differentiable."""
+    _check(x, weight, eps, residual)
+    if x.numel() == 0:  # no rows: torch's own empty products keep the graph
+        total = x if residual is None else x.to(residual.dtype) + residual
+        y = (total if weight is None else total * weight).to(x.dtype)
+        return y if residual is None else (y, total)
+    rows = _as_rows(x)
+    stream = None if residual is None else _as_rows(residual)
+    weight = weight if weight is None else weight.contiguous()
+    if differentiates(rows, stream, weight):
+        y, total = _Norm.apply(rows, stream, weight, eps, None)
+    else:
+        y, total, _ = hip_ops.rms_norm(rows, weight, eps, stream)
+    y = y.view(x.shape)
+    return y if residual is None else (y, total.view(x.shape))
+
+
+def _version(t: torch.Tensor | None) -> int:
+    return 0 if t is None or t.is_inference() else t._version
+
+
+def _token_runs(of: tuple, versions: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
+    if [_version(t) for t in of] != versions:
+        raise RuntimeError("what an 8-bit norm was made of was changed in place before a weight gradient's form of it was made")
+    return hip_ops.rms_norm_token_runs(*of)
+
+
+def rms_norm_fp8(
+    x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6, *, residual: torch.Tensor | None = None
+) -> Fp8Activation | tuple[Fp8Activation, torch.Tensor]:
+    """:func:`rms_norm`, its output rounded to bf16 and quantized like the
+    activations of the blockwise FP8 linears, which take it as it is."""
+    _check(x, weight, eps, residual)
+    rows = _as_rows(x)
+    stream = None if residual is None else _as_rows(residual)
+    weight = weight if weight is None else weight.contiguous()
+    if x.numel() == 0:
+        y = rms_norm(x, weight, eps, residual=residual)
+        y, total = (y, None) if residual is None else y
+        (q, scales), _, rstd = hip_ops.rms_norm(rows.detach(), None, eps, fp8=True, keep_rstd=True)
+        normed, carrier = rows.detach(), y.to(torch.bfloat16)
+    elif differentiates(rows, stream, weight):
+        kept: list = []
+        carrier, total = _Norm.apply(rows, stream, weight, eps, kept)
+        q, scales, normed, rstd = kept
+        carrier = carrier.view(x.shape)
+    else:
+        (q, scales), total, rstd = hip_ops.rms_norm(rows, weight, eps, stream, fp8=True, keep_rstd=True)
+        normed, carrier = rows if total is None else total, _carrier(x.shape, x.device)
+    of = (normed.detach(), None if weight is None else weight.detach(), rstd)
+    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, of, [_version(t) for t in of]))
+    return activation if residual is None else (activation, total.view(x.shape))
+
+
+class FlexShardRMSNorm(nn.RMSNorm):
+    """``nn.RMSNorm`` over the last dimension on the kernels here.  ``forward(x,
+    residual)`` adds first and returns the sum too; with ``fp8`` the output is an
+    :class:`~flex_shard_amd.blockwise_fp8.Fp8Activation`."""
+
+    @classmethod
+    def from_float(cls, mod: nn.RMSNorm) -> "FlexShardRMSNorm":
+        if len(mod.normalized_shape) != 1:
+            raise NotImplementedError(f"the norm is over the last dimension, got {tuple(mod.normalized_shape)}")
+        new_mod = cls(mod.normalized_shape, eps=mod.eps, elementwise_affine=mod.elementwise_affine, device="meta")
+        new_mod.weight = mod.weight
+        new_mod.train(mod.training)
+        return new_mod
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, fp8: bool = False):
+        if len(self.normalized_shape) != 1 or x.shape[-1:] != tuple(self.normalized_shape):
+            raise ValueError(f"the norm is over a last dimension {tuple(self.normalized_shape)}, got {tuple(x.shape)}")
+        eps = torch.finfo(x.dtype).eps if self.eps is None else self.eps
+        return (rms_norm_fp8 if fp8 else rms_norm)(x, self.weight, eps, residual=residual)
+
+
+def convert_to_flex_shard_rms_norm(module: nn.Module, filter_fn=None) -> nn.Module:
+    """Swap every ``nn.RMSNorm`` over one dimension below ``module`` that
+    ``filter_fn(fqn, child)`` accepts (all, when it is None) for a
+    :class:`FlexShardRMSNorm` sharing its weight."""
+    _convert_children(module, "", filter_fn)
+    return module
+
+
+def _convert_children(parent: nn.Module, prefix: str, filter_fn) -> None:
+    for name, child in list(parent.named_children()):
+        fqn = f"{prefix}{name}"
+        if type(child) is nn.RMSNorm and len(child.normalized_shape) == 1 and (filter_fn is None or filter_fn(fqn, child)):
+            setattr(parent, name, FlexShardRMSNorm.from_float(child))
+        else:
+            _convert_children(child, f"{fqn}.", filter_fn)
+
+
+__all__ = ["FlexShardRMSNorm", "convert_to_flex_shard_rms_norm", "rms_norm", "rms_norm_fp8"]

@@ -139,7 +139,7 @@ int fsh_zero_segments(void* dst_dev, const int64_t* numels_dev, const int64_t* d
 
 #define FSH_DT_BF16 0
 #define FSH_DT_F32 1
-#define FSH_DT_F16 2 /* fsh_unpack_dequant's dequantized output only */
+#define FSH_DT_F16 2 /* fsh_unpack_dequant's dequantized output, and from section 11 on */
 /* out[dst_off[s]+i] = cast(inputs[tensor_idx[s]][src_off[s]+i]), i < numel[s];
  * offsets in elements; input_ptrs_dev holds the inputs' device addresses.  A
  * negative tensor index makes the segment a zero fill, so one launch can
@@ -651,6 +651,124 @@ int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, cons
                                 const int32_t* offsets_dev, int32_t experts, const void* weights_dev, int32_t weights_dtype,
                                 int64_t tokens, int32_t top_k, int64_t width, int32_t dtype, void* grad_rows_dev,
                                 void* grad_weights_dev, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 14. Root-mean-square norm of rows of `cols` elements, the layer ahead of the
+ * linears, with the residual's addition and with an output that the FP8 linear
+ * multiplies as it is.  The reference leaves norms to its models.
+ *
+ * fsh_rms_norm: h = x + residual, rounded to residual_dtype (that of x, or fp32)
+ * and written to total (contiguous); h = x without a residual.  s = 1 /
+ * sqrt(mean(h^2) + eps) in fp32, to rstd [rows] unless that is null.  y = h s
+ * weight (weight null: 1).
+ *   FSH_NORM_VALUES  out [rows, cols] of x_dtype, contiguous
+ *   FSH_NORM_FP8     y rounded to bf16 and quantized like section 8's activations:
+ *                    out [rows][cols rounded up to 128] E4M3FN bytes (pad zero),
+ *                    scales [that / 128][rows]; the bits of fsh_act_quant_1x128
+ * ldx, ldr: row strides of x and residual.
+ *
+ * fsh_rms_norm_backward: of h (total, x_dtype's or fp32, row stride ldh), the
+ * output's gradient (x_dtype or, for the FP8 form, bf16; ldg) and, or null, the
+ * gradient of h from what reads it besides (of h's type; ldt): grad_x [rows, cols] of
+ * x_dtype, grad_residual of h's type (either null; the second is not written where the
+ * types are the same: it is grad_x), and grad_weight of weight_dtype, or null.  The
+ * workspace is for grad_weight alone.
+ *
+ * fsh_rms_norm_token_runs: the FP8 form's y in runs of 128 rows, transposed, as
+ * fsh_act_quant_128x1_transposed writes it (q [cols rounded up to 8][ldq = rows
+ * rounded up to 128], scales [ldq / 128][cols rounded up to 8]): what a weight gradient
+ * contracts over.  From h and rstd.
+ *
+ * fsh_act_dequant_1x128: the values [rows, cols], contiguous, of section 8's
+ * quantized activations.
+ * ---------------------------------------------------------------------- */
+#define FSH_NORM_VALUES 0
+#define FSH_NORM_FP8 1
+typedef struct fsh_norm {
+  const void* x_dev;
+  const void* residual_dev;
+  const void* weight_dev;
+  void* total_dev;
+  void* out_dev;
+  float* scales_dev;
+  float* rstd_dev;
+  int64_t rows, cols, ldx, ldr;
+  int32_t x_dtype, residual_dtype, weight_dtype, form;
+  float eps;
+  int32_t reserved;
+} fsh_norm;
+int fsh_rms_norm(const fsh_norm* norm, void* stream);
+typedef struct fsh_norm_gradient {
+  const void* grad_dev;
+  const void* total_dev;
+  const void* weight_dev;
+  const float* rstd_dev;
+  const void* grad_total_dev;
+  void* grad_x_dev;
+  void* grad_residual_dev;
+  void* grad_weight_dev;
+  void* workspace_dev;
+  int64_t workspace_nbytes;
+  int64_t rows, cols, ldg, ldh, ldt;
+  int32_t grad_dtype, total_dtype, x_dtype, weight_dtype;
+} fsh_norm_gradient;
+int64_t fsh_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int fsh_rms_norm_backward(const fsh_norm_gradient* gradient, void* stream);
+int fsh_rms_norm_token_runs(const void* total_dev, int32_t dtype, int64_t rows, int64_t cols, int64_t ldh, const float* rstd_dev,
+                            const void* weight_dev, int32_t weight_dtype, void* q_dev, int64_t ldq, float* scales_dev, void* stream);
+int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, int64_t rows, int64_t cols, int64_t ldq, void* out_dev,
+                          int32_t dtype, void* stream);
+
+/* ------------------------------------------------------------------------
+ * 15. AdamW over many tensors at once, for the parameters that section 10's step
+ * does not take (or all), and the sum of squares that their gradients are clipped by.
+ *
+ * fsh_grad_square_sum: *out = the sum of the squares of `count` tensors' elements,
+ * in 64 bits, in a fixed order.  tensors: three numbers each, address, elements,
+ * dtype (host memory).  workspace: at least ..._workspace_bytes(tensors, count), 8-byte aligned.
+ *
+ * fsh_adamw_step: per tensor, in fp32 with one rounding to the parameter's type,
+ *   c = min(1, max_norm / (sqrt(square_sum) + 1e-6)), 1 without a sum or a positive max_norm
+ *   g = c g;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  t = step + 1, kept
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * A square_sum that is an infinity or not a number leaves everything, step counts
+ * included, as it is.  Tensors and groups are host tables, read within the call; lr_dev, if not
+ * null, is read by the step in place of lr.  Parameters and gradients: bf16 or fp32, contiguous,
+ * aligned to their elements.  States: fp32, or 8-bit codes with an fp32 scale for each
+ * FSH_ADAMW_BLOCK elements (the last block may be shorter):
+ *   magnitude of a code c > 0: the fp32 number of bits (c + 889) << 20 (first moment, c =
+ *   code & 127, negative with bit 7) or (c + 761) << 20 (second), times the scale; c = 0: zero
+ * rounded up or down evenly over elements and steps.  All zero is the start of both.
+ * workspace: ..._workspace_bytes(count), 16-byte aligned; only the call itself uses it.
+ *
+ * fsh_adamw_state_values: what the codes stand for, in dtype.
+ * ---------------------------------------------------------------------- */
+#define FSH_ADAMW_BLOCK 128
+#define FSH_ADAMW_GROUPS 16
+typedef struct fsh_adamw_tensor {
+  void* param_dev;
+  const void* grad_dev;
+  void* exp_avg_dev;
+  void* exp_avg_sq_dev;
+  float* exp_avg_scale_dev;    /* 8 bits: [ceil(numel / FSH_ADAMW_BLOCK)] */
+  float* exp_avg_sq_scale_dev;
+  int32_t* step_dev;
+  int64_t numel;
+  int64_t param_dtype, grad_dtype, state_bits, group;
+} fsh_adamw_tensor;
+typedef struct fsh_adamw_group {
+  double lr;
+  const float* lr_dev;
+  double beta1, beta2, eps, weight_decay;
+} fsh_adamw_group;
+int64_t fsh_grad_square_sum_workspace_bytes(const int64_t* tensors, int32_t count);
+int fsh_grad_square_sum(const int64_t* tensors, int32_t count, double* out_dev, void* workspace_dev, int64_t workspace_nbytes, void* stream);
+int64_t fsh_adamw_step_workspace_bytes(int32_t count);
+int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count,
+                   const double* square_sum_dev, double max_norm, void* workspace_dev, int64_t workspace_nbytes, void* stream);
+int fsh_adamw_state_values(const void* exp_avg_dev, const float* exp_avg_scale_dev, const void* exp_avg_sq_dev,
+                           const float* exp_avg_sq_scale_dev, int64_t numel, void* exp_avg_out_dev, void* exp_avg_sq_out_dev,
+                           int32_t dtype, void* stream);
 
 #ifdef __cplusplus
 }

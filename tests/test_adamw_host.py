@@ -1,0 +1,151 @@
+"""What the optimizer's entry points refuse before anything reaches a GPU, and the
+definition of its 8-bit states that the GPU tests compare with."""
+
+import ctypes
+
+import pytest
+import torch
+from adamw_definition import FIRST, SECOND, decode, dither, encode
+
+from flex_shard_amd import _native
+from flex_shard_amd.adamw import FlexShardAdamW, grad_square_sum
+
+OK, EINVAL, ENOTSUP = 0, -22, -95
+SOMEWHERE = 1 << 20  # an aligned address that no refused call touches
+
+
+def _message():
+    return _native.lib().fsh_last_error().decode()
+
+
+def _table(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def test_square_sum():
+    lib = _native.lib()
+    for tensor, status, word in (
+        ((SOMEWHERE, -1, 0), EINVAL, "negative"), ((SOMEWHERE, 5, 3), EINVAL, "dtype"), ((SOMEWHERE, 5, -1), EINVAL, "dtype"),
+        ((SOMEWHERE, 5, 1 << 40), EINVAL, "dtype"), ((0, 5, 0), EINVAL, "null"), ((SOMEWHERE + 1, 5, 0), ENOTSUP, "aligned"),
+        ((SOMEWHERE + 2, 5, 1), ENOTSUP, "aligned"),
+    ):
+        assert lib.fsh_grad_square_sum(_table(SOMEWHERE, 8, 0, *tensor), 2, SOMEWHERE, SOMEWHERE, 1 << 20, None) == status
+        assert word in _message() and _message().startswith("fsh_grad_square_sum")
+    good = _table(SOMEWHERE, 8, 0)
+    assert lib.fsh_grad_square_sum(good, -1, SOMEWHERE, SOMEWHERE, 64, None) == EINVAL
+    assert lib.fsh_grad_square_sum(good, 1, None, SOMEWHERE, 64, None) == EINVAL
+    assert lib.fsh_grad_square_sum(good, 1, SOMEWHERE + 4, SOMEWHERE, 64, None) == ENOTSUP
+    assert lib.fsh_grad_square_sum(good, 1, SOMEWHERE, SOMEWHERE, 7, None) == EINVAL and "workspace" in _message()
+    size = lib.fsh_grad_square_sum_workspace_bytes
+    assert size(good, 1) == 8 and size(good, 0) == size(None, 1) == size(good, -1) == 0
+    assert size(_table(SOMEWHERE, 1 << 40, 1), 1) <= 8 * 4096
+
+
+def _step(tensor=(), group=(), count=1, groups=1, square_sum=None, max_norm=0.0, workspace=SOMEWHERE, nbytes=1 << 20):
+    values = [SOMEWHERE] * 7 + [1000, _native.DT_F32, _native.DT_F32, 8, 0]
+    for at, value in dict(tensor).items():
+        values[at] = value
+    entry = dict(lr=1e-3, lr_dev=None, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1) | dict(group)
+    table = (_native.AdamWGroup * 1)(tuple(entry.values()))
+    return _native.lib().fsh_adamw_step(_table(*values), count, table, groups, square_sum, max_norm, workspace, nbytes, None)
+
+
+@pytest.mark.parametrize(
+    "arguments,status,word",
+    [
+        (dict(count=-1), EINVAL, "negative"), (dict(groups=0), ENOTSUP, "groups"), (dict(groups=17), ENOTSUP, "groups"),
+        (dict(workspace=None), EINVAL, "null"), (dict(nbytes=8), EINVAL, "workspace"), (dict(workspace=SOMEWHERE + 8), EINVAL, "workspace"),
+        (dict(square_sum=SOMEWHERE + 4), ENOTSUP, "sum"), (dict(max_norm=float("nan")), EINVAL, "max_norm"),
+        (dict(group=dict(beta1=1.0)), EINVAL, "betas"), (dict(group=dict(beta2=-0.1)), EINVAL, "betas"),
+        (dict(group=dict(beta2=float("nan"))), EINVAL, "betas"), (dict(group=dict(eps=-1.0)), EINVAL, "betas"),
+        (dict(group=dict(lr_dev=SOMEWHERE + 2)), ENOTSUP, "learning rate"), (dict(tensor={7: -1}), EINVAL, "size"),
+        (dict(tensor={11: 1}), EINVAL, "group"), (dict(tensor={11: -1}), EINVAL, "group"), (dict(tensor={8: 2}), EINVAL, "bf16"),
+        (dict(tensor={9: 2}), EINVAL, "bf16"), (dict(tensor={10: 16}), EINVAL, "bits"), (dict(tensor={8: 1 << 33}), EINVAL, "bf16"),
+        *((dict(tensor={at: 0}), EINVAL, "null") for at in range(7)),
+        *((dict(tensor={at: SOMEWHERE + 2}), ENOTSUP, "aligned") for at in (0, 1, 4, 5, 6)),
+        (dict(tensor={2: SOMEWHERE + 2, 10: 32}), ENOTSUP, "aligned"), (dict(tensor={7: 1 << 50}), ENOTSUP, "long"),
+    ],
+)
+def test_step(arguments, status, word):
+    assert _step(**arguments) == status
+    assert word in _message() and _message().startswith("fsh_adamw_step")
+
+
+def test_nothing_to_do():
+    assert _step(count=0) == OK
+    assert _native.lib().fsh_adamw_state_values(None, None, None, None, 0, None, None, 0, None) == OK
+    assert _native.lib().fsh_adamw_step_workspace_bytes(-1) == 0
+    assert ctypes.sizeof(_native.AdamWGroup) == 48
+
+
+def test_state_values():
+    call = _native.lib().fsh_adamw_state_values
+    args = [SOMEWHERE] * 4 + [100, SOMEWHERE, SOMEWHERE, 0, None]
+    for at, value, status in ((4, -1, EINVAL), (7, 3, EINVAL), (0, None, EINVAL), (6, None, EINVAL), (1, SOMEWHERE + 2, ENOTSUP), (5, SOMEWHERE + 1, ENOTSUP)):
+        assert call(*args[:at], value, *args[at + 1 :]) == status, (at, value)
+
+
+def test_there_is_no_cpu_path():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    with pytest.raises(RuntimeError, match="CPU"):
+        FlexShardAdamW([p]).step()
+    with pytest.raises(RuntimeError, match="CPU"):
+        grad_square_sum([p.grad])
+    p.grad = None
+    assert FlexShardAdamW([p]).step() is None  # nothing to do
+
+
+def test_a_refused_group_is_not_added():
+    p, q = (torch.nn.Parameter(torch.zeros(4)) for _ in range(2))
+    optimizer = FlexShardAdamW([p])
+    with pytest.raises(ValueError):
+        optimizer.add_param_group(dict(params=[q], betas=(0.9, 2.0)))
+    assert len(optimizer.param_groups) == 1
+
+
+# ---------------------------------------------------------------- the definition
+@pytest.mark.parametrize("codes", [FIRST, SECOND])
+def test_every_code_stands_for_itself(codes):
+    """A block of all codes and its largest is encoded to the codes again, whatever the dither."""
+    for sign in (0, 128) if codes == FIRST else (0,):
+        code = torch.arange(codes + 1).add(torch.where(torch.arange(codes + 1) > 0, sign, 0)).to(torch.uint8)
+        for part in code.split(127):
+            part = torch.cat((part, torch.tensor([codes + sign], dtype=torch.uint8)))
+            value = decode(part, torch.tensor([0.37]), codes)
+            for t in (1, 2, 1000):
+                again, scale = encode(value, t, codes)
+                got = decode(again, scale, codes)
+                # (0.37 times a code over 0.37 may miss it by a rounding, which the dither can take a step down)
+                assert ((got - value).abs() <= value.abs() / 8).all() and scale[0] == torch.tensor(0.37)
+            exact = decode(part, torch.ones(1), codes)
+            assert torch.equal(encode(exact, 7, codes)[0], part)
+
+
+@pytest.mark.parametrize("codes", [FIRST, SECOND])
+def test_rounding_is_even_on_average(codes):
+    """A value's mean over many steps and elements is the value: the dither's
+    spread is a step of at most an eighth over 4000 draws, its error an eighth / sqrt(12 * 4000)."""
+    for target in (0.7, 0.013, 3e-4):
+        x = torch.full((128,), target)
+        x[0] = 1.0
+        values = torch.stack([decode(*encode(x, t, codes), codes)[1:] for t in range(1, 33)])
+        assert abs(values.mean().item() / target - 1) < 5 * 0.125 / (12 * 32 * 127) ** 0.5
+    if codes == FIRST:  # below the smallest code: that, or zero, as often as it takes
+        x = torch.full((128,), 0.3 * 1.25 * 2.0**-16)
+        x[0] = 1.0
+        values = torch.stack([decode(*encode(x, t, codes), codes)[1:] for t in range(1, 33)])
+        assert abs((values > 0).float().mean().item() - 0.3) < 5 * (0.21 / (32 * 127)) ** 0.5
+    else:
+        x = torch.full((128,), 1e-30)
+        x[0] = 1.0
+        assert (decode(*encode(x, 1, codes), codes) > 0).all()
+
+
+def test_the_dither_is_uniform():
+    for codes in (FIRST, SECOND):
+        u = torch.cat([dither(1 << 16, t, codes) for t in (1, 2, 12345)]).double() / 2**32
+        count = u.numel()
+        assert abs(u.mean().item() - 0.5) < 5 / (12 * count) ** 0.5
+        bins = torch.histc(u, 64, 0, 1)
+        assert (bins - count / 64).abs().max() < 5 * (count / 64) ** 0.5
