@@ -26,12 +26,18 @@ struct NormGradParams {
   int32_t weight_dtype;
 };
 
-constexpr int kGradGroups = 1024;      // workgroups of 256 threads: four a compute unit
-constexpr int kGradGroupsWide = 512;   // of 1024
+// Workgroups that rows are dealt out to, so many that all are resident: of 256
+// threads, of 512, of 1024.  More leave more parts of dw: 8192 rows of 4096 bf16 take 56 us with 512
+// of 512 threads, 58 with 768, 68 with 256; of 7168 93 with 256 of 1024, 99 with 512.
+template <typename L>
+constexpr int kGradGroups = L::THREADS == 256 ? 1024 : L::THREADS == 512 ? 512 : 256;
 
 template <int GT, int HT, int XT, typename L>
 __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGradParams p) {
   constexpr int VEC = L::VEC, ITEMS = L::ITEMS;
+  // fp32 outputs leave past the caches: 8192 rows of 7168 on an fp32 stream 187 -> 167 us; bf16 ones
+  // the layer behind finds there (4096 of bf16: 56 us either way).
+  constexpr bool kStreamOut = HT == FSH_DT_F32;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : L::ROWS * L::LANES * L::PER];
   const int lane = threadIdx.x % L::LANES, group = threadIdx.x / L::LANES;
   float w[ITEMS][VEC], part[ITEMS][VEC];
@@ -55,13 +61,13 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGra
     for (int i = 0; i < ITEMS; ++i) {
       const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
       const int64_t count = live ? p.cols - col : 0;
-      g[i] = load_vec<GT, VEC>(p.grad, row * p.ldg + col, count);
-      h[i] = load_vec<HT, VEC>(p.h, row * p.ldh + col, count);
+      g[i] = load_vec<GT, VEC, true>(p.grad, row * p.ldg + col, count);
+      h[i] = load_vec<HT, VEC, true>(p.h, row * p.ldh + col, count);
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      t[i] = load_vec<HT, VEC>(p.grad_total, row * p.ldt + col, live && p.grad_total ? p.cols - col : 0);
+      t[i] = load_vec<HT, VEC, true>(p.grad_total, row * p.ldt + col, live && p.grad_total ? p.cols - col : 0);
     }
     const float s = live ? p.rstd[row] : 0.0f;
     float sum = 0.0f;
@@ -84,8 +90,8 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGra
         const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
         d[j] = s * (dy * w[i][j] - n * c) + element<HT, VEC>(t[i], j);
       }
-      if (p.grad_x) store_vec<XT, VEC>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
-      if (HT != XT && p.grad_residual) store_vec<HT, VEC>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
+      if (p.grad_x) store_vec<XT, VEC, kStreamOut>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
+      if (HT != XT && p.grad_residual) store_vec<HT, VEC, kStreamOut>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
     }
   }
   if (!p.parts) return;
@@ -160,34 +166,46 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_wide_kernel(const No
   }
 }
 
-// dw[c] = the sum of the workgroups' parts: 64 columns a workgroup, sixteen
-// threads a column, always in the same order.
+// dw[c] = the sum of the workgroups' parts: 32 columns a workgroup, 32 threads a
+// column, always in the same order.
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* parts, void* out, int64_t groups, int64_t cols) {
-  __shared__ float lds[16][64];
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  __shared__ float lds[32][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sum = 0.0f;
   if (c < cols) {
-#pragma unroll 8
-    for (int64_t r = slice; r < groups; r += 16) sum += parts[r * cols + c];
+#pragma unroll 16
+    for (int64_t r = slice; r < groups; r += 32) sum += parts[r * cols + c];
   }
   lds[slice][lane] = sum;
   __syncthreads();
-  if (slice == 0 && c < cols) {
-    sum = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) sum += lds[k][lane];
-    if (DT == FSH_DT_F32) static_cast<float*>(out)[c] = sum;
-    else static_cast<uint16_t*>(out)[c] = static_cast<uint16_t>(bits_of<DT>(sum));
-  }
+  // (a slice's threads now share a column, a half-wave)
+  sum = sum32(lds[lane][slice]);
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + slice;
+  if (lane != 0 || mine >= cols) return;
+  if (DT == FSH_DT_F32) static_cast<float*>(out)[mine] = sum;
+  else static_cast<uint16_t*>(out)[mine] = static_cast<uint16_t>(bits_of<DT>(sum));
+}
+
+// launch(layout) with the layout for rows of `cols` columns.
+template <int VEC, typename Launch>
+void by_columns(int64_t cols, Launch launch) {
+  if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC>{});
+  else if (cols <= 512) launch(NormLayout<64, 8, VEC>{});
+  else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
+  else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});
+  else if (cols <= 4096) launch(NormLayout<512, 8, VEC>{});
+  else if (cols <= 8192) launch(NormLayout<1024, 8, VEC>{});
+  else if (cols <= 16384) launch(NormLayout<1024, 16, VEC>{});
+  else launch(NormLayout<1024, 0, VEC>{});
 }
 
 // Workgroups that a gradient's rows are dealt out to.
 template <typename L>
 int64_t grad_groups(int64_t rows) {
-  const int64_t blocks = ceil_div(rows, (int64_t)L::ROWS), most = L::THREADS == 256 ? kGradGroups : kGradGroupsWide;
-  return blocks < most ? blocks : most;
+  const int64_t blocks = ceil_div(rows, (int64_t)L::ROWS);
+  return blocks < kGradGroups<L> ? blocks : kGradGroups<L>;
 }
 
 // Launches the gradients; returns how many parts of dw they leave.
@@ -245,7 +263,7 @@ FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
   if (q->grad_weight_dev && (!q->workspace_dev || q->workspace_nbytes < fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols)))
     return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)q->workspace_nbytes,
                 (long long)fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols));
-  if (ceil_div(q->cols, (int64_t)64) > (1LL << 22) - 1) return fail(FSH_ENOTSUP, "%s: too many columns", who);
+  if (ceil_div(q->cols, (int64_t)32) > (1LL << 22) - 1) return fail(FSH_ENOTSUP, "%s: too many columns", who);
   NormGradParams p = {};
   p.grad = q->grad_dev;
   p.h = q->total_dev;
@@ -270,7 +288,7 @@ FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
   else groups = launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F32>(p, on);
   if (int rc = check_launch("rms_norm_grad_kernel")) return rc;
   if (!q->grad_weight_dev) return FSH_OK;
-  const dim3 grid(static_cast<uint32_t>(ceil_div(q->cols, (int64_t)64))), block(1024);
+  const dim3 grid(static_cast<uint32_t>(ceil_div(q->cols, (int64_t)32))), block(1024);
   if (q->weight_dtype == FSH_DT_BF16) hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_BF16>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);
   else if (q->weight_dtype == FSH_DT_F16) hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_F16>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);
   else hipLaunchKernelGGL(norm_weight_grad_kernel<FSH_DT_F32>, grid, block, 0, on, p.parts, q->grad_weight_dev, groups, q->cols);

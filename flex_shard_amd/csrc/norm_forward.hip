@@ -52,7 +52,7 @@ __device__ __forceinline__ void add_residual(const RawVec<XT, VEC>& x, const Raw
 template <int XT, bool kQuant, int VEC>
 __device__ __forceinline__ void write_out(const NormParams& p, int64_t row, int64_t col, int64_t count, bool live, const float (&y)[VEC]) {
   if constexpr (!kQuant) {
-    if (live && count > 0) store_vec<XT, VEC>(p.out, row * p.cols + col, count, to_vec<XT, VEC>(y));
+    if (live && count > 0) store_vec<XT, VEC, true>(p.out, row * p.cols + col, count, to_vec<XT, VEC>(y));
   } else {
     // (128 / VEC neighbouring lanes have a run; columns from p.cols on are zero)
     float b[VEC];
@@ -81,7 +81,7 @@ __device__ __forceinline__ void write_out(const NormParams& p, int64_t row, int6
 
 template <int XT, int RT, bool kQuant, typename L>
 __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p) {
-  constexpr int VEC = L::VEC, ITEMS = L::ITEMS;
+  constexpr int VEC = L::VEC, ITEMS = L::ITEMS, TURN = L::TURN;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : 1];
   const int lane = threadIdx.x % L::LANES;
   float w[ITEMS][VEC];
@@ -93,43 +93,50 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p
     if (p.weight && col < p.cols) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w[i]);
   }
   int turn = 0;
-  for (int64_t block = blockIdx.x; block < p.row_blocks; block += gridDim.x, ++turn) {
-    const int64_t row = block * L::ROWS + threadIdx.x / L::LANES;
-    const bool live = row < p.rows;
-    RawVec<XT, VEC> x[ITEMS];
-    RawVec<RT, VEC> r[ITEMS];
+  for (int64_t block = blockIdx.x; block < p.row_blocks; block += gridDim.x) {
+    RawVec<XT, VEC> x[TURN][ITEMS];
+    RawVec<RT, VEC> r[TURN][ITEMS];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      const int64_t count = live ? p.cols - col : 0;
-      x[i] = load_vec<XT, VEC>(p.x, row * p.ldx + col, count);
-      r[i] = load_vec<RT, VEC>(p.residual, row * p.ldr + col, count);
-    }
-    float h[ITEMS][VEC];
-    float sum = 0.0f;
+    for (int k = 0; k < TURN; ++k) {
+      const int64_t row = (block * TURN + k) * L::ROWS + threadIdx.x / L::LANES;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      add_residual<XT, RT, VEC>(x[i], r[i], h[i]);
-      if constexpr (RT != kNoType) {
-        const auto rounded = to_vec<RT, VEC>(h[i]);
-        if (live && col < p.cols) store_vec<RT, VEC>(p.total, row * p.cols + col, p.cols - col, rounded);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) h[i][j] = element<RT, VEC>(rounded, j);
+      for (int i = 0; i < ITEMS; ++i) {
+        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+        const int64_t count = row < p.rows ? p.cols - col : 0;
+        x[k][i] = load_vec<XT, VEC, true>(p.x, row * p.ldx + col, count);
+        r[k][i] = load_vec<RT, VEC, true>(p.residual, row * p.ldr + col, count);
       }
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum += h[i][j] * h[i][j];
     }
-    sum = sum_over_row<L::LANES>(sum, lds, turn);
-    const float s = inverse_root(sum, p.cols, p.eps);
-    if (p.rstd && live && lane == 0) p.rstd[row] = s;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      float y[VEC];
+    for (int k = 0; k < TURN; ++k, ++turn) {
+      const int64_t row = (block * TURN + k) * L::ROWS + threadIdx.x / L::LANES;
+      const bool live = row < p.rows;
+      float h[ITEMS][VEC];
+      float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) y[j] = col + j < p.cols ? h[i][j] * s * w[i][j] : 0.0f;
-      write_out<XT, kQuant, VEC>(p, row, col, p.cols - col, live, y);
+      for (int i = 0; i < ITEMS; ++i) {
+        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+        add_residual<XT, RT, VEC>(x[k][i], r[k][i], h[i]);
+        if constexpr (RT != kNoType) {
+          const auto rounded = to_vec<RT, VEC>(h[i]);
+          if (live && col < p.cols) store_vec<RT, VEC, true>(p.total, row * p.cols + col, p.cols - col, rounded);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) h[i][j] = element<RT, VEC>(rounded, j);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum += h[i][j] * h[i][j];
+      }
+      sum = sum_over_row<L::LANES>(sum, lds, turn);
+      const float s = inverse_root(sum, p.cols, p.eps);
+      if (p.rstd && live && lane == 0) p.rstd[row] = s;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+        float y[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] = col + j < p.cols ? h[i][j] * s * w[i][j] : 0.0f;
+        write_out<XT, kQuant, VEC>(p, row, col, p.cols - col, live, y);
+      }
     }
   }
 }
@@ -182,12 +189,28 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
   }
 }
 
+// launch(layout) with the layout for rows of `cols` columns.
+template <int VEC, typename Launch>
+void by_columns(int64_t cols, int64_t rows, Launch launch) {
+  const bool few = rows <= 512;
+  if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC, 2>{});
+  else if (cols <= 512) launch(NormLayout<64, 8, VEC, 2>{});
+  else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
+  else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});
+  else if (cols <= 4096 && !few) launch(NormLayout<256, 16, VEC>{});
+  else if (cols <= 4096) launch(NormLayout<512, 8, VEC>{});
+  else if (cols <= 8192 && !few) launch(NormLayout<256, 32, VEC>{});
+  else if (cols <= 8192) launch(NormLayout<1024, 8, VEC>{});
+  else if (cols <= 16384) launch(NormLayout<1024, 16, VEC>{});
+  else launch(NormLayout<1024, 0, VEC>{});
+}
+
 template <int XT, int RT, bool kQuant>
 void launch_norm(NormParams& p, hipStream_t stream) {
   constexpr int VEC = XT == FSH_DT_F32 || RT == FSH_DT_F32 ? 4 : 8;  // 16 bytes of the wider type
-  by_columns<VEC>(p.cols, [&](auto layout) {
+  by_columns<VEC>(p.cols, p.rows, [&](auto layout) {
     using L = decltype(layout);
-    p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS);
+    p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS * L::TURN);
     constexpr int64_t kMaxGrid = (1LL << 32) / L::THREADS - 1;  // a launch's threads are counted in 32 bits
     const dim3 grid(static_cast<uint32_t>(p.row_blocks < kMaxGrid ? p.row_blocks : kMaxGrid)), block(L::THREADS);
     if constexpr (L::PER == 0)

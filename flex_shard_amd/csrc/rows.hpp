@@ -19,10 +19,40 @@ struct RawVec {
   uint32_t w[DT == kNoType ? 1 : VEC * bytes_of(DT) / 4];
 };
 
-// Elements [0, count) of the VEC at element `at`, the others zero.  A whole
-// vector is one access of up to 16 bytes, or two, whatever the address: global memory
-// instructions may be unaligned.
-template <int DT, int VEC>
+// 8 or 16 bytes, or several 16, at any address (global memory instructions may be
+// unaligned).  STREAM: with the nontemporal hint, for what is not read again.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+template <bool STREAM, int N>
+__device__ __forceinline__ void load_words(const uint8_t* src, uint32_t (&w)[N]) {
+  if constexpr (!STREAM || N < 2) {
+    __builtin_memcpy(w, src, sizeof(w));
+  } else if constexpr (N == 2) {
+    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_any*>(src));
+    __builtin_memcpy(w, &v, 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(src + 4 * i));
+      __builtin_memcpy(w + i, &v, 16);
+    }
+  }
+}
+template <bool STREAM, int N>
+__device__ __forceinline__ void store_words(uint8_t* dst, const uint32_t (&w)[N]) {
+  if constexpr (!STREAM || N < 2) {
+    __builtin_memcpy(dst, w, sizeof(w));
+  } else if constexpr (N == 2) {
+    __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2_any*>(dst));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      __builtin_nontemporal_store(u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]}, reinterpret_cast<u32x4_any*>(dst + 4 * i));
+  }
+}
+
+// Elements [0, count) of the VEC at element `at`, the others zero.
+template <int DT, int VEC, bool STREAM = false>
 __device__ __forceinline__ RawVec<DT, VEC> load_vec(const void* base, int64_t at, int64_t count) {
   RawVec<DT, VEC> r;
 #pragma unroll
@@ -30,7 +60,7 @@ __device__ __forceinline__ RawVec<DT, VEC> load_vec(const void* base, int64_t at
   if constexpr (DT != kNoType) {
     const uint8_t* src = static_cast<const uint8_t*>(base) + at * bytes_of(DT);
     if (count >= VEC) {
-      __builtin_memcpy(&r, src, sizeof(r));
+      load_words<STREAM>(src, r.w);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -88,11 +118,11 @@ __device__ __forceinline__ RawVec<DT, VEC> to_vec(const float (&f)[VEC]) {
   return r;
 }
 
-template <int DT, int VEC>
+template <int DT, int VEC, bool STREAM = false>
 __device__ __forceinline__ void store_vec(void* base, int64_t at, int64_t count, const RawVec<DT, VEC>& r) {
   uint8_t* dst = static_cast<uint8_t*>(base) + at * bytes_of(DT);
   if (count >= VEC) {
-    __builtin_memcpy(dst, &r, sizeof(r));
+    store_words<STREAM>(dst, r.w);
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
