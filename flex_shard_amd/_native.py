@@ -321,9 +321,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int32, c_void_p,
          c_void_p, c_void_p],
     ),
-    "fsh_rms_norm": (c_int, [POINTER(Norm), c_void_p]),
+    "fsh_rms_norm": (c_int, [c_void_p, c_void_p]),  # (a Norm by reference, or its bytes)
     "fsh_rms_norm_backward_workspace_bytes": (c_int64, [c_int64, c_int64]),
-    "fsh_rms_norm_backward": (c_int, [POINTER(NormGradient), c_void_p]),
+    "fsh_rms_norm_backward": (c_int, [c_void_p, c_void_p]),
     "fsh_rms_norm_token_runs": (
         c_int,
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p],

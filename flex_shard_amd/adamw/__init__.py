@@ -10,7 +10,7 @@ gradients' norm is part of the step's one pass over them:
 
 from __future__ import annotations
 
-from typing import Any, Iterable, Sequence
+from typing import Any, Iterable
 
 import torch
 
@@ -25,7 +25,7 @@ def grad_square_sum(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     one GPU; None is left out), a float64 scalar there: the square of their
     common norm.  Products and sums in 64 bits, in an order that the sizes alone decide.  Of
     sharded gradients it is this rank's part: add the ranks' up before it is used."""
-    present = [g.detach() if g.is_contiguous() else g.detach().contiguous() for g in grads if g is not None]
+    present = [g if g.is_contiguous() else g.detach().contiguous() for g in grads if g is not None]
     if not present:
         raise ValueError("at least one gradient")
     return hip_ops.grad_square_sum(present)
@@ -133,67 +133,74 @@ class FlexShardAdamW(torch.optim.Optimizer):
                 loss = closure()
         if max_norm is not None and (square_sum is None or not max_norm > 0):
             raise ValueError(f"clipping needs the gradients' square_sum and a positive max_norm, got {max_norm}")
-        device = None
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is not None:
-                    device = p.device if device is None else device
-                    _check_pair(p, p.grad, device)
-        if device is None:
-            return loss
-        if square_sum is not None and (square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device):
-            raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
+        device, index = None, -1
         groups: list[tuple] = []
         table: list[int] = []
         calls = [(table, groups)]
         stepped, copies = [], []  # (the queued kernels read the copies)
+        states = self.state
         for group in self.param_groups:
-            lr, address = group["lr"], None
-            if isinstance(lr, torch.Tensor):
+            lr, bits, number = group["lr"], group["state_bits"], len(groups)
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if device is None:
+                    device, index = p.device, p.get_device()
+                    _check_sum(square_sum, device)
+                param_dt, grad_dt = _DT.get(p.dtype), _DT.get(g.dtype)
+                if (
+                    param_dt is None or grad_dt is None or p.get_device() != index or g.get_device() != index or index < 0
+                    or g.layout is not torch.strided or g.shape != p.shape or not p.is_contiguous()
+                ):
+                    _refuse_pair(p, g, device)
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    copies.append(g)
+                state = states[p]
+                if not state:
+                    state.update(self._new_state(p, bits))
+                m, v = state["exp_avg"], state["exp_avg_sq"]
+                if (m.dtype is torch.uint8) is not (bits == 8):
+                    raise ValueError(f"states of {m.dtype} do not go with state_bits={bits}")
+                m_scale = v_scale = 0
+                if bits == 8:
+                    m_scale, v_scale = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
+                # (an fsh_adamw_tensor)
+                table += (
+                    p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale, v_scale, state["step"].data_ptr(), p.numel(),
+                    param_dt, grad_dt, bits, number,
+                )
+                stepped.append(p)
+            address = None
+            if isinstance(lr, torch.Tensor) and device is not None:
                 lr, address = _learning_rate(lr, device)
+            groups.append((lr, address, *group["betas"], group["eps"], group["weight_decay"]))
             if len(groups) == ADAMW_GROUPS:
                 table, groups = [], []
                 calls.append((table, groups))
-            bits, index = group["state_bits"], len(groups)
-            for p in group["params"]:
-                if p.grad is not None:
-                    stepped.append(p)
-                    table += self._row(p, bits, index, copies)
-            groups.append((lr, address, *group["betas"], group["eps"], group["weight_decay"]))
         for table, groups in calls:  # (nothing is queued before all of it has been checked)
-            hip_ops.adamw_step(table, groups, device, square_sum, max_norm or 0.0)
-        torch.autograd.graph.increment_version(stepped)
+            if table:
+                hip_ops.adamw_step(table, groups, device, square_sum, max_norm or 0.0)
+        if stepped:
+            torch.autograd.graph.increment_version(stepped)
         return loss
 
-    def _row(self, p: torch.Tensor, bits: int, group: int, copies: list) -> Sequence[int]:
-        """The twelve numbers of an ``fsh_adamw_tensor``."""
-        g = p.grad
-        if not g.is_contiguous():
-            g = g.contiguous()
-            copies.append(g)
-        state = self.state[p]
-        if not state:
-            state.update(self._new_state(p, bits))
-        m, v = state["exp_avg"], state["exp_avg_sq"]
-        if (m.dtype == torch.uint8) != (bits == 8):
-            raise ValueError(f"states of {m.dtype} do not go with state_bits={bits}")
-        scales = (state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()) if bits == 8 else (0, 0)
-        return (
-            p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), *scales, state["step"].data_ptr(), p.numel(),
-            _DT[p.dtype], _DT[g.dtype], bits, group,
-        )
+
+def _check_sum(square_sum: torch.Tensor | None, device: torch.device) -> None:
+    if square_sum is not None and (square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device):
+        raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
 
 
-def _check_pair(p: torch.Tensor, g: torch.Tensor, device: torch.device) -> None:
-    """That the kernels can take a parameter and its gradient."""
+def _refuse_pair(p: torch.Tensor, g: torch.Tensor, device: torch.device) -> None:
+    """Why the kernels cannot take a parameter and its gradient."""
     if p.device.type != "cuda":
         raise RuntimeError("flex_shard_amd kernels run on the GPU only; there is no CPU path.")
     if p.dtype not in _DT or g.dtype not in _DT or g.layout != torch.strided:
         raise NotImplementedError(f"the AdamW kernels take dense bf16 or fp32 parameters and gradients, got {p.dtype} and {g.dtype} ({g.layout})")
     if p.device != device or g.device != device:
         raise ValueError(f"all parameters and gradients of a step must live on {device}, got {p.device} and {g.device}")
-    if not p.is_contiguous() or g.shape != p.shape:
-        raise ValueError(f"contiguous parameters with gradients of their shape, got {tuple(p.shape)} / {p.stride()} and {tuple(g.shape)}")
+    raise ValueError(f"contiguous parameters with gradients of their shape, got {tuple(p.shape)} / {p.stride()} and {tuple(g.shape)}")
 
 
 def _learning_rate(lr: torch.Tensor, device: torch.device) -> tuple[float, int | None]:

@@ -57,7 +57,7 @@ class Fp8Activation:
         return self._values(dtype)
 
     def _values(self, dtype: torch.dtype) -> torch.Tensor:
-        return hip_ops.act_dequant_1x128(self.q, self.scales, self.shape[-1], dtype).view(self.shape)
+        return hip_ops.act_dequant_1x128(self.q, self.scales, self.shape[-1], dtype, self.shape)
 
     def __repr__(self) -> str:
         return f"Fp8Activation(shape={tuple(self.shape)})"

@@ -9,6 +9,7 @@ only.  Nothing here synchronizes the host.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Sequence
 
 import torch
@@ -1489,75 +1490,95 @@ def expert_combine_backward_at(
     return grad_rows, grad_weights
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _queue(entry: str, device: torch.device, *args) -> None:
     """Call a C entry with the current stream of ``device`` behind its arguments,
     ``device`` being the current one meanwhile."""
     fn = getattr(_native.lib(), entry)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, stream_ptr(device))
+    index = device.index
+    if _current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, stream_ptr(device))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _native.check(status, entry)
 
 
-def _norm_stride(name: str, t: torch.Tensor, shape: tuple[int, int]) -> int:
-    rows, cols = shape
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {t.stride()}")
-    return t.stride(0) if rows > 1 else cols
+def _norm_stride(name: str, t: torch.Tensor, shape: torch.Size) -> int:
+    """The row stride of rows [..., cols]: contiguous ones, or a matrix whose rows
+    are contiguous and do not overlap."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    cols = shape[-1]
+    if t.is_contiguous():
+        return cols
+    along = t.stride(0)
+    if t.ndim != 2 or (cols > 1 and t.stride(1) != 1) or (shape[0] > 1 and along < cols):
+        raise ValueError(f"{name} must be contiguous, or a matrix of contiguous rows that do not overlap, got strides {t.stride()}")
+    return along if shape[0] > 1 else cols
 
 
-def _check_norm_weight(weight: torch.Tensor | None, cols: int) -> int:
+def _norm_weight(weight: torch.Tensor | None, cols: int) -> tuple[int, int]:
+    """Address and dtype code."""
     if weight is None:
-        return DT_F32
-    if tuple(weight.shape) != (cols,) or (cols > 1 and weight.stride(0) != 1):
+        return 0, DT_F32
+    if weight.shape != (cols,) or not weight.is_contiguous():
         raise ValueError(f"weight must be {[cols]}, contiguous, got {tuple(weight.shape)} / {weight.stride()}")
-    return _float_dt(weight.dtype)
+    return weight.data_ptr(), _float_dt(weight.dtype)
+
+
+# (packed by hand: a ctypes structure takes 4 us to fill)
+_PACK_NORM = struct.Struct("@7P4q4ifi").pack
+_PACK_NORM_GRADIENT = struct.Struct("@9P6q4i").pack
+assert struct.calcsize("@7P4q4ifi") == ctypes.sizeof(_native.Norm) and struct.calcsize("@9P6q4i") == ctypes.sizeof(_native.NormGradient)
 
 
 def rms_norm(
     x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None = None, *, fp8: bool = False,
     keep_rstd: bool = False,
 ) -> tuple[torch.Tensor | tuple[torch.Tensor, torch.Tensor], torch.Tensor | None, torch.Tensor | None]:
-    """``(out, total, rstd)`` of the rows of ``x`` [rows, cols]: ``total`` = x +
+    """``(out, total, rstd)`` of the rows of ``x`` [..., cols]: ``total`` = x +
     residual (None without one), ``out`` its norm in the type of ``x``, or with ``fp8``
     what :func:`act_quant_1x128` makes of it in bf16; ``rstd`` [rows] if kept."""
     _require_gpu(x, *(t for t in (weight, residual) if t is not None))
-    if x.ndim != 2:
-        raise ValueError(f"expected rows [rows, cols], got {tuple(x.shape)}")
-    rows, cols = shape = tuple(x.shape)
-    q = _native.Norm()
-    q.x_dtype, q.weight_dtype = _float_dt(x.dtype), _check_norm_weight(weight, cols)
-    q.rows, q.cols, q.eps = rows, cols, eps
-    q.ldx = _norm_stride("x", x, shape)
-    q.x_dev = x.data_ptr()
+    shape, device, dtype = x.shape, x.device, x.dtype
+    if x.ndim < 1 or shape[-1] == 0:
+        raise ValueError(f"expected rows [..., cols], got {tuple(shape)}")
+    cols = shape[-1]
+    rows = x.numel() // cols
+    ldx, code = _norm_stride("x", x, shape), _float_dt(dtype)
+    weight_ptr, weight_code = _norm_weight(weight, cols)
     total = rstd = scales = None
-    if weight is not None:
-        q.weight_dev = weight.data_ptr()
+    residual_ptr = total_ptr = ldr = residual_code = 0
     if residual is not None:
-        if residual.dtype not in (x.dtype, torch.float32):
-            raise NotImplementedError(f"a residual is of the type of x ({x.dtype}) or fp32, got {residual.dtype}")
-        q.residual_dtype, q.ldr = _float_dt(residual.dtype), _norm_stride("residual", residual, shape)
-        total = torch.empty(shape, dtype=residual.dtype, device=x.device)
-        q.residual_dev, q.total_dev = residual.data_ptr(), total.data_ptr()
+        if residual.dtype not in (dtype, torch.float32):
+            raise NotImplementedError(f"a residual is of the type of x ({dtype}) or fp32, got {residual.dtype}")
+        residual_code, ldr = _float_dt(residual.dtype), _norm_stride("residual", residual, shape)
+        total = torch.empty(shape, dtype=residual.dtype, device=device)
+        residual_ptr, total_ptr = residual.data_ptr(), total.data_ptr()
     if fp8:
         padded = -(-cols // 128) * 128
-        out = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=x.device)
-        scales = torch.empty((padded // 128, rows), dtype=torch.float32, device=x.device)
-        q.form, q.scales_dev = _native.NORM_FP8, scales.data_ptr()
+        out = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty((padded // 128, rows), dtype=torch.float32, device=device)
     else:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    q.out_dev = out.data_ptr()
+        out = torch.empty(shape, dtype=dtype, device=device)
     if keep_rstd:
-        rstd = torch.empty((rows,), dtype=torch.float32, device=x.device)
-        q.rstd_dev = rstd.data_ptr()
-    if rows and cols:
-        _queue("fsh_rms_norm", x.device, ctypes.byref(q))
+        rstd = torch.empty((rows,), dtype=torch.float32, device=device)
+    if rows:
+        _queue("fsh_rms_norm", device, _PACK_NORM(
+            x.data_ptr(), residual_ptr, weight_ptr, total_ptr, out.data_ptr(), scales.data_ptr() if fp8 else 0,
+            rstd.data_ptr() if keep_rstd else 0, rows, cols, ldx, ldr, code, residual_code, weight_code,
+            _native.NORM_FP8 if fp8 else _native.NORM_VALUES, eps, 0,
+        ))
     return (out, scales) if fp8 else out, total, rstd
+
+
+def _check_rstd(rstd: torch.Tensor, rows: int) -> None:
+    if rstd.shape != (rows,) or rstd.dtype != torch.float32 or not rstd.is_contiguous():
+        raise ValueError(f"rstd must be contiguous fp32 [{rows}], got {rstd.dtype} {tuple(rstd.shape)}")
 
 
 def rms_norm_backward(
@@ -1568,36 +1589,37 @@ def rms_norm_backward(
     what it normed (``x`` without a residual).  The first two are one tensor where
     ``total`` is of ``x_dtype``."""
     _require_gpu(grad, total, rstd, *(t for t in (weight, grad_total) if t is not None))
-    rows, cols = shape = tuple(total.shape)
+    shape, device = total.shape, total.device
+    cols = shape[-1]
+    rows = total.numel() // cols
     same = total.dtype == x_dtype
-    q = _native.NormGradient()
-    q.grad_dtype, q.total_dtype, q.x_dtype = _float_dt(grad.dtype), _float_dt(total.dtype), _float_dt(x_dtype)
-    q.weight_dtype = _check_norm_weight(weight, cols)
-    q.rows, q.cols = shape
-    q.ldg, q.ldh = _norm_stride("grad", grad, shape), _norm_stride("total", total, shape)
-    if tuple(rstd.shape) != (rows,) or rstd.dtype != torch.float32 or not rstd.is_contiguous():
-        raise ValueError(f"rstd must be contiguous fp32 [{rows}], got {rstd.dtype} {tuple(rstd.shape)}")
-    q.grad_dev, q.total_dev, q.rstd_dev = grad.data_ptr(), total.data_ptr(), rstd.data_ptr()
-    if weight is not None:
-        q.weight_dev = weight.data_ptr()
+    weight_ptr, weight_code = _norm_weight(weight, cols)
+    ldg, ldh = _norm_stride("grad", grad, shape), _norm_stride("total", total, shape)
+    _check_rstd(rstd, rows)
+    ldt = grad_total_ptr = 0
     if grad_total is not None:
         if grad_total.dtype != total.dtype:
             raise ValueError(f"the gradient of a sum of {total.dtype} is of that type, got {grad_total.dtype}")
-        q.ldt, q.grad_total_dev = _norm_stride("grad_total", grad_total, shape), grad_total.data_ptr()
+        ldt, grad_total_ptr = _norm_stride("grad_total", grad_total, shape), grad_total.data_ptr()
     grad_x = grad_residual = grad_weight = None
+    grad_x_ptr = grad_residual_ptr = grad_weight_ptr = workspace_ptr = nbytes = 0
     if needs_x or (same and needs_residual):
-        grad_x = torch.empty(shape, dtype=x_dtype, device=grad.device)
-        q.grad_x_dev = grad_x.data_ptr()
+        grad_x = torch.empty(shape, dtype=x_dtype, device=device)
+        grad_x_ptr = grad_x.data_ptr()
     if needs_residual:
-        grad_residual = grad_x if same else torch.empty(shape, dtype=total.dtype, device=grad.device)
+        grad_residual = grad_x if same else torch.empty(shape, dtype=total.dtype, device=device)
         if not same:
-            q.grad_residual_dev = grad_residual.data_ptr()
+            grad_residual_ptr = grad_residual.data_ptr()
     if needs_weight and weight is not None:
-        grad_weight = torch.empty((cols,), dtype=weight.dtype, device=grad.device)
+        grad_weight = torch.empty((cols,), dtype=weight.dtype, device=device)
         nbytes = _native.lib().fsh_rms_norm_backward_workspace_bytes(rows, cols)
-        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=grad.device)
-        q.grad_weight_dev, q.workspace_dev, q.workspace_nbytes = grad_weight.data_ptr(), workspace.data_ptr(), nbytes
-    _queue("fsh_rms_norm_backward", grad.device, ctypes.byref(q))
+        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+        grad_weight_ptr, workspace_ptr = grad_weight.data_ptr(), workspace.data_ptr()
+    _queue("fsh_rms_norm_backward", device, _PACK_NORM_GRADIENT(
+        grad.data_ptr(), total.data_ptr(), weight_ptr, rstd.data_ptr(), grad_total_ptr, grad_x_ptr, grad_residual_ptr,
+        grad_weight_ptr, workspace_ptr, nbytes, rows, cols, ldg, ldh, ldt, _float_dt(grad.dtype), _float_dt(total.dtype),
+        _float_dt(x_dtype), weight_code,
+    ))
     return grad_x if needs_x else None, grad_residual, grad_weight
 
 
@@ -1605,23 +1627,25 @@ def rms_norm_token_runs(total: torch.Tensor, weight: torch.Tensor | None, rstd: 
     """What :func:`act_quant_128x1_transposed` makes of the norm in bf16 (its columns
     padded with zeros to a multiple of 8), from what was normed and ``rstd``."""
     _require_gpu(total, rstd, *(() if weight is None else (weight,)))
-    rows, cols = shape = tuple(total.shape)
-    if tuple(rstd.shape) != (rows,) or rstd.dtype != torch.float32 or not rstd.is_contiguous():
-        raise ValueError(f"rstd must be contiguous fp32 [{rows}], got {rstd.dtype} {tuple(rstd.shape)}")
+    cols = total.shape[-1]
+    rows = total.numel() // cols
+    _check_rstd(rstd, rows)
     width, padded = -(-cols // 8) * 8, -(-rows // 128) * 128
     q = torch.empty((width, padded), dtype=torch.float8_e4m3fn, device=total.device)
     scales = torch.empty((padded // 128, width), dtype=torch.float32, device=total.device)
-    if rows and cols:
+    if rows:
         _queue(
             "fsh_rms_norm_token_runs", total.device, total.data_ptr(), _float_dt(total.dtype), rows, cols,
-            _norm_stride("total", total, shape), rstd.data_ptr(), None if weight is None else weight.data_ptr(),
-            _check_norm_weight(weight, cols), q.data_ptr(), padded, scales.data_ptr(),
+            _norm_stride("total", total, total.shape), rstd.data_ptr(), *_norm_weight(weight, cols), q.data_ptr(), padded,
+            scales.data_ptr(),
         )
     return q, scales
 
 
-def act_dequant_1x128(q: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values [rows, cols] of what :func:`act_quant_1x128` returned."""
+def act_dequant_1x128(
+    q: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype = torch.bfloat16, shape: Sequence[int] | None = None
+) -> torch.Tensor:
+    """The values [rows, cols], or of ``shape``, of what :func:`act_quant_1x128` returned."""
     _require_gpu(q, scales)
     _fp8_matrix("q", q)
     rows, padded = q.shape
@@ -1629,7 +1653,9 @@ def act_dequant_1x128(q: torch.Tensor, scales: torch.Tensor, cols: int, dtype: t
         raise ValueError(f"q must be [rows, {cols} rounded up to 128], rows 8-byte aligned, got {tuple(q.shape)} / {q.stride()}")
     if scales.dtype != torch.float32 or not scales.is_contiguous() or tuple(scales.shape) != (padded // 128, rows):
         raise ValueError(f"scales must be contiguous fp32 of shape {(padded // 128, rows)}, got {tuple(scales.shape)}")
-    out = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    out = torch.empty((rows, cols) if shape is None else shape, dtype=dtype, device=q.device)
+    if out.numel() != rows * cols:
+        raise ValueError(f"{rows} rows of {cols} do not fill {tuple(shape)}")
     if rows and cols:
         _queue(
             "fsh_act_dequant_1x128", q.device, q.data_ptr(), scales.data_ptr(), rows, cols, q.stride(0) if rows > 1 else padded,
@@ -1644,16 +1670,16 @@ def grad_square_sum(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     device = _require_gpu(*tensors)
     table = []
     for t in tensors:
-        if not t.is_contiguous():
-            raise ValueError(f"contiguous tensors, got strides {t.stride()} of {tuple(t.shape)}")
-        table += (t.data_ptr(), t.numel(), _float_dt(t.dtype))
+        code = _FLOAT_DT.get(t.dtype)
+        if code is None or not t.is_contiguous():
+            raise NotImplementedError(f"contiguous bf16, fp16 or fp32 tensors, got {t.dtype} {tuple(t.shape)} / {t.stride()}")
+        table += (t.data_ptr(), t.numel(), code)
     table = (ctypes.c_int64 * len(table))(*table)
     nbytes = _native.lib().fsh_grad_square_sum_workspace_bytes(table, len(tensors))
-    # the sum, and behind it the workgroups' parts
-    buffer = torch.empty((1 + nbytes // 8,), dtype=torch.float64, device=device)
-    out = buffer.data_ptr()
-    _queue("fsh_grad_square_sum", device, table, len(tensors), out, out + 8, nbytes)
-    return buffer[0]
+    out = torch.empty((), dtype=torch.float64, device=device)
+    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    _queue("fsh_grad_square_sum", device, table, len(tensors), out.data_ptr(), workspace.data_ptr(), nbytes)
+    return out
 
 
 def adamw_step(
@@ -1667,7 +1693,6 @@ def adamw_step(
     if rest:
         raise ValueError(f"{_native.ADAMW_TENSOR_INT64S} numbers a tensor, got {len(table)}")
     if square_sum is not None:
-        _require_gpu(square_sum)
         if square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device:
             raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
     if not count:

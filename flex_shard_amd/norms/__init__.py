@@ -25,13 +25,13 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
-    """[rows, cols] with contiguous rows that do not overlap; a copy if need be."""
-    if t.ndim != 2:
-        t = t.reshape(-1, t.shape[-1])
-    rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t
+    """Contiguous rows [..., cols], or a matrix of contiguous rows that do not
+    overlap; a copy if need be."""
+    if t.is_contiguous() or (
+        t.ndim == 2 and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+    ):
+        return t
+    return t.contiguous()
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None) -> None:
@@ -51,7 +51,8 @@ def _check(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: t
 
 
 def _carrier(shape, device: torch.device) -> torch.Tensor:
-    return torch.empty((), dtype=torch.bfloat16, device=device).expand(shape)
+    # (of one element, and not an expanded view of it: autograd would go back through its strides)
+    return torch.empty_strided(shape, (0,) * len(shape), dtype=torch.bfloat16, device=device)
 
 
 class _Norm(torch.autograd.Function):
@@ -98,25 +99,24 @@ def rms_norm(
         total = x if residual is None else x.to(residual.dtype) + residual
         y = (total if weight is None else total * weight).to(x.dtype)
         return y if residual is None else (y, total)
-    rows = _as_rows(x)
+    x = _as_rows(x)
     stream = None if residual is None else _as_rows(residual)
-    weight = weight if weight is None else weight.contiguous()
-    if differentiates(rows, stream, weight):
-        y, total = _Norm.apply(rows, stream, weight, eps, None)
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    if differentiates(x, stream, weight):
+        y, total = _Norm.apply(x, stream, weight, eps, None)
     else:
-        y, total, _ = hip_ops.rms_norm(rows, weight, eps, stream)
-    y = y.view(x.shape)
-    return y if residual is None else (y, total.view(x.shape))
+        y, total, _ = hip_ops.rms_norm(x, weight, eps, stream)
+    return y if residual is None else (y, total)
 
 
 def _version(t: torch.Tensor | None) -> int:
     return 0 if t is None or t.is_inference() else t._version
 
 
-def _token_runs(of: tuple, versions: list[int]) -> tuple[torch.Tensor, torch.Tensor]:
-    if [_version(t) for t in of] != versions:
+def _token_runs(normed, normed_version: int, weight, weight_version: int, rstd) -> tuple[torch.Tensor, torch.Tensor]:
+    if _version(normed) != normed_version or _version(weight) != weight_version:
         raise RuntimeError("what an 8-bit norm was made of was changed in place before a weight gradient's form of it was made")
-    return hip_ops.rms_norm_token_runs(*of)
+    return hip_ops.rms_norm_token_runs(normed, weight, rstd)
 
 
 def rms_norm_fp8(
@@ -125,25 +125,23 @@ def rms_norm_fp8(
     """:func:`rms_norm`, its output rounded to bf16 and quantized like the
     activations of the blockwise FP8 linears, which take it as it is."""
     _check(x, weight, eps, residual)
-    rows = _as_rows(x)
+    x = _as_rows(x)
     stream = None if residual is None else _as_rows(residual)
-    weight = weight if weight is None else weight.contiguous()
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
     if x.numel() == 0:
         y = rms_norm(x, weight, eps, residual=residual)
-        y, total = (y, None) if residual is None else y
-        (q, scales), _, rstd = hip_ops.rms_norm(rows.detach(), None, eps, fp8=True, keep_rstd=True)
-        normed, carrier = rows.detach(), y.to(torch.bfloat16)
-    elif differentiates(rows, stream, weight):
+        carrier, total = (y, None) if residual is None else y
+        (q, scales), _, rstd = hip_ops.rms_norm(x, None, eps, fp8=True, keep_rstd=True)
+        normed, carrier = x, carrier.to(torch.bfloat16)
+    elif differentiates(x, stream, weight):
         kept: list = []
-        carrier, total = _Norm.apply(rows, stream, weight, eps, kept)
+        carrier, total = _Norm.apply(x, stream, weight, eps, kept)
         q, scales, normed, rstd = kept
-        carrier = carrier.view(x.shape)
     else:
-        (q, scales), total, rstd = hip_ops.rms_norm(rows, weight, eps, stream, fp8=True, keep_rstd=True)
-        normed, carrier = rows if total is None else total, _carrier(x.shape, x.device)
-    of = (normed.detach(), None if weight is None else weight.detach(), rstd)
-    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, of, [_version(t) for t in of]))
-    return activation if residual is None else (activation, total.view(x.shape))
+        (q, scales), total, rstd = hip_ops.rms_norm(x, weight, eps, stream, fp8=True, keep_rstd=True)
+        normed, carrier = x if total is None else total, _carrier(x.shape, x.device)
+    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, _version(normed), weight, _version(weight), rstd))
+    return activation if residual is None else (activation, total)
 
 
 class FlexShardRMSNorm(nn.RMSNorm):
