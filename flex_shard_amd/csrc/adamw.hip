@@ -127,31 +127,36 @@ __device__ __forceinline__ int tensor_of(const uint32_t (&first)[N], uint32_t ch
 }
 
 // ------------------------------------------------------------------ 8-bit codes
-constexpr int kOne = 1016;  // the upper 12 bits of 1.0f
-__device__ __forceinline__ float code_value(uint32_t code, int codes) {
-  return code ? u32_as_f32((code + kOne - codes) << 20) : 0.0f;
-}
+constexpr uint32_t kFirstBase = 1016 - 127, kSecondBase = 1016 - 255;  // 1016: the upper 12 bits of 1.0f
 __device__ __forceinline__ float first_value(uint32_t code) {
-  return u32_as_f32(f32_as_u32(code_value(code & 127u, 127)) | ((code & 128u) << 24));
+  const uint32_t size = code & 127u;
+  return u32_as_f32((size ? (size + kFirstBase) << 20 : 0u) | ((code & 128u) << 24));
 }
-// size in [0, 1]; u: the dither.
-__device__ __forceinline__ uint32_t first_code(float size, uint32_t sign, uint32_t u) {
+__device__ __forceinline__ float second_value(uint32_t code) { return u32_as_f32(code ? (code + kSecondBase) << 20 : 0u); }
+// The codes of a value over its block's scale, of at most 1 and a few units in the last
+// place, which the dither cannot carry further (of a block that is not a number: any bits).
+// half: the dither in units of 2^-16.
+__device__ __forceinline__ uint32_t first_code(float value, uint32_t half) {
   constexpr float kSmallest = 1.25f / 65536.0f;
-  const uint32_t up = ((f32_as_u32(size) + (u >> 12)) >> 20) - (kOne - 127);
-  const uint32_t few = size * (1.0f / kSmallest) > static_cast<float>(u >> 8) * (1.0f / 16777216.0f) ? 1u : 0u;
-  return (size < kSmallest ? few : up) | (sign ? 128u : 0u);
+  const uint32_t bits = f32_as_u32(value) & 0x7FFFFFFFu;
+  const float size = u32_as_f32(bits);
+  const uint32_t up = ((bits + (half << 4)) >> 20) - kFirstBase;
+  // (the product with 1 / kSmallest, rounded as such, against half / 65536)
+  const uint32_t few = size * (1.0f / kSmallest * 65536.0f) > static_cast<float>(half) ? 1u : 0u;
+  return (size < kSmallest ? few : up) | ((f32_as_u32(value) >> 24) & 128u);
 }
-__device__ __forceinline__ uint32_t second_code(float size, uint32_t u) {
-  const int up = static_cast<int>((f32_as_u32(size) + (u >> 12)) >> 20) - (kOne - 255);
-  return size > 0.0f ? static_cast<uint32_t>(up > 1 ? up : 1) : 0u;
+__device__ __forceinline__ uint32_t second_code(float size, uint32_t half) {
+  const int up = static_cast<int>((f32_as_u32(size) + (half << 4)) >> 20) - static_cast<int>(kSecondBase);
+  const int least = static_cast<int>(min(f32_as_u32(size), 1u));  // 1 of what is not zero
+  return static_cast<uint32_t>(max(up, least));
 }
-// The dither of an element in a step, 16 bits for each moment: multiples of the
-// golden ratio and of the square root of 2, modulo 2^32, mixed by one product with the
-// square root of 3 between two shifts, which leaves no correlation beyond chance between
-// neighbours, steps or the halves (2^20 elements).
-__device__ __forceinline__ uint32_t dither(uint32_t index, uint32_t t) {
-  uint32_t z = index * 0x9E3779B9u + t * 0x6A09E667u;
-  z = (z ^ (z >> 16)) * 0xBB67AE85u;
+// The dither of an element in a step, 16 bits for each moment (the first's below):
+// multiples of the golden ratio and of the square root of 2, modulo 2^32, mixed by one
+// product with the square root of 3 between two shifts, which leaves no correlation beyond
+// chance between neighbours, steps or the halves (2^20 elements).
+constexpr uint32_t kOverElements = 0x9E3779B9u, kOverSteps = 0x6A09E667u;
+__device__ __forceinline__ uint32_t dither(uint32_t multiple) {
+  const uint32_t z = (multiple ^ (multiple >> 16)) * 0xBB67AE85u;
   return z ^ (z >> 15);
 }
 
@@ -165,98 +170,149 @@ __device__ __forceinline__ float block_scale(uint32_t largest, float& inverse) {
 }
 
 // --------------------------------------------------------------------- the step
-constexpr int kChunk = 4 * kThreads;  // elements: four neighbours a thread
+// A workgroup takes a chunk: vectors of four neighbours a thread, the loads of all
+// of them requested first.  With 32-bit states one vector, with 8-bit ones, where instructions
+// count and what is done once per chunk is spread, four (218 M parameters, us with one, two
+// and four: bf16 and 32 bits 768, 855, 820; bf16 and 8 bits 535, 490, 470; fp32 and 8 bits 600 each).
+// Everything streams: through the caches the 32-bit step takes 919 us, and workgroups that stay for more chunks than
+// one are slower still (2048 of them: 1049).
+constexpr int chunk_of(bool eight) { return (eight ? 4 : 1) * 4 * kThreads; }
 
+// What a vector's step reads.
 template <int PT, int GT, bool kEight>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamTable a) {
-  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-    const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
-    const StepFactors f = a.all_factors[a.factors[k]];
-    if (f.skip) continue;
-    const int64_t numel = a.numel[k];
-    const int64_t at = (chunk - a.first_chunk[k]) * kChunk + 4 * static_cast<int64_t>(threadIdx.x);
-    const int64_t count = numel - at;
-    const auto pr = load_vec<PT, 4>(a.param[k], at, count);
-    const auto gr = load_vec<GT, 4>(a.grad[k], at, count);
-    float m[4], v[4], p[4];
-    const int64_t block = at / kStateBlock;
+struct StepInput {
+  RawVec<PT, 4> p;
+  RawVec<GT, 4> g;
+  RawVec<FSH_DT_F32, 4> m, v;
+  uint32_t mc, vc;
+  float ms, vs;
+};
+
+// Where a chunk's part of a tensor lies.
+struct ChunkOf {
+  uint8_t* param;
+  const uint8_t* grad;
+  uint8_t* m;
+  uint8_t* v;
+  float* m_scale;
+  float* v_scale;
+};
+
+// Up to four codes, the others zero.
+template <bool kFull>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int count) {
+  uint32_t c = 0;
+  if (kFull || count >= 4) {
+    __builtin_memcpy(&c, src, 4);
+  } else {
+    for (int j = 0; j < count; ++j) c |= static_cast<uint32_t>(src[j]) << (8 * j);
+  }
+  return c;
+}
+template <bool kFull>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int count, uint32_t c) {
+  if (kFull || count >= 4) {
+    __builtin_memcpy(dst, &c, 4);
+  } else {
+    for (int j = 0; j < count; ++j) dst[j] = static_cast<uint8_t>(c >> (8 * j));
+  }
+}
+
+// kFull: the chunk ends inside the tensor; `left`: elements from the chunk's first on.
+template <int PT, int GT, bool kEight, bool kFull>
+__device__ __forceinline__ void step_chunk(const ChunkOf& c, const StepFactors& f, uint32_t first_index, int left) {
+  constexpr int kVectors = chunk_of(kEight) / (4 * kThreads);
+  StepInput<PT, GT, kEight> in[kVectors];
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * 4;
+    const int count = kFull ? 4 : left - at;
+    in[i].p = load_vec<PT, 4, true>(c.param, at, count);
+    in[i].g = load_vec<GT, 4, true>(c.grad, at, count);
     if constexpr (kEight) {
-      // (codes lie in fours at 4-byte addresses; a tensor's last four may be fewer)
-      uint32_t mc = 0, vc = 0;
-      float ms = 0.0f, vs = 0.0f;
-      if (count > 0) {
-        ms = a.m_scale[k][block];
-        vs = a.v_scale[k][block];
-      }
-      if (count >= 4) {
-        __builtin_memcpy(&mc, static_cast<const uint8_t*>(a.m[k]) + at, 4);
-        __builtin_memcpy(&vc, static_cast<const uint8_t*>(a.v[k]) + at, 4);
-      } else {
-        for (int j = 0; j < count; ++j) {
-          mc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.m[k])[at + j]) << (8 * j);
-          vc |= static_cast<uint32_t>(static_cast<const uint8_t*>(a.v[k])[at + j]) << (8 * j);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = first_value((mc >> (8 * j)) & 255u) * ms;
-        v[j] = code_value((vc >> (8 * j)) & 255u, 255) * vs;
-      }
+      in[i].mc = load_codes<kFull>(c.m + at, count);
+      in[i].vc = load_codes<kFull>(c.v + at, count);
+      in[i].ms = count > 0 ? c.m_scale[at / kStateBlock] : 0.0f;
+      in[i].vs = count > 0 ? c.v_scale[at / kStateBlock] : 0.0f;
     } else {
-      const auto mr = load_vec<FSH_DT_F32, 4>(a.m[k], at, count);
-      const auto vr = load_vec<FSH_DT_F32, 4>(a.v[k], at, count);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = element<FSH_DT_F32, 4>(mr, j);
-        v[j] = element<FSH_DT_F32, 4>(vr, j);
-      }
+      in[i].m = load_vec<FSH_DT_F32, 4, true>(c.m, at, count);
+      in[i].v = load_vec<FSH_DT_F32, 4, true>(c.v, at, count);
     }
+  }
+#pragma unroll
+  for (int i = 0; i < kVectors; ++i) {
+    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * 4;
+    const int count = kFull ? 4 : left - at;
+    float m[4], v[4], p[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float g = element<GT, 4>(gr, j) * f.clip;
+      if constexpr (kEight) {
+        m[j] = first_value((in[i].mc >> (8 * j)) & 255u) * in[i].ms;
+        v[j] = second_value((in[i].vc >> (8 * j)) & 255u) * in[i].vs;
+      } else {
+        m[j] = element<FSH_DT_F32, 4>(in[i].m, j);
+        v[j] = element<FSH_DT_F32, 4>(in[i].v, j);
+      }
+      const float g = element<GT, 4>(in[i].g, j) * f.clip;
       m[j] = m[j] * f.b1 + g * f.one_b1;
       v[j] = v[j] * f.b2 + (g * g) * f.one_b2;
-      const float root = sqrtf(v[j]) * f.root_factor + f.eps;
-      p[j] = element<PT, 4>(pr, j) * f.decay - f.step_size * (m[j] / root);
+      float update;
+      if constexpr (kEight) {
+        // (root and quotient to one unit in the last place: this form is bound by instructions
+        // otherwise.  A v below 2^-126 may count as zero.)
+        update = m[j] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[j]) * f.root_factor + f.eps);
+      } else {
+        update = m[j] / (sqrtf(v[j]) * f.root_factor + f.eps);
+      }
+      p[j] = element<PT, 4>(in[i].p, j) * f.decay - f.step_size * update;
     }
-    if (count > 0) store_vec<PT, 4>(a.param[k], at, count, to_vec<PT, 4>(p));
+    if (kFull || count > 0) store_vec<PT, 4, true>(c.param, at, count, to_vec<PT, 4>(p));
     if constexpr (kEight) {
       // Half a wave has a block; elements behind the tensor's last are zero.
       uint32_t m_max = 0, v_max = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (j >= count) m[j] = v[j] = 0.0f;
+        if (!kFull && j >= count) m[j] = v[j] = 0.0f;
         m_max = max(m_max, f32_as_u32(m[j]) & 0x7FFFFFFFu);
         v_max = max(v_max, f32_as_u32(v[j]) & 0x7FFFFFFFu);
       }
       float m_inverse, v_inverse;
       const float ms = block_scale(max32_u32(m_max), m_inverse), vs = block_scale(max32_u32(v_max), v_inverse);
+      const uint32_t multiple = (first_index + static_cast<uint32_t>(at)) * kOverElements + f.t * kOverSteps;
       uint32_t mc = 0, vc = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t u = dither(static_cast<uint32_t>(at) + j, f.t);
-        const float m_size = fminf(u32_as_f32(f32_as_u32(m[j]) & 0x7FFFFFFFu) * m_inverse, 1.0f);
-        const float v_size = fminf(v[j] * v_inverse, 1.0f);
-        mc |= (first_code(m_size, m[j] < 0.0f, u << 16) & 255u) << (8 * j);
-        vc |= (second_code(v_size, u & 0xFFFF0000u) & 255u) << (8 * j);
+        const uint32_t u = dither(multiple + static_cast<uint32_t>(j) * kOverElements);
+        mc |= first_code(m[j] * m_inverse, u & 0xFFFFu) << (8 * j);
+        vc |= second_code(v[j] * v_inverse, u >> 16) << (8 * j);
       }
-      if (count >= 4) {
-        __builtin_memcpy(static_cast<uint8_t*>(a.m[k]) + at, &mc, 4);
-        __builtin_memcpy(static_cast<uint8_t*>(a.v[k]) + at, &vc, 4);
-      } else {
-        for (int j = 0; j < count; ++j) {
-          static_cast<uint8_t*>(a.m[k])[at + j] = static_cast<uint8_t>(mc >> (8 * j));
-          static_cast<uint8_t*>(a.v[k])[at + j] = static_cast<uint8_t>(vc >> (8 * j));
-        }
+      store_codes<kFull>(c.m + at, count, mc);
+      store_codes<kFull>(c.v + at, count, vc);
+      if ((kFull || count > 0) && at % kStateBlock == 0) {
+        c.m_scale[at / kStateBlock] = ms;
+        c.v_scale[at / kStateBlock] = vs;
       }
-      if (count > 0 && at % kStateBlock == 0) {
-        a.m_scale[k][block] = ms;
-        a.v_scale[k][block] = vs;
-      }
-    } else if (count > 0) {
-      store_vec<FSH_DT_F32, 4>(a.m[k], at, count, to_vec<FSH_DT_F32, 4>(m));
-      store_vec<FSH_DT_F32, 4>(a.v[k], at, count, to_vec<FSH_DT_F32, 4>(v));
+    } else if (kFull || count > 0) {
+      store_vec<FSH_DT_F32, 4, true>(c.m, at, count, to_vec<FSH_DT_F32, 4>(m));
+      store_vec<FSH_DT_F32, 4, true>(c.v, at, count, to_vec<FSH_DT_F32, 4>(v));
     }
+  }
+}
+
+template <int PT, int GT, bool kEight>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const AdamTable a) {
+  constexpr int kChunk = chunk_of(kEight);
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
+    const StepFactors f = a.all_factors[a.factors[k]];
+    if (f.skip) continue;
+    const int64_t at = (chunk - a.first_chunk[k]) * kChunk, left = a.numel[k] - at;
+    constexpr int kStateBytes = kEight ? 1 : 4;
+    const ChunkOf c = {static_cast<uint8_t*>(a.param[k]) + at * bytes_of(PT), static_cast<const uint8_t*>(a.grad[k]) + at * bytes_of(GT),
+                       static_cast<uint8_t*>(a.m[k]) + at * kStateBytes, static_cast<uint8_t*>(a.v[k]) + at * kStateBytes,
+                       a.m_scale[k] + at / kStateBlock, a.v_scale[k] + at / kStateBlock};
+    if (left >= kChunk) step_chunk<PT, GT, kEight, true>(c, f, static_cast<uint32_t>(at), kChunk);
+    else step_chunk<PT, GT, kEight, false>(c, f, static_cast<uint32_t>(at), static_cast<int>(left));
   }
 }
 
@@ -280,7 +336,7 @@ __global__ __launch_bounds__(kThreads) void adamw_values_kernel(const uint8_t* m
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       mf[j] = first_value(mc[j]) * ms;
-      vf[j] = code_value(vc[j], 255) * vs;
+      vf[j] = second_value(vc[j]) * vs;
     }
     store_vec<DT, 8>(m_out, at, count, to_vec<DT, 8>(mf));
     store_vec<DT, 8>(v_out, at, count, to_vec<DT, 8>(vf));
@@ -290,10 +346,14 @@ __global__ __launch_bounds__(kThreads) void adamw_values_kernel(const uint8_t* m
 // --------------------------------------------------------------- sum of squares
 // In 64 bits, where the squares of bf16, fp16 and fp32 values are exact or nearly: a
 // workgroup adds up its chunks, its threads' sums are joined in a fixed order, and
-// one workgroup joins the workgroups'.
+// one workgroup joins the workgroups'.  Bound by memory.  Gradients that the last-level cache
+// cannot hold for the step behind (256 MB) are read past the caches: 218 M, us without and with, bf16 77 and
+// 70, fp32 152 and 130; of 55 M the step then takes 10 more.  Fewer workgroups leave the memory idle
+// between their chunks (2048: 83 and 178).
 constexpr int kSquareTensors = 160;
 constexpr int kSquareChunk = 8 * kThreads * 4;  // elements: four vectors of eight a thread
-constexpr int kSquareGroups = 2048;
+constexpr int kSquareGroups = 4096;
+constexpr int64_t kSquareStream = 256LL << 20;  // bytes
 struct SquareTable {
   const void* grad[kSquareTensors];
   int64_t numel[kSquareTensors];
@@ -304,14 +364,15 @@ struct SquareTable {
 };
 static_assert(sizeof(SquareTable) <= 4096, "kernel arguments");
 
-template <int DT>
-__device__ __forceinline__ double squares_of(const void* g, int64_t at, int64_t numel) {
+// The sum of a thread's squares of elements [at, at + kSquareChunk); `thread` of kThreads.
+template <int DT, bool kStream>
+__device__ __forceinline__ double squares_of(const void* g, int64_t at, int64_t numel, int thread) {
   constexpr int VEC = DT == FSH_DT_F32 ? 4 : 8, kVectors = kSquareChunk / kThreads / VEC;
   RawVec<DT, VEC> r[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int64_t here = at + (static_cast<int64_t>(i) * kThreads + threadIdx.x) * VEC;
-    r[i] = load_vec<DT, VEC>(g, here, numel - here);
+    const int64_t here = at + (static_cast<int64_t>(i) * kThreads + thread) * VEC;
+    r[i] = load_vec<DT, VEC, kStream>(g, here, numel - here);
   }
   double sum = 0.0;
 #pragma unroll
@@ -323,30 +384,34 @@ __device__ __forceinline__ double squares_of(const void* g, int64_t at, int64_t 
     }
   return sum;
 }
+template <bool kStream>
+__device__ __forceinline__ double squares_of_chunk(const SquareTable& a, int64_t chunk, int thread) {
+  const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
+  const int64_t at = (chunk - a.first_chunk[k]) * kSquareChunk;
+  const int dtype = a.dtype[k];
+  if (dtype == FSH_DT_F32) return squares_of<FSH_DT_F32, kStream>(a.grad[k], at, a.numel[k], thread);
+  if (dtype == FSH_DT_BF16) return squares_of<FSH_DT_BF16, kStream>(a.grad[k], at, a.numel[k], thread);
+  return squares_of<FSH_DT_F16, kStream>(a.grad[k], at, a.numel[k], thread);
+}
 
-__device__ double workgroup_sum(double v, double* lds) {
+template <int THREADS>
+__device__ __forceinline__ double workgroup_sum(double v, double* lds) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   double sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) sum += lds[w];
+  for (int w = 0; w < THREADS / 64; ++w) sum += lds[w];
   return sum;
 }
 
+template <bool kStream>
 __global__ __launch_bounds__(kThreads) void square_sum_kernel(const SquareTable a) {
   __shared__ double lds[kThreads / 64];
   double sum = 0.0;
-  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-    const int k = tensor_of(a.first_chunk, static_cast<uint32_t>(chunk));
-    const int64_t at = (chunk - a.first_chunk[k]) * kSquareChunk;
-    const int dtype = a.dtype[k];
-    if (dtype == FSH_DT_F32) sum += squares_of<FSH_DT_F32>(a.grad[k], at, a.numel[k]);
-    else if (dtype == FSH_DT_BF16) sum += squares_of<FSH_DT_BF16>(a.grad[k], at, a.numel[k]);
-    else sum += squares_of<FSH_DT_F16>(a.grad[k], at, a.numel[k]);
-  }
-  sum = workgroup_sum(sum, lds);
+  for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) sum += squares_of_chunk<kStream>(a, chunk, threadIdx.x);
+  sum = workgroup_sum<kThreads>(sum, lds);
   if (threadIdx.x == 0) a.parts[blockIdx.x] = sum;
 }
 
@@ -355,14 +420,31 @@ __global__ __launch_bounds__(kThreads) void square_join_kernel(const double* par
   double sum = 0.0;
 #pragma unroll 8
   for (int64_t i = threadIdx.x; i < count; i += kThreads) sum += parts[i];
-  sum = workgroup_sum(sum, lds);
+  sum = workgroup_sum<kThreads>(sum, lds);
   if (threadIdx.x == 0) *out = sum;
+}
+
+// A few chunks in one workgroup, two at a time for each quarter of it, which writes
+// the sum itself: norm weights and biases, where a second launch would be the longer part.
+constexpr int kFewChunks = 32, kFewThreads = 1024;
+__global__ __launch_bounds__(kFewThreads) void square_sum_few_kernel(const SquareTable a) {
+  __shared__ double lds[kFewThreads / 64];
+  constexpr int kParts = kFewThreads / kThreads;
+  const int part = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kThreads), thread = threadIdx.x % kThreads;
+  double sum = 0.0, other = 0.0;
+  for (int64_t chunk = part; chunk < a.chunks; chunk += 2 * kParts) {
+    sum += squares_of_chunk<false>(a, chunk, thread);
+    if (chunk + kParts < a.chunks) other += squares_of_chunk<false>(a, chunk + kParts, thread);
+  }
+  sum = workgroup_sum<kFewThreads>(sum + other, lds);
+  if (threadIdx.x == 0) a.parts[0] = sum;
 }
 
 // Chunks of one launch are numbered in 32 bits.
 constexpr int64_t kMaxChunks = 0xFFFFFFFELL;
 
-// Workgroups of each of the launches that the tensors take; their number.
+// Workgroups of each of the launches that the tensors take; their number.  One of a
+// single workgroup where one can do it all.
 template <typename Each>
 int square_launches(const int64_t* tensors, int32_t count, Each each) {
   int32_t begin = 0;
@@ -377,7 +459,8 @@ int square_launches(const int64_t* tensors, int32_t count, Each each) {
       ++end;
     }
     if (end == begin) return -1;  // a tensor of more than 2^44 elements
-    if (chunks) each(begin, end, chunks, chunks < kSquareGroups ? chunks : static_cast<int64_t>(kSquareGroups));
+    const bool few = begin == 0 && end == count && chunks <= kFewChunks;
+    if (chunks) each(begin, end, chunks, few ? 0 : chunks < kSquareGroups ? chunks : static_cast<int64_t>(kSquareGroups));
     ++launches;
     begin = end;
   }
@@ -419,7 +502,9 @@ FSH_API int fsh_grad_square_sum(const int64_t* tensors, int32_t count, double* o
   if (need && (!workspace_dev || workspace_nbytes < need)) return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_nbytes, (long long)need);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   double* const parts = static_cast<double*>(workspace_dev);
-  int64_t used = 0;
+  int64_t used = 0, nbytes = 0;
+  for (int32_t i = 0; i < count; ++i) nbytes += tensors[3 * i + 1] * bytes_of(static_cast<int>(tensors[3 * i + 2]));
+  bool done = false;
   int rc = FSH_OK;
   const int launches = square_launches(tensors, count, [&](int32_t begin, int32_t end, int64_t chunks, int64_t groups) {
     SquareTable a;
@@ -433,16 +518,19 @@ FSH_API int fsh_grad_square_sum(const int64_t* tensors, int32_t count, double* o
       a.first_chunk[k] = here ? first : 0xFFFFFFFFu;
       if (here) first += static_cast<uint32_t>(ceil_div(t[1], (int64_t)kSquareChunk));
     }
-    a.parts = parts + used;
+    a.parts = groups ? parts + used : out_dev;
     a.chunks = chunks;
+    done = groups == 0;
     if (rc == FSH_OK) {
-      hipLaunchKernelGGL(square_sum_kernel, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, on, a);
+      if (done) hipLaunchKernelGGL(square_sum_few_kernel, dim3(1), dim3(kFewThreads), 0, on, a);
+      else if (nbytes > kSquareStream) hipLaunchKernelGGL(square_sum_kernel<true>, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, on, a);
+      else hipLaunchKernelGGL(square_sum_kernel<false>, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), 0, on, a);
       rc = check_launch("square_sum_kernel");
     }
     used += groups;
   });
   if (launches < 0) return fail(FSH_ENOTSUP, "%s: a tensor is too long", who);
-  if (rc) return rc;
+  if (rc || done) return rc;
   hipLaunchKernelGGL(square_join_kernel, dim3(1), dim3(kThreads), 0, on, parts, used, out_dev);
   return check_launch("square_join_kernel");
 }
@@ -478,7 +566,7 @@ FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const
     if (!aligned(t.param_dev, bytes_of(t.param_dtype)) || !aligned(t.grad_dev, bytes_of(t.grad_dtype)) || !aligned(t.exp_avg_dev, t.state_bits == 8 ? 1 : 4) ||
         !aligned(t.exp_avg_sq_dev, t.state_bits == 8 ? 1 : 4) || !aligned(t.exp_avg_scale_dev, 4) || !aligned(t.exp_avg_sq_scale_dev, 4) || !aligned(t.step_dev, 4))
       return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
-    if (ceil_div(t.numel, (int64_t)kChunk) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
+    if (ceil_div(t.numel, (int64_t)chunk_of(t.state_bits == 8)) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
   }
   const hipStream_t on = static_cast<hipStream_t>(stream);
   StepFactors* const factors = static_cast<StepFactors*>(workspace_dev);
@@ -507,7 +595,7 @@ FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const
       for (; next < count && n < kTensors; ++next) {
         const fsh_adamw_tensor& t = tensors[next];
         if (t.param_dtype != pt || t.grad_dtype != gt || (t.state_bits == 8) != eight || t.numel == 0) continue;
-        const int64_t more = ceil_div(t.numel, (int64_t)kChunk);
+        const int64_t more = ceil_div(t.numel, (int64_t)chunk_of(eight));
         if (a.chunks + more > kMaxChunks) break;
         a.param[n] = t.param_dev;
         a.grad[n] = t.grad_dev;

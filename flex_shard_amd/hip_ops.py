@@ -1677,8 +1677,8 @@ def grad_square_sum(tensors: Sequence[torch.Tensor]) -> torch.Tensor:
     table = (ctypes.c_int64 * len(table))(*table)
     nbytes = _native.lib().fsh_grad_square_sum_workspace_bytes(table, len(tensors))
     out = torch.empty((), dtype=torch.float64, device=device)
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
-    _queue("fsh_grad_square_sum", device, table, len(tensors), out.data_ptr(), workspace.data_ptr(), nbytes)
+    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
+    _queue("fsh_grad_square_sum", device, table, len(tensors), out.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes)
     return out
 
 

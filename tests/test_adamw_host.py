@@ -35,10 +35,12 @@ def test_square_sum():
     assert lib.fsh_grad_square_sum(good, -1, SOMEWHERE, SOMEWHERE, 64, None) == EINVAL
     assert lib.fsh_grad_square_sum(good, 1, None, SOMEWHERE, 64, None) == EINVAL
     assert lib.fsh_grad_square_sum(good, 1, SOMEWHERE + 4, SOMEWHERE, 64, None) == ENOTSUP
-    assert lib.fsh_grad_square_sum(good, 1, SOMEWHERE, SOMEWHERE, 7, None) == EINVAL and "workspace" in _message()
+    many = _table(SOMEWHERE, 1 << 30, 0)
+    assert lib.fsh_grad_square_sum(many, 1, SOMEWHERE, SOMEWHERE, 7, None) == EINVAL and "workspace" in _message()
+    assert lib.fsh_grad_square_sum(many, 1, SOMEWHERE, None, 1 << 20, None) == EINVAL and "workspace" in _message()
     size = lib.fsh_grad_square_sum_workspace_bytes
-    assert size(good, 1) == 8 and size(good, 0) == size(None, 1) == size(good, -1) == 0
-    assert size(_table(SOMEWHERE, 1 << 40, 1), 1) <= 8 * 4096
+    assert size(good, 1) == size(good, 0) == size(None, 1) == size(good, -1) == 0  # one workgroup does a few
+    assert size(many, 1) == size(_table(SOMEWHERE, 1 << 40, 1), 1) == 8 * 4096
 
 
 def _step(tensor=(), group=(), count=1, groups=1, square_sum=None, max_norm=0.0, workspace=SOMEWHERE, nbytes=1 << 20):

@@ -198,7 +198,7 @@ def test_a_sum_that_is_not_finite_skips_the_step(bad, bits):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
-@pytest.mark.parametrize("sizes", [[1], [7, 0, 8191, 8192, 8193], [3] * 400, [1 << 20, 5], [25_000_003]])
+@pytest.mark.parametrize("sizes", [[1], [7, 0, 8191, 8192, 8193], [3] * 32, [8192] * 31 + [0, 9], [3] * 33, [3] * 400, [1 << 20, 5], [25_000_003], [140_000_000, 77]])
 def test_square_sums(sizes, dtype):
     gen = _gen(6)
     flat = torch.randn(sum(sizes) + 1, generator=gen, device="cuda").to(dtype)
