@@ -191,7 +191,9 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* par
 // launch(layout) with the layout for rows of `cols` columns.
 template <int VEC, typename Launch>
 void by_columns(int64_t cols, Launch launch) {
-  if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC>{});
+  if (cols <= 64) launch(NormLayout<64 / VEC, VEC, VEC>{});
+  else if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC>{});
+  else if (cols <= 256) launch(NormLayout<256 / VEC, VEC, VEC>{});
   else if (cols <= 512) launch(NormLayout<64, 8, VEC>{});
   else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
   else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});

@@ -190,10 +190,13 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
 }
 
 // launch(layout) with the layout for rows of `cols` columns.
-template <int VEC, typename Launch>
+// (a run of 128 columns that is quantized takes all the lanes that it needs)
+template <int VEC, bool kQuant, typename Launch>
 void by_columns(int64_t cols, int64_t rows, Launch launch) {
   const bool few = rows <= 512;
-  if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC, 2>{});
+  if (cols <= 64 && !kQuant) launch(NormLayout<64 / VEC, VEC, VEC, 2>{});
+  else if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC, 2>{});
+  else if (cols <= 256) launch(NormLayout<256 / VEC, VEC, VEC, 2>{});
   else if (cols <= 512) launch(NormLayout<64, 8, VEC, 2>{});
   else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
   else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});
@@ -208,7 +211,7 @@ void by_columns(int64_t cols, int64_t rows, Launch launch) {
 template <int XT, int RT, bool kQuant>
 void launch_norm(NormParams& p, hipStream_t stream) {
   constexpr int VEC = XT == FSH_DT_F32 || RT == FSH_DT_F32 ? 4 : 8;  // 16 bytes of the wider type
-  by_columns<VEC>(p.cols, p.rows, [&](auto layout) {
+  by_columns<VEC, kQuant>(p.cols, p.rows, [&](auto layout) {
     using L = decltype(layout);
     p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS * L::TURN);
     constexpr int64_t kMaxGrid = (1LL << 32) / L::THREADS - 1;  // a launch's threads are counted in 32 bits

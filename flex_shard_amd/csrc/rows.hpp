@@ -155,18 +155,18 @@ __device__ __forceinline__ void load_floats(const void* base, int32_t dtype, int
   }
 }
 
-// Sums over a row of 16 lanes, half a wave, a wave, in every lane of it: moves
+// Sums over 8 lanes, a row of 16, half a wave, a wave, in every lane of them: moves
 // between lanes (DPP), always in the same order.
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
   return v + u32_as_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(f32_as_u32(v)), CTRL, 0xF, 0xF, true)));
 }
-__device__ __forceinline__ float sum16(float v) {
-  v = dpp_add<0xB1>(v);   // quad_perm [1,0,3,2]
-  v = dpp_add<0x4E>(v);   // quad_perm [2,3,0,1]
-  v = dpp_add<0x141>(v);  // row_half_mirror
-  return dpp_add<0x140>(v);  // row_mirror
+__device__ __forceinline__ float sum8(float v) {
+  v = dpp_add<0xB1>(v);      // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E>(v);      // quad_perm [2,3,0,1]
+  return dpp_add<0x141>(v);  // row_half_mirror
 }
+__device__ __forceinline__ float sum16(float v) { return dpp_add<0x140>(sum8(v)); }  // row_mirror
 __device__ __forceinline__ float sum32(float v) {
   v = sum16(v);
   return v + __shfl_xor(v, 16, kWave);
@@ -185,10 +185,11 @@ __device__ __forceinline__ uint32_t max32_u32(uint32_t v) {
   return o > v ? o : v;
 }
 
-// The sum over the LANES threads that share a row (16, 32, 64, or a workgroup of
-// 256 or 1024: then `lds` holds a float for each of its waves, twice over, used in turn).
+// The sum over the LANES threads that share a row (8, 16, 32, 64, or a workgroup of
+// 256, 512 or 1024: then `lds` holds a float for each of its waves, twice over, used in turn).
 template <int LANES>
 __device__ __forceinline__ float sum_over_row(float v, float* lds, int turn) {
+  if constexpr (LANES == 8) return sum8(v);
   if constexpr (LANES == 16) return sum16(v);
   if constexpr (LANES == 32) return sum32(v);
   if constexpr (LANES == 64) return sum64(v);

@@ -1543,35 +1543,40 @@ def rms_norm(
     """``(out, total, rstd)`` of the rows of ``x`` [..., cols]: ``total`` = x +
     residual (None without one), ``out`` its norm in the type of ``x``, or with ``fp8``
     what :func:`act_quant_1x128` makes of it in bf16; ``rstd`` [rows] if kept."""
-    _require_gpu(x, *(t for t in (weight, residual) if t is not None))
-    shape, device, dtype = x.shape, x.device, x.dtype
-    if x.ndim < 1 or shape[-1] == 0:
+    index = x.get_device()
+    if (
+        index < 0 or (weight is not None and weight.get_device() != index) or (residual is not None and residual.get_device() != index)
+    ):
+        _refuse_devices([t for t in (x, weight, residual) if t is not None])
+    shape, dtype = x.shape, x.dtype
+    if not shape or shape[-1] == 0:
         raise ValueError(f"expected rows [..., cols], got {tuple(shape)}")
     cols = shape[-1]
     rows = x.numel() // cols
     ldx, code = _norm_stride("x", x, shape), _float_dt(dtype)
     weight_ptr, weight_code = _norm_weight(weight, cols)
     total = rstd = scales = None
-    residual_ptr = total_ptr = ldr = residual_code = 0
+    residual_ptr = total_ptr = ldr = residual_code = scales_ptr = rstd_ptr = form = 0
     if residual is not None:
-        if residual.dtype not in (dtype, torch.float32):
+        if residual.dtype is not dtype and residual.dtype is not torch.float32:
             raise NotImplementedError(f"a residual is of the type of x ({dtype}) or fp32, got {residual.dtype}")
         residual_code, ldr = _float_dt(residual.dtype), _norm_stride("residual", residual, shape)
-        total = torch.empty(shape, dtype=residual.dtype, device=device)
+        total = torch.empty_like(residual, memory_format=torch.contiguous_format)
         residual_ptr, total_ptr = residual.data_ptr(), total.data_ptr()
     if fp8:
         padded = -(-cols // 128) * 128
-        out = torch.empty((rows, padded), dtype=torch.float8_e4m3fn, device=device)
-        scales = torch.empty((padded // 128, rows), dtype=torch.float32, device=device)
+        out = x.new_empty((rows, padded), dtype=torch.float8_e4m3fn)
+        scales = x.new_empty((padded // 128, rows), dtype=torch.float32)
+        scales_ptr, form = scales.data_ptr(), _native.NORM_FP8
     else:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if keep_rstd:
-        rstd = torch.empty((rows,), dtype=torch.float32, device=device)
+        rstd = x.new_empty((rows,), dtype=torch.float32)
+        rstd_ptr = rstd.data_ptr()
     if rows:
-        _queue("fsh_rms_norm", device, _PACK_NORM(
-            x.data_ptr(), residual_ptr, weight_ptr, total_ptr, out.data_ptr(), scales.data_ptr() if fp8 else 0,
-            rstd.data_ptr() if keep_rstd else 0, rows, cols, ldx, ldr, code, residual_code, weight_code,
-            _native.NORM_FP8 if fp8 else _native.NORM_VALUES, eps, 0,
+        _queue("fsh_rms_norm", x.device, _PACK_NORM(
+            x.data_ptr(), residual_ptr, weight_ptr, total_ptr, out.data_ptr(), scales_ptr, rstd_ptr, rows, cols, ldx, ldr,
+            code, residual_code, weight_code, form, eps, 0,
         ))
     return (out, scales) if fp8 else out, total, rstd
 
@@ -1588,36 +1593,40 @@ def rms_norm_backward(
     """``(grad_x, grad_residual, grad_weight)`` of :func:`rms_norm`; ``total`` is
     what it normed (``x`` without a residual).  The first two are one tensor where
     ``total`` is of ``x_dtype``."""
-    _require_gpu(grad, total, rstd, *(t for t in (weight, grad_total) if t is not None))
-    shape, device = total.shape, total.device
+    index = total.get_device()
+    if index < 0 or grad.get_device() != index or rstd.get_device() != index or (
+        weight is not None and weight.get_device() != index) or (grad_total is not None and grad_total.get_device() != index
+    ):
+        _refuse_devices([t for t in (grad, total, rstd, weight, grad_total) if t is not None])
+    shape, dtype = total.shape, total.dtype
     cols = shape[-1]
     rows = total.numel() // cols
-    same = total.dtype == x_dtype
+    same = dtype is x_dtype
     weight_ptr, weight_code = _norm_weight(weight, cols)
     ldg, ldh = _norm_stride("grad", grad, shape), _norm_stride("total", total, shape)
     _check_rstd(rstd, rows)
     ldt = grad_total_ptr = 0
     if grad_total is not None:
-        if grad_total.dtype != total.dtype:
-            raise ValueError(f"the gradient of a sum of {total.dtype} is of that type, got {grad_total.dtype}")
+        if grad_total.dtype is not dtype:
+            raise ValueError(f"the gradient of a sum of {dtype} is of that type, got {grad_total.dtype}")
         ldt, grad_total_ptr = _norm_stride("grad_total", grad_total, shape), grad_total.data_ptr()
     grad_x = grad_residual = grad_weight = None
     grad_x_ptr = grad_residual_ptr = grad_weight_ptr = workspace_ptr = nbytes = 0
     if needs_x or (same and needs_residual):
-        grad_x = torch.empty(shape, dtype=x_dtype, device=device)
+        grad_x = torch.empty_like(total, dtype=x_dtype, memory_format=torch.contiguous_format)
         grad_x_ptr = grad_x.data_ptr()
     if needs_residual:
-        grad_residual = grad_x if same else torch.empty(shape, dtype=total.dtype, device=device)
+        grad_residual = grad_x if same else torch.empty_like(total, memory_format=torch.contiguous_format)
         if not same:
             grad_residual_ptr = grad_residual.data_ptr()
     if needs_weight and weight is not None:
-        grad_weight = torch.empty((cols,), dtype=weight.dtype, device=device)
+        grad_weight = torch.empty_like(weight)
         nbytes = _native.lib().fsh_rms_norm_backward_workspace_bytes(rows, cols)
-        workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+        workspace = rstd.new_empty((nbytes // 4,))
         grad_weight_ptr, workspace_ptr = grad_weight.data_ptr(), workspace.data_ptr()
-    _queue("fsh_rms_norm_backward", device, _PACK_NORM_GRADIENT(
+    _queue("fsh_rms_norm_backward", total.device, _PACK_NORM_GRADIENT(
         grad.data_ptr(), total.data_ptr(), weight_ptr, rstd.data_ptr(), grad_total_ptr, grad_x_ptr, grad_residual_ptr,
-        grad_weight_ptr, workspace_ptr, nbytes, rows, cols, ldg, ldh, ldt, _float_dt(grad.dtype), _float_dt(total.dtype),
+        grad_weight_ptr, workspace_ptr, nbytes, rows, cols, ldg, ldh, ldt, _float_dt(grad.dtype), _float_dt(dtype),
         _float_dt(x_dtype), weight_code,
     ))
     return grad_x if needs_x else None, grad_residual, grad_weight
