@@ -24,6 +24,7 @@ import torch
 import torch.nn as nn
 from torch.utils._python_dispatch import is_traceable_wrapper_subclass
 
+from ..blockwise_fp8.fp8_activation import Fp8Activation
 from ..bucket_storage import ParamInfo, create_param_infos
 from ..placement_contract import GradientReduction, Placement
 from .bucket_comm import (
@@ -472,8 +473,10 @@ class BucketRuntime:
 
         def post_forward(mod: nn.Module, args: Any, output: Any) -> Any:
             self.reshard()
-            tensors = [t for t in (output if isinstance(output, (tuple, list)) else (output,))
-                       if isinstance(t, torch.Tensor) and t.requires_grad]
+            outputs = output if isinstance(output, (tuple, list)) else (output,)
+            # (a quantized activation is a tensor to autograd through its carrier)
+            outputs = [t.carrier if isinstance(t, Fp8Activation) else t for t in outputs]
+            tensors = [t for t in outputs if isinstance(t, torch.Tensor) and t.requires_grad]
             if tensors:
                 torch.autograd.graph.register_multi_grad_hook(tensors, pre_backward, mode="any")
             return output

@@ -1527,7 +1527,10 @@ def _norm_weight(weight: torch.Tensor | None, cols: int) -> tuple[int, int]:
         return 0, DT_F32
     if weight.shape != (cols,) or not weight.is_contiguous():
         raise ValueError(f"weight must be {[cols]}, contiguous, got {tuple(weight.shape)} / {weight.stride()}")
-    return weight.data_ptr(), _float_dt(weight.dtype)
+    address = weight.data_ptr()
+    if address == 0:  # (to the kernels no weight at all)
+        raise RuntimeError("the norm's weight has no memory: its bucket is resharded")
+    return address, _float_dt(weight.dtype)
 
 
 # (packed by hand: a ctypes structure takes 4 us to fill)

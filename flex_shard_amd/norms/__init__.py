@@ -109,12 +109,12 @@ def rms_norm(
     return y if residual is None else (y, total)
 
 
-def _version(t: torch.Tensor | None) -> int:
-    return 0 if t is None or t.is_inference() else t._version
+def _version(t: torch.Tensor) -> int:
+    return 0 if t.is_inference() else t._version
 
 
-def _token_runs(normed, normed_version: int, weight, weight_version: int, rstd) -> tuple[torch.Tensor, torch.Tensor]:
-    if _version(normed) != normed_version or _version(weight) != weight_version:
+def _token_runs(normed, version: int, weight, rstd) -> tuple[torch.Tensor, torch.Tensor]:
+    if _version(normed) != version:
         raise RuntimeError("what an 8-bit norm was made of was changed in place before a weight gradient's form of it was made")
     return hip_ops.rms_norm_token_runs(normed, weight, rstd)
 
@@ -140,7 +140,11 @@ def rms_norm_fp8(
     else:
         (q, scales), total, rstd = hip_ops.rms_norm(x, weight, eps, stream, fp8=True, keep_rstd=True)
         normed, carrier = x if total is None else total, _carrier(x.shape, x.device)
-    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, _version(normed), weight, _version(weight), rstd))
+    if weight is not None and torch.is_grad_enabled():
+        # The token runs are made when a linear asks for them, and by then the weight's
+        # bucket may be resharded, or an optimizer have been at it.
+        weight = weight.detach().clone()
+    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, _version(normed), weight, rstd))
     return activation if residual is None else (activation, total)
 
 

@@ -19,7 +19,7 @@ EPS = 1e-5
 # types of x and of the residual
 PAIRS = [(BF16, None), (BF16, BF16), (BF16, F32), (F16, None), (F16, F16), (F16, F32), (F32, None), (F32, F32)]
 # one and more columns, up to the borders of every layout and past them
-WIDTHS = [1, 7, 8, 127, 128, 129, 512, 515, 1001, 1024, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16385, 20001]
+WIDTHS = [1, 7, 8, 63, 64, 65, 127, 128, 129, 200, 256, 257, 512, 515, 1001, 1024, 2048, 2056, 4095, 4096, 4104, 8192, 8200, 16384, 16385, 20001]
 
 
 def _step(dtype):
@@ -58,6 +58,14 @@ def _check_forward(x, residual, w, eps=EPS):
 @pytest.mark.parametrize("dtype,stream", PAIRS)
 def test_widths(dtype, stream, cols):
     x, residual, w, _ = _make(5, cols, dtype, stream)
+    _check_forward(x, residual, w)
+
+
+@pytest.mark.parametrize("cols", [64, 256, 1001, 2048, 4000, 4096, 7168, 8192])
+@pytest.mark.parametrize("dtype,stream", PAIRS)
+def test_many_rows(dtype, stream, cols):
+    """More rows than those that get more lanes each."""
+    x, residual, w, _ = _make(777, cols, dtype, stream)
     _check_forward(x, residual, w)
 
 

@@ -16,7 +16,7 @@ BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 EPS = 1e-6
 # types of which the bf16 norm can be had elsewhere in the same bits: fp32 and bf16
 PAIRS = [(BF16, None), (BF16, BF16), (BF16, F32), (F32, None), (F32, F32)]
-WIDTHS = [1, 8, 100, 128, 130, 256, 520, 1000, 1024, 2048, 2050, 4096, 4232, 7168, 8192, 8200, 12288, 16384, 16390, 20001]
+WIDTHS = [1, 8, 64, 100, 128, 130, 256, 257, 520, 1000, 1024, 2048, 2050, 4096, 4232, 7168, 8192, 8200, 12288, 16384, 16390, 20001]
 
 
 def _make(rows, cols, dtype, stream, weight=F32):
@@ -58,9 +58,10 @@ def test_bits_of_the_norm_and_the_quantizer(dtype, stream, cols):
     assert got.token_runs()[0] is mine
 
 
-@pytest.mark.parametrize("rows", [1, 5, 16, 127, 128, 129, 300])
-def test_rows(rows):
-    x, residual, w, _ = _make(rows, 700, BF16, BF16, BF16)
+@pytest.mark.parametrize("cols", [64, 700, 2048, 4096, 7168])
+@pytest.mark.parametrize("rows", [1, 5, 16, 127, 128, 129, 300, 600])
+def test_rows(rows, cols):
+    x, residual, w, _ = _make(rows, cols, BF16, BF16, BF16)
     got, _ = rms_norm_fp8(x, w, EPS, residual=residual)
     padded = _quantized(rms_norm(x, w, EPS, residual=residual)[0])
     assert _same(got.q, hip_ops.act_quant_1x128(padded)[0])
