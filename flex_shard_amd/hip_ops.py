@@ -1521,16 +1521,21 @@ def _norm_stride(name: str, t: torch.Tensor, shape: torch.Size) -> int:
     return along if shape[0] > 1 else cols
 
 
+def _address(name: str, t: torch.Tensor) -> int:
+    """Of an operand that may be left out: one without memory would be to the kernels."""
+    address = t.data_ptr()
+    if address == 0 and t.numel():
+        raise RuntimeError(f"{name} has no memory (a parameter of a resharded bucket, or a wrapper)")
+    return address
+
+
 def _norm_weight(weight: torch.Tensor | None, cols: int) -> tuple[int, int]:
     """Address and dtype code."""
     if weight is None:
         return 0, DT_F32
     if weight.shape != (cols,) or not weight.is_contiguous():
         raise ValueError(f"weight must be {[cols]}, contiguous, got {tuple(weight.shape)} / {weight.stride()}")
-    address = weight.data_ptr()
-    if address == 0:  # (to the kernels no weight at all)
-        raise RuntimeError("the norm's weight has no memory: its bucket is resharded")
-    return address, _float_dt(weight.dtype)
+    return _address("the norm's weight", weight), _float_dt(weight.dtype)
 
 
 # (packed by hand: a ctypes structure takes 4 us to fill)
@@ -1565,7 +1570,7 @@ def rms_norm(
             raise NotImplementedError(f"a residual is of the type of x ({dtype}) or fp32, got {residual.dtype}")
         residual_code, ldr = _float_dt(residual.dtype), _norm_stride("residual", residual, shape)
         total = torch.empty_like(residual, memory_format=torch.contiguous_format)
-        residual_ptr, total_ptr = residual.data_ptr(), total.data_ptr()
+        residual_ptr, total_ptr = _address("residual", residual), total.data_ptr()
     if fp8:
         padded = -(-cols // 128) * 128
         out = x.new_empty((rows, padded), dtype=torch.float8_e4m3fn)
@@ -1612,7 +1617,7 @@ def rms_norm_backward(
     if grad_total is not None:
         if grad_total.dtype is not dtype:
             raise ValueError(f"the gradient of a sum of {dtype} is of that type, got {grad_total.dtype}")
-        ldt, grad_total_ptr = _norm_stride("grad_total", grad_total, shape), grad_total.data_ptr()
+        ldt, grad_total_ptr = _norm_stride("grad_total", grad_total, shape), _address("grad_total", grad_total)
     grad_x = grad_residual = grad_weight = None
     grad_x_ptr = grad_residual_ptr = grad_weight_ptr = workspace_ptr = nbytes = 0
     if needs_x or (same and needs_residual):

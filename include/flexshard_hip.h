@@ -740,6 +740,8 @@ int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, int64_t ro
  *   code & 127, negative with bit 7) or (c + 761) << 20 (second), times the scale; c = 0: zero
  * rounded up or down evenly over elements and steps.  All zero is the start of both.
  * workspace: ..._workspace_bytes(count), 16-byte aligned; only the call itself uses it.
+ * All argument checks come before any launch; a launch that the runtime then rejects leaves
+ * the step half done, as in section 10.
  *
  * fsh_adamw_state_values: what the codes stand for, in dtype.
  * ---------------------------------------------------------------------- */

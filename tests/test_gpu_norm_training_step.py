@@ -145,9 +145,20 @@ def test_states_get_their_shards_layouts(device):
 
 def test_a_resharded_weight_is_refused(device):
     norm = FlexShardRMSNorm(DIM, device=device, dtype=torch.bfloat16)
+    x = torch.zeros(3, DIM, dtype=torch.bfloat16, device=device)
+    freed = torch.zeros_like(x)
+    freed.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="residual has no memory"):
+        norm(x, freed)
     norm.weight.untyped_storage().resize_(0)
-    with pytest.raises(RuntimeError, match="resharded"):
-        norm(torch.zeros(3, DIM, dtype=torch.bfloat16, device=device))
+    for fp8 in (False, True):
+        with pytest.raises(RuntimeError, match="resharded"):
+            norm(x, fp8=fp8)
+    p = nn.Parameter(torch.zeros(5, device=device))
+    p.grad = torch.ones_like(p)
+    p.untyped_storage().resize_(0)
+    with pytest.raises(RuntimeError, match="null pointer"):
+        FlexShardAdamW([p]).step()
 
 
 def test_beside_muon(device):
