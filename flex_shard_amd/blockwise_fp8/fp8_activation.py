@@ -5,7 +5,6 @@ from __future__ import annotations
 from typing import Any, Callable
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import hip_ops
 
@@ -69,9 +68,8 @@ class _Dequantize(torch.autograd.Function):
         return activation._values(dtype)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad: torch.Tensor):
-        return grad.to(torch.bfloat16), None, None
+    def backward(ctx: Any, grad: torch.Tensor):  # (linear in the gradient: differentiable again)
+        return grad if grad.dtype is torch.bfloat16 else grad.to(torch.bfloat16), None, None
 
 
 __all__ = ["Fp8Activation"]

@@ -35,6 +35,7 @@ def _as_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor | None, eps: float, residual: torch.Tensor | None) -> None:
+    """For a call without rows; any other one is checked with its operands."""
     if x.dtype not in _DTYPES:
         raise NotImplementedError(f"the norm takes bf16, fp16 or fp32 rows, got {x.dtype}")
     if x.ndim < 1 or x.shape[-1] == 0:
@@ -67,24 +68,40 @@ class _Norm(torch.autograd.Function):
             kept += (*out, normed, rstd)
             out = _carrier(x.shape, x.device)
         ctx.save_for_backward(normed, weight, rstd)
+        # what the backward's thread need not find out again
+        cols, types = x.shape[-1], hip_ops.FLOAT_CODES
+        ldh = cols if normed.is_contiguous() else normed.stride(0)
         ctx.x_dtype = x.dtype
+        ctx.call = (x.numel() // cols, cols, ldh), (types[out.dtype], types[normed.dtype], types[x.dtype], 0 if weight is None else types[weight.dtype])
         ctx.set_materialize_grads(False)
         return out, total
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
-        normed, weight, rstd = ctx.saved_tensors
-        needs_x, needs_residual, needs_weight = ctx.needs_input_grad[:3]
-        if grad is None:  # the stream alone was used
-            if grad_total is None:
-                return None, None, None, None, None
-            return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
-        grads = hip_ops.rms_norm_backward(
-            _as_rows(grad), normed, weight, rstd, ctx.x_dtype, None if grad_total is None else _as_rows(grad_total),
-            needs_x=needs_x, needs_residual=needs_residual, needs_weight=needs_weight,
-        )
-        return (*grads, None, None)
+        # (recorded only for a second differentiation, which the wrapper refuses: 3 us of the backward's thread else)
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, grad, grad_total)
+
+
+def _norm_backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
+    normed, weight, rstd = ctx.saved_tensors
+    needs_x, needs_residual, needs_weight, _, _ = ctx.needs_input_grad
+    if grad is None:  # the stream alone was used
+        if grad_total is None:
+            return None, None, None, None, None
+        return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
+    (rows, cols, ldh), codes = ctx.call
+    grad = _as_rows(grad)
+    ldg, ldt = cols if grad.is_contiguous() else grad.stride(0), 0
+    if grad_total is not None:
+        grad_total = _as_rows(grad_total)
+        ldt = cols if grad_total.is_contiguous() else grad_total.stride(0)
+    grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward_checked(
+        grad, normed, weight, rstd, ctx.x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
+    )
+    return grad_x, grad_residual, grad_weight, None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
 
 
 def rms_norm(
@@ -94,8 +111,8 @@ def rms_norm(
     times ``weight`` [cols] (any of these types, or None).  With ``residual``, of the
     shape of ``x`` and its type or fp32, ``(norm of x + residual, x + residual)``, the sum in
     the residual's type.  Statistics in fp32, every output rounded once; differentiable."""
-    _check(x, weight, eps, residual)
     if x.numel() == 0:  # no rows: torch's own empty products keep the graph
+        _check(x, weight, eps, residual)
         total = x if residual is None else x.to(residual.dtype) + residual
         y = (total if weight is None else total * weight).to(x.dtype)
         return y if residual is None else (y, total)
@@ -124,7 +141,6 @@ def rms_norm_fp8(
 ) -> Fp8Activation | tuple[Fp8Activation, torch.Tensor]:
     """:func:`rms_norm`, its output rounded to bf16 and quantized like the
     activations of the blockwise FP8 linears, which take it as it is."""
-    _check(x, weight, eps, residual)
     x = _as_rows(x)
     stream = None if residual is None else _as_rows(residual)
     weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
