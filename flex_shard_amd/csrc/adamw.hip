@@ -10,8 +10,8 @@
 //
 // Bound by memory: everything is read once and written once, 22 bytes an element
 // (bf16 parameters and gradients, 32-bit states), 10 1/8 with 8-bit states.  218 M
-// parameters: 756 us, 6.3 TB/s, and fp32 with 8-bit states 595, 5.9; bf16 with those 470, 4.7, bound by
-// instructions.  The tensors of a launch come with its arguments, so that nothing is uploaded and a
+// parameters: 756 us, 6.3 TB/s, and fp32 with 8-bit states 593, 5.9; bf16 with those 430, 5.1, half
+// of it instructions.  The tensors of a launch come with its arguments, so that nothing is uploaded and a
 // captured launch keeps its own table; what a step's number and learning rate make of the
 // hyperparameters is worked out once for each tensor, by a launch of a single workgroup ahead (4.6 us).
 //
@@ -137,18 +137,22 @@ __device__ __forceinline__ float first_value(uint32_t code) {
 __device__ __forceinline__ float second_value(uint32_t code) { return u32_as_f32(code ? (code + kSecondBase) << 20 : 0u); }
 // The codes of a value over its block's scale, of at most 1 and a few units in the last
 // place, which the dither cannot carry further (of a block that is not a number: any bits).
-// half: the dither in units of 2^-16.
+// half: the dither in units of 2^-16.  kSmall: the value may be below the smallest code.
+constexpr float kFirstSmallest = 1.25f / 65536.0f, kSecondSmallest = kFirstSmallest / 65536.0f;
+template <bool kSmall>
 __device__ __forceinline__ uint32_t first_code(float value, uint32_t half) {
-  constexpr float kSmallest = 1.25f / 65536.0f;
-  const uint32_t bits = f32_as_u32(value) & 0x7FFFFFFFu;
-  const float size = u32_as_f32(bits);
+  const uint32_t bits = f32_as_u32(value) & 0x7FFFFFFFu, sign = (f32_as_u32(value) >> 24) & 128u;
   const uint32_t up = ((bits + (half << 4)) >> 20) - kFirstBase;
-  // (the product with 1 / kSmallest, rounded as such, against half / 65536)
-  const uint32_t few = size * (1.0f / kSmallest * 65536.0f) > static_cast<float>(half) ? 1u : 0u;
-  return (size < kSmallest ? few : up) | ((f32_as_u32(value) >> 24) & 128u);
+  if constexpr (!kSmall) return up | sign;
+  const float size = u32_as_f32(bits);
+  // (the product with 1 / kFirstSmallest, rounded as such, against half / 65536)
+  const uint32_t few = size * (1.0f / kFirstSmallest * 65536.0f) > static_cast<float>(half) ? 1u : 0u;
+  return (size < kFirstSmallest ? few : up) | sign;
 }
+template <bool kSmall>
 __device__ __forceinline__ uint32_t second_code(float size, uint32_t half) {
   const int up = static_cast<int>((f32_as_u32(size) + (half << 4)) >> 20) - static_cast<int>(kSecondBase);
+  if constexpr (!kSmall) return static_cast<uint32_t>(up);
   const int least = static_cast<int>(min(f32_as_u32(size), 1u));  // 1 of what is not zero
   return static_cast<uint32_t>(max(up, least));
 }
@@ -160,6 +164,17 @@ constexpr uint32_t kOverElements = 0x9E3779B9u, kOverSteps = 0x6A09E667u;
 __device__ __forceinline__ uint32_t dither(uint32_t multiple) {
   const uint32_t z = (multiple ^ (multiple >> 16)) * 0xBB67AE85u;
   return z ^ (z >> 15);
+}
+
+template <bool kSmall>
+__device__ __forceinline__ void codes_of(const float (&m)[4], const float (&v)[4], uint32_t multiple, uint32_t& mc, uint32_t& vc) {
+  mc = vc = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t u = dither(multiple + static_cast<uint32_t>(j) * kOverElements);
+    mc |= first_code<kSmall>(m[j], u & 0xFFFFu) << (8 * j);
+    vc |= second_code<kSmall>(v[j], u >> 16) << (8 * j);
+  }
 }
 
 // The scale of a block from its largest magnitude's bits, and 1 over it.
@@ -175,7 +190,8 @@ __device__ __forceinline__ float block_scale(uint32_t largest, float& inverse) {
 // A workgroup takes a chunk: vectors of four neighbours a thread, the loads of all
 // of them requested first.  With 32-bit states one vector, with 8-bit ones, where instructions
 // count and what is done once per chunk is spread, four (218 M parameters, us with one, two
-// and four: bf16 and 32 bits 768, 855, 820; bf16 and 8 bits 535, 490, 470; fp32 and 8 bits 600 each).
+// and four: bf16 and 32 bits 768, 855, 820; bf16 and 8 bits, with a division for each moment, 535, 490,
+// 470; fp32 and 8 bits 600 each).
 // Everything streams: through the caches the 32-bit step takes 919 us, and workgroups that stay for more chunks than
 // one are slower still (2048 of them: 1049).
 constexpr int chunk_of(bool eight) { return (eight ? 4 : 1) * 4 * kThreads; }
@@ -278,21 +294,33 @@ __device__ __forceinline__ void step_chunk(const ChunkOf& c, const StepFactors& 
         m_max = max(m_max, f32_as_u32(m[j]) & 0x7FFFFFFFu);
         v_max = max(v_max, f32_as_u32(v[j]) & 0x7FFFFFFFu);
       }
-      float m_inverse, v_inverse;
-      const float ms = block_scale(max32_u32(m_max), m_inverse), vs = block_scale(max32_u32(v_max), v_inverse);
-      const uint32_t multiple = (first_index + static_cast<uint32_t>(at)) * kOverElements + f.t * kOverSteps;
-      uint32_t mc = 0, vc = 0;
+      // Both moments' maxima over each row of 16 lanes; a swap of the first's odd rows
+      // with the second's even ones joins the pairs, the first's in even rows and the second's in
+      // odd ones, so that one division does for both, and another swap hands its results out.
+      const auto pair = __builtin_amdgcn_permlane16_swap(row16_max_u32(m_max), row16_max_u32(v_max), false, false);
+      float inverse;
+      const float scale = block_scale(max(pair[0], pair[1]), inverse);
+      const auto inverses = __builtin_amdgcn_permlane16_swap(f32_as_u32(inverse), f32_as_u32(inverse), false, false);
+      float m_least = 1.0f, v_least = 1.0f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t u = dither(multiple + static_cast<uint32_t>(j) * kOverElements);
-        mc |= first_code(m[j] * m_inverse, u & 0xFFFFu) << (8 * j);
-        vc |= second_code(v[j] * v_inverse, u >> 16) << (8 * j);
+        m[j] *= u32_as_f32(inverses[0]);
+        v[j] *= u32_as_f32(inverses[1]);
+        m_least = fminf(m_least, fabsf(m[j]));
+        v_least = fminf(v_least, v[j]);
       }
+      const uint32_t multiple = (first_index + static_cast<uint32_t>(at)) * kOverElements + f.t * kOverSteps;
+      uint32_t mc, vc;
+      // (a wave rarely has a value below the smallest code; with this and the one division, bf16
+      // parameters take 430 us for 485)
+      if (__ballot(m_least < kFirstSmallest || v_least < kSecondSmallest)) codes_of<true>(m, v, multiple, mc, vc);
+      else codes_of<false>(m, v, multiple, mc, vc);
       store_codes<kFull>(c.m + at, count, mc);
       store_codes<kFull>(c.v + at, count, vc);
-      if ((kFull || count > 0) && at % kStateBlock == 0) {
-        c.m_scale[at / kStateBlock] = ms;
-        c.v_scale[at / kStateBlock] = vs;
+      // (a block's first lane has its first moment's scale, the sixteenth behind it the second's)
+      if (threadIdx.x % 16 == 0) {
+        const int of = at - (threadIdx.x & 16) * 4;  // the block's first element
+        if (kFull || left > of) (threadIdx.x & 16 ? c.v_scale : c.m_scale)[of / kStateBlock] = scale;
       }
     } else if (kFull || count > 0) {
       store_vec<FSH_DT_F32, 4, true>(c.m, at, count, to_vec<FSH_DT_F32, 4>(m));
