@@ -69,10 +69,11 @@ class _Norm(torch.autograd.Function):
             out = _carrier(x.shape, x.device)
         ctx.save_for_backward(normed, weight, rstd)
         # what the backward's thread need not find out again
-        cols, types = x.shape[-1], hip_ops.FLOAT_CODES
-        ldh = cols if normed.is_contiguous() else normed.stride(0)
-        ctx.x_dtype = x.dtype
-        ctx.call = (x.numel() // cols, cols, ldh), (types[out.dtype], types[normed.dtype], types[x.dtype], 0 if weight is None else types[weight.dtype])
+        cols, types, x_dtype = x.shape[-1], hip_ops.FLOAT_CODES, x.dtype
+        ctx.call = (
+            x_dtype, x.numel() // cols, cols, cols if normed.is_contiguous() else normed.stride(0),
+            (types[out.dtype], types[normed.dtype], types[x_dtype], 0 if weight is None else types[weight.dtype]),
+        )
         ctx.set_materialize_grads(False)
         return out, total
 
@@ -83,20 +84,22 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm_backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
-    normed, weight, rstd = ctx.saved_tensors
+    x_dtype, rows, cols, ldh, codes = ctx.call
     needs_x, needs_residual, needs_weight, _, _ = ctx.needs_input_grad
     if grad is None:  # the stream alone was used
         if grad_total is None:
             return None, None, None, None, None
-        return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
-    (rows, cols, ldh), codes = ctx.call
-    grad = _as_rows(grad)
-    ldg, ldt = cols if grad.is_contiguous() else grad.stride(0), 0
-    if grad_total is not None:
+        return grad_total.to(x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
+    normed, weight, rstd = ctx.saved_tensors
+    ldg = ldt = cols
+    if not grad.is_contiguous():
+        grad = _as_rows(grad)
+        ldg = cols if grad.is_contiguous() else grad.stride(0)
+    if grad_total is not None and not grad_total.is_contiguous():
         grad_total = _as_rows(grad_total)
         ldt = cols if grad_total.is_contiguous() else grad_total.stride(0)
     grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward_checked(
-        grad, normed, weight, rstd, ctx.x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
+        grad, normed, weight, rstd, x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
     )
     return grad_x, grad_residual, grad_weight, None, None
 
