@@ -40,7 +40,9 @@ class FlexShardAdamW(torch.optim.Optimizer):
     ``exp_avg_sq_scale``; :meth:`state_values` gives what they stand for): 2 1/16
     bytes an element for 8.  Arithmetic is in fp32, the parameter rounded once.  ``step`` is
     an int32 on the GPU, so that a captured step counts on; ``lr`` may be an fp32 scalar
-    there, which a captured step reads anew.  Parameters without a gradient are left alone."""
+    there, which a captured step reads anew.  A captured step keeps the addresses that it was
+captured with: load states, and take new gradients' memory, before.  Parameters without a gradient
+are left alone; two that overlap are refused."""
 
     def __init__(
         self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -89,7 +91,7 @@ class FlexShardAdamW(torch.optim.Optimizer):
         if not state:
             raise KeyError("this parameter has no state yet")
         if state["exp_avg"].dtype != torch.uint8:
-            return state["exp_avg"].to(dtype), state["exp_avg_sq"].to(dtype)
+            return state["exp_avg"].to(dtype, copy=True), state["exp_avg_sq"].to(dtype, copy=True)
         return hip_ops.adamw_state_values(
             state["exp_avg"], state["exp_avg_scale"], state["exp_avg_sq"], state["exp_avg_sq_scale"], dtype
         )
@@ -138,7 +140,7 @@ class FlexShardAdamW(torch.optim.Optimizer):
         table: list[int] = []
         calls = [(table, groups)]
         stepped, copies = [], []  # (the queued kernels read the copies)
-        states = self.state
+        states, strided, int32 = self.state, torch.strided, torch.int32
         for group in self.param_groups:
             lr, bits, number = group["lr"], group["state_bits"], len(groups)
             for p in group["params"]:
@@ -151,7 +153,7 @@ class FlexShardAdamW(torch.optim.Optimizer):
                 param_dt, grad_dt = _DT.get(p.dtype), _DT.get(g.dtype)
                 if (
                     param_dt is None or grad_dt is None or p.get_device() != index or g.get_device() != index or index < 0
-                    or g.layout is not torch.strided or g.shape != p.shape or not p.is_contiguous()
+                    or g.layout is not strided or g.shape != p.shape or not p.is_contiguous()
                 ):
                     _refuse_pair(p, g, device)
                 if not g.is_contiguous():
@@ -160,15 +162,28 @@ class FlexShardAdamW(torch.optim.Optimizer):
                 state = states[p]
                 if not state:
                     state.update(self._new_state(p, bits))
-                m, v = state["exp_avg"], state["exp_avg_sq"]
-                if (m.dtype is torch.uint8) is not (bits == 8):
-                    raise ValueError(f"states of {m.dtype} do not go with state_bits={bits}")
+                m, v, count, numel = state["exp_avg"], state["exp_avg_sq"], state["step"], p.numel()
+                # (they may have been replaced, or the parameter's memory since they were made)
+                nbytes = numel if bits == 8 else 4 * numel
+                if (
+                    m.nbytes != nbytes or v.nbytes != nbytes or not m.is_contiguous() or not v.is_contiguous()
+                    or m.get_device() != index or v.get_device() != index
+                    or count.dtype is not int32 or count.nbytes != 4 or count.get_device() != index
+                ):
+                    _check_state(state, numel, bits, index)
                 m_scale = v_scale = 0
                 if bits == 8:
-                    m_scale, v_scale = state["exp_avg_scale"].data_ptr(), state["exp_avg_sq_scale"].data_ptr()
+                    m_scale, v_scale = state["exp_avg_scale"], state["exp_avg_sq_scale"]
+                    nbytes = 4 * -(-numel // ADAMW_BLOCK)
+                    if (
+                        m_scale.nbytes != nbytes or v_scale.nbytes != nbytes or not m_scale.is_contiguous() or not v_scale.is_contiguous()
+                        or m_scale.get_device() != index or v_scale.get_device() != index
+                    ):
+                        _check_state(state, numel, bits, index)
+                    m_scale, v_scale = m_scale.data_ptr(), v_scale.data_ptr()
                 # (an fsh_adamw_tensor)
                 table += (
-                    p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale, v_scale, state["step"].data_ptr(), p.numel(),
+                    p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), m_scale, v_scale, count.data_ptr(), numel,
                     param_dt, grad_dt, bits, number,
                 )
                 stepped.append(p)
@@ -201,6 +216,20 @@ def _refuse_pair(p: torch.Tensor, g: torch.Tensor, device: torch.device) -> None
     if p.device != device or g.device != device:
         raise ValueError(f"all parameters and gradients of a step must live on {device}, got {p.device} and {g.device}")
     raise ValueError(f"contiguous parameters with gradients of their shape, got {tuple(p.shape)} / {p.stride()} and {tuple(g.shape)}")
+
+
+def _check_state(state: dict[str, torch.Tensor], numel: int, bits: int, index: int) -> None:
+    """That a parameter's states are of its size and on its device, as the kernels take them."""
+    kind = torch.float32 if bits == 32 else torch.uint8
+    wanted = {"step": (torch.int32, 1), "exp_avg": (kind, numel), "exp_avg_sq": (kind, numel)}
+    if bits == 8:
+        wanted |= dict.fromkeys(("exp_avg_scale", "exp_avg_sq_scale"), (torch.float32, -(-numel // ADAMW_BLOCK)))
+    for name, (dtype, count) in wanted.items():
+        t = state[name]
+        if t.dtype != dtype or t.numel() != count or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError(
+                f"{bits}-bit states need {name} as {count} contiguous {dtype} where the parameter is, got {t.dtype} {tuple(t.shape)} on {t.device}"
+            )
 
 
 def _learning_rate(lr: torch.Tensor, device: torch.device) -> tuple[float, int | None]:

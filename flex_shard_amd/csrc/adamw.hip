@@ -30,6 +30,10 @@
 // What is an infinity or not a number makes the whole block not a number.
 #include "rows.hpp"
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 namespace fsh {
 namespace {
 
@@ -528,6 +532,26 @@ int square_launches(const int64_t* tensors, int32_t count, Each each) {
   return launches;
 }
 
+// Whether two tensors of a step share memory of their parameters or a step count (one
+// that is listed twice, say): their updates would race.  -1 without memory for the list.
+int tensors_overlap(const fsh_adamw_tensor* tensors, int32_t count) {
+  struct Span {
+    uintptr_t begin, end;
+  };
+  std::unique_ptr<Span[]> spans(new (std::nothrow) Span[2 * static_cast<size_t>(count)]);
+  if (!spans) return -1;
+  size_t n = 0;
+  for (int32_t i = 0; i < count; ++i) {
+    const uintptr_t step = reinterpret_cast<uintptr_t>(tensors[i].step_dev), param = reinterpret_cast<uintptr_t>(tensors[i].param_dev);
+    spans[n++] = {step, step + sizeof(int32_t)};
+    if (tensors[i].numel) spans[n++] = {param, param + static_cast<uintptr_t>(tensors[i].numel) * bytes_of(static_cast<int>(tensors[i].param_dtype))};
+  }
+  std::sort(spans.get(), spans.get() + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < n; ++i)
+    if (spans[i].begin < spans[i - 1].end) return 1;
+  return 0;
+}
+
 template <int PT, int GT>
 void launch_step(const AdamTable& a, bool eight, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(a.chunks < kMaxGrid ? a.chunks : kMaxGrid)), block(kThreads);
@@ -631,6 +655,9 @@ FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const
       return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
     if (ceil_div(t.numel, (int64_t)chunk_of(t.state_bits == 8)) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
   }
+  if (const int overlap = tensors_overlap(tensors, count))
+    return overlap < 0 ? fail(FSH_ENOTSUP, "%s: no host memory for %d tensors", who, count)
+                       : fail(FSH_EINVAL, "%s: two tensors overlap, or share a step count", who);
   const hipStream_t on = static_cast<hipStream_t>(stream);
   StepFactors* const factors = static_cast<StepFactors*>(workspace_dev);
   for (int32_t begin = 0; begin < count; begin += kFactorTensors) {

@@ -8,7 +8,7 @@ import torch
 from adamw_definition import FIRST, SECOND, decode, dither, encode
 
 from flex_shard_amd import _native
-from flex_shard_amd.adamw import FlexShardAdamW, grad_square_sum
+from flex_shard_amd.adamw import FlexShardAdamW, _check_state, grad_square_sum
 
 OK, EINVAL, ENOTSUP = 0, -22, -95
 SOMEWHERE = 1 << 20  # an aligned address that no refused call touches
@@ -151,3 +151,44 @@ def test_the_dither_is_uniform():
         assert abs(u.mean().item() - 0.5) < 5 / (12 * count) ** 0.5
         bins = torch.histc(u, 64, 0, 1)
         assert (bins - count / 64).abs().max() < 5 * (count / 64) ** 0.5
+
+
+def test_tensors_that_overlap():
+    """A parameter that is listed twice, one inside another, a shared step count: refused before anything is queued."""
+    groups = (_native.AdamWGroup * 1)((1e-3, None, 0.9, 0.95, 1e-8, 0.1))
+
+    def call(*tensors):  # (param, step, elements, dtype)
+        rows = [(param, 1 << 40, 2 << 40, 3 << 40, 4 << 40, 5 << 40, step, n, dtype, _native.DT_F32, 32, 0) for param, step, n, dtype in tensors]
+        return _native.lib().fsh_adamw_step(_table(*(v for row in rows for v in row)), len(rows), groups, 1, None, 0.0, 6 << 40, 1 << 20, None)
+
+    far, steps = 1 << 30, 7 << 40
+    for tensors in (
+        ((SOMEWHERE, steps, 8, 1), (SOMEWHERE, steps + 4, 8, 1)),
+        ((SOMEWHERE + 28, steps, 8, 1), (far, steps + 4, 8, 1), (SOMEWHERE, steps + 8, 8, 1)),
+        ((SOMEWHERE, steps, 8, 0), (SOMEWHERE + 14, steps + 4, 1, 0)),
+        ((SOMEWHERE, steps, 8, 1), (far, steps, 8, 1)),
+        ((SOMEWHERE, steps, 0, 1), (far, steps, 0, 1)),
+    ):
+        assert call(*tensors) == EINVAL and "overlap" in _message(), tensors
+
+
+def test_states_of_another_size_or_type():
+    def state(**changed):
+        return dict(
+            step=torch.zeros((), dtype=torch.int32), exp_avg=torch.zeros(300, dtype=torch.uint8), exp_avg_sq=torch.zeros(300, dtype=torch.uint8),
+            exp_avg_scale=torch.zeros(3), exp_avg_sq_scale=torch.zeros(3),
+        ) | changed
+
+    _check_state(state(), 300, 8, -1)  # (-1: on the CPU)
+    _check_state(dict(step=torch.zeros((), dtype=torch.int32), exp_avg=torch.zeros(20, 15), exp_avg_sq=torch.zeros(20, 15)), 300, 32, -1)
+    for name, value in (
+        ("step", torch.zeros(())), ("exp_avg", torch.zeros(299, dtype=torch.uint8)), ("exp_avg", torch.zeros(300)),
+        ("exp_avg_sq", torch.zeros(600, dtype=torch.uint8)[::2]), ("exp_avg_scale", torch.zeros(2)),
+        ("exp_avg_sq_scale", torch.zeros(3, dtype=torch.float64)),
+    ):
+        with pytest.raises(ValueError, match=name):
+            _check_state(state(**{name: value}), 300, 8, -1)
+    with pytest.raises(ValueError, match="exp_avg"):
+        _check_state(state(), 300, 32, -1)
+    with pytest.raises(ValueError, match="step"):
+        _check_state(state(), 300, 8, 0)

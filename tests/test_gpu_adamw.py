@@ -469,3 +469,33 @@ def test_refusals():
         grad_square_sum([torch.zeros(3)])
     with pytest.raises(KeyError):
         optimizer.state_values(p)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replaced_states_and_parameters_listed_twice(bits):
+    p = torch.nn.Parameter(torch.zeros(300, device="cuda"))
+    p.grad = torch.ones(300, device="cuda")
+    optimizer = FlexShardAdamW([p], state_bits=bits)
+    optimizer.step()
+    before = p.detach().clone()
+    state = dict(optimizer.state[p])
+    for name, kept in state.items():
+        for other in (kept.double(), kept.cpu(), kept.reshape(-1)[:0]):
+            optimizer.state[p][name] = other
+            with pytest.raises(ValueError, match=name):
+                optimizer.step()
+        optimizer.state[p][name] = kept
+    p.data = torch.zeros(400, device="cuda")  # a parameter that has grown
+    p.grad = torch.ones(400, device="cuda")
+    with pytest.raises(ValueError, match="exp_avg"):
+        optimizer.step()
+    whole = torch.zeros(300, device="cuda")
+    parts = [torch.nn.Parameter(whole), torch.nn.Parameter(whole[100:200])]
+    for t in parts:
+        t.grad = torch.ones_like(t)
+    with pytest.raises(RuntimeError, match="overlap"):
+        FlexShardAdamW(parts, state_bits=bits).step()
+    assert before.any() and not p.any() and not whole.any()
+    values = optimizer.state_values(p)
+    values[0].zero_()  # (a copy)
+    assert optimizer.state_values(p)[0].any()
