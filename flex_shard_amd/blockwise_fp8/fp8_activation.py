@@ -19,7 +19,7 @@ class Fp8Activation:
     shape without values of its own, through which the linears' gradients reach what
     made the activation, unrounded by the quantizer (straight through)."""
 
-    __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_runs")
+    __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_runs", "_captured")
 
     def __init__(
         self, q: torch.Tensor, scales: torch.Tensor, carrier: torch.Tensor,
@@ -31,6 +31,7 @@ class Fp8Activation:
         self.carrier = carrier
         self._make_runs = make_token_runs
         self._runs: tuple | None = None
+        self._captured = torch.cuda.is_current_stream_capturing()
 
     @property
     def ndim(self) -> int:
@@ -43,7 +44,10 @@ class Fp8Activation:
     def token_runs(self) -> tuple[torch.Tensor, torch.Tensor]:
         """The activation in runs of 128 tokens, transposed, with its scales: what a
         weight gradient contracts over.  Made when the first linear asks for it, for
-        all that do so on the same stream."""
+        all that do so on the same stream (but anew for a capture that the activation
+        is not part of: a graph's memory holds nothing before its first replay)."""
+        if torch.cuda.is_current_stream_capturing() != self._captured:
+            return self._make_runs()
         stream = hip_ops.stream_ptr(self.q.device)
         if self._runs is None or self._runs[0] != stream:
             self._runs = (stream, self._make_runs())

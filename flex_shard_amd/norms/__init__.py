@@ -68,12 +68,7 @@ class _Norm(torch.autograd.Function):
             kept += (*out, normed, rstd)
             out = _carrier(x.shape, x.device)
         ctx.save_for_backward(normed, weight, rstd)
-        # what the backward's thread need not find out again
-        cols, types, x_dtype = x.shape[-1], hip_ops.FLOAT_CODES, x.dtype
-        ctx.call = (
-            x_dtype, x.numel() // cols, cols, cols if normed.is_contiguous() else normed.stride(0),
-            (types[out.dtype], types[normed.dtype], types[x_dtype], 0 if weight is None else types[weight.dtype]),
-        )
+        ctx.x_dtype = x.dtype
         ctx.set_materialize_grads(False)
         return out, total
 
@@ -84,22 +79,16 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm_backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
-    x_dtype, rows, cols, ldh, codes = ctx.call
     needs_x, needs_residual, needs_weight, _, _ = ctx.needs_input_grad
     if grad is None:  # the stream alone was used
         if grad_total is None:
             return None, None, None, None, None
-        return grad_total.to(x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
+        return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
+    # (hooks on saved tensors may give back others than were kept, so that these are checked like any)
     normed, weight, rstd = ctx.saved_tensors
-    ldg = ldt = cols
-    if not grad.is_contiguous():
-        grad = _as_rows(grad)
-        ldg = cols if grad.is_contiguous() else grad.stride(0)
-    if grad_total is not None and not grad_total.is_contiguous():
-        grad_total = _as_rows(grad_total)
-        ldt = cols if grad_total.is_contiguous() else grad_total.stride(0)
-    grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward_checked(
-        grad, normed, weight, rstd, x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
+    grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward(
+        _as_rows(grad), _as_rows(normed), weight, rstd, ctx.x_dtype, None if grad_total is None else _as_rows(grad_total),
+        needs_x=needs_x, needs_residual=needs_residual, needs_weight=needs_weight,
     )
     return grad_x, grad_residual, grad_weight, None, None
 
@@ -129,12 +118,12 @@ def rms_norm(
     return y if residual is None else (y, total)
 
 
-def _version(t: torch.Tensor) -> int:
-    return 0 if t.is_inference() else t._version
+def _version(t: torch.Tensor | None) -> int:
+    return 0 if t is None or t.is_inference() else t._version
 
 
-def _token_runs(normed, version: int, weight, rstd) -> tuple[torch.Tensor, torch.Tensor]:
-    if _version(normed) != version:
+def _token_runs(normed, weight, rstd, versions: tuple[int, int]) -> tuple[torch.Tensor, torch.Tensor]:
+    if versions != (_version(normed), _version(weight)):
         raise RuntimeError("what an 8-bit norm was made of was changed in place before a weight gradient's form of it was made")
     return hip_ops.rms_norm_token_runs(normed, weight, rstd)
 
@@ -163,7 +152,7 @@ def rms_norm_fp8(
         # The token runs are made when a linear asks for them, and by then the weight's
         # bucket may be resharded, or an optimizer have been at it.
         weight = weight.detach().clone()
-    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, _version(normed), weight, rstd))
+    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, weight, rstd, (_version(normed), _version(weight))))
     return activation if residual is None else (activation, total)
 
 

@@ -350,3 +350,22 @@ def test_refusals():
         torch.autograd.grad(d.sum(), leaf)
     with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
         rms_norm(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)), w)
+
+
+def test_saved_tensors_that_come_back_otherwise():
+    """Strided rows that a hook keeps on the host come back contiguous; what stays there is refused."""
+    x, residual, w, gen = _make(20, 200, BF16, BF16)
+    g = torch.randn(20, 200, generator=gen, device="cuda").to(BF16)
+    wide = torch.zeros(20, 500, dtype=BF16, device="cuda")
+    wide[:, 11:211] = x.detach()
+    rows, weight = wide[:, 11:211].requires_grad_(), w.detach().clone().requires_grad_()
+    want = torch.autograd.grad(rms_norm(rows, weight, EPS), (rows, weight), g)
+    with torch.autograd.graph.save_on_cpu():
+        y = rms_norm(rows, weight, EPS)
+    for a, b in zip(torch.autograd.grad(y, (rows, weight), g), want):
+        assert torch.equal(a, b)
+    for back in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten()[:-1]):
+        with torch.autograd.graph.saved_tensors_hooks(back, lambda t: t):
+            y = rms_norm(rows, weight, EPS)
+        with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
+            torch.autograd.grad(y, (rows, weight), g)

@@ -214,3 +214,44 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, once()))
+
+
+def test_made_eagerly_and_read_by_two_graphs():
+    """Neither graph may rely on token runs that the other one makes, nor eager work on either's."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    weight = _weight(256, 384, gen)
+    x = torch.randn(60, 384, generator=gen, device="cuda").to(BF16)
+    g = torch.randn(60, 256, generator=gen, device="cuda").to(BF16)
+    a = rms_norm_fp8(x, torch.ones(384, device="cuda"), EPS)
+
+    def once(activation):
+        return torch.autograd.grad(prequantized_linear(activation, weight), weight, g)[0]
+
+    want = once(rms_norm_fp8(x, torch.ones(384, device="cuda"), EPS))
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(once(a))
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], want) and torch.equal(once(a), want)
+    for _ in range(3):
+        outs[0].zero_()
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want)
+
+
+def test_weight_changed_before_the_token_runs():
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn(9, 256, generator=gen, device="cuda").to(BF16)
+    w = torch.ones(256, device="cuda")
+    kept = rms_norm_fp8(x, w, EPS)
+    with torch.no_grad():  # (no copy of the weight is kept)
+        unkept = rms_norm_fp8(x, w, EPS)
+    want = [t.clone() for t in rms_norm_fp8(x, w.clone(), EPS).token_runs()]
+    w.mul_(2)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kept.token_runs(), want))
+    with pytest.raises(RuntimeError, match="in place"):
+        unkept.token_runs()
