@@ -52,28 +52,15 @@ are left alone; two that overlap are refused."""
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
         try:
-            beta1, beta2 = group["betas"]
-            if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
-                raise ValueError(f"betas must be in [0, 1), got {group['betas']}")
-            for name in ("eps", "weight_decay"):
-                if not group[name] >= 0:
-                    raise ValueError(f"{name} must not be negative, got {group[name]}")
-            if not isinstance(group["lr"], torch.Tensor) and not group["lr"] >= 0:
-                raise ValueError(f"lr must not be negative, got {group['lr']}")
-            if group["state_bits"] not in (8, 32):
-                raise NotImplementedError(f"states have 8 or 32 bits, got {group['state_bits']}")
-            for p in group["params"]:
-                if p.dtype not in _DT:
-                    raise NotImplementedError(f"the AdamW kernels update bf16 or fp32 parameters, got {p.dtype}")
+            _check_group(self.param_groups[-1])
         except Exception:
             self.param_groups.pop()
             raise
 
     # ------------------------------------------------------------------- states
     def _new_state(self, p: torch.Tensor, bits: int) -> dict[str, torch.Tensor]:
-        if torch.cuda.is_current_stream_capturing():
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
             # the zeros would be part of the graph, and every replay would begin with them
             raise RuntimeError("the states of an AdamW step must exist before it is captured: run one step, or load them")
         blocks = -(-p.numel() // ADAMW_BLOCK)
@@ -98,15 +85,23 @@ are left alone; two that overlap are refused."""
 
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
         """Copies of the saved states, of the types that they have here (``torch``'s
-        own loading would cast them to the parameters')."""
-        saved_groups = state_dict["param_groups"]
+        own loading would cast them to the parameters').  Groups that name no ``state_bits``, ``torch``'s own
+        AdamW's, have 32."""
+        groups = []
+        for group in state_dict["param_groups"]:
+            group = {"state_bits": 32, **group}
+            for option in ("amsgrad", "maximize"):
+                if group.get(option):
+                    raise NotImplementedError(f"the AdamW kernels have no {option}")
+            _check_group({**group, "params": ()})
+            groups.append(group)
         loaded = {}
-        if [len(g["params"]) for g in saved_groups] == [len(g["params"]) for g in self.param_groups]:
-            for group, saved in zip(self.param_groups, saved_groups):
+        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:
+            for group, saved in zip(self.param_groups, groups):
                 for p, index in zip(group["params"], saved["params"]):
                     if index in state_dict["state"]:
-                        loaded[p] = self._copy_of(p, saved.get("state_bits", 32), state_dict["state"][index])
-        super().load_state_dict({**state_dict, "state": {}})
+                        loaded[p] = self._copy_of(p, saved["state_bits"], state_dict["state"][index])
+        super().load_state_dict({**state_dict, "param_groups": groups, "state": {}})
         self.state.update(loaded)
 
     def _copy_of(self, p: torch.Tensor, bits: int, saved: dict[str, Any]) -> dict[str, torch.Tensor]:
@@ -200,6 +195,22 @@ are left alone; two that overlap are refused."""
         if stepped:
             torch.autograd.graph.increment_version(stepped)
         return loss
+
+
+def _check_group(group: dict[str, Any]) -> None:
+    beta1, beta2 = group["betas"]
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1):
+        raise ValueError(f"betas must be in [0, 1), got {group['betas']}")
+    for name in ("eps", "weight_decay"):
+        if not group[name] >= 0:
+            raise ValueError(f"{name} must not be negative, got {group[name]}")
+    if not isinstance(group["lr"], torch.Tensor) and not group["lr"] >= 0:
+        raise ValueError(f"lr must not be negative, got {group['lr']}")
+    if group["state_bits"] not in (8, 32):
+        raise NotImplementedError(f"states have 8 or 32 bits, got {group['state_bits']}")
+    for p in group["params"]:
+        if p.dtype not in _DT:
+            raise NotImplementedError(f"the AdamW kernels update bf16 or fp32 parameters, got {p.dtype}")
 
 
 def _check_sum(square_sum: torch.Tensor | None, device: torch.device) -> None:

@@ -31,7 +31,7 @@ class Fp8Activation:
         self.carrier = carrier
         self._make_runs = make_token_runs
         self._runs: tuple | None = None
-        self._captured = torch.cuda.is_current_stream_capturing()
+        self._captured = q.is_cuda and torch.cuda.is_current_stream_capturing()
 
     @property
     def ndim(self) -> int:

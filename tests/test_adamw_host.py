@@ -192,3 +192,26 @@ def test_states_of_another_size_or_type():
         _check_state(state(), 300, 32, -1)
     with pytest.raises(ValueError, match="step"):
         _check_state(state(), 300, 8, 0)
+
+
+def test_states_of_torchs_own_are_loaded():
+    p = torch.nn.Parameter(torch.ones(5))
+    p.grad = torch.arange(5.0)
+    for options in ({}, {"amsgrad": True}, {"maximize": True}):
+        its = torch.optim.AdamW([p], lr=0.1, **options)
+        its.step()
+        mine = FlexShardAdamW([torch.nn.Parameter(torch.ones(5))], lr=0.5, state_bits=8)
+        if options:
+            with pytest.raises(NotImplementedError, match=next(iter(options))):
+                mine.load_state_dict(its.state_dict())
+            assert mine.param_groups[0]["state_bits"] == 8 and not mine.state
+            continue
+        mine.load_state_dict(its.state_dict())
+        group = mine.param_groups[0]
+        assert group["lr"] == 0.1 and group["state_bits"] == 32 and "state_bits" not in its.state_dict()["param_groups"][0]
+        state = mine.state[group["params"][0]]
+        assert torch.equal(state["exp_avg"], its.state[p]["exp_avg"]) and int(state["step"]) == 1 and state["step"].dtype == torch.int32
+    bad = mine.state_dict()
+    bad["param_groups"][0]["betas"] = (0.9, 1.0)
+    with pytest.raises(ValueError, match="betas"):
+        mine.load_state_dict(bad)

@@ -499,3 +499,23 @@ def test_replaced_states_and_parameters_listed_twice(bits):
     values = optimizer.state_values(p)
     values[0].zero_()  # (a copy)
     assert optimizer.state_values(p)[0].any()
+
+
+def test_more_tensors_than_a_table_holds():
+    """300 tensors: two launches of the factors, five of the steps, two of the sums."""
+    gen = _gen(21)
+    params = _params([(40 + i,) for i in range(300)], F32, gen)
+    _set_grads(params, BF16, gen)
+    total = grad_square_sum([p.grad for p in params])
+    want = sum(p.grad.double().square().sum() for p in params)
+    assert abs(total / want - 1) < 1e-12  # (sums of some 57000 squares in 64 bits)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    for p, q in zip(params, twins):
+        q.grad_dtype = None  # (any type)
+        q.grad = p.grad.clone()
+    optimizer = FlexShardAdamW(params, **HYPER)
+    optimizer.step(square_sum=total, max_norm=0.5)
+    for q in twins:
+        FlexShardAdamW([q], **HYPER).step(square_sum=total, max_norm=0.5)
+    assert all(torch.equal(p, q) for p, q in zip(params, twins))
+    assert all(int(optimizer.state[p]["step"]) == 1 for p in params)
