@@ -10,8 +10,8 @@
 //
 // Bound by memory: everything is read once and written once, 22 bytes an element
 // (bf16 parameters and gradients, 32-bit states), 10 1/8 with 8-bit states.  218 M
-// parameters: 756 us, 6.3 TB/s, and fp32 with 8-bit states 593, 5.9; bf16 with those 430, 5.1, half
-// of it instructions.  The tensors of a launch come with its arguments, so that nothing is uploaded and a
+// parameters: 756 us, 6.3 TB/s, and fp32 with 8-bit states 550 to 595, 5.9 to 6.4; bf16 with those
+// 405, 5.4, half of it instructions.  The tensors of a launch come with its arguments, so that nothing is uploaded and a
 // captured launch keeps its own table; what a step's number and learning rate make of the
 // hyperparameters is worked out once for each tensor, by a launch of a single workgroup ahead (4.6 us).
 //
@@ -170,14 +170,14 @@ __device__ __forceinline__ uint32_t dither(uint32_t multiple) {
   return z ^ (z >> 15);
 }
 
-template <bool kSmall>
-__device__ __forceinline__ void codes_of(const float (&m)[4], const float (&v)[4], uint32_t multiple, uint32_t& mc, uint32_t& vc) {
-  mc = vc = 0;
+template <bool kSmall, int VEC>
+__device__ __forceinline__ void codes_of(const float (&m)[VEC], const float (&v)[VEC], uint32_t multiple, uint32_t (&mc)[VEC / 4], uint32_t (&vc)[VEC / 4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < VEC; ++j) {
     const uint32_t u = dither(multiple + static_cast<uint32_t>(j) * kOverElements);
-    mc |= first_code<kSmall>(m[j], u & 0xFFFFu) << (8 * j);
-    vc |= second_code<kSmall>(v[j], u >> 16) << (8 * j);
+    const uint32_t first = first_code<kSmall>(m[j], u & 0xFFFFu) << (8 * (j % 4)), second = second_code<kSmall>(v[j], u >> 16) << (8 * (j % 4));
+    mc[j / 4] = j % 4 ? mc[j / 4] | first : first;
+    vc[j / 4] = j % 4 ? vc[j / 4] | second : second;
   }
 }
 
@@ -193,20 +193,24 @@ __device__ __forceinline__ float block_scale(uint32_t largest, float& inverse) {
 // --------------------------------------------------------------------- the step
 // A workgroup takes a chunk: vectors of four neighbours a thread, the loads of all
 // of them requested first.  With 32-bit states one vector, with 8-bit ones, where instructions
-// count and what is done once per chunk is spread, four (218 M parameters, us with one, two
-// and four: bf16 and 32 bits 768, 855, 820; bf16 and 8 bits, with a division for each moment, 535, 490,
-// 470; fp32 and 8 bits 600 each).
+// count and what is done once per chunk is spread, 16 elements (218 M parameters, us with 4, 8
+// and 16: bf16 and 32 bits 768, 855, 820; with 8 bits 16 and 32 elements, after 8: bf16 420, 405, 420, fp32 595, 595, 615).
 // Everything streams: through the caches the 32-bit step takes 919 us, and workgroups that stay for more chunks than
 // one are slower still (2048 of them: 1049).
 constexpr int chunk_of(bool eight) { return (eight ? 4 : 1) * 4 * kThreads; }
 
+// Neighbours in a vector: eight of bf16 parameters with 8-bit states, which makes a block a
+// row of 16 lanes and halves what is done once a block (428 us for 405 with four; fp32 parameters, whose
+// vectors would be two loads: 595 with four, 720 with eight).
+constexpr int vector_of(int param_dtype, bool eight) { return eight && param_dtype == FSH_DT_BF16 ? 8 : 4; }
+
 // What a vector's step reads.
-template <int PT, int GT, bool kEight>
+template <int PT, int GT, bool kEight, int VEC>
 struct StepInput {
-  RawVec<PT, 4> p;
-  RawVec<GT, 4> g;
-  RawVec<FSH_DT_F32, 4> m, v;
-  uint32_t mc, vc;
+  RawVec<PT, VEC> p;
+  RawVec<GT, VEC> g;
+  RawVec<FSH_DT_F32, VEC> m, v;
+  uint32_t mc[VEC / 4], vc[VEC / 4];
   float ms, vs;
 };
 
@@ -220,62 +224,66 @@ struct ChunkOf {
   float* v_scale;
 };
 
-// Up to four codes, the others zero.
-template <bool kFull>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* src, int count) {
-  uint32_t c = 0;
-  if (kFull || count >= 4) {
-    __builtin_memcpy(&c, src, 4);
+// Up to VEC codes, the others zero.
+template <bool kFull, int WORDS>
+__device__ __forceinline__ void load_codes(const uint8_t* src, int count, uint32_t (&c)[WORDS]) {
+  if (kFull || count >= 4 * WORDS) {
+    __builtin_memcpy(c, src, sizeof(c));
   } else {
-    for (int j = 0; j < count; ++j) c |= static_cast<uint32_t>(src[j]) << (8 * j);
+#pragma unroll
+    for (int j = 0; j < 4 * WORDS; ++j) {
+      const uint32_t code = j < count ? src[j] : 0u;
+      c[j / 4] = j % 4 ? c[j / 4] | code << (8 * (j % 4)) : code;
+    }
   }
-  return c;
 }
-template <bool kFull>
-__device__ __forceinline__ void store_codes(uint8_t* dst, int count, uint32_t c) {
-  if (kFull || count >= 4) {
-    __builtin_memcpy(dst, &c, 4);
+template <bool kFull, int WORDS>
+__device__ __forceinline__ void store_codes(uint8_t* dst, int count, const uint32_t (&c)[WORDS]) {
+  if (kFull || count >= 4 * WORDS) {
+    __builtin_memcpy(dst, c, sizeof(c));
   } else {
-    for (int j = 0; j < count; ++j) dst[j] = static_cast<uint8_t>(c >> (8 * j));
+#pragma unroll
+    for (int j = 0; j < 4 * WORDS; ++j)
+      if (j < count) dst[j] = static_cast<uint8_t>(c[j / 4] >> (8 * (j % 4)));
   }
 }
 
 // kFull: the chunk ends inside the tensor; `left`: elements from the chunk's first on.
 template <int PT, int GT, bool kEight, bool kFull>
 __device__ __forceinline__ void step_chunk(const ChunkOf& c, const StepFactors& f, uint32_t first_index, int left) {
-  constexpr int kVectors = chunk_of(kEight) / (4 * kThreads);
-  StepInput<PT, GT, kEight> in[kVectors];
+  constexpr int VEC = vector_of(PT, kEight), kVectors = chunk_of(kEight) / (VEC * kThreads);
+  StepInput<PT, GT, kEight, VEC> in[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * 4;
-    const int count = kFull ? 4 : left - at;
-    in[i].p = load_vec<PT, 4, true>(c.param, at, count);
-    in[i].g = load_vec<GT, 4, true>(c.grad, at, count);
+    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * VEC;
+    const int count = kFull ? VEC : left - at;
+    in[i].p = load_vec<PT, VEC, true>(c.param, at, count);
+    in[i].g = load_vec<GT, VEC, true>(c.grad, at, count);
     if constexpr (kEight) {
-      in[i].mc = load_codes<kFull>(c.m + at, count);
-      in[i].vc = load_codes<kFull>(c.v + at, count);
+      load_codes<kFull>(c.m + at, count, in[i].mc);
+      load_codes<kFull>(c.v + at, count, in[i].vc);
       in[i].ms = count > 0 ? c.m_scale[at / kStateBlock] : 0.0f;
       in[i].vs = count > 0 ? c.v_scale[at / kStateBlock] : 0.0f;
     } else {
-      in[i].m = load_vec<FSH_DT_F32, 4, true>(c.m, at, count);
-      in[i].v = load_vec<FSH_DT_F32, 4, true>(c.v, at, count);
+      in[i].m = load_vec<FSH_DT_F32, VEC, true>(c.m, at, count);
+      in[i].v = load_vec<FSH_DT_F32, VEC, true>(c.v, at, count);
     }
   }
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * 4;
-    const int count = kFull ? 4 : left - at;
-    float m[4], v[4], p[4];
+    const int at = (i * kThreads + static_cast<int>(threadIdx.x)) * VEC;
+    const int count = kFull ? VEC : left - at;
+    float m[VEC], v[VEC], p[VEC];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < VEC; ++j) {
       if constexpr (kEight) {
-        m[j] = first_value((in[i].mc >> (8 * j)) & 255u) * in[i].ms;
-        v[j] = second_value((in[i].vc >> (8 * j)) & 255u) * in[i].vs;
+        m[j] = first_value((in[i].mc[j / 4] >> (8 * (j % 4))) & 255u) * in[i].ms;
+        v[j] = second_value((in[i].vc[j / 4] >> (8 * (j % 4))) & 255u) * in[i].vs;
       } else {
-        m[j] = element<FSH_DT_F32, 4>(in[i].m, j);
-        v[j] = element<FSH_DT_F32, 4>(in[i].v, j);
+        m[j] = element<FSH_DT_F32, VEC>(in[i].m, j);
+        v[j] = element<FSH_DT_F32, VEC>(in[i].v, j);
       }
-      const float g = element<GT, 4>(in[i].g, j) * f.clip;
+      const float g = element<GT, VEC>(in[i].g, j) * f.clip;
       m[j] = m[j] * f.b1 + g * f.one_b1;
       v[j] = v[j] * f.b2 + (g * g) * f.one_b2;
       float update;
@@ -286,49 +294,62 @@ __device__ __forceinline__ void step_chunk(const ChunkOf& c, const StepFactors& 
       } else {
         update = m[j] / (sqrtf(v[j]) * f.root_factor + f.eps);
       }
-      p[j] = element<PT, 4>(in[i].p, j) * f.decay - f.step_size * update;
+      p[j] = element<PT, VEC>(in[i].p, j) * f.decay - f.step_size * update;
     }
-    if (kFull || count > 0) store_vec<PT, 4, true>(c.param, at, count, to_vec<PT, 4>(p));
+    if (kFull || count > 0) store_vec<PT, VEC, true>(c.param, at, count, to_vec<PT, VEC>(p));
     if constexpr (kEight) {
-      // Half a wave has a block; elements behind the tensor's last are zero.
+      // A block is half a wave's, or a row's of 16 lanes; elements behind the tensor's last are zero.
       uint32_t m_max = 0, v_max = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < VEC; ++j) {
         if (!kFull && j >= count) m[j] = v[j] = 0.0f;
         m_max = max(m_max, f32_as_u32(m[j]) & 0x7FFFFFFFu);
         v_max = max(v_max, f32_as_u32(v[j]) & 0x7FFFFFFFu);
       }
-      // Both moments' maxima over each row of 16 lanes; a swap of the first's odd rows
-      // with the second's even ones joins the pairs, the first's in even rows and the second's in
-      // odd ones, so that one division does for both, and another swap hands its results out.
-      const auto pair = __builtin_amdgcn_permlane16_swap(row16_max_u32(m_max), row16_max_u32(v_max), false, false);
-      float inverse;
-      const float scale = block_scale(max(pair[0], pair[1]), inverse);
-      const auto inverses = __builtin_amdgcn_permlane16_swap(f32_as_u32(inverse), f32_as_u32(inverse), false, false);
+      // Both moments' maxima over each row of 16 lanes.  One division does for both: the
+      // first's in even rows and the second's in odd ones, which a swap of the first's odd rows with
+      // the second's even ones gives (and joins the two rows of a block); with a block in a
+      // row, in even and odd lanes.
+      m_max = row16_max_u32(m_max);
+      v_max = row16_max_u32(v_max);
+      float inverse, m_inverse, v_inverse, scale;
+      if constexpr (VEC == 4) {
+        const auto pair = __builtin_amdgcn_permlane16_swap(m_max, v_max, false, false);
+        scale = block_scale(max(pair[0], pair[1]), inverse);
+        const auto inverses = __builtin_amdgcn_permlane16_swap(f32_as_u32(inverse), f32_as_u32(inverse), false, false);
+        m_inverse = u32_as_f32(inverses[0]);
+        v_inverse = u32_as_f32(inverses[1]);
+      } else {
+        scale = block_scale(threadIdx.x & 1 ? v_max : m_max, inverse);
+        const int both = static_cast<int>(f32_as_u32(inverse));
+        m_inverse = u32_as_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, both, 0xA0, 0xF, 0xF, true)));  // quad_perm [0,0,2,2]
+        v_inverse = u32_as_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, both, 0xF5, 0xF, 0xF, true)));  // quad_perm [1,1,3,3]
+      }
       float m_least = 1.0f, v_least = 1.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] *= u32_as_f32(inverses[0]);
-        v[j] *= u32_as_f32(inverses[1]);
+      for (int j = 0; j < VEC; ++j) {
+        m[j] *= m_inverse;
+        v[j] *= v_inverse;
         m_least = fminf(m_least, fabsf(m[j]));
         v_least = fminf(v_least, v[j]);
       }
       const uint32_t multiple = (first_index + static_cast<uint32_t>(at)) * kOverElements + f.t * kOverSteps;
-      uint32_t mc, vc;
-      // (a wave rarely has a value below the smallest code; with this and the one division, bf16
-      // parameters take 430 us for 485)
+      uint32_t mc[VEC / 4], vc[VEC / 4];
+      // (a wave rarely has a value below the smallest code; with this and the one division, in
+      // vectors of four, bf16 parameters took 430 us for 485)
       if (__ballot(m_least < kFirstSmallest || v_least < kSecondSmallest)) codes_of<true>(m, v, multiple, mc, vc);
       else codes_of<false>(m, v, multiple, mc, vc);
       store_codes<kFull>(c.m + at, count, mc);
       store_codes<kFull>(c.v + at, count, vc);
-      // (a block's first lane has its first moment's scale, the sixteenth behind it the second's)
-      if (threadIdx.x % 16 == 0) {
-        const int of = at - (threadIdx.x & 16) * 4;  // the block's first element
-        if (kFull || left > of) (threadIdx.x & 16 ? c.v_scale : c.m_scale)[of / kStateBlock] = scale;
+      // (a block's first lane has its first moment's scale, the sixteenth behind it, or the next, the second's)
+      constexpr int kSecond = VEC == 4 ? 16 : 1;
+      if ((threadIdx.x & (kStateBlock / VEC - 1) & ~kSecond) == 0) {
+        const int of = at - (threadIdx.x & kSecond) * VEC;  // the block's first element
+        if (kFull || left > of) (threadIdx.x & kSecond ? c.v_scale : c.m_scale)[of / kStateBlock] = scale;
       }
     } else if (kFull || count > 0) {
-      store_vec<FSH_DT_F32, 4, true>(c.m, at, count, to_vec<FSH_DT_F32, 4>(m));
-      store_vec<FSH_DT_F32, 4, true>(c.v, at, count, to_vec<FSH_DT_F32, 4>(v));
+      store_vec<FSH_DT_F32, VEC, true>(c.m, at, count, to_vec<FSH_DT_F32, VEC>(m));
+      store_vec<FSH_DT_F32, VEC, true>(c.v, at, count, to_vec<FSH_DT_F32, VEC>(v));
     }
   }
 }
