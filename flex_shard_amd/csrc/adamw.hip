@@ -193,15 +193,15 @@ __device__ __forceinline__ float block_scale(uint32_t largest, float& inverse) {
 // --------------------------------------------------------------------- the step
 // A workgroup takes a chunk: vectors of four neighbours a thread, the loads of all
 // of them requested first.  With 32-bit states one vector, with 8-bit ones, where instructions
-// count and what is done once per chunk is spread, 16 elements (218 M parameters, us with 4, 8
-// and 16: bf16 and 32 bits 768, 855, 820; with 8 bits 16 and 32 elements, after 8: bf16 420, 405, 420, fp32 595, 595, 615).
+// count and what is done once per chunk is spread, 16 elements (218 M parameters, us: bf16 and 32
+// bits with 4, 8 and 16 elements 768, 855, 820; 8 bits with 8, 16 and 32 bf16 420, 405, 420, fp32 590, 595, 615).
 // Everything streams: through the caches the 32-bit step takes 919 us, and workgroups that stay for more chunks than
 // one are slower still (2048 of them: 1049).
 constexpr int chunk_of(bool eight) { return (eight ? 4 : 1) * 4 * kThreads; }
 
 // Neighbours in a vector: eight of bf16 parameters with 8-bit states, which makes a block a
-// row of 16 lanes and halves what is done once a block (428 us for 405 with four; fp32 parameters, whose
-// vectors would be two loads: 595 with four, 720 with eight).
+// row of 16 lanes and halves what is done once a block (405 us; with four 428).  Of fp32 parameters, where
+// eight are two loads of lanes apart, four (595 us; with eight 720).
 constexpr int vector_of(int param_dtype, bool eight) { return eight && param_dtype == FSH_DT_BF16 ? 8 : 4; }
 
 // What a vector's step reads.
