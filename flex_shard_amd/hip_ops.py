@@ -45,7 +45,7 @@ __all__ = [
     "mxfp4_linear", "mxfp4_quantize", "mxfp4_quantize_segments", "newton_schulz_multi", "newton_schulz", "newton_schulz_large_tiles", "newton_schulz_noalloc",
     "newton_schulz_product_tiles",
     "newton_schulz_workspace_bytes", "pack_segments", "quantize_pack", "reduce_rows", "rms_norm", "rms_norm_backward",
-    "rms_norm_token_runs", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
+    "rms_norm_backward_checked", "rms_norm_token_runs", "stream_ptr", "sum_runs", "unpack_dequant", "zero_segments",
 ]
 
 
@@ -1023,6 +1023,7 @@ class MuonStepPlan:
 
 
 _FLOAT_DT = {torch.bfloat16: DT_BF16, torch.float16: DT_F16, torch.float32: DT_F32}
+FLOAT_CODES = _FLOAT_DT  # (of the types that the kernels read and write)
 
 
 def _float_dt(dtype: torch.dtype) -> int:
@@ -1623,10 +1624,22 @@ def rms_norm_backward(
             raise ValueError(f"the gradient of a sum of {dtype} is of that type, got {grad_total.dtype}")
         ldt = _norm_stride("grad_total", grad_total, shape)
         _address("grad_total", grad_total)
-    grad_code, total_code, x_code = _float_dt(grad.dtype), _float_dt(dtype), _float_dt(x_dtype)
-    same = total_code == x_code
+    codes = _float_dt(grad.dtype), _float_dt(dtype), _float_dt(x_dtype), weight_code
+    return rms_norm_backward_checked(
+        grad, total, weight, rstd, x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
+    )
+
+
+def rms_norm_backward_checked(
+    grad: torch.Tensor, total: torch.Tensor, weight: torch.Tensor | None, rstd: torch.Tensor, x_dtype: torch.dtype,
+    grad_total: torch.Tensor | None, sizes: tuple, codes: tuple, needs_x: bool, needs_residual: bool, needs_weight: bool,
+) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """:func:`rms_norm_backward` of operands that are known to belong together.
+    ``sizes``: rows, cols and the row strides of the gradient, of ``total`` and of its
+    gradient; ``codes``: the types of the first two, of x and of the weight."""
+    same = codes[1] == codes[2]
     grad_x = grad_residual = grad_weight = None
-    grad_x_ptr = grad_residual_ptr = grad_weight_ptr = workspace_ptr = nbytes = 0
+    grad_x_ptr = grad_residual_ptr = weight_ptr = grad_weight_ptr = workspace_ptr = nbytes = 0
     if needs_x or (same and needs_residual):
         grad_x = torch.empty_like(total, dtype=x_dtype, memory_format=torch.contiguous_format)
         grad_x_ptr = grad_x.data_ptr()
@@ -1634,15 +1647,16 @@ def rms_norm_backward(
         grad_residual = grad_x if same else torch.empty_like(total, memory_format=torch.contiguous_format)
         if not same:
             grad_residual_ptr = grad_residual.data_ptr()
-    if weight is not None and needs_weight:
-        grad_weight = torch.empty_like(weight)
-        nbytes = _native.lib().fsh_rms_norm_backward_workspace_bytes(rows, cols)
-        workspace = rstd.new_empty((nbytes // 4,))
-        grad_weight_ptr, workspace_ptr = grad_weight.data_ptr(), workspace.data_ptr()
+    if weight is not None:
+        weight_ptr = _address("the norm's weight", weight)
+        if needs_weight:
+            grad_weight = torch.empty_like(weight)
+            nbytes = _native.lib().fsh_rms_norm_backward_workspace_bytes(sizes[0], sizes[1])
+            workspace = rstd.new_empty((nbytes // 4,))
+            grad_weight_ptr, workspace_ptr = grad_weight.data_ptr(), workspace.data_ptr()
     _queue("fsh_rms_norm_backward", total.device, _PACK_NORM_GRADIENT(
         grad.data_ptr(), total.data_ptr(), weight_ptr, rstd.data_ptr(), 0 if grad_total is None else grad_total.data_ptr(),
-        grad_x_ptr, grad_residual_ptr, grad_weight_ptr, workspace_ptr, nbytes, rows, cols, ldg, ldh, ldt,
-        grad_code, total_code, x_code, weight_code,
+        grad_x_ptr, grad_residual_ptr, grad_weight_ptr, workspace_ptr, nbytes, *sizes, *codes,
     ))
     return grad_x if needs_x else None, grad_residual, grad_weight
 

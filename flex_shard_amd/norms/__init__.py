@@ -68,7 +68,11 @@ class _Norm(torch.autograd.Function):
             kept += (*out, normed, rstd)
             out = _carrier(x.shape, x.device)
         ctx.save_for_backward(normed, weight, rstd)
-        ctx.x_dtype = x.dtype
+        # what the backward's thread need not find out again
+        cols, types, x_dtype = x.shape[-1], hip_ops.FLOAT_CODES, x.dtype
+        codes = types[out.dtype], types[normed.dtype], types[x_dtype], 0 if weight is None else types[weight.dtype]
+        ctx.call = x_dtype, x.numel() // cols, cols, codes
+        ctx.kept = x.get_device(), normed.nbytes, normed.dtype, 0 if weight is None else weight.nbytes, None if weight is None else weight.dtype
         ctx.set_materialize_grads(False)
         return out, total
 
@@ -79,16 +83,36 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm_backward(ctx: Any, grad: torch.Tensor | None, grad_total: torch.Tensor | None):
+    x_dtype, rows, cols, codes = ctx.call
     needs_x, needs_residual, needs_weight, _, _ = ctx.needs_input_grad
     if grad is None:  # the stream alone was used
         if grad_total is None:
             return None, None, None, None, None
-        return grad_total.to(ctx.x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
-    # (hooks on saved tensors may give back others than were kept, so that these are checked like any)
+        return grad_total.to(x_dtype) if needs_x else None, grad_total if needs_residual else None, None, None, None
     normed, weight, rstd = ctx.saved_tensors
-    grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward(
-        _as_rows(grad), _as_rows(normed), weight, rstd, ctx.x_dtype, None if grad_total is None else _as_rows(grad_total),
-        needs_x=needs_x, needs_residual=needs_residual, needs_weight=needs_weight,
+    ldg = ldh = ldt = cols
+    if not grad.is_contiguous():
+        grad = _as_rows(grad)
+        ldg = cols if grad.is_contiguous() else grad.stride(0)
+    if not normed.is_contiguous():
+        normed = _as_rows(normed) if normed.shape[-1] == cols else normed.contiguous()
+        ldh = cols if normed.is_contiguous() else normed.stride(0)
+    if grad_total is not None and not grad_total.is_contiguous():
+        grad_total = _as_rows(grad_total)
+        ldt = cols if grad_total.is_contiguous() else grad_total.stride(0)
+    # (autograd answers for the gradients; hooks on saved tensors may give back others than were kept)
+    index, nbytes, dtype, weight_nbytes, weight_dtype = ctx.kept
+    if (
+        normed.get_device() != index or normed.nbytes != nbytes or normed.dtype is not dtype or rstd.get_device() != index
+        or rstd.dtype is not torch.float32 or rstd.nbytes != 4 * rows or not rstd.is_contiguous()
+    ) or (
+        weight is not None and (
+            weight.get_device() != index or weight.nbytes != weight_nbytes or weight.dtype is not weight_dtype or not weight.is_contiguous()
+        )
+    ):
+        raise RuntimeError("a hook on saved tensors gave back other tensors than the norm kept")
+    grad_x, grad_residual, grad_weight = hip_ops.rms_norm_backward_checked(
+        grad, normed, weight, rstd, x_dtype, grad_total, (rows, cols, ldg, ldh, ldt), codes, needs_x, needs_residual, needs_weight
     )
     return grad_x, grad_residual, grad_weight, None, None
 
