@@ -17,7 +17,8 @@ class Fp8Activation:
     ``FlexShardFloat8BlockwiseLinear`` and ``prequantized_linear`` take one in place of
     an activation.  ``carrier`` stands for it in autograd: a bf16 tensor of that
     shape without values of its own, through which the linears' gradients reach what
-    made the activation, unrounded by the quantizer (straight through)."""
+    made the activation, unrounded by the quantizer (straight through).  (Reentrant
+    checkpointing sees tensors alone: make and read one inside the same region, or hand on ``dequantize()``.)"""
 
     __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_runs", "_captured")
 

@@ -255,3 +255,40 @@ def test_weight_changed_before_the_token_runs():
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(kept.token_runs(), want))
     with pytest.raises(RuntimeError, match="in place"):
         unkept.token_runs()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_in_the_backward(reentrant):
+    """A checkpointed norm and its linear: the gradients of a run without one."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    weight = _weight(256, 384, gen)
+    x = torch.randn(60, 384, generator=gen, device="cuda").to(BF16).requires_grad_()
+    w = torch.ones(384, device="cuda", requires_grad=True)
+    g = torch.randn(60, 256, generator=gen, device="cuda").to(BF16)
+
+    def block(x):
+        a, total = rms_norm_fp8(x, w, EPS, residual=x)
+        return prequantized_linear(a, weight), total
+
+    def grads(run):
+        for leaf in (x, w, weight):
+            leaf.grad = None
+        out, total = run(x)
+        torch.autograd.backward([out, total], [g, total.detach()])
+        return [leaf.grad for leaf in (x, w, weight)]
+
+    want = grads(block)
+    got = grads(lambda x: torch.utils.checkpoint.checkpoint(block, x, use_reentrant=reentrant))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_made_in_a_checkpoint_and_read_behind_it():
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    weight = _weight(256, 384, gen)
+    x = torch.randn(60, 384, generator=gen, device="cuda").to(BF16).requires_grad_()
+    w = torch.ones(384, device="cuda", requires_grad=True)
+    g = torch.randn(60, 256, generator=gen, device="cuda").to(BF16)
+    want = torch.autograd.grad(prequantized_linear(rms_norm_fp8(x, w, EPS), weight), (x, w, weight), g)
+    a = torch.utils.checkpoint.checkpoint(rms_norm_fp8, x, w, EPS, use_reentrant=False)
+    got = torch.autograd.grad(prequantized_linear(a, weight), (x, w, weight), g)
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
