@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from typing import Any, Callable
+from typing import Any, Callable, Sequence
 
 import torch
 
@@ -20,17 +20,18 @@ class Fp8Activation:
     made the activation, unrounded by the quantizer (straight through).  (Reentrant
     checkpointing sees tensors alone: make and read one inside the same region, or hand on ``dequantize()``.)"""
 
-    __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_runs", "_captured")
+    __slots__ = ("q", "scales", "shape", "carrier", "_make_runs", "_sources", "_runs", "_captured")
 
     def __init__(
         self, q: torch.Tensor, scales: torch.Tensor, carrier: torch.Tensor,
-        make_token_runs: Callable[[], tuple[torch.Tensor, torch.Tensor]],
+        make_token_runs: Callable[[], tuple[torch.Tensor, torch.Tensor]], sources: Sequence[torch.Tensor] = (),
     ) -> None:
         self.q = q
         self.scales = scales
         self.shape = carrier.shape
         self.carrier = carrier
         self._make_runs = make_token_runs
+        self._sources = sources  # (what that reads)
         self._runs: tuple | None = None
         self._captured = q.is_cuda and torch.cuda.is_current_stream_capturing()
 
@@ -53,6 +54,11 @@ class Fp8Activation:
         if self._runs is None or self._runs[0] != stream:
             self._runs = (stream, self._make_runs())
         return self._runs[1]
+
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """As for a tensor: what work on ``stream`` reads is not reused before that work is done."""
+        for t in (self.q, self.scales, *self._sources):
+            t.record_stream(stream)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, differentiable straight through the quantizer."""

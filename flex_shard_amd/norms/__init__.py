@@ -176,7 +176,10 @@ def rms_norm_fp8(
         # The token runs are made when a linear asks for them, and by then the weight's
         # bucket may be resharded, or an optimizer have been at it.
         weight = weight.detach().clone()
-    activation = Fp8Activation(q, scales, carrier, partial(_token_runs, normed, weight, rstd, (_version(normed), _version(weight))))
+    activation = Fp8Activation(
+        q, scales, carrier, partial(_token_runs, normed, weight, rstd, (_version(normed), _version(weight))),
+        (normed, rstd) if weight is None else (normed, rstd, weight),
+    )
     return activation if residual is None else (activation, total)
 
 

@@ -292,3 +292,34 @@ def test_made_in_a_checkpoint_and_read_behind_it():
     a = torch.utils.checkpoint.checkpoint(rms_norm_fp8, x, w, EPS, use_reentrant=False)
     got = torch.autograd.grad(prequantized_linear(a, weight), (x, w, weight), g)
     assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+def test_read_on_another_stream():
+    """Made on one stream, multiplied on another, dropped, and its memory asked for again meanwhile."""
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    weight = _weight(256, 1024, gen)
+    x = torch.randn(2000, 1024, generator=gen, device="cuda").to(BF16)
+    w = torch.ones(1024, device="cuda")
+    g = torch.randn(2000, 256, generator=gen, device="cuda").to(BF16)
+
+    def once(a):
+        out = prequantized_linear(a, weight)
+        return [out.detach(), *torch.autograd.grad(out, weight, g)]
+
+    want = once(rms_norm_fp8(x, w, EPS))
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(3):
+        a = rms_norm_fp8(x, w, EPS)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                busy = busy @ busy * 1e-3
+            got = once(a)
+        a.record_stream(side)
+        del a
+        for _ in range(4):
+            rms_norm_fp8(x + 1, w * 2, EPS)
+        side.synchronize()
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
