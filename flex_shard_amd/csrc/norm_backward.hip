@@ -206,22 +206,33 @@ void by_columns(int64_t cols, Launch launch) {
   else launch(NormLayout<1024, 0, VEC>{});
 }
 
-// Workgroups that a gradient's rows are dealt out to.
+// Workgroups that a gradient's rows are dealt out to: as many parts of dw.
 template <typename L>
-int64_t grad_groups(int64_t rows) {
+int64_t groups_of(int64_t rows) {
   const int64_t blocks = ceil_div(rows, (int64_t)L::ROWS);
   return blocks < kGradGroups<L> ? blocks : kGradGroups<L>;
 }
+template <int VEC>
+int64_t groups_of(int64_t rows, int64_t cols) {
+  int64_t groups = 0;
+  by_columns<VEC>(cols, [&](auto layout) { groups = groups_of<decltype(layout)>(rows); });
+  return groups;
+}
 
-// Launches the gradients; returns how many parts of dw they leave.
+// Launches the gradients; returns how many parts of dw they leave, or -1 without
+// room for them.
 template <int GT, int HT, int XT>
-int64_t launch_grad(NormGradParams& p, hipStream_t stream) {
+int64_t launch_grad(NormGradParams& p, int64_t room, hipStream_t stream) {
   constexpr int VEC = GT == FSH_DT_F32 || HT == FSH_DT_F32 || XT == FSH_DT_F32 ? 4 : 8;
   int64_t groups = 0;
   by_columns<VEC>(p.cols, [&](auto layout) {
     using L = decltype(layout);
     p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS);
-    groups = grad_groups<L>(p.rows);
+    groups = groups_of<L>(p.rows);
+    if (p.parts && groups * p.cols > room) {
+      groups = -1;
+      return;
+    }
     const dim3 grid(static_cast<uint32_t>(groups)), block(L::THREADS);
     if constexpr (L::PER == 0)
       hipLaunchKernelGGL((rms_norm_grad_wide_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
@@ -237,8 +248,7 @@ int64_t launch_grad(NormGradParams& p, hipStream_t stream) {
 FSH_API int64_t fsh_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   using namespace fsh;
   if (rows <= 0 || cols <= 0) return 0;
-  int64_t groups = 0;
-  by_columns<4>(cols, [&](auto layout) { groups = grad_groups<decltype(layout)>(rows); });  // (never fewer than with vectors of 8)
+  const int64_t four = groups_of<4>(rows, cols), eight = groups_of<8>(rows, cols), groups = four > eight ? four : eight;
   return groups * cols * static_cast<int64_t>(sizeof(float));
 }
 
@@ -285,12 +295,14 @@ FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
   p.ldt = q->ldt;
   p.weight_dtype = q->weight_dtype;
   const hipStream_t on = static_cast<hipStream_t>(stream);
+  const int64_t room = q->workspace_nbytes / static_cast<int64_t>(sizeof(float));
   int64_t groups;
-  if (x == FSH_DT_BF16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_BF16, FSH_DT_BF16>(p, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_BF16>(p, on);
-  else if (x == FSH_DT_F16 && g == x) groups = h == x ? launch_grad<FSH_DT_F16, FSH_DT_F16, FSH_DT_F16>(p, on) : launch_grad<FSH_DT_F16, FSH_DT_F32, FSH_DT_F16>(p, on);
-  else if (x == FSH_DT_F16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_F16, FSH_DT_F16>(p, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F16>(p, on);
-  else if (g == x) groups = launch_grad<FSH_DT_F32, FSH_DT_F32, FSH_DT_F32>(p, on);
-  else groups = launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F32>(p, on);
+  if (x == FSH_DT_BF16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_BF16, FSH_DT_BF16>(p, room, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_BF16>(p, room, on);
+  else if (x == FSH_DT_F16 && g == x) groups = h == x ? launch_grad<FSH_DT_F16, FSH_DT_F16, FSH_DT_F16>(p, room, on) : launch_grad<FSH_DT_F16, FSH_DT_F32, FSH_DT_F16>(p, room, on);
+  else if (x == FSH_DT_F16) groups = h == x ? launch_grad<FSH_DT_BF16, FSH_DT_F16, FSH_DT_F16>(p, room, on) : launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F16>(p, room, on);
+  else if (g == x) groups = launch_grad<FSH_DT_F32, FSH_DT_F32, FSH_DT_F32>(p, room, on);
+  else groups = launch_grad<FSH_DT_BF16, FSH_DT_F32, FSH_DT_F32>(p, room, on);
+  if (groups < 0) return fail(FSH_EINVAL, "%s: workspace of %lld bytes", who, (long long)q->workspace_nbytes);
   if (int rc = check_launch("rms_norm_grad_kernel")) return rc;
   if (!q->grad_weight_dev) return FSH_OK;
   const dim3 grid(static_cast<uint32_t>(ceil_div(q->cols, (int64_t)32))), block(1024);
