@@ -7,7 +7,7 @@
 // Bound by memory: dy, h and the gradient of h are read once, dx is written once.
 // A workgroup takes rows in turn and keeps its part of dw in registers, in fp32;
 // the parts are added up in a fixed order by a second kernel.  Measured, both: 8192 x 4096 bf16 with a
-// residual 48 + 4 us, 5.6 TB/s in the first; 262144 x 128 37 + 4, 5.4; 1000 x 1001 fp32 6.3 + 4.6.
+// residual 46 + 4 us, 5.8 TB/s in the first; 262144 x 128 37 + 4, 5.4; 1000 x 1001 fp32 6.3 + 4.6.
 // Requesting the next row ahead of the present one's sum changed nothing up to 8192 columns
 // and spilled at 16384.
 #include "norm_layout.hpp"
@@ -30,29 +30,27 @@ struct NormGradParams {
 };
 
 // Workgroups that rows are dealt out to, so many that all are resident: of 256
-// threads, of 512, of 1024.  More leave more parts of dw: 8192 rows of 4096 bf16 take 56 us with 512
-// of 512 threads, 58 with 768, 68 with 256; of 7168 93 with 256 of 1024, 99 with 512.
+// threads, of up to 512, of 1024.  More leave more parts of dw: 8192 rows of 4096 bf16 take 56 us with 512
+// of 512 threads, 58 with 768, 68 with 256; of 7168 93 with 256 of 1024, 99 with 512; 24576 of 1280 51 with 512 of 256
+// threads, 61 with 768.
 template <typename L>
-constexpr int kGradGroups = L::THREADS == 256 ? 1024 : L::THREADS == 512 ? 512 : 256;
+constexpr int kGradGroups = L::THREADS == 256 ? (L::PER > 16 ? 512 : 1024) : L::THREADS <= 512 ? 512 : 256;
 
+// (two workgroups of 448 in a compute unit: 128 registers)
 template <int GT, int HT, int XT, typename L>
-__global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGradParams p) {
+__global__ __launch_bounds__(L::THREADS, L::THREADS == 448 ? 4 : 1) void rms_norm_grad_kernel(const NormGradParams p) {
   constexpr int VEC = L::VEC, ITEMS = L::ITEMS;
   // fp32 outputs leave past the caches: 8192 rows of 7168 on an fp32 stream 187 -> 167 us; bf16 ones
   // the layer behind finds there (4096 of bf16: 56 us either way).
   constexpr bool kStreamOut = HT == FSH_DT_F32;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : L::ROWS * L::LANES * L::PER];
-  const int lane = threadIdx.x % L::LANES, group = threadIdx.x / L::LANES;
+  const int lane = threadIdx.x % L::LANES, group = threadIdx.x / L::LANES, cols = static_cast<int>(p.cols);
   float w[ITEMS][VEC], part[ITEMS][VEC];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+    NormVector<L>((i * L::LANES + lane) * VEC, cols).weights(p.weight, p.weight_dtype, w[i]);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      w[i][j] = 1.0f;
-      part[i][j] = 0.0f;
-    }
-    if (p.weight && col < p.cols) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w[i]);
+    for (int j = 0; j < VEC; ++j) part[i][j] = 0.0f;
   }
   int turn = 0;
   for (int64_t block = blockIdx.x; block < p.row_blocks; block += gridDim.x, ++turn) {
@@ -62,39 +60,38 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGra
     RawVec<HT, VEC> h[ITEMS], t[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      const int64_t count = live ? p.cols - col : 0;
-      g[i] = load_vec<GT, VEC, true>(p.grad, row * p.ldg + col, count);
-      h[i] = load_vec<HT, VEC, true>(p.h, row * p.ldh + col, count);
+      const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
+      g[i] = c.template load<GT>(p.grad, row * p.ldg, live);
+      h[i] = c.template load<HT>(p.h, row * p.ldh, live);
     }
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      t[i] = load_vec<HT, VEC, true>(p.grad_total, row * p.ldt + col, live && p.grad_total ? p.cols - col : 0);
-    }
+    for (int i = 0; i < ITEMS; ++i)
+      t[i] = NormVector<L>((i * L::LANES + lane) * VEC, cols).template load<HT>(p.grad_total, row * p.ldt, live && p.grad_total);
     const float s = live ? p.rstd[row] : 0.0f;
     float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i) {
+      const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
-        sum += dy * w[i][j] * n;
+        sum += j < c.skip ? 0.0f : dy * w[i][j] * n;
         part[i][j] += dy * n;
       }
+    }
     const float c = sum_over_row<L::LANES>(sum, lds, turn) / static_cast<float>(p.cols);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-      if (!live || col >= p.cols) continue;
+      const NormVector<L> v((i * L::LANES + lane) * VEC, cols);
+      if (!live || !v.inside) continue;
       float d[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
         d[j] = s * (dy * w[i][j] - n * c) + element<HT, VEC>(t[i], j);
       }
-      if (p.grad_x) store_vec<XT, VEC, kStreamOut>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
-      if (HT != XT && p.grad_residual) store_vec<HT, VEC, kStreamOut>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
+      if (p.grad_x) v.template store<XT, kStreamOut>(p.grad_x, row * p.cols, to_vec<XT, VEC>(d));
+      if (HT != XT && p.grad_residual) v.template store<HT, kStreamOut>(p.grad_residual, row * p.cols, to_vec<HT, VEC>(d));
     }
   }
   if (!p.parts) return;
@@ -102,20 +99,23 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_kernel(const NormGra
   if constexpr (L::ROWS == 1) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+      const NormVector<L> v((i * L::LANES + lane) * VEC, cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        if (col + j < p.cols) mine[col + j] = part[i][j];
+        if (v.inside && j < v.count) mine[v.at + j] = part[i][j];
     }
   } else {
     // (LANES <= 64: no sum over a row goes through LDS)
     constexpr int kWidth = L::LANES * L::PER;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int i = 0; i < ITEMS; ++i) {
+      const NormVector<L> v((i * L::LANES + lane) * VEC, cols);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) lds[group * kWidth + (i * L::LANES + lane) * VEC + j] = part[i][j];
+      for (int j = 0; j < VEC; ++j)
+        if (v.inside) lds[group * kWidth + v.at + j] = part[i][j];
+    }
     __syncthreads();
-    for (int64_t col = threadIdx.x; col < p.cols; col += L::THREADS) {
+    for (int col = threadIdx.x; col < cols; col += L::THREADS) {
       float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < L::ROWS; ++k) sum += lds[k * kWidth + col];
@@ -191,19 +191,24 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* par
   else static_cast<uint16_t*>(out)[mine] = static_cast<uint16_t>(bits_of<DT>(sum));
 }
 
-// launch(layout) with the layout for rows of `cols` columns.
-template <int VEC, typename Launch>
-void by_columns(int64_t cols, Launch launch) {
-  if (cols <= 64) launch(NormLayout<64 / VEC, VEC, VEC>{});
-  else if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC>{});
-  else if (cols <= 256) launch(NormLayout<256 / VEC, VEC, VEC>{});
-  else if (cols <= 512) launch(NormLayout<64, 8, VEC>{});
-  else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
-  else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});
-  else if (cols <= 4096) launch(NormLayout<512, 8, VEC>{});
-  else if (cols <= 8192) launch(NormLayout<1024, 8, VEC>{});
-  else if (cols <= 16384) launch(NormLayout<1024, 16, VEC>{});
-  else launch(NormLayout<1024, 0, VEC>{});
+// launch(layout) with the layout for rows of `cols` columns.  Two workgroups or more to a
+// compute unit: 8192 rows of 5120 bf16 take 63 us by 448 threads, 78 by 1024 (but 1000 of 7168 28 for 26, and with
+// an fp32 stream 178 for 166); 24576 of 1040 47 by 64 and 56 by 256; 16384 of 2048 51 and 54.
+template <int ENDS, int VEC, typename Launch>
+void by_columns(int64_t rows, int64_t cols, Launch launch) {
+  if (cols <= 64) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC>{});
+  else if constexpr (ENDS == kPieces) return;
+  else if (cols <= 128) launch(NormLayout<ENDS, 128 / VEC, VEC, VEC>{});
+  else if (cols <= 256) launch(NormLayout<ENDS, 256 / VEC, VEC, VEC>{});
+  else if (cols <= 512) launch(NormLayout<ENDS, 64, 8, VEC>{});
+  else if (cols <= 1024) launch(NormLayout<ENDS, 64, 16, VEC>{});
+  else if (cols <= 1536) launch(NormLayout<ENDS, 64, 24, VEC>{});
+  else if (cols <= 2048) launch(NormLayout<ENDS, 64, 32, VEC>{});
+  else if (cols <= 4096) launch(NormLayout<ENDS, 512, 8, VEC>{});
+  else if (cols <= 7168 && VEC == 8 && rows > 2048) launch(NormLayout<ENDS, 448, 16, VEC>{});
+  else if (cols <= 8192) launch(NormLayout<ENDS, 1024, 8, VEC>{});
+  else if (cols <= 16384) launch(NormLayout<ENDS, 1024, 16, VEC>{});
+  else launch(NormLayout<kEven, 1024, 0, VEC>{});  // (any columns)
 }
 
 // Workgroups that a gradient's rows are dealt out to: as many parts of dw.
@@ -215,7 +220,7 @@ int64_t groups_of(int64_t rows) {
 template <int VEC>
 int64_t groups_of(int64_t rows, int64_t cols) {
   int64_t groups = 0;
-  by_columns<VEC>(cols, [&](auto layout) { groups = groups_of<decltype(layout)>(rows); });
+  by_ends<VEC>(cols, [&](auto ends) { by_columns<ends.value, VEC>(rows, cols, [&](auto layout) { groups = groups_of<decltype(layout)>(rows); }); });
   return groups;
 }
 
@@ -225,19 +230,21 @@ template <int GT, int HT, int XT>
 int64_t launch_grad(NormGradParams& p, int64_t room, hipStream_t stream) {
   constexpr int VEC = GT == FSH_DT_F32 || HT == FSH_DT_F32 || XT == FSH_DT_F32 ? 4 : 8;
   int64_t groups = 0;
-  by_columns<VEC>(p.cols, [&](auto layout) {
-    using L = decltype(layout);
-    p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS);
-    groups = groups_of<L>(p.rows);
-    if (p.parts && groups * p.cols > room) {
-      groups = -1;
-      return;
-    }
-    const dim3 grid(static_cast<uint32_t>(groups)), block(L::THREADS);
-    if constexpr (L::PER == 0)
-      hipLaunchKernelGGL((rms_norm_grad_wide_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((rms_norm_grad_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
+  by_ends<VEC>(p.cols, [&](auto ends) {
+    by_columns<ends.value, VEC>(p.rows, p.cols, [&](auto layout) {
+      using L = decltype(layout);
+      p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS);
+      groups = groups_of<L>(p.rows);
+      if (p.parts && groups * p.cols > room) {
+        groups = -1;
+        return;
+      }
+      const dim3 grid(static_cast<uint32_t>(groups)), block(L::THREADS);
+      if constexpr (L::PER == 0)
+        hipLaunchKernelGGL((rms_norm_grad_wide_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
+      else
+        hipLaunchKernelGGL((rms_norm_grad_kernel<GT, HT, XT, L>), grid, block, 0, stream, p);
+    });
   });
   return groups;
 }
@@ -279,6 +286,16 @@ FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
     return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed", who, (long long)q->workspace_nbytes,
                 (long long)fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols));
   if (ceil_div(q->cols, (int64_t)32) > (1LL << 22) - 1) return fail(FSH_ENOTSUP, "%s: too many columns", who);
+  // (the last columns of a row are written twice, by two lanes that have read them)
+  const RowSpan inputs[] = {{q->grad_dev, q->rows, q->cols, q->ldg, bytes_of(g)},
+                            {q->total_dev, q->rows, q->cols, q->ldh, bytes_of(h)},
+                            {q->grad_total_dev, q->rows, q->cols, q->ldt, bytes_of(h)},
+                            {q->weight_dev, 1, q->cols, q->cols, bytes_of(q->weight_dtype)}};
+  const RowSpan outputs[] = {{q->grad_x_dev, q->rows, q->cols, q->cols, bytes_of(x)},
+                             {h == x ? nullptr : q->grad_residual_dev, q->rows, q->cols, q->cols, bytes_of(h)}};
+  for (const RowSpan& in : inputs)
+    for (const RowSpan& out : outputs)
+      if (share(in, out)) return fail(FSH_EINVAL, "%s: an output overlaps an input", who);
   NormGradParams p = {};
   p.grad = q->grad_dev;
   p.h = q->total_dev;

@@ -14,12 +14,10 @@
 // Bound by memory: x, r and w are read once, h and y written once, the row stays
 // in registers in between.  All but w streams, past the caches: with h written through them
 // 8192 rows of 4096 (bf16, quantized) take 49 us for 44, of 7168 on an fp32 stream 140 for 120.
-// Measured: 8192 x 4096 bf16 with a residual 46 us, 5.8 TB/s; quantized 44, 5.3; 8192 x 7168 quantized, on
-// an fp32 stream, 120, 5.4; 262144 x 128 25, 5.3; one row of 4096 3.1 us, a launch's chain of loads.
+// Measured: 8192 x 4096 bf16 with a residual 47 us, 5.7 TB/s; quantized 43, 5.5; 8192 x 7168 quantized, on
+// an fp32 stream, 108, 6.0; 262144 x 128 25, 5.3; one row of 4096 3.1 us, a launch's chain of loads.
 //
-// LANES threads share a row (norm_layout.hpp); 256 have up to 8192 columns, so that
-// many rows are under way in a compute unit (4096 by 512 threads: 49 us for 47).  Narrow rows go two a
-// turn, for more bytes in flight (262144 x 128: 30 us with one a turn, 26 with four).
+// LANES threads share a row (norm_layout.hpp).
 #include "norm_layout.hpp"
 
 namespace fsh {
@@ -55,34 +53,34 @@ __device__ __forceinline__ void add_residual(const RawVec<XT, VEC>& x, const Raw
   }
 }
 
-// One vector of y, in its type or in 8 bits.  `count`: columns from `col` on.
-template <int XT, bool kQuant, int VEC>
-__device__ __forceinline__ void write_out(const NormParams& p, int64_t row, int64_t col, int64_t count, bool live, const float (&y)[VEC]) {
-  if constexpr (!kQuant) {
-    if (live && count > 0) store_vec<XT, VEC, true>(p.out, row * p.cols + col, count, to_vec<XT, VEC>(y));
-  } else {
-    // (128 / VEC neighbouring lanes have a run; columns from p.cols on are zero)
-    float b[VEC];
-    uint32_t largest = 0;
+// A vector of y in 8 bits: the lane's columns from `col` on are the VEC of y behind
+// the first `skip`, and zero from there.  128 / VEC neighbouring lanes have a run.
+template <int VEC>
+__device__ __forceinline__ void write_quantized(const NormParams& p, int64_t row, int64_t col, int skip, bool live, const float (&y)[VEC]) {
+  float b[VEC];
+  uint32_t largest = 0;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const uint32_t bits = f32_to_bf16_bits(y[j]);
-      b[j] = bf16_bits_to_f32(bits);
-      largest = max(largest, bits & 0x7FFFu);
-    }
-    largest = VEC == 8 ? row16_max_u32(largest) : max32_u32(largest);
-    float scale, recip;
-    tile_scale(bf16_bits_to_f32(largest), 1e-12f, scale, recip);
-    if (live && col < p.ldq) {
-      uint32_t w[VEC / 4];
+  for (int j = 0; j < VEC; ++j) {
+    const uint32_t bits = f32_to_bf16_bits(y[j]);
+    b[j] = bf16_bits_to_f32(bits);
+    largest = max(largest, j < skip ? 0u : bits & 0x7FFFu);
+  }
+  largest = VEC == 8 ? row16_max_u32(largest) : max32_u32(largest);
+  float scale, recip;
+  tile_scale(bf16_bits_to_f32(largest), 1e-12f, scale, recip);
+  if (live && col < p.ldq) {
+    uint32_t w[VEC / 4];
 #pragma unroll
-      for (int j = 0; j < VEC / 4; ++j) {
-        w[j] = cvt2_fp8(b[4 * j] * scale, b[4 * j + 1] * scale, 0, false);
-        w[j] = cvt2_fp8(b[4 * j + 2] * scale, b[4 * j + 3] * scale, w[j], true);
-      }
-      __builtin_memcpy(static_cast<uint8_t*>(p.out) + row * p.ldq + col, w, sizeof(w));
-      if (col % 128 == 0) p.scales[col / 128 * p.rows + row] = recip;
+    for (int j = 0; j < VEC / 4; ++j) {
+      w[j] = cvt2_fp8(b[4 * j] * scale, b[4 * j + 1] * scale, 0, false);
+      w[j] = cvt2_fp8(b[4 * j + 2] * scale, b[4 * j + 3] * scale, w[j], true);
     }
+    typename std::conditional<VEC == 8, uint64_t, uint32_t>::type bytes;
+    static_assert(sizeof(bytes) == sizeof(w));
+    __builtin_memcpy(&bytes, w, sizeof(w));
+    bytes >>= 8 * skip;
+    __builtin_memcpy(static_cast<uint8_t*>(p.out) + row * p.ldq + col, &bytes, sizeof(bytes));
+    if (col % 128 == 0) p.scales[col / 128 * p.rows + row] = recip;
   }
 }
 
@@ -90,15 +88,10 @@ template <int XT, int RT, bool kQuant, typename L>
 __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p) {
   constexpr int VEC = L::VEC, ITEMS = L::ITEMS, TURN = L::TURN;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : 1];
-  const int lane = threadIdx.x % L::LANES;
+  const int lane = threadIdx.x % L::LANES, cols = static_cast<int>(p.cols);
   float w[ITEMS][VEC];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[i][j] = 1.0f;
-    if (p.weight && col < p.cols) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w[i]);
-  }
+  for (int i = 0; i < ITEMS; ++i) NormVector<L>((i * L::LANES + lane) * VEC, cols).weights(p.weight, p.weight_dtype, w[i]);
   int turn = 0;
   for (int64_t block = blockIdx.x; block < p.row_blocks; block += gridDim.x) {
     RawVec<XT, VEC> x[TURN][ITEMS];
@@ -108,10 +101,9 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p
       const int64_t row = (block * TURN + k) * L::ROWS + threadIdx.x / L::LANES;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
-        const int64_t count = row < p.rows ? p.cols - col : 0;
-        x[k][i] = load_vec<XT, VEC, true>(p.x, row * p.ldx + col, count);
-        r[k][i] = load_vec<RT, VEC, true>(p.residual, row * p.ldr + col, count);
+        const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
+        x[k][i] = c.template load<XT>(p.x, row * p.ldx, row < p.rows);
+        r[k][i] = c.template load<RT>(p.residual, row * p.ldr, row < p.rows);
       }
     }
 #pragma unroll
@@ -122,27 +114,29 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p
       float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+        const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
         add_residual<XT, RT, VEC>(x[k][i], r[k][i], h[i]);
         if constexpr (RT != kNoType) {
           const auto rounded = to_vec<RT, VEC>(h[i]);
-          if (live && col < p.cols) store_vec<RT, VEC, true>(p.total, row * p.cols + col, p.cols - col, rounded);
+          if (live && c.inside) c.template store<RT, true>(p.total, row * p.cols, rounded);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) h[i][j] = element<RT, VEC>(rounded, j);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sum += h[i][j] * h[i][j];
+        for (int j = 0; j < VEC; ++j) sum += j < c.skip ? 0.0f : h[i][j] * h[i][j];
       }
       sum = sum_over_row<L::LANES>(sum, lds, turn);
       const float s = inverse_root(sum, p.cols, p.eps);
       if (p.rstd && live && lane == 0) p.rstd[row] = s;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int64_t col = (static_cast<int64_t>(i) * L::LANES + lane) * VEC;
+        const int col = (i * L::LANES + lane) * VEC;
+        const NormVector<L> c(col, cols);
         float y[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = col + j < p.cols ? h[i][j] * s * w[i][j] : 0.0f;
-        write_out<XT, kQuant, VEC>(p, row, col, p.cols - col, live, y);
+        for (int j = 0; j < VEC; ++j) y[j] = c.inside && j < c.count ? h[i][j] * s * w[i][j] : 0.0f;
+        if constexpr (kQuant) write_quantized<VEC>(p, row, col, c.skip, live, y);
+        else if (live && c.inside) c.template store<XT, true>(p.out, row * p.cols, to_vec<XT, VEC>(y));
       }
     }
   }
@@ -191,43 +185,54 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
       if (p.weight && col < p.cols) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) y[j] = col + j < p.cols ? y[j] * s * w[j] : 0.0f;
-      write_out<XT, kQuant, VEC>(p, row, col, p.cols - col, true, y);
+      if constexpr (kQuant) write_quantized<VEC>(p, row, col, 0, true, y);
+      else if (col < p.cols) store_vec<XT, VEC, true>(p.out, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(y));
     }
   }
 }
 
-// launch(layout) with the layout for rows of `cols` columns.  Few rows get more lanes
-// each: 48 of 7168, quantized, 5.0 us for 6.7; of 2048 the other way round, 33 for 27.
-// (a run of 128 columns that is quantized takes all the lanes that it needs)
-template <int VEC, bool kQuant, typename Launch>
+// launch(layout) with the layout for rows of `cols` columns.  Threads as few as keep
+// two or more workgroups in a compute unit, for the bytes in flight, and as have few idle at
+// the row's end: 24576 rows of 1040 bf16 take 41 us by 64 threads, 57 by 256; 8192 of 5120, quantized, 62 by 320 and
+// 68 by 256; of 6144 68 by 512, 72 by 256; of 7168 with an fp32 stream, in vectors of four, 108 by 256, and 2 to 4 %
+// more by 512; 4096 of 12288 69 by 768, 81 by 1024.  Narrow rows go two a turn (262144 x 128: 30 us
+// with one, 26 with four).  Few rows get more lanes each: 48 of 7168, quantized, 5.0 us for 6.7; of 2048 the
+// other way round, 33 for 27.  Values and bytes take the same sums: kQuant alone picks whole runs of 128.
+template <int ENDS, int VEC, bool kQuant, typename Launch>
 void by_columns(int64_t cols, int64_t rows, Launch launch) {
   const bool few = rows <= 512;
-  if (cols <= 64 && !kQuant) launch(NormLayout<64 / VEC, VEC, VEC, 2>{});
-  else if (cols <= 128) launch(NormLayout<128 / VEC, VEC, VEC, 2>{});
-  else if (cols <= 256) launch(NormLayout<256 / VEC, VEC, VEC, 2>{});
-  else if (cols <= 512) launch(NormLayout<64, 8, VEC, 2>{});
-  else if (cols <= 1024) launch(NormLayout<64, 16, VEC>{});
-  else if (cols <= 2048) launch(NormLayout<256, 8, VEC>{});
-  else if (cols <= 4096 && !few) launch(NormLayout<256, 16, VEC>{});
-  else if (cols <= 4096) launch(NormLayout<512, 8, VEC>{});
-  else if (cols <= 8192 && !few) launch(NormLayout<256, 32, VEC>{});
-  else if (cols <= 8192) launch(NormLayout<1024, 8, VEC>{});
-  else if (cols <= 16384) launch(NormLayout<1024, 16, VEC>{});
-  else launch(NormLayout<1024, 0, VEC>{});
+  if (cols <= 64 && !kQuant) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC, 2>{});
+  else if (cols <= 128) launch(NormLayout<ENDS, 128 / VEC, VEC, VEC, 2>{});
+  else if constexpr (ENDS == kPieces) return;
+  else if (cols <= 256) launch(NormLayout<ENDS, 256 / VEC, VEC, VEC, 2>{});
+  else if (cols <= 512) launch(NormLayout<ENDS, 64, 8, VEC, 2>{});
+  else if (cols <= 1024) launch(NormLayout<ENDS, 64, 16, VEC>{});
+  else if (cols <= 1536) launch(NormLayout<ENDS, 64, 24, VEC>{});
+  else if (cols <= 2048) launch(NormLayout<ENDS, 256, 8, VEC>{});
+  else if (cols <= 4096 && !few) launch(NormLayout<ENDS, 256, 16, VEC>{});
+  else if (cols <= 4096) launch(NormLayout<ENDS, 512, 8, VEC>{});
+  else if (cols <= 8192 && few) launch(NormLayout<ENDS, 1024, 8, VEC>{});
+  else if (cols <= 5120) launch(NormLayout<ENDS, 320, 16, VEC>{});
+  else if (cols <= 8192) launch(NormLayout<ENDS, VEC == 8 ? 512 : 256, VEC == 8 ? 16 : 32, VEC>{});
+  else if (cols <= 12288 && VEC == 8) launch(NormLayout<ENDS, 768, 16, VEC>{});
+  else if (cols <= 16384) launch(NormLayout<ENDS, VEC == 8 ? 512 : 1024, VEC == 8 ? 32 : 16, VEC>{});
+  else launch(NormLayout<kEven, 1024, 0, VEC>{});  // (any columns)
 }
 
 template <int XT, int RT, bool kQuant>
 void launch_norm(NormParams& p, hipStream_t stream) {
   constexpr int VEC = XT == FSH_DT_F32 || RT == FSH_DT_F32 ? 4 : 8;  // 16 bytes of the wider type
-  by_columns<VEC, kQuant>(p.cols, p.rows, [&](auto layout) {
-    using L = decltype(layout);
-    p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS * L::TURN);
-    constexpr int64_t kMaxGrid = (1LL << 32) / L::THREADS - 1;  // a launch's threads are counted in 32 bits
-    const dim3 grid(static_cast<uint32_t>(p.row_blocks < kMaxGrid ? p.row_blocks : kMaxGrid)), block(L::THREADS);
-    if constexpr (L::PER == 0)
-      hipLaunchKernelGGL((rms_norm_wide_kernel<XT, RT, kQuant, L>), grid, block, 0, stream, p);
-    else
-      hipLaunchKernelGGL((rms_norm_kernel<XT, RT, kQuant, L>), grid, block, 0, stream, p);
+  by_ends<VEC>(p.cols, [&](auto ends) {
+    by_columns<ends.value, VEC, kQuant>(p.cols, p.rows, [&](auto layout) {
+      using L = decltype(layout);
+      p.row_blocks = ceil_div(p.rows, (int64_t)L::ROWS * L::TURN);
+      constexpr int64_t kMaxGrid = (1LL << 32) / L::THREADS - 1;  // a launch's threads are counted in 32 bits
+      const dim3 grid(static_cast<uint32_t>(p.row_blocks < kMaxGrid ? p.row_blocks : kMaxGrid)), block(L::THREADS);
+      if constexpr (L::PER == 0)
+        hipLaunchKernelGGL((rms_norm_wide_kernel<XT, RT, kQuant, L>), grid, block, 0, stream, p);
+      else
+        hipLaunchKernelGGL((rms_norm_kernel<XT, RT, kQuant, L>), grid, block, 0, stream, p);
+    });
   });
 }
 
@@ -292,6 +297,16 @@ FSH_API int fsh_rms_norm(const fsh_norm* q, void* stream) {
       (q->weight_dev && !aligned(q->weight_dev, bytes_of(q->weight_dtype))) || !aligned(q->out_dev, quant ? 8 : bytes_of(q->x_dtype)) ||
       !aligned(q->scales_dev, 4) || !aligned(q->rstd_dev, 4))
     return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements, bytes to 8", who);
+  // (the last columns of a row are written twice, by two lanes that have read them)
+  const int64_t n = q->rows, k = q->cols, kq = ceil_div(k, (int64_t)128) * 128;
+  const RowSpan inputs[] = {{q->x_dev, n, k, q->ldx, bytes_of(q->x_dtype)},
+                            {q->residual_dev, n, k, q->ldr, bytes_of(q->residual_dtype)},
+                            {q->weight_dev, 1, k, k, bytes_of(q->weight_dtype)}};
+  const RowSpan outputs[] = {{residual ? q->total_dev : nullptr, n, k, k, bytes_of(q->residual_dtype)},
+                             {q->out_dev, n, quant ? kq : k, quant ? kq : k, quant ? 1 : bytes_of(q->x_dtype)}};
+  for (const RowSpan& in : inputs)
+    for (const RowSpan& out : outputs)
+      if (share(in, out)) return fail(FSH_EINVAL, "%s: an output overlaps an input", who);
   NormParams p = {};
   p.x = q->x_dev;
   p.residual = q->residual_dev;

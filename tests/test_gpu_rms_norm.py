@@ -369,3 +369,31 @@ def test_saved_tensors_that_come_back_otherwise():
             y = rms_norm(rows, weight, EPS)
         with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
             torch.autograd.grad(y, (rows, weight), g)
+
+
+@pytest.mark.parametrize("cols", [*range(1, 34), 393, 771, 1030, 1283, 1539, 1805, 2049, 2305, 3003, 5001, 5119, 6001, 7169, 9001, 12290, 14001])
+@pytest.mark.parametrize("dtype,stream", [(BF16, None), (BF16, F32), (F16, F16), (F32, F32)])
+def test_row_ends(dtype, stream, cols):
+    """Every number of columns behind the last whole vector, in rows with neighbours that are not theirs: no
+    value of one row's end counts twice, or gets into another row."""
+    rows = 6
+    gen = torch.Generator(device="cuda").manual_seed(cols)
+    wide = torch.full((rows, cols + 5), float("nan"), device="cuda", dtype=dtype)
+    wide[:, 2 : cols + 2] = torch.randn(rows, cols, generator=gen, device="cuda").to(dtype)
+    wide[:, cols + 1] *= 3  # the last column weighs the most
+    x = wide[:, 2 : cols + 2]
+    residual = None if stream is None else torch.randn(rows, cols, generator=gen, device="cuda").to(stream)
+    w = (1 + 0.3 * torch.randn(cols, generator=gen, device="cuda")).to(dtype)
+    _check_forward(x, residual, w)
+    x = x.detach()
+    g, gt, got = _run_grads(x, residual, w, gen)
+    _check_grads(x, residual, w, g, gt, got)
+
+
+@pytest.mark.parametrize("cols", [500, 1500, 1777, 2000, 4097, 5120, 6001, 7168])
+def test_gradients_of_rows_by_the_thousand(cols):
+    """Rows enough that those of 4097 to 7168 columns are dealt out otherwise."""
+    for stream in (BF16, F32):
+        x, residual, w, gen = _make(2500, cols, BF16, stream, BF16)
+        g, gt, got = _run_grads(x, residual, w, gen)
+        _check_grads(x, residual, w, g, gt, got)

@@ -323,3 +323,17 @@ def test_read_on_another_stream():
             rms_norm_fp8(x + 1, w * 2, EPS)
         side.synchronize()
         assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+@pytest.mark.parametrize("cols", [*range(1, 18), 121, 135, 255, 259, 383, 389, 513, 767, 771, 1285, 1530, 2305, 5113, 6001, 7161, 9001, 12290, 14001])
+@pytest.mark.parametrize("dtype,stream", [(BF16, None), (BF16, F32), (F32, F32)])
+def test_row_ends(dtype, stream, cols):
+    """Every number of columns behind the last whole vector; the run that ends the row has its largest value last."""
+    for rows in (3, 600):
+        x, residual, w, _ = _make(rows, cols, dtype, stream)
+        x[:, -1] = 40
+        got, want = rms_norm_fp8(x, w, EPS, residual=residual), rms_norm(x, w, EPS, residual=residual)
+        got, want = (got, want) if residual is None else (got[0], want[0])
+        q, scales = hip_ops.act_quant_1x128(_quantized(want))
+        assert _same(got.q, q) and torch.equal(got.scales, scales)
+        assert not got.q.view(torch.uint8)[:, cols:].any()

@@ -122,3 +122,18 @@ def test_there_is_no_cpu_path():
             call()
     with pytest.raises(NotImplementedError):
         FlexShardRMSNorm.from_float(torch.nn.RMSNorm((2, 64)))
+
+
+def test_outputs_that_overlap_inputs():
+    far = [SOMEWHERE + (i << 20) for i in range(9)]
+    apart = dict(zip(("x_dev", "residual_dev", "weight_dev", "total_dev", "out_dev", "scales_dev", "rstd_dev"), far))
+    for fields in (
+        dict(out_dev=apart["x_dev"]), dict(total_dev=apart["residual_dev"]), dict(total_dev=apart["x_dev"] + 798),
+        dict(out_dev=apart["residual_dev"] + 2 * (3 * 200 + 100) - 2, ldr=200), dict(out_dev=apart["weight_dev"] + 198),
+        dict(form=_native.NORM_FP8, out_dev=apart["x_dev"] - 8),
+    ):
+        assert _native.lib().fsh_rms_norm(_norm(**apart | fields), None) == EINVAL and "overlaps" in _message(), fields
+    names = ("grad_dev", "total_dev", "weight_dev", "rstd_dev", "grad_total_dev", "grad_x_dev", "grad_residual_dev", "grad_weight_dev", "workspace_dev")
+    apart = dict(zip(names, far))
+    for fields in (dict(grad_x_dev=apart["grad_dev"]), dict(grad_x_dev=apart["grad_total_dev"] + 2), dict(grad_x_dev=apart["total_dev"])):
+        assert _native.lib().fsh_rms_norm_backward(_gradient(**apart | fields), None) == EINVAL and "overlaps" in _message(), fields
