@@ -125,7 +125,9 @@ __global__ __launch_bounds__(L::THREADS, L::THREADS == 448 ? 4 : 1) void rms_nor
 }
 
 // Rows that do not fit the registers: the sum first, then the gradients, with dw's
-// part of a workgroup read and written for every row it takes.
+// part of a workgroup read and written for every row it takes.  What is read or written
+// for the last time streams, so that the parts stay in the caches (2048 rows of 20480 bf16 131 us; with the
+// parts read and written by elements 200, and nothing streamed 213).
 template <int GT, int HT, int XT, typename L>
 __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_wide_kernel(const NormGradParams p) {
   constexpr int VEC = L::VEC, STEP = L::THREADS * VEC;
@@ -142,18 +144,21 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_wide_kernel(const No
 #pragma unroll
       for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
       if (p.weight) load_floats<VEC>(p.weight, p.weight_dtype, col, p.cols - col, w);
+      const auto before = load_vec<FSH_DT_F32, VEC>(mine, col, mine && turn ? p.cols - col : 0);
+      float part[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float dy = element<GT, VEC>(g, j), n = element<HT, VEC>(h, j) * s;
         sum += dy * w[j] * n;
-        if (mine && col + j < p.cols) mine[col + j] = (turn ? mine[col + j] : 0.0f) + dy * n;
+        part[j] = element<FSH_DT_F32, VEC>(before, j) + dy * n;
       }
+      if (mine) store_vec<FSH_DT_F32, VEC>(mine, col, p.cols - col, to_vec<FSH_DT_F32, VEC>(part));
     }
     const float c = sum_over_row<L::THREADS>(sum, lds, turn) / static_cast<float>(p.cols);
     for (int64_t col = threadIdx.x * VEC; col < p.cols; col += STEP) {
-      const auto g = load_vec<GT, VEC>(p.grad, row * p.ldg + col, p.cols - col);
-      const auto h = load_vec<HT, VEC>(p.h, row * p.ldh + col, p.cols - col);
-      const auto t = load_vec<HT, VEC>(p.grad_total, row * p.ldt + col, p.grad_total ? p.cols - col : 0);
+      const auto g = load_vec<GT, VEC, true>(p.grad, row * p.ldg + col, p.cols - col);
+      const auto h = load_vec<HT, VEC, true>(p.h, row * p.ldh + col, p.cols - col);
+      const auto t = load_vec<HT, VEC, true>(p.grad_total, row * p.ldt + col, p.grad_total ? p.cols - col : 0);
       float w[VEC], d[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) w[j] = 1.0f;
@@ -163,8 +168,8 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_grad_wide_kernel(const No
         const float dy = element<GT, VEC>(g, j), n = element<HT, VEC>(h, j) * s;
         d[j] = s * (dy * w[j] - n * c) + element<HT, VEC>(t, j);
       }
-      if (p.grad_x) store_vec<XT, VEC>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
-      if (HT != XT && p.grad_residual) store_vec<HT, VEC>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
+      if (p.grad_x) store_vec<XT, VEC, true>(p.grad_x, row * p.cols + col, p.cols - col, to_vec<XT, VEC>(d));
+      if (HT != XT && p.grad_residual) store_vec<HT, VEC, true>(p.grad_residual, row * p.cols + col, p.cols - col, to_vec<HT, VEC>(d));
     }
   }
 }
