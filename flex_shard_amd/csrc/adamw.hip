@@ -492,8 +492,10 @@ __global__ __launch_bounds__(kThreads) void square_join_kernel(const double* par
 // A few chunks of one type in one workgroup, two at a time for each quarter of it,
 // which writes the sum itself: norm weights and biases, where a second launch would be the
 // longer part.  Bound by latency and by what one compute unit reads; the table is fetched once, into
-// LDS.  20 vectors of 4096 fp32: 10.4 us; as two launches 7.6, but 20 of the host's instead of 16.
+// LDS.  20 vectors of 4096 fp32: 10.4 us; as two launches 7.6, but 20 of the host's instead of 16.  (A
+// replayed graph of the call on 262144 elements, 32 whole chunks: 21 us this way, 12.5 as two.)
 constexpr int kFewChunks = 32, kFewThreads = 1024;
+constexpr int64_t kFewElements = 16 * kSquareChunk;
 template <int DT>
 __global__ __launch_bounds__(kFewThreads) void square_sum_few_kernel(const SquareTable a) {
   __shared__ double lds[kFewThreads / 64];
@@ -545,7 +547,11 @@ int square_launches(const int64_t* tensors, int32_t count, Each each) {
     }
     if (end == begin) return -1;  // a tensor of more than 2^44 elements
     bool few = begin == 0 && end == count && chunks <= kFewChunks;
-    for (int32_t i = 1; few && i < count; ++i) few = tensors[3 * i + 2] == tensors[2];  // (of one type)
+    int64_t elements = 0;
+    for (int32_t i = 0; few && i < count; ++i) {
+      elements += tensors[3 * i + 1];
+      few = tensors[3 * i + 2] == tensors[2] && elements <= kFewElements;  // (of one type)
+    }
     if (chunks) each(begin, end, chunks, few ? 0 : chunks < kSquareGroups ? chunks : static_cast<int64_t>(kSquareGroups));
     ++launches;
     begin = end;

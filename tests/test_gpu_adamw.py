@@ -519,3 +519,12 @@ def test_more_tensors_than_a_table_holds():
         FlexShardAdamW([q], **HYPER).step(square_sum=total, max_norm=0.5)
     assert all(torch.equal(p, q) for p, q in zip(params, twins))
     assert all(int(optimizer.state[p]["step"]) == 1 for p in params)
+
+
+@pytest.mark.parametrize("sizes", [[131072], [131073], [8192] * 16, [8192] * 15 + [8191, 2], [65536, 0, 65536], [4096] * 31 + [1]])
+def test_square_sums_around_a_single_workgroups_share(sizes):
+    gen = _gen(22)
+    for dtype in (BF16, F32):
+        parts = [torch.randn(n, generator=gen, device="cuda").to(dtype) for n in sizes]
+        want = sum(p.double().square().sum() for p in parts)
+        assert abs(grad_square_sum(parts) - want) <= 2 * 4096 * 2.0**-53 * want
