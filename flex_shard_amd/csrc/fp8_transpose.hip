@@ -242,7 +242,8 @@ struct LoadMatrix {
 
 // The thread's part of a tile of a norm's output h s w (norm_forward.hip), made again
 // from its sum h [rows, cols], the rows' factors s and the weight, and rounded to bf16 as there.
-// (y itself is then never written, nor kept for the backward pass.)
+// (y itself is then never written, nor kept for the backward pass.)  Bound by memory and by the tiles'
+// way through LDS, like the matrix's own: 8192 x 4096 bf16 24.1 us for 23.5, 4.2 TB/s; fp32 34.2, 4.9.
 struct NormRunsParams {
   const void* h;
   const float* rstd;
