@@ -43,6 +43,8 @@ __global__ __launch_bounds__(L::THREADS, L::THREADS == 448 ? 4 : 1) void rms_nor
   // fp32 outputs leave past the caches: 8192 rows of 7168 on an fp32 stream 187 -> 167 us; bf16 ones
   // the layer behind finds there (4096 of bf16: 56 us either way).
   constexpr bool kStreamOut = HT == FSH_DT_F32;
+  // Where the registers would not do: 4096 rows of 9001 on an fp32 stream 122 us for 151 (of bf16 82 for 79).
+  constexpr bool kAgain = L::ENDS == kOverlapping && VEC == 4 && L::THREADS == 1024 && L::PER == 16;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : L::ROWS * L::LANES * L::PER];
   const int lane = threadIdx.x % L::LANES, group = threadIdx.x / L::LANES, cols = static_cast<int>(p.cols);
   float w[ITEMS][VEC], part[ITEMS][VEC];
@@ -69,9 +71,10 @@ __global__ __launch_bounds__(L::THREADS, L::THREADS == 448 ? 4 : 1) void rms_nor
       t[i] = NormVector<L>((i * L::LANES + lane) * VEC, cols).template load<HT>(p.grad_total, row * p.ldt, live && p.grad_total);
     const float s = live ? p.rstd[row] : 0.0f;
     float sum = 0.0f;
+    const int lane_sum = lane_again<kAgain>(lane);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
+      const NormVector<L> c((i * L::LANES + lane_sum) * VEC, cols);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float dy = element<GT, VEC>(g[i], j), n = element<HT, VEC>(h[i], j) * s;
@@ -80,9 +83,10 @@ __global__ __launch_bounds__(L::THREADS, L::THREADS == 448 ? 4 : 1) void rms_nor
       }
     }
     const float c = sum_over_row<L::LANES>(sum, lds, turn) / static_cast<float>(p.cols);
+    const int lane_out = lane_again<kAgain>(lane);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const NormVector<L> v((i * L::LANES + lane) * VEC, cols);
+      const NormVector<L> v((i * L::LANES + lane_out) * VEC, cols);
       if (!live || !v.inside) continue;
       float d[VEC];
 #pragma unroll
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* par
 // an fp32 stream 178 for 166); 24576 of 1040 47 by 64 and 56 by 256; 16384 of 2048 51 and 54.
 template <int ENDS, int VEC, typename Launch>
 void by_columns(int64_t rows, int64_t cols, Launch launch) {
-  if (cols <= 64) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC>{});
+  if (ENDS == kPieces || cols <= 64) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC>{});
   else if constexpr (ENDS == kPieces) return;
   else if (cols <= 128) launch(NormLayout<ENDS, 128 / VEC, VEC, VEC>{});
   else if (cols <= 256) launch(NormLayout<ENDS, 256 / VEC, VEC, VEC>{});
@@ -210,7 +214,7 @@ void by_columns(int64_t rows, int64_t cols, Launch launch) {
   else if (cols <= 1536) launch(NormLayout<ENDS, 64, 24, VEC>{});
   else if (cols <= 2048) launch(NormLayout<ENDS, 64, 32, VEC>{});
   else if (cols <= 4096) launch(NormLayout<ENDS, 512, 8, VEC>{});
-  else if (cols <= 7168 && VEC == 8 && rows > 2048) launch(NormLayout<ENDS, 448, 16, VEC>{});
+  else if (cols <= 7168 && VEC == 8 && rows > 2048) launch(NormLayout<ENDS, VEC == 8 ? 448 : 1024, VEC == 8 ? 16 : 8, VEC>{});
   else if (cols <= 8192) launch(NormLayout<ENDS, 1024, 8, VEC>{});
   else if (cols <= 16384) launch(NormLayout<ENDS, 1024, 16, VEC>{});
   else launch(NormLayout<kEven, 1024, 0, VEC>{});  // (any columns)

@@ -87,6 +87,8 @@ __device__ __forceinline__ void write_quantized(const NormParams& p, int64_t row
 template <int XT, int RT, bool kQuant, typename L>
 __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p) {
   constexpr int VEC = L::VEC, ITEMS = L::ITEMS, TURN = L::TURN;
+  // (8192 rows of 7161 on an fp32 stream, quantized: 120 us for 163; with one vector 35 for 33)
+  constexpr bool kAgain = L::ENDS == kOverlapping && ITEMS > 1;
   __shared__ float lds[L::LANES > 64 ? 2 * L::LANES / 64 : 1];
   const int lane = threadIdx.x % L::LANES, cols = static_cast<int>(p.cols);
   float w[ITEMS][VEC];
@@ -112,9 +114,10 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p
       const bool live = row < p.rows;
       float h[ITEMS][VEC];
       float sum = 0.0f;
+      const int lane_sum = lane_again<kAgain>(lane);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const NormVector<L> c((i * L::LANES + lane) * VEC, cols);
+        const NormVector<L> c((i * L::LANES + lane_sum) * VEC, cols);
         add_residual<XT, RT, VEC>(x[k][i], r[k][i], h[i]);
         if constexpr (RT != kNoType) {
           const auto rounded = to_vec<RT, VEC>(h[i]);
@@ -128,9 +131,10 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_kernel(const NormParams p
       sum = sum_over_row<L::LANES>(sum, lds, turn);
       const float s = inverse_root(sum, p.cols, p.eps);
       if (p.rstd && live && lane == 0) p.rstd[row] = s;
+      const int lane_out = lane_again<kAgain>(lane);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
-        const int col = (i * L::LANES + lane) * VEC;
+        const int col = (i * L::LANES + lane_out) * VEC;
         const NormVector<L> c(col, cols);
         float y[VEC];
 #pragma unroll
@@ -201,9 +205,9 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
 template <int ENDS, int VEC, bool kQuant, typename Launch>
 void by_columns(int64_t cols, int64_t rows, Launch launch) {
   const bool few = rows <= 512;
-  if (cols <= 64 && !kQuant) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC, 2>{});
-  else if (cols <= 128) launch(NormLayout<ENDS, 128 / VEC, VEC, VEC, 2>{});
+  if (ENDS == kPieces || (cols <= 64 && !kQuant)) launch(NormLayout<ENDS, (kQuant ? 128 : 64) / VEC, VEC, VEC, 2>{});
   else if constexpr (ENDS == kPieces) return;
+  else if (cols <= 128) launch(NormLayout<ENDS, 128 / VEC, VEC, VEC, 2>{});
   else if (cols <= 256) launch(NormLayout<ENDS, 256 / VEC, VEC, VEC, 2>{});
   else if (cols <= 512) launch(NormLayout<ENDS, 64, 8, VEC, 2>{});
   else if (cols <= 1024) launch(NormLayout<ENDS, 64, 16, VEC>{});
@@ -214,7 +218,7 @@ void by_columns(int64_t cols, int64_t rows, Launch launch) {
   else if (cols <= 8192 && few) launch(NormLayout<ENDS, 1024, 8, VEC>{});
   else if (cols <= 5120) launch(NormLayout<ENDS, 320, 16, VEC>{});
   else if (cols <= 8192) launch(NormLayout<ENDS, VEC == 8 ? 512 : 256, VEC == 8 ? 16 : 32, VEC>{});
-  else if (cols <= 12288 && VEC == 8) launch(NormLayout<ENDS, 768, 16, VEC>{});
+  else if (cols <= 12288 && VEC == 8) launch(NormLayout<ENDS, VEC == 8 ? 768 : 1024, 16, VEC>{});
   else if (cols <= 16384) launch(NormLayout<ENDS, VEC == 8 ? 512 : 1024, VEC == 8 ? 32 : 16, VEC>{});
   else launch(NormLayout<kEven, 1024, 0, VEC>{});  // (any columns)
 }

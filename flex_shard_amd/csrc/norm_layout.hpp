@@ -57,6 +57,14 @@ struct NormVector {
   }
 };
 
+// The lane once more, for a loop that works out again where its vectors lie rather than
+// to keep that in registers since the loop before it.
+template <bool AGAIN>
+__device__ __forceinline__ int lane_again(int lane) {
+  if constexpr (AGAIN) asm volatile("" : "+v"(lane));
+  return lane;
+}
+
 // launch(ends) for rows of `cols` columns in vectors of VEC, as an integral constant.
 template <int VEC, typename Launch>
 void by_ends(int64_t cols, Launch launch) {
