@@ -22,6 +22,9 @@ from ..blockwise_fp8.fp8_activation import Fp8Activation
 from ..experts import differentiates
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+# Of a module that names none: torch's own takes that of the type it computes in, also for bf16 and fp16
+# rows.  (Of rows of 0.01 the norm with bf16's would be 0.11, not 1.)
+_EPS = torch.finfo(torch.float32).eps
 
 
 def _as_rows(t: torch.Tensor) -> torch.Tensor:
@@ -186,7 +189,7 @@ def rms_norm_fp8(
 class FlexShardRMSNorm(nn.RMSNorm):
     """``nn.RMSNorm`` over the last dimension on the kernels here.  ``forward(x,
     residual)`` adds first and returns the sum too; with ``fp8`` the output is an
-    :class:`~flex_shard_amd.blockwise_fp8.Fp8Activation`."""
+    :class:`~flex_shard_amd.blockwise_fp8.Fp8Activation`.  ``eps`` None is fp32's."""
 
     @classmethod
     def from_float(cls, mod: nn.RMSNorm) -> "FlexShardRMSNorm":
@@ -200,7 +203,7 @@ class FlexShardRMSNorm(nn.RMSNorm):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, *, fp8: bool = False):
         if len(self.normalized_shape) != 1 or x.shape[-1:] != tuple(self.normalized_shape):
             raise ValueError(f"the norm is over a last dimension {tuple(self.normalized_shape)}, got {tuple(x.shape)}")
-        eps = torch.finfo(x.dtype).eps if self.eps is None else self.eps
+        eps = _EPS if self.eps is None else self.eps
         return (rms_norm_fp8 if fp8 else rms_norm)(x, self.weight, eps, residual=residual)
 
 

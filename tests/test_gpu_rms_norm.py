@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from flex_shard_amd import hip_ops
-from flex_shard_amd.norms import FlexShardRMSNorm, convert_to_flex_shard_rms_norm, rms_norm
+from flex_shard_amd.norms import FlexShardRMSNorm, convert_to_flex_shard_rms_norm, rms_norm, rms_norm_fp8
 
 pytestmark = pytest.mark.gpu
 
@@ -397,3 +397,45 @@ def test_gradients_of_rows_by_the_thousand(cols):
         x, residual, w, gen = _make(2500, cols, BF16, stream, BF16)
         g, gt, got = _run_grads(x, residual, w, gen)
         _check_grads(x, residual, w, g, gt, got)
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.02, 1e-3])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_converted_module_without_eps(dtype, scale):
+    """A module that names no eps has that of fp32 whatever the type of its rows, as torch's own: of small bf16 or fp16
+    rows another one changes the outputs by a factor."""
+    x, _, w, gen = _make(6, 300, dtype, None, weight=dtype, scale=scale)
+    g = torch.randn(x.shape, generator=gen, device="cuda").to(dtype)
+    model = torch.nn.Sequential(torch.nn.RMSNorm(300, device="cuda", dtype=dtype))
+    its = model[0]
+    its.weight.data.copy_(w)
+    convert_to_flex_shard_rms_norm(model)
+    mine = model[0]
+    assert type(mine) is FlexShardRMSNorm and mine.eps is None
+    rows, others = x.clone().requires_grad_(), x.clone().requires_grad_()
+    y, want = mine(rows), _norm64(x, w, torch.finfo(F32).eps)[0]
+    least = 2.0**-25 if dtype == F16 else 1e-38
+    assert ((y.double() - want).abs() <= want.abs() * (_step(dtype) + 64 * U) + least).all()
+    theirs = its(others)  # (which may round the norm before the weight's product too)
+    assert theirs.dtype == y.dtype
+    assert ((y.double() - theirs.double()).abs() <= want.abs() * (3 * _step(dtype) + 128 * U) + 3 * least).all()
+    # gradients, of the formula: dh = s (a - n mean(a n)), each sum's error that of its terms' magnitudes
+    got = torch.autograd.grad(y, rows, g)[0].double()
+    n, s = _norm64(x, None, torch.finfo(F32).eps)
+    a = g.double() * w.double()
+    mean, size = (a * n).mean(-1, keepdim=True), (a * n).abs().mean(-1, keepdim=True)
+    wanted = s * (a - n * mean)
+    assert ((got - wanted).abs() <= wanted.abs() * _step(dtype) + 256 * U * s * (a.abs() + n.abs() * size) + least).all()
+
+
+def test_a_converted_module_without_eps_in_8_bits():
+    x, _, w, _ = _make(6, 300, BF16, None, weight=BF16, scale=0.02)
+    model = torch.nn.Sequential(torch.nn.RMSNorm(300, device="cuda", dtype=BF16))
+    model[0].weight.data.copy_(w)
+    mine = convert_to_flex_shard_rms_norm(model)[0]
+    with torch.no_grad():
+        got, want = mine(x, fp8=True), rms_norm_fp8(x, w, torch.finfo(F32).eps)
+        assert torch.equal(got.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(got.scales, want.scales)
+        # an E4M3 value is off by half a step of 2**-3, or of 2**-9 of its scale, which is the largest bf16 value over 448
+        values, y = got.dequantize(F32).double(), _norm64(x, w, torch.finfo(F32).eps)[0]
+        assert ((values - y).abs() <= y.abs() * (2.0**-4 + 2 * _step(BF16)) + y.abs().amax() * (1 + 2 * _step(BF16)) / 448 * 2.0**-10).all()
