@@ -210,18 +210,23 @@ class FlexShardRMSNorm(nn.RMSNorm):
 def convert_to_flex_shard_rms_norm(module: nn.Module, filter_fn=None) -> nn.Module:
     """Swap every ``nn.RMSNorm`` over one dimension below ``module`` that
     ``filter_fn(fqn, child)`` accepts (all, when it is None) for a
-    :class:`FlexShardRMSNorm` sharing its weight."""
-    _convert_children(module, "", filter_fn)
+    :class:`FlexShardRMSNorm` sharing its weight; one that has several names for the
+    same module under each of them."""
+    _convert_children(module, "", filter_fn, {})
     return module
 
 
-def _convert_children(parent: nn.Module, prefix: str, filter_fn) -> None:
-    for name, child in list(parent.named_children()):
+def _convert_children(parent: nn.Module, prefix: str, filter_fn, converted: dict[nn.Module, nn.Module]) -> None:
+    for name, child in list(parent._modules.items()):  # (named_children leaves second names out)
+        if child is None:
+            continue
         fqn = f"{prefix}{name}"
         if type(child) is nn.RMSNorm and len(child.normalized_shape) == 1 and (filter_fn is None or filter_fn(fqn, child)):
-            setattr(parent, name, FlexShardRMSNorm.from_float(child))
+            if child not in converted:
+                converted[child] = FlexShardRMSNorm.from_float(child)
+            setattr(parent, name, converted[child])
         else:
-            _convert_children(child, f"{fqn}.", filter_fn)
+            _convert_children(child, f"{fqn}.", filter_fn, converted)
 
 
 __all__ = ["FlexShardRMSNorm", "convert_to_flex_shard_rms_norm", "rms_norm", "rms_norm_fp8"]

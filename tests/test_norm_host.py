@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from flex_shard_amd import _native
-from flex_shard_amd.norms import FlexShardRMSNorm, rms_norm, rms_norm_fp8
+from flex_shard_amd.norms import FlexShardRMSNorm, convert_to_flex_shard_rms_norm, rms_norm, rms_norm_fp8
 
 OK, EINVAL, ENOTSUP = 0, -22, -95
 SOMEWHERE = 1 << 20  # an aligned address that no refused call touches
@@ -137,3 +137,24 @@ def test_outputs_that_overlap_inputs():
     apart = dict(zip(names, far))
     for fields in (dict(grad_x_dev=apart["grad_dev"]), dict(grad_x_dev=apart["grad_total_dev"] + 2), dict(grad_x_dev=apart["total_dev"])):
         assert _native.lib().fsh_rms_norm_backward(_gradient(**apart | fields), None) == EINVAL and "overlaps" in _message(), fields
+
+
+def test_a_norm_under_several_names_is_converted_once():
+    """Twice in one parent, and in two: one module under all of its names, as before."""
+    norm, other = torch.nn.RMSNorm(8), torch.nn.RMSNorm(8)
+    block = torch.nn.ModuleDict({"a": norm, "b": norm, "c": other, "d": torch.nn.Linear(2, 2)})
+    model = torch.nn.ModuleList([block, torch.nn.Sequential(norm, other), block])
+    model.register_module("nothing", None)
+    names = []
+    assert convert_to_flex_shard_rms_norm(model, lambda fqn, child: names.append(fqn) or True) is model
+    assert type(block["a"]) is FlexShardRMSNorm and block["b"] is block["a"] and model[1][0] is block["a"]
+    assert type(block["c"]) is FlexShardRMSNorm and model[1][1] is block["c"] and block["c"] is not block["a"]
+    assert block["a"].weight is norm.weight and type(block["d"]) is torch.nn.Linear and model[2] is block
+    assert names == ["0.a", "0.b", "0.c", "1.0", "1.1"]
+
+
+def test_a_name_that_the_filter_leaves_out_keeps_its_norm():
+    norm = torch.nn.RMSNorm(8)
+    model = torch.nn.ModuleDict({"a": norm, "b": norm, "c": norm})
+    convert_to_flex_shard_rms_norm(model, lambda fqn, child: fqn != "b")
+    assert type(model["a"]) is FlexShardRMSNorm and model["c"] is model["a"] and model["b"] is norm
