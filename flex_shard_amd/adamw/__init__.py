@@ -137,7 +137,7 @@ are left alone; two that overlap are refused."""
         stepped, copies = [], []  # (the queued kernels read the copies)
         states, strided, int32 = self.state, torch.strided, torch.int32
         for group in self.param_groups:
-            lr, bits, number = group["lr"], group["state_bits"], len(groups)
+            lr, bits, number, begin = group["lr"], group["state_bits"], len(groups), len(table)
             for p in group["params"]:
                 g = p.grad
                 if g is None:
@@ -182,8 +182,10 @@ are left alone; two that overlap are refused."""
                     param_dt, grad_dt, bits, number,
                 )
                 stepped.append(p)
+            if len(table) == begin:  # (no gradients: nothing of the group is looked at)
+                continue
             address = None
-            if isinstance(lr, torch.Tensor) and device is not None:
+            if isinstance(lr, torch.Tensor):
                 lr, address = _learning_rate(lr, device)
             groups.append((lr, address, *group["betas"], group["eps"], group["weight_decay"]))
             if len(groups) == ADAMW_GROUPS:

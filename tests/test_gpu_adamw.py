@@ -528,3 +528,44 @@ def test_square_sums_around_a_single_workgroups_share(sizes):
         parts = [torch.randn(n, generator=gen, device="cuda").to(dtype) for n in sizes]
         want = sum(p.double().square().sum() for p in parts)
         assert abs(grad_square_sum(parts) - want) <= 2 * 4096 * 2.0**-53 * want
+
+
+def _learning_rates(captured):
+    """A step of two groups, the first without gradients, with one learning rate on the GPU, and its twin's with a number."""
+    gen = _gen(23)
+    params = _params([(300,), (300,)], F32, gen)
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    lr = torch.tensor(2e-3, device="cuda")
+    mine = FlexShardAdamW([dict(params=[p]) for p in params], lr=lr)
+    other = FlexShardAdamW([dict(params=[q]) for q in twins], lr=lr.item())
+    _set_grads(params[1:], F32, gen)
+    twins[1].grad = params[1].grad.clone()
+    other.step()
+    if captured:
+        mine.step()  # the states must exist
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            mine.step()
+        for _ in range(3):
+            graph.replay()
+            other.step()
+            torch.cuda.synchronize()
+            assert torch.equal(params[1], twins[1])
+    else:
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            mine.step()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(params[1], twins[1]) and torch.equal(params[0], twins[0])
+    assert not mine.state.get(params[0])
+
+
+def test_learning_rate_on_the_gpu_of_a_group_without_gradients():
+    """Nothing waits for the GPU."""
+    _learning_rates(captured=False)
+
+
+def test_learning_rate_on_the_gpu_of_a_group_without_gradients_captured():
+    _learning_rates(captured=True)
