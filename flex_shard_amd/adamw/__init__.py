@@ -87,22 +87,36 @@ are left alone; two that overlap are refused."""
         """Copies of the saved states, of the types that they have here (``torch``'s
         own loading would cast them to the parameters').  Groups that name no ``state_bits``, ``torch``'s own
         AdamW's, have 32."""
-        groups = []
-        for group in state_dict["param_groups"]:
-            group = {"state_bits": 32, **group}
-            for option in ("amsgrad", "maximize"):
-                if group.get(option):
-                    raise NotImplementedError(f"the AdamW kernels have no {option}")
-            _check_group({**group, "params": ()})
-            groups.append(group)
-        loaded = {}
-        if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:
-            for group, saved in zip(self.param_groups, groups):
-                for p, index in zip(group["params"], saved["params"]):
-                    if index in state_dict["state"]:
-                        loaded[p] = self._copy_of(p, saved["state_bits"], state_dict["state"][index])
-        super().load_state_dict({**state_dict, "param_groups": groups, "state": {}})
-        self.state.update(loaded)
+        loaded: dict[torch.Tensor, dict[str, torch.Tensor]] = {}
+
+        def take(_, state_dict: dict[str, Any]) -> dict[str, Any]:
+            groups, states = [], dict(state_dict["state"])
+            for group in state_dict["param_groups"]:
+                group = {"state_bits": 32, **group}
+                for option in ("amsgrad", "maximize"):
+                    if group.get(option):
+                        raise NotImplementedError(f"the AdamW kernels have no {option}")
+                _check_group({**group, "params": ()})
+                groups.append(group)
+            if [len(g["params"]) for g in groups] == [len(g["params"]) for g in self.param_groups]:
+                for group, saved in zip(self.param_groups, groups):
+                    for p, index in zip(group["params"], saved["params"]):
+                        if states.get(index):
+                            loaded[p] = self._copy_of(p, saved["state_bits"], states[index])
+                            states[index] = {name: value for name, value in states[index].items() if name not in loaded[p]}
+            return {**state_dict, "param_groups": groups, "state": states}
+
+        def put(_) -> None:
+            for p, state in loaded.items():
+                self.state[p] = state | self.state.get(p, {})
+
+        # (behind the hooks that change what is loaded, and ahead of those that look at it)
+        handles = self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(put, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
 
     def _copy_of(self, p: torch.Tensor, bits: int, saved: dict[str, Any]) -> dict[str, torch.Tensor]:
         state = self._new_state(p, bits)

@@ -215,3 +215,76 @@ def test_states_of_torchs_own_are_loaded():
     bad["param_groups"][0]["betas"] = (0.9, 1.0)
     with pytest.raises(ValueError, match="betas"):
         mine.load_state_dict(bad)
+
+
+def _saved(bits):
+    """A saved optimizer of two parameters, the first with states."""
+    params = [torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(3))]
+    optimizer = FlexShardAdamW(params, state_bits=bits)
+    optimizer.state[params[0]] = optimizer._new_state(params[0], bits)
+    optimizer.state[params[0]]["exp_avg"].copy_(torch.arange(5))
+    optimizer.state[params[0]]["step"].fill_(7)
+    return optimizer.state_dict()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_hooks_see_the_states(bits):
+    """A hook ahead of the loading gets all that was saved, and what it puts in its place is loaded; one behind
+    it finds the states loaded."""
+    params = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
+    optimizer = FlexShardAdamW(params, state_bits=bits)
+    seen = []
+
+    def before(which, state_dict):
+        seen.append((which, sorted(state_dict["state"]), sorted(state_dict["state"][0])))
+        state = dict(state_dict["state"][0])
+        state["exp_avg"] = state["exp_avg"] + 2  # (renamed, cut or converted, say)
+        return {**state_dict, "state": {0: state}, "param_groups": [{**group, "lr": 0.25} for group in state_dict["param_groups"]]}
+
+    def behind(which):
+        seen.append((which, int(which.state[params[0]]["step"]), which.state[params[0]]["exp_avg"].tolist()))
+
+    optimizer.register_load_state_dict_pre_hook(before)
+    optimizer.register_load_state_dict_post_hook(behind)
+    saved = _saved(bits)
+    names = sorted(saved["state"][0])
+    for _ in range(2):
+        optimizer.load_state_dict(saved)
+        assert seen == [(optimizer, [0], names), (optimizer, 7, [2, 3, 4, 5, 6])]
+        state = optimizer.state[params[0]]
+        assert state["exp_avg"].dtype == (torch.uint8 if bits == 8 else torch.float32) and state["step"].dtype == torch.int32
+        assert optimizer.param_groups[0]["lr"] == 0.25 and not optimizer.state.get(params[1])
+        seen.clear()
+    assert saved["state"][0]["exp_avg"].tolist() == [0, 1, 2, 3, 4]
+
+
+def test_what_else_was_saved_is_loaded():
+    """States of other names, of no parameter, and of a parameter that has none yet."""
+    params = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
+    optimizer = FlexShardAdamW(params)
+    saved = _saved(32)
+    saved["state"][0]["note"] = torch.tensor([4.0])
+    saved["state"][1] = {}
+    saved["state"]["all"] = torch.tensor(3.0)
+    optimizer.load_state_dict(saved)
+    assert optimizer.state["all"].item() == 3 and not optimizer.state.get(params[1])
+    state = optimizer.state[params[0]]
+    assert state["note"].item() == 4 and int(state["step"]) == 7 and state["exp_avg"].tolist() == [0, 1, 2, 3, 4]
+    assert state["exp_avg"] is not saved["state"][0]["exp_avg"] and state["step"].dtype == torch.int32
+
+
+def test_a_refused_loading_changes_nothing():
+    params = [torch.nn.Parameter(torch.zeros(5)), torch.nn.Parameter(torch.zeros(3))]
+    optimizer = FlexShardAdamW(params, lr=0.5)
+    optimizer.load_state_dict(_saved(32) | {"param_groups": [{**_saved(32)["param_groups"][0], "lr": 0.5}]})
+    kept = optimizer.state[params[0]]
+    calls = []
+    optimizer.register_load_state_dict_post_hook(calls.append)
+    other = _saved(32)
+    other["state"][0]["exp_avg_sq"] = torch.zeros(4)
+    fewer = _saved(32)
+    fewer["param_groups"][0]["params"] = [0]
+    for bad in (other, fewer):
+        with pytest.raises(ValueError):
+            optimizer.load_state_dict(bad)
+        assert optimizer.state[params[0]] is kept and optimizer.param_groups[0]["lr"] == 0.5 and not calls
