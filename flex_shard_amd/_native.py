@@ -335,6 +335,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "fsh_adamw_step": (
         c_int, [POINTER(c_int64), c_int32, POINTER(AdamWGroup), c_int32, c_void_p, c_double, c_void_p, c_int64, c_void_p],
     ),
+    "fsh_adamw_check": (c_int, [POINTER(c_int64), c_int32, POINTER(AdamWGroup), c_int32]),
     "fsh_adamw_state_values": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p],
     ),

@@ -15,7 +15,7 @@ from typing import Any, Iterable
 import torch
 
 from .. import _native, hip_ops
-from .._native import ADAMW_BLOCK, ADAMW_GROUPS, DT_BF16, DT_F32
+from .._native import ADAMW_BLOCK, DT_BF16, DT_F32
 
 _DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32}
 
@@ -147,7 +147,6 @@ are left alone; two that overlap are refused."""
         device, index = None, -1
         groups: list[tuple] = []
         table: list[int] = []
-        calls = [(table, groups)]
         stepped, copies = [], []  # (the queued kernels read the copies)
         states, strided, int32 = self.state, torch.strided, torch.int32
         for group in self.param_groups:
@@ -202,13 +201,8 @@ are left alone; two that overlap are refused."""
             if isinstance(lr, torch.Tensor):
                 lr, address = _learning_rate(lr, device)
             groups.append((lr, address, *group["betas"], group["eps"], group["weight_decay"]))
-            if len(groups) == ADAMW_GROUPS:
-                table, groups = [], []
-                calls.append((table, groups))
-        for table, groups in calls:  # (nothing is queued before all of it has been checked)
-            if table:
-                hip_ops.adamw_step(table, groups, device, square_sum, max_norm or 0.0)
         if stepped:
+            hip_ops.adamw_step(table, groups, device, square_sum, max_norm or 0.0)  # (checks all of it before any of it is queued)
             torch.autograd.graph.increment_version(stepped)
         return loss
 

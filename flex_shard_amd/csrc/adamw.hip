@@ -579,6 +579,31 @@ int tensors_overlap(const fsh_adamw_tensor* tensors, int32_t count) {
   return 0;
 }
 
+// What a step refuses of its tensors and groups.
+int check_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const char* who) {
+  for (int32_t i = 0; i < group_count; ++i) {
+    const fsh_adamw_group& g = groups[i];
+    if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return fail(FSH_EINVAL, "%s: group %d: betas in [0, 1), eps not negative", who, i);
+    if (!aligned(g.lr_dev, 4)) return fail(FSH_ENOTSUP, "%s: group %d: the learning rate must be 4-byte aligned", who, i);
+  }
+  for (int32_t i = 0; i < count; ++i) {
+    const fsh_adamw_tensor& t = tensors[i];
+    if (t.numel < 0 || t.group < 0 || t.group >= group_count) return fail(FSH_EINVAL, "%s: tensor %d: negative size, or group %lld of %d", who, i, (long long)t.group, group_count);
+    if ((t.param_dtype != FSH_DT_BF16 && t.param_dtype != FSH_DT_F32) || (t.grad_dtype != FSH_DT_BF16 && t.grad_dtype != FSH_DT_F32) || (t.state_bits != 8 && t.state_bits != 32))
+      return fail(FSH_EINVAL, "%s: tensor %d: bf16 or fp32 parameters and gradients, states of 8 or 32 bits", who, i);
+    if (!t.step_dev || (t.numel && (!t.param_dev || !t.grad_dev || !t.exp_avg_dev || !t.exp_avg_sq_dev || (t.state_bits == 8 && (!t.exp_avg_scale_dev || !t.exp_avg_sq_scale_dev)))))
+      return fail(FSH_EINVAL, "%s: tensor %d: null pointer", who, i);
+    if (!aligned(t.param_dev, bytes_of(t.param_dtype)) || !aligned(t.grad_dev, bytes_of(t.grad_dtype)) || !aligned(t.exp_avg_dev, t.state_bits == 8 ? 1 : 4) ||
+        !aligned(t.exp_avg_sq_dev, t.state_bits == 8 ? 1 : 4) || !aligned(t.exp_avg_scale_dev, 4) || !aligned(t.exp_avg_sq_scale_dev, 4) || !aligned(t.step_dev, 4))
+      return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
+    if (ceil_div(t.numel, (int64_t)chunk_of(t.state_bits == 8)) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
+  }
+  if (const int overlap = tensors_overlap(tensors, count))
+    return overlap < 0 ? fail(FSH_ENOTSUP, "%s: no host memory for %d tensors", who, count)
+                       : fail(FSH_EINVAL, "%s: two tensors overlap, or share a step count", who);
+  return FSH_OK;
+}
+
 template <int PT, int GT>
 void launch_step(const AdamTable& a, bool eight, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(a.chunks < kMaxGrid ? a.chunks : kMaxGrid)), block(kThreads);
@@ -653,6 +678,15 @@ FSH_API int64_t fsh_adamw_step_workspace_bytes(int32_t count) {
   return count < 0 ? 0 : static_cast<int64_t>(count) * static_cast<int64_t>(sizeof(fsh::StepFactors));
 }
 
+FSH_API int fsh_adamw_check(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count) {
+  using namespace fsh;
+  const char* who = "fsh_adamw_check";
+  if (count < 0 || group_count < 0) return fail(FSH_EINVAL, "%s: negative count", who);
+  if (count == 0) return FSH_OK;
+  if (!tensors || !groups) return fail(FSH_EINVAL, "%s: null pointer", who);
+  return check_step(tensors, count, groups, group_count, who);
+}
+
 FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const double* square_sum_dev,
                            double max_norm, void* workspace_dev, int64_t workspace_nbytes, void* stream) {
   using namespace fsh;
@@ -665,26 +699,7 @@ FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const
     return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", who, (long long)workspace_nbytes, (long long)fsh_adamw_step_workspace_bytes(count));
   if (!aligned(square_sum_dev, 8)) return fail(FSH_ENOTSUP, "%s: the sum of squares must be 8-byte aligned", who);
   if (max_norm != max_norm) return fail(FSH_EINVAL, "%s: max_norm is not a number", who);
-  for (int32_t i = 0; i < group_count; ++i) {
-    const fsh_adamw_group& g = groups[i];
-    if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return fail(FSH_EINVAL, "%s: group %d: betas in [0, 1), eps not negative", who, i);
-    if (!aligned(g.lr_dev, 4)) return fail(FSH_ENOTSUP, "%s: group %d: the learning rate must be 4-byte aligned", who, i);
-  }
-  for (int32_t i = 0; i < count; ++i) {
-    const fsh_adamw_tensor& t = tensors[i];
-    if (t.numel < 0 || t.group < 0 || t.group >= group_count) return fail(FSH_EINVAL, "%s: tensor %d: negative size, or group %lld of %d", who, i, (long long)t.group, group_count);
-    if ((t.param_dtype != FSH_DT_BF16 && t.param_dtype != FSH_DT_F32) || (t.grad_dtype != FSH_DT_BF16 && t.grad_dtype != FSH_DT_F32) || (t.state_bits != 8 && t.state_bits != 32))
-      return fail(FSH_EINVAL, "%s: tensor %d: bf16 or fp32 parameters and gradients, states of 8 or 32 bits", who, i);
-    if (!t.step_dev || (t.numel && (!t.param_dev || !t.grad_dev || !t.exp_avg_dev || !t.exp_avg_sq_dev || (t.state_bits == 8 && (!t.exp_avg_scale_dev || !t.exp_avg_sq_scale_dev)))))
-      return fail(FSH_EINVAL, "%s: tensor %d: null pointer", who, i);
-    if (!aligned(t.param_dev, bytes_of(t.param_dtype)) || !aligned(t.grad_dev, bytes_of(t.grad_dtype)) || !aligned(t.exp_avg_dev, t.state_bits == 8 ? 1 : 4) ||
-        !aligned(t.exp_avg_sq_dev, t.state_bits == 8 ? 1 : 4) || !aligned(t.exp_avg_scale_dev, 4) || !aligned(t.exp_avg_sq_scale_dev, 4) || !aligned(t.step_dev, 4))
-      return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
-    if (ceil_div(t.numel, (int64_t)chunk_of(t.state_bits == 8)) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
-  }
-  if (const int overlap = tensors_overlap(tensors, count))
-    return overlap < 0 ? fail(FSH_ENOTSUP, "%s: no host memory for %d tensors", who, count)
-                       : fail(FSH_EINVAL, "%s: two tensors overlap, or share a step count", who);
+  if (int rc = check_step(tensors, count, groups, group_count, who)) return rc;
   const hipStream_t on = static_cast<hipStream_t>(stream);
   StepFactors* const factors = static_cast<StepFactors*>(workspace_dev);
   for (int32_t begin = 0; begin < count; begin += kFactorTensors) {

@@ -1726,21 +1726,43 @@ def adamw_step(
     """``fsh_adamw_step``.  ``table``: the twelve numbers of an ``fsh_adamw_tensor``
     for each tensor, one after the other; the caller answers for the memory that
     they name.  ``groups``: ``(lr, address of a device lr or None, beta1, beta2, eps,
-    weight_decay)`` each, at most ``_native.ADAMW_GROUPS``."""
-    count, rest = divmod(len(table), _native.ADAMW_TENSOR_INT64S)
+    weight_decay)`` each.  More than ``_native.ADAMW_GROUPS`` go in several calls, which begin once all
+    of them have been checked."""
+    width, most = _native.ADAMW_TENSOR_INT64S, _native.ADAMW_GROUPS
+    count, rest = divmod(len(table), width)
     if rest:
-        raise ValueError(f"{_native.ADAMW_TENSOR_INT64S} numbers a tensor, got {len(table)}")
+        raise ValueError(f"{width} numbers a tensor, got {len(table)}")
     if square_sum is not None:
         if square_sum.dtype != torch.float64 or square_sum.numel() != 1 or square_sum.device != device:
             raise ValueError(f"square_sum must be one float64 on {device}, got {square_sum.dtype} {tuple(square_sum.shape)} on {square_sum.device}")
     if not count:
         return
-    of_groups = (_native.AdamWGroup * len(groups))(*groups)
-    nbytes = _native.lib().fsh_adamw_step_workspace_bytes(count)
-    workspace = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+    workspace = torch.empty((_native.lib().fsh_adamw_step_workspace_bytes(count),), dtype=torch.uint8, device=device)
+    if len(groups) <= most:
+        return _adamw_call(table, groups, device, square_sum, max_norm, workspace)
+    _native.check(
+        _native.lib().fsh_adamw_check(
+            (ctypes.c_int64 * len(table))(*table), count, (_native.AdamWGroup * len(groups))(*groups), len(groups)
+        ),
+        "fsh_adamw_check",
+    )
+    parts: list[list[int]] = [[] for _ in range(0, len(groups), most)]
+    for at in range(0, len(table), width):
+        of, number = divmod(table[at + width - 1], most)
+        parts[of] += (*table[at : at + width - 1], number)
+    for i, part in enumerate(parts):
+        if part:
+            _adamw_call(part, groups[most * i : most * (i + 1)], device, square_sum, max_norm, workspace)
+
+
+def _adamw_call(
+    table: Sequence[int], groups: Sequence[tuple], device: torch.device, square_sum: torch.Tensor | None, max_norm: float,
+    workspace: torch.Tensor,
+) -> None:
     _queue(
-        "fsh_adamw_step", device, (ctypes.c_int64 * len(table))(*table), count, of_groups, len(groups),
-        None if square_sum is None else square_sum.data_ptr(), max_norm, workspace.data_ptr(), nbytes,
+        "fsh_adamw_step", device, (ctypes.c_int64 * len(table))(*table), len(table) // _native.ADAMW_TENSOR_INT64S,
+        (_native.AdamWGroup * len(groups))(*groups), len(groups), None if square_sum is None else square_sum.data_ptr(), max_norm,
+        workspace.data_ptr(), workspace.numel(),
     )
 
 

@@ -743,6 +743,9 @@ int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, int64_t ro
  * All argument checks come before any launch; a launch that the runtime then rejects leaves
  * the step half done, as in section 10.
  *
+ * fsh_adamw_check: what the step refuses of its tensors and groups, of any number of groups and without
+ * a launch: ahead of a step that takes several calls, of FSH_ADAMW_GROUPS groups each.
+ *
  * fsh_adamw_state_values: what the codes stand for, in dtype.
  * ---------------------------------------------------------------------- */
 #define FSH_ADAMW_BLOCK 128
@@ -768,6 +771,7 @@ int fsh_grad_square_sum(const int64_t* tensors, int32_t count, double* out_dev, 
 int64_t fsh_adamw_step_workspace_bytes(int32_t count);
 int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count,
                    const double* square_sum_dev, double max_norm, void* workspace_dev, int64_t workspace_nbytes, void* stream);
+int fsh_adamw_check(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count);
 int fsh_adamw_state_values(const void* exp_avg_dev, const float* exp_avg_scale_dev, const void* exp_avg_sq_dev,
                            const float* exp_avg_sq_scale_dev, int64_t numel, void* exp_avg_out_dev, void* exp_avg_sq_out_dev,
                            int32_t dtype, void* stream);

@@ -7,7 +7,7 @@ import pytest
 import torch
 from adamw_definition import FIRST, SECOND, decode, dither, encode
 
-from flex_shard_amd import _native
+from flex_shard_amd import _native, hip_ops
 from flex_shard_amd.adamw import FlexShardAdamW, _check_state, grad_square_sum
 
 OK, EINVAL, ENOTSUP = 0, -22, -95
@@ -288,3 +288,54 @@ def test_a_refused_loading_changes_nothing():
         with pytest.raises(ValueError):
             optimizer.load_state_dict(bad)
         assert optimizer.state[params[0]] is kept and optimizer.param_groups[0]["lr"] == 0.5 and not calls
+
+
+def _many_groups(count, params, group=()):
+    """The tables of as many tensors of 8 fp32 elements, a group each; ``params``: addresses other than their own."""
+    rows = [[(1 << 20) * (i + 1) + (at << 30) for at in range(7)] + [8, _native.DT_F32, _native.DT_F32, 8, i] for i in range(count)]
+    for at, address in params.items():
+        rows[at][0] = address
+    groups = [(1e-3, None, 0.9, 0.95, 1e-8, 0.1)] * count
+    for at, values in dict(group).items():
+        groups[at] = values
+    return rows, groups
+
+
+@pytest.mark.parametrize(
+    "params,group,word",
+    [
+        ({18: (1 << 20) + 28}, {}, "overlap"), ({18: (1 << 20) * 2 - 28}, {}, "overlap"), ({19: 0}, {}, "null"), ({19: (1 << 30) - 2}, {}, "aligned"),
+        ({}, {19: (1e-3, None, 1.0, 0.95, 1e-8, 0.1)}, "group 19"), ({}, {19: (1e-3, SOMEWHERE + 2, 0.9, 0.95, 1e-8, 0.1)}, "group 19"),
+    ],
+)
+def test_groups_of_several_calls_are_checked_together(params, group, word, monkeypatch):
+    """Twenty groups: what is wrong with the last is found before the first call, and so is what overlaps between calls."""
+    rows, groups = _many_groups(20, params, group)
+    table = _table(*(v for row in rows for v in row))
+    check = _native.lib().fsh_adamw_check
+    of_groups = (_native.AdamWGroup * 20)(*groups)
+    assert check(table, 20, of_groups, 20) in (EINVAL, ENOTSUP)
+    assert word in _message() and _message().startswith("fsh_adamw_check")
+    queued = []
+    monkeypatch.setattr(hip_ops, "_queue", lambda *args: queued.append(args))
+    cpu = torch.device("cpu")
+    with pytest.raises(RuntimeError, match=word):
+        hip_ops.adamw_step([v for row in rows for v in row], groups, cpu)
+    assert not queued
+
+
+def test_groups_of_several_calls(monkeypatch):
+    rows, groups = _many_groups(40, {})
+    groups = [(1e-3 * (i + 1), *group[1:]) for i, group in enumerate(groups)]
+    rows = rows[::2] + [rows[i] for i in range(1, 40, 2) if i not in (17, 19)]  # (in any order, two without tensors)
+    queued = []
+    monkeypatch.setattr(hip_ops, "_queue", lambda *args: queued.append(args))
+    hip_ops.adamw_step([v for row in rows for v in row], groups, torch.device("cpu"))
+    got = {}
+    for entry, _, table, count, of_groups, group_count, *_ in queued:
+        assert entry == "fsh_adamw_step" and group_count <= _native.ADAMW_GROUPS and len(table) == 12 * count
+        for at in range(0, 12 * count, 12):
+            got[tuple(table[at : at + 11])] = of_groups[table[at + 11]].lr
+    assert len(queued) == 3 and got == {tuple(row[:11]): groups[row[11]][0] for row in rows}
+    check = _native.lib().fsh_adamw_check
+    assert check(None, 0, None, 0) == OK and check(None, 1, None, 0) == EINVAL and check(None, -1, None, 0) == EINVAL

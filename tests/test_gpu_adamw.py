@@ -569,3 +569,31 @@ def test_learning_rate_on_the_gpu_of_a_group_without_gradients():
 
 def test_learning_rate_on_the_gpu_of_a_group_without_gradients_captured():
     _learning_rates(captured=True)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_is_stepped_when_a_late_group_is_refused(bits):
+    """More groups than one launch takes: all are checked before the first is stepped."""
+    gen = _gen(24)
+    params = _params([(200,)] * 20, F32, gen)
+    whole = torch.zeros(300, device="cuda")
+    params[1], params[18] = (torch.nn.Parameter(whole[a : a + 200]) for a in (0, 100))
+    _set_grads(params, F32, gen)
+    before = [p.detach().clone() for p in params]
+    versions = [p._version for p in params]
+    optimizer = FlexShardAdamW([dict(params=[p]) for p in params], **HYPER, state_bits=bits)
+    with pytest.raises(RuntimeError, match="overlap"):
+        optimizer.step()
+    params[18].data = torch.zeros(200, device="cuda")
+    optimizer.param_groups[19]["betas"] = (0.9, 1.0)
+    with pytest.raises(RuntimeError, match="betas"):
+        optimizer.step()
+    before[18].zero_()
+    assert all(torch.equal(p, q) for p, q in zip(params, before)) and versions == [p._version for p in params]
+    assert all(int(optimizer.state[p]["step"]) == 0 for p in params)
+    optimizer.param_groups[19]["betas"] = HYPER["betas"]
+    optimizer.step()
+    assert all(int(optimizer.state[p]["step"]) == 1 for p in params)
+    for p, q in zip(params, before):
+        want = step64(q, p.grad, torch.zeros_like(q), torch.zeros_like(q), 1, **HYPER)[0]
+        assert torch.allclose(p.detach().double(), want, rtol=8 * U, atol=1e-8)
