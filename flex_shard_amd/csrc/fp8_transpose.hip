@@ -460,6 +460,9 @@ FSH_API int fsh_rms_norm_token_runs(const void* total_dev, int32_t dtype, int64_
   if (int rc = act_quant_params(p, tiles, nullptr, rows, padded, padded, nullptr, 0, nullptr, q_dev, ldq, scales_dev, nullptr, FSH_EPS_FP32, who))
     return rc;
   if (tiles > (1LL << 32) / kTransposeThreads - 1) return fail(FSH_ENOTSUP, "%s: too many tiles", who);  // a launch's threads are counted in 32 bits
+  const RowSpan inputs[] = {{total_dev, rows, cols, ldh, bytes_of(dtype)}, span_of(rstd_dev, rows, 4), span_of(weight_dev, cols, bytes_of(weight_dtype))};
+  const RowSpan outputs[] = {span_of(q_dev, padded * ldq, 1), span_of(scales_dev, ldq / 128 * padded, 4)};
+  if (outputs_overlap(inputs, outputs)) return fail(FSH_EINVAL, "%s: an output overlaps an input or the other output", who);
   const NormRunsParams norm = {total_dev, rstd_dev, weight_dev, cols, ldh, weight_dtype};
   const dim3 grid(static_cast<uint32_t>(tiles)), block(kTransposeThreads);
   const hipStream_t on = static_cast<hipStream_t>(stream);

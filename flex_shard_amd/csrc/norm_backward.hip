@@ -296,15 +296,17 @@ FSH_API int fsh_rms_norm_backward(const fsh_norm_gradient* q, void* stream) {
                 (long long)fsh_rms_norm_backward_workspace_bytes(q->rows, q->cols));
   if (ceil_div(q->cols, (int64_t)32) > (1LL << 22) - 1) return fail(FSH_ENOTSUP, "%s: too many columns", who);
   // (the last columns of a row are written twice, by two lanes that have read them)
-  const RowSpan inputs[] = {{q->grad_dev, q->rows, q->cols, q->ldg, bytes_of(g)},
-                            {q->total_dev, q->rows, q->cols, q->ldh, bytes_of(h)},
-                            {q->grad_total_dev, q->rows, q->cols, q->ldt, bytes_of(h)},
-                            {q->weight_dev, 1, q->cols, q->cols, bytes_of(q->weight_dtype)}};
-  const RowSpan outputs[] = {{q->grad_x_dev, q->rows, q->cols, q->cols, bytes_of(x)},
-                             {h == x ? nullptr : q->grad_residual_dev, q->rows, q->cols, q->cols, bytes_of(h)}};
-  for (const RowSpan& in : inputs)
-    for (const RowSpan& out : outputs)
-      if (share(in, out)) return fail(FSH_EINVAL, "%s: an output overlaps an input", who);
+  const int64_t n = q->rows, k = q->cols;
+  const RowSpan inputs[] = {{q->grad_dev, n, k, q->ldg, bytes_of(g)},
+                            {q->total_dev, n, k, q->ldh, bytes_of(h)},
+                            {q->grad_total_dev, n, k, q->ldt, bytes_of(h)},
+                            span_of(q->weight_dev, k, bytes_of(q->weight_dtype)),
+                            span_of(q->rstd_dev, n, 4)};
+  const RowSpan outputs[] = {span_of(q->grad_x_dev, n * k, bytes_of(x)),
+                             span_of(h == x ? nullptr : q->grad_residual_dev, n * k, bytes_of(h)),
+                             span_of(q->grad_weight_dev, k, bytes_of(q->weight_dtype)),
+                             span_of(q->grad_weight_dev ? q->workspace_dev : nullptr, fsh_rms_norm_backward_workspace_bytes(n, k), 1)};
+  if (outputs_overlap(inputs, outputs)) return fail(FSH_EINVAL, "%s: an output or the workspace overlaps an input or another output", who);
   NormGradParams p = {};
   p.grad = q->grad_dev;
   p.h = q->total_dev;

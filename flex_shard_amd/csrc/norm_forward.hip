@@ -301,16 +301,15 @@ FSH_API int fsh_rms_norm(const fsh_norm* q, void* stream) {
       (q->weight_dev && !aligned(q->weight_dev, bytes_of(q->weight_dtype))) || !aligned(q->out_dev, quant ? 8 : bytes_of(q->x_dtype)) ||
       !aligned(q->scales_dev, 4) || !aligned(q->rstd_dev, 4))
     return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements, bytes to 8", who);
-  // (the last columns of a row are written twice, by two lanes that have read them)
-  const int64_t n = q->rows, k = q->cols, kq = ceil_div(k, (int64_t)128) * 128;
+  // (the last columns of a row are written twice, by two lanes that have read them; wide rows read the total back)
+  const int64_t n = q->rows, k = q->cols, runs = ceil_div(k, (int64_t)128);
   const RowSpan inputs[] = {{q->x_dev, n, k, q->ldx, bytes_of(q->x_dtype)},
                             {q->residual_dev, n, k, q->ldr, bytes_of(q->residual_dtype)},
-                            {q->weight_dev, 1, k, k, bytes_of(q->weight_dtype)}};
-  const RowSpan outputs[] = {{residual ? q->total_dev : nullptr, n, k, k, bytes_of(q->residual_dtype)},
-                             {q->out_dev, n, quant ? kq : k, quant ? kq : k, quant ? 1 : bytes_of(q->x_dtype)}};
-  for (const RowSpan& in : inputs)
-    for (const RowSpan& out : outputs)
-      if (share(in, out)) return fail(FSH_EINVAL, "%s: an output overlaps an input", who);
+                            span_of(q->weight_dev, k, bytes_of(q->weight_dtype))};
+  const RowSpan outputs[] = {span_of(residual ? q->total_dev : nullptr, n * k, bytes_of(q->residual_dtype)),
+                             span_of(q->out_dev, quant ? n * runs * 128 : n * k, quant ? 1 : bytes_of(q->x_dtype)),
+                             span_of(quant ? q->scales_dev : nullptr, n * runs, 4), span_of(q->rstd_dev, n, 4)};
+  if (outputs_overlap(inputs, outputs)) return fail(FSH_EINVAL, "%s: an output overlaps an input or another output", who);
   NormParams p = {};
   p.x = q->x_dev;
   p.residual = q->residual_dev;
@@ -351,6 +350,10 @@ FSH_API int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, in
     return fail(FSH_EINVAL, "%s: ldq %lld is less than cols %lld rounded up to 128", who, (long long)ldq, (long long)cols);
   if (ldq % 8 || !aligned(q_dev, 8) || !aligned(scales_dev, 4) || !aligned(out_dev, bytes_of(dtype)))
     return fail(FSH_ENOTSUP, "%s: the bytes' rows must be 8-byte aligned, the others to their elements", who);
+  const int64_t runs = ceil_div(cols, (int64_t)128);
+  const RowSpan inputs[] = {{q_dev, rows, runs * 128, ldq, 1}, span_of(scales_dev, rows * runs, 4)};
+  const RowSpan outputs[] = {span_of(out_dev, rows * cols, bytes_of(dtype))};
+  if (outputs_overlap(inputs, outputs)) return fail(FSH_EINVAL, "%s: the output overlaps an input", who);
   DequantParams p = {static_cast<const uint8_t*>(q_dev), scales_dev, out_dev, rows, cols, ldq, ceil_div(cols, (int64_t)8)};
   constexpr int64_t kMaxGrid = (1LL << 32) / 256 - 1;
   const int64_t blocks = ceil_div(rows * p.chunks, (int64_t)256);

@@ -73,17 +73,5 @@ void by_ends(int64_t cols, Launch launch) {
   else launch(std::integral_constant<int, kEven>{});
 }
 
-// Rows in memory; whether two of them may share some (a null one never does).
-struct RowSpan {
-  const void* base;
-  int64_t rows, cols, ld, size;
-};
-inline bool share(const RowSpan& a, const RowSpan& b) {
-  if (!a.base || !b.base) return false;
-  const auto from = [](const RowSpan& r) { return reinterpret_cast<uintptr_t>(r.base); };
-  const auto to = [&](const RowSpan& r) { return from(r) + static_cast<uintptr_t>(((r.rows - 1) * r.ld + r.cols) * r.size); };
-  return from(a) < to(b) && from(b) < to(a);
-}
-
 }  // namespace
 }  // namespace fsh

@@ -13,6 +13,31 @@ constexpr int kNoType = -1;  // of an operand that is not there
 inline bool is_dtype(int32_t dtype) { return dtype == FSH_DT_BF16 || dtype == FSH_DT_F32 || dtype == FSH_DT_F16; }
 constexpr int bytes_of(int dtype) { return dtype == FSH_DT_F32 ? 4 : dtype == kNoType ? 0 : 2; }
 
+// Rows in memory (base null: none); whether two of them may share some of it.
+struct RowSpan {
+  const void* base;
+  int64_t rows, cols, ld, size;
+};
+inline bool share(const RowSpan& a, const RowSpan& b) {
+  if (!a.base || !b.base) return false;
+  const auto from = [](const RowSpan& r) { return reinterpret_cast<uintptr_t>(r.base); };
+  const auto to = [&](const RowSpan& r) { return from(r) + static_cast<uintptr_t>(((r.rows - 1) * r.ld + r.cols) * r.size); };
+  return from(a) < to(b) && from(b) < to(a);
+}
+// `count` elements of `size` bytes.
+inline RowSpan span_of(const void* base, int64_t count, int64_t size) { return {base, 1, count, count, size}; }
+// Whether an output lies over an input or another output.
+template <int M, int N>
+bool outputs_overlap(const RowSpan (&inputs)[M], const RowSpan (&outputs)[N]) {
+  for (int i = 0; i < N; ++i) {
+    for (const RowSpan& in : inputs)
+      if (share(in, outputs[i])) return true;
+    for (int j = 0; j < i; ++j)
+      if (share(outputs[j], outputs[i])) return true;
+  }
+  return false;
+}
+
 // VEC elements as they lie in memory.
 template <int DT, int VEC>
 struct RawVec {

@@ -665,7 +665,8 @@ int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, cons
  *   FSH_NORM_FP8     y rounded to bf16 and quantized like section 8's activations:
  *                    out [rows][cols rounded up to 128] E4M3FN bytes (pad zero),
  *                    scales [that / 128][rows]; the bits of fsh_act_quant_1x128
- * ldx, ldr: row strides of x and residual.  No output may overlap an input, here or in the backward.
+ * ldx, ldr: row strides of x and residual.  In this section no output (nor the workspace) may overlap an
+ * input or another output.
  *
  * fsh_rms_norm_backward: of h (total, x_dtype's or fp32, row stride ldh), the
  * output's gradient (x_dtype or, for the FP8 form, bf16; ldg) and, or null, the

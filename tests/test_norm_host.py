@@ -158,3 +158,34 @@ def test_a_name_that_the_filter_leaves_out_keeps_its_norm():
     model = torch.nn.ModuleDict({"a": norm, "b": norm, "c": norm})
     convert_to_flex_shard_rms_norm(model, lambda fqn, child: fqn != "b")
     assert type(model["a"]) is FlexShardRMSNorm and model["c"] is model["a"] and model["b"] is norm
+
+
+def test_outputs_that_overlap_each_other():
+    """Or an input that is read late: the factors over a row's end, the scales over the weight, the sum under the norm."""
+    lib = _native.lib()
+    apart = {name: SOMEWHERE + (i << 20) for i, name in enumerate(("x_dev", "residual_dev", "weight_dev", "total_dev", "out_dev", "scales_dev", "rstd_dev"))}
+    fp8 = dict(form=_native.NORM_FP8)
+    for fields in (
+        dict(out_dev=apart["total_dev"] + 798), dict(total_dev=apart["out_dev"] + 798), fp8 | dict(out_dev=apart["total_dev"] - 504),
+        dict(rstd_dev=apart["x_dev"] + 796), dict(rstd_dev=apart["weight_dev"] - 12), dict(rstd_dev=apart["out_dev"]),
+        dict(rstd_dev=apart["total_dev"] + 796), fp8 | dict(scales_dev=apart["x_dev"]), fp8 | dict(scales_dev=apart["weight_dev"] - 12),
+        fp8 | dict(scales_dev=apart["out_dev"] + 508), fp8 | dict(scales_dev=apart["rstd_dev"] + 12),
+    ):
+        assert lib.fsh_rms_norm(_norm(**apart | fields), None) == EINVAL and "overlaps" in _message(), fields
+    names = ("grad_dev", "total_dev", "weight_dev", "rstd_dev", "grad_total_dev", "grad_x_dev", "grad_residual_dev", "grad_weight_dev", "workspace_dev")
+    apart = {name: SOMEWHERE + (i << 20) for i, name in enumerate(names)} | dict(workspace_nbytes=1600)
+    wide = dict(total_dtype=F32)
+    assert lib.fsh_rms_norm_backward_workspace_bytes(4, 100) == 400  # (what is used of it)
+    for fields in (
+        dict(grad_x_dev=apart["rstd_dev"] - 796), dict(grad_weight_dev=apart["weight_dev"] + 198), dict(grad_weight_dev=apart["grad_x_dev"] + 798),
+        dict(workspace_dev=apart["grad_dev"]), dict(workspace_dev=apart["grad_weight_dev"] - 396), dict(workspace_dev=apart["grad_x_dev"] + 796),
+        wide | dict(grad_residual_dev=apart["grad_x_dev"] - 1596), wide | dict(grad_residual_dev=apart["total_dev"] + 1596),
+    ):
+        assert lib.fsh_rms_norm_backward(_gradient(**apart | fields), None) == EINVAL and "overlaps" in _message(), fields
+    h, rstd, weight, q, scales = (SOMEWHERE + (i << 20) for i in range(5))
+    for fields in (dict(q=h + 39984), dict(q=rstd - 16), dict(scales=weight), dict(scales=q + 104 * 256 - 4), dict(scales=h)):
+        at = dict(q=q, scales=scales) | fields
+        assert lib.fsh_rms_norm_token_runs(h, BF16, 200, 100, 100, rstd, weight, BF16, at["q"], 256, at["scales"], None) == EINVAL, fields
+        assert "overlaps" in _message()
+    for out in (q, q + 199 * 128 + 126, scales + 796):
+        assert lib.fsh_act_dequant_1x128(q, scales, 200, 100, 128, out, BF16, None) == EINVAL and "overlaps" in _message()
