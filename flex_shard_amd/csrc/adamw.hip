@@ -559,28 +559,49 @@ int square_launches(const int64_t* tensors, int32_t count, Each each) {
   return launches;
 }
 
-// Whether two tensors of a step share memory of their parameters or a step count (one
-// that is listed twice, say): their updates would race.  -1 without memory for the list.
-int tensors_overlap(const fsh_adamw_tensor* tensors, int32_t count) {
+// Whether a step writes memory that it also reads or writes elsewhere (a parameter that is listed
+// twice, say): parameters, states, scales, step counts and the workspace, each once, and no gradient
+// over them, but for one that is its own parameter, which every thread reads before it writes there. -1 without
+// memory for the list.
+int tensors_overlap(const fsh_adamw_tensor* tensors, int32_t count, const void* workspace) {
   struct Span {
     uintptr_t begin, end;
+    bool written;
   };
-  std::unique_ptr<Span[]> spans(new (std::nothrow) Span[2 * static_cast<size_t>(count)]);
+  std::unique_ptr<Span[]> spans(new (std::nothrow) Span[7 * static_cast<size_t>(count) + 1]);
   if (!spans) return -1;
   size_t n = 0;
+  const auto add = [&](const void* base, int64_t nbytes, bool written) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(base);
+    if (base) spans[n++] = {begin, begin + static_cast<uintptr_t>(nbytes), written};
+  };
+  add(workspace, fsh_adamw_step_workspace_bytes(count), true);
   for (int32_t i = 0; i < count; ++i) {
-    const uintptr_t step = reinterpret_cast<uintptr_t>(tensors[i].step_dev), param = reinterpret_cast<uintptr_t>(tensors[i].param_dev);
-    spans[n++] = {step, step + sizeof(int32_t)};
-    if (tensors[i].numel) spans[n++] = {param, param + static_cast<uintptr_t>(tensors[i].numel) * bytes_of(static_cast<int>(tensors[i].param_dtype))};
+    const fsh_adamw_tensor& t = tensors[i];
+    add(t.step_dev, sizeof(int32_t), true);
+    if (t.numel == 0) continue;
+    const int64_t state = t.state_bits == 8 ? 1 : 4;
+    add(t.param_dev, t.numel * bytes_of(static_cast<int>(t.param_dtype)), true);
+    if (t.grad_dev != t.param_dev || t.grad_dtype != t.param_dtype) add(t.grad_dev, t.numel * bytes_of(static_cast<int>(t.grad_dtype)), false);
+    add(t.exp_avg_dev, t.numel * state, true);
+    add(t.exp_avg_sq_dev, t.numel * state, true);
+    if (t.state_bits != 8) continue;
+    add(t.exp_avg_scale_dev, 4 * ceil_div(t.numel, (int64_t)kStateBlock), true);
+    add(t.exp_avg_sq_scale_dev, 4 * ceil_div(t.numel, (int64_t)kStateBlock), true);
   }
   std::sort(spans.get(), spans.get() + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
-  for (size_t i = 1; i < n; ++i)
-    if (spans[i].begin < spans[i - 1].end) return 1;
+  uintptr_t written = 0, touched = 0;  // ends of those before
+  for (size_t i = 0; i < n; ++i) {
+    const Span& s = spans[i];
+    if (s.begin < (s.written ? touched : written)) return 1;
+    touched = std::max(touched, s.end);
+    if (s.written) written = std::max(written, s.end);
+  }
   return 0;
 }
 
 // What a step refuses of its tensors and groups.
-int check_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const char* who) {
+int check_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const void* workspace, const char* who) {
   for (int32_t i = 0; i < group_count; ++i) {
     const fsh_adamw_group& g = groups[i];
     if (!(g.beta1 >= 0.0 && g.beta1 < 1.0 && g.beta2 >= 0.0 && g.beta2 < 1.0 && g.eps >= 0.0)) return fail(FSH_EINVAL, "%s: group %d: betas in [0, 1), eps not negative", who, i);
@@ -598,9 +619,9 @@ int check_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_g
       return fail(FSH_ENOTSUP, "%s: tensor %d is not aligned to its elements", who, i);
     if (ceil_div(t.numel, (int64_t)chunk_of(t.state_bits == 8)) > kMaxChunks) return fail(FSH_ENOTSUP, "%s: tensor %d is too long", who, i);
   }
-  if (const int overlap = tensors_overlap(tensors, count))
+  if (const int overlap = tensors_overlap(tensors, count, workspace))
     return overlap < 0 ? fail(FSH_ENOTSUP, "%s: no host memory for %d tensors", who, count)
-                       : fail(FSH_EINVAL, "%s: two tensors overlap, or share a step count", who);
+                       : fail(FSH_EINVAL, "%s: parameters, gradients, states, step counts or the workspace overlap", who);
   return FSH_OK;
 }
 
@@ -684,7 +705,7 @@ FSH_API int fsh_adamw_check(const fsh_adamw_tensor* tensors, int32_t count, cons
   if (count < 0 || group_count < 0) return fail(FSH_EINVAL, "%s: negative count", who);
   if (count == 0) return FSH_OK;
   if (!tensors || !groups) return fail(FSH_EINVAL, "%s: null pointer", who);
-  return check_step(tensors, count, groups, group_count, who);
+  return check_step(tensors, count, groups, group_count, nullptr, who);
 }
 
 FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const fsh_adamw_group* groups, int32_t group_count, const double* square_sum_dev,
@@ -699,7 +720,7 @@ FSH_API int fsh_adamw_step(const fsh_adamw_tensor* tensors, int32_t count, const
     return fail(FSH_EINVAL, "%s: workspace of %lld bytes, %lld needed, 16-byte aligned", who, (long long)workspace_nbytes, (long long)fsh_adamw_step_workspace_bytes(count));
   if (!aligned(square_sum_dev, 8)) return fail(FSH_ENOTSUP, "%s: the sum of squares must be 8-byte aligned", who);
   if (max_norm != max_norm) return fail(FSH_EINVAL, "%s: max_norm is not a number", who);
-  if (int rc = check_step(tensors, count, groups, group_count, who)) return rc;
+  if (int rc = check_step(tensors, count, groups, group_count, workspace_dev, who)) return rc;
   const hipStream_t on = static_cast<hipStream_t>(stream);
   StepFactors* const factors = static_cast<StepFactors*>(workspace_dev);
   for (int32_t begin = 0; begin < count; begin += kFactorTensors) {
@@ -764,6 +785,10 @@ FSH_API int fsh_adamw_state_values(const void* exp_avg_dev, const float* exp_avg
   if (!exp_avg_dev || !exp_avg_scale_dev || !exp_avg_sq_dev || !exp_avg_sq_scale_dev || !exp_avg_out_dev || !exp_avg_sq_out_dev) return fail(FSH_EINVAL, "%s: null pointer", who);
   if (!aligned(exp_avg_scale_dev, 4) || !aligned(exp_avg_sq_scale_dev, 4) || !aligned(exp_avg_out_dev, bytes_of(dtype)) || !aligned(exp_avg_sq_out_dev, bytes_of(dtype)))
     return fail(FSH_ENOTSUP, "%s: tensors must be aligned to their elements", who);
+  const int64_t scales = ceil_div(numel, (int64_t)kStateBlock);
+  const RowSpan inputs[] = {span_of(exp_avg_dev, numel, 1), span_of(exp_avg_sq_dev, numel, 1), span_of(exp_avg_scale_dev, scales, 4), span_of(exp_avg_sq_scale_dev, scales, 4)};
+  const RowSpan outputs[] = {span_of(exp_avg_out_dev, numel, bytes_of(dtype)), span_of(exp_avg_sq_out_dev, numel, bytes_of(dtype))};
+  if (outputs_overlap(inputs, outputs)) return fail(FSH_EINVAL, "%s: an output overlaps an input or the other output", who);
   const int64_t blocks = ceil_div(numel, (int64_t)kThreads * 8);
   const dim3 grid(static_cast<uint32_t>(blocks < kMaxGrid ? blocks : kMaxGrid)), block(kThreads);
   const hipStream_t on = static_cast<hipStream_t>(stream);

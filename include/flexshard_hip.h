@@ -735,7 +735,8 @@ int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, int64_t ro
  * A square_sum that is an infinity or not a number leaves everything, step counts
  * included, as it is.  Tensors and groups are host tables, read within the call; lr_dev, if not
  * null, is read by the step in place of lr.  Parameters and gradients: bf16 or fp32, contiguous,
- * aligned to their elements; no two tensors of a call overlap.  States: fp32, or 8-bit codes with an fp32 scale for each
+ * aligned to their elements.  Parameters, states, scales, step counts and the workspace do not overlap each
+ * other, nor a gradient (which may be shared, or be its own parameter).  States: fp32, or 8-bit codes with an fp32 scale for each
  * FSH_ADAMW_BLOCK elements (the last block may be shorter):
  *   magnitude of a code c > 0: the fp32 number of bits (c + 889) << 20 (first moment, c =
  *   code & 127, negative with bit 7) or (c + 761) << 20 (second), times the scale; c = 0: zero

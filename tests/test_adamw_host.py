@@ -339,3 +339,57 @@ def test_groups_of_several_calls(monkeypatch):
     assert len(queued) == 3 and got == {tuple(row[:11]): groups[row[11]][0] for row in rows}
     check = _native.lib().fsh_adamw_check
     assert check(None, 0, None, 0) == OK and check(None, 1, None, 0) == EINVAL and check(None, -1, None, 0) == EINVAL
+
+
+# 0 parameter, 1 gradient, 2 and 3 moments, 4 and 5 scales, 6 step count
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize(
+    "at,over,status",
+    [
+        *(((1, one), (0, other), EINVAL) for one in (0, 2, 3, 6) for other in (0, 2, 3, 6)),
+        *(((1, 1), (0, other), EINVAL) for other in (0, 2, 3, 6)), *(((0, one), (0, other), EINVAL) for one in (2, 3, 6) for other in (0, 1)),
+        ((0, 3), (0, 2), EINVAL), ((1, 1), (0, 1), OK), ((0, 1), (0, 0), OK),
+    ],
+)
+def test_states_and_gradients_that_overlap(bits, at, over, status):
+    """A step's parameters, states and step counts lie apart, and no gradient lies over them; one gradient may serve two."""
+    rows, groups = _many_groups(2, {})
+    for row in rows:
+        row[10] = bits
+    rows[at[0]][at[1]] = rows[over[0]][over[1]]
+    _expect(rows, groups, status)
+
+
+@pytest.mark.parametrize("one", range(7))
+def test_scales_that_overlap(one):
+    for scale in (4, 5):
+        rows, groups = _many_groups(2, {})
+        for row in rows:
+            row[7] = 300  # three blocks
+        rows[1][scale] = rows[0][one] - 8 if one not in (2, 3) else rows[0][one] + 296
+        _expect(rows, groups, EINVAL)
+        rows[1][scale] = rows[0][one] - 12
+        _expect(rows, groups, OK)
+    rows[1][10] = rows[0][10] = 32  # states that have none
+    rows[1][4] = rows[1][5] = rows[0][4]
+    _expect(rows, groups, OK)
+
+
+def _expect(rows, groups, status):
+    of_groups = (_native.AdamWGroup * len(groups))(*groups)
+    assert _native.lib().fsh_adamw_check(_table(*(v for row in rows for v in row)), len(rows), of_groups, len(groups)) == status, rows
+    assert status == OK or "overlap" in _message()
+
+
+def test_a_workspace_over_a_state():
+    rows, groups = _many_groups(1, {})
+    of_groups = (_native.AdamWGroup * 1)(*groups)
+    for at in range(7):
+        table = _table(*rows[0])
+        assert _native.lib().fsh_adamw_step(table, 1, of_groups, 1, None, 0.0, rows[0][at] - 32, 1 << 20, None) == EINVAL and "overlap" in _message()
+
+
+def test_state_values_over_their_codes():
+    call, far = _native.lib().fsh_adamw_state_values, [SOMEWHERE + (i << 20) for i in range(6)]
+    for first, second in ((far[0], far[5]), (far[4], far[2] - 198), (far[1] - 196, far[5]), (far[4], far[4] + 198)):
+        assert call(*far[:4], 100, first, second, _native.DT_BF16, None) == EINVAL and "overlaps" in _message()
