@@ -102,8 +102,10 @@ are left alone; two that overlap are refused."""
                 for group, saved in zip(self.param_groups, groups):
                     for p, index in zip(group["params"], saved["params"]):
                         if states.get(index):
-                            loaded[p] = self._copy_of(p, saved["state_bits"], states[index])
-                            states[index] = {name: value for name, value in states[index].items() if name not in loaded[p]}
+                            state = states.pop(index)
+                            loaded[p] = mine = self._copy_of(p, saved["state_bits"], state)
+                            if len(state) > len(mine):  # (states of other names)
+                                states[index] = {name: value for name, value in state.items() if name not in mine}
             return {**state_dict, "param_groups": groups, "state": states}
 
         def put(_) -> None:
