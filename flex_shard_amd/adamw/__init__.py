@@ -38,11 +38,13 @@ class FlexShardAdamW(torch.optim.Optimizer):
     ``state_bits`` 32: ``exp_avg`` and ``exp_avg_sq`` are fp32 whatever the parameter's type.
     8: they are uint8 codes with fp32 scales for every 128 elements (``exp_avg_scale``,
     ``exp_avg_sq_scale``; :meth:`state_values` gives what they stand for): 2 1/16
-    bytes an element for 8.  Arithmetic is in fp32, the parameter rounded once.  ``step`` is
+    bytes an element for 8.  Arithmetic is in fp32, the parameter rounded once; with 8 bits the
+    second moment's root and the moments' quotient are the hardware's, each to one unit in
+    fp32's last place, and a second moment below 2**-126 may count as zero.  ``step`` is
     an int32 on the GPU, so that a captured step counts on; ``lr`` may be an fp32 scalar
     there, which a captured step reads anew.  A captured step keeps the addresses that it was
-captured with: load states, and take new gradients' memory, before.  Parameters without a gradient
-are left alone; two that overlap are refused."""
+    captured with: load states, and take new gradients' memory, before.  Parameters without a gradient
+    are left alone; parameters or states that overlap are refused, before anything is stepped."""
 
     def __init__(
         self, params, lr: float | torch.Tensor = 1e-3, betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,

@@ -201,8 +201,9 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* par
 }
 
 // launch(layout) with the layout for rows of `cols` columns.  Two workgroups or more to a
-// compute unit: 8192 rows of 5120 bf16 take 63 us by 448 threads, 78 by 1024 (but 1000 of 7168 28 for 26, and with
-// an fp32 stream 178 for 166); 24576 of 1040 47 by 64 and 56 by 256; 16384 of 2048 51 and 54.
+// compute unit: 8192 rows of 5120 bf16 take 63 us by 448 threads, 78 by 1024 (but with
+// an fp32 stream 178 for 166).  With few rows the parts of dw count for more: 512 of 7168 take 19.0 us for 17.6, of 5120 16.1 for 15.4; the
+// two are alike at 1000 and at 768, and at the border 1024 threads take 1.7 and 2.4 us longer.  24576 of 1040 47 by 64 and 56 by 256; 16384 of 2048 51 and 54.
 template <int ENDS, int VEC, typename Launch>
 void by_columns(int64_t rows, int64_t cols, Launch launch) {
   if (ENDS == kPieces || cols <= 64) launch(NormLayout<ENDS, 64 / VEC, VEC, VEC>{});

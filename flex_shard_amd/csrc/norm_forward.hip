@@ -200,8 +200,10 @@ __global__ __launch_bounds__(L::THREADS) void rms_norm_wide_kernel(const NormPar
 // the row's end: 24576 rows of 1040 bf16 take 41 us by 64 threads, 57 by 256; 8192 of 5120, quantized, 62 by 320 and
 // 68 by 256; of 6144 68 by 512, 72 by 256; of 7168 with an fp32 stream, in vectors of four, 108 by 256, and 2 to 4 %
 // more by 512; 4096 of 12288 69 by 768, 81 by 1024.  Narrow rows go two a turn (262144 x 128: 30 us
-// with one, 26 with four).  Few rows get more lanes each: 48 of 7168, quantized, 5.0 us for 6.7; of 2048 the
-// other way round, 33 for 27.  Values and bytes take the same sums: kQuant alone picks whole runs of 128.
+// with one, 26 with four).  Rows of 2049 to 8192 columns get more lanes each where they are few: 48 of 7168, quantized, 5.0 us
+// for 6.7; of 2048 the other way round, 33 for 27.  The two cross between 512 and 768 rows (quantized, with the events around
+// them: 512 of 8192 10.3 for 11.0, 640 alike, 768 14.2 for 13.5; 512 of 4096 7.4 for 7.8), values earlier (512 of 7168 10.0
+// for 8.9).  Values and bytes take the same sums, of an order that this choice changes: kQuant alone picks whole runs of 128.
 template <int ENDS, int VEC, bool kQuant, typename Launch>
 void by_columns(int64_t cols, int64_t rows, Launch launch) {
   const bool few = rows <= 512;

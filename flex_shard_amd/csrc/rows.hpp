@@ -210,8 +210,8 @@ __device__ __forceinline__ uint32_t max32_u32(uint32_t v) {
   return o > v ? o : v;
 }
 
-// The sum over the LANES threads that share a row (8, 16, 32, 64, or a workgroup of
-// 256, 512 or 1024: then `lds` holds a float for each of its waves, twice over, used in turn).
+// The sum over the LANES threads that share a row (8, 16, 32, 64, or a whole workgroup of
+// several waves: then `lds` holds a float for each of them, twice over, used in turn).
 template <int LANES>
 __device__ __forceinline__ float sum_over_row(float v, float* lds, int turn) {
   if constexpr (LANES == 8) return sum8(v);

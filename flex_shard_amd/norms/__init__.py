@@ -129,7 +129,10 @@ def rms_norm(
     """The norm of the rows of ``x`` [..., cols] (bf16, fp16 or fp32), in its type,
     times ``weight`` [cols] (any of these types, or None).  With ``residual``, of the
     shape of ``x`` and its type or fp32, ``(norm of x + residual, x + residual)``, the sum in
-    the residual's type.  Statistics in fp32, every output rounded once; differentiable."""
+    the residual's type.  Statistics in fp32, every output rounded once; differentiable.
+    A row's bits are the same on every run, but a call of more than 512 rows of 2049 to 8192 columns
+    adds up a row in another order than one of fewer: a prompt's row and the same one alone may
+    differ by a rounding."""
     if x.numel() == 0:  # no rows: torch's own empty products keep the graph
         _check(x, weight, eps, residual)
         total = x if residual is None else x.to(residual.dtype) + residual

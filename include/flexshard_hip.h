@@ -660,7 +660,8 @@ int fsh_expert_combine_backward(const void* grad_dev, const void* rows_dev, cons
  * fsh_rms_norm: h = x + residual, rounded to residual_dtype (that of x, or fp32)
  * and written to total (contiguous); h = x without a residual.  s = 1 /
  * sqrt(mean(h^2) + eps) in fp32, to rstd [rows] unless that is null.  y = h s
- * weight (weight null: 1).
+ * weight (weight null: 1).  The order of a row's sum depends on cols and, from 2049 to 8192 of them, on whether
+ * there are more than 512 rows.
  *   FSH_NORM_VALUES  out [rows, cols] of x_dtype, contiguous
  *   FSH_NORM_FP8     y rounded to bf16 and quantized like section 8's activations:
  *                    out [rows][cols rounded up to 128] E4M3FN bytes (pad zero),
@@ -728,7 +729,8 @@ int fsh_act_dequant_1x128(const void* q_dev, const float* scales_dev, int64_t ro
  * in 64 bits, in a fixed order.  tensors: three numbers each, address, elements,
  * dtype (host memory).  workspace: at least ..._workspace_bytes(tensors, count), 8-byte aligned.
  *
- * fsh_adamw_step: per tensor, in fp32 with one rounding to the parameter's type,
+ * fsh_adamw_step: per tensor, in fp32 with one rounding to the parameter's type (with 8-bit states the root
+ * and the quotient to one unit in the last place),
  *   c = min(1, max_norm / (sqrt(square_sum) + 1e-6)), 1 without a sum or a positive max_norm
  *   g = c g;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  t = step + 1, kept
  *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
